@@ -33,7 +33,8 @@ typedef struct CUstream_st* tb200_stream_t; /* == cudaStream_t */
 
 enum tb200_dtype {
   TB200_I8 = 0, TB200_U8 = 1, TB200_I16 = 2, TB200_U16 = 3, TB200_I32 = 4,
-  TB200_U32 = 5, TB200_I64 = 6, TB200_U64 = 7, TB200_F32 = 8, TB200_F64 = 9
+  TB200_U32 = 5, TB200_I64 = 6, TB200_U64 = 7, TB200_F32 = 8, TB200_F64 = 9,
+  TB200_F16 = 10, TB200_BF16 = 11 /* only the operators on rows at the end of this file take these two */
 };
 enum tb200_op { TB200_PLUS = 0, TB200_MIN = 1, TB200_MAX = 2 };
 /* MOD_EQ: x % a == b    LT: x < a    GE: x >= a    NE: x != a */
@@ -346,6 +347,68 @@ int tb200_ipc_export(const void* d_ptr, void* h_handle64, size_t* h_offset);
 int tb200_ipc_open(const void* h_handle64, size_t offset, void** d_ptr_out);
 int tb200_ipc_close(const void* h_handle64);
 int tb200_ipc_close_all(void);
+
+/* ---- Operators on rows of channels: what a language model's layers ask of gather, scan, sort and reduce_by_key.
+ *
+ * Rows hold `dim` neighbouring elements of type t (F32, F16 or BF16); row i of an input begins at i * stride elements
+ * (stride >= dim; outputs are packed).  Arithmetic is in 32 bits, rounded once, to nearest, where a result is stored.  Ids are I32 or I64; an
+ * id outside its range names nothing: its row of a result is zero and nothing that belongs to it is read.
+ * Outputs must not overlap inputs.  None of these has a counterpart in the reference. */
+
+/* d_out[i] = scale * d_weight[d_tokens[i]] for i < n (n < 2^31); zero where the token is outside [0, rows). */
+int tb200_embedding(const void* d_weight, size_t rows, size_t weight_stride, const void* d_tokens, int token_t,
+                    size_t n, size_t dim, int t, float scale, void* d_out, tb200_stream_t stream);
+
+/* Its gradient: d_out[v] = scale * the sum of d_dout[i] over the i with d_tokens[i] == v, for all v < rows; with accumulate != 0
+ * that is added to d_out (of type out_t) instead.  The tokens are sorted with their positions, and the sum of a row goes
+ * over its places in that order: the same inputs give the same bits.  n, rows < 2^31.  The sort's waits are
+ * bounded: one that ran out leaves NaNs in d_out (with accumulate too) and status 1 in the workspace. */
+int tb200_embedding_grad(const void* d_dout, size_t dout_stride, const void* d_tokens, int token_t, size_t n,
+                         size_t rows, size_t dim, int t, int out_t, float scale, int accumulate, void* d_out,
+                         void* d_ws, size_t* ws_bytes, tb200_stream_t stream);
+
+/* A gated linear recurrence along each sequence, channel by channel:
+ *     a = 1 / (1 + exp(-gate[r])),   h[r] = a * h[r - 1] + (1 - a) * x[r],
+ * begun from d_h0[s] (F32, batch x dim, packed; NULL: zero); d_last[s] (F32) is the state behind the sequence's last row, unrounded, or
+ * d_h0[s] if it has none.  Sequence s has rows [d_offsets[s], d_offsets[s + 1]) (batch + 1 of type offset_t, not decreasing); d_offsets ==
+ * NULL: n / batch rows each, which must divide.  Rows before the first and behind the last offset have h = 0. */
+int tb200_gated_scan(const void* d_x, size_t x_stride, const void* d_gate, size_t gate_stride, const void* d_h0,
+                     const void* d_offsets, int offset_t, size_t batch, size_t n, size_t dim, int t, void* d_h,
+                     void* d_last, tb200_stream_t stream);
+
+/* Its gradient.  d_h is what tb200_gated_scan returned; d_dh the gradient of h, d_dlast (F32, may be NULL: zero) that of d_last.
+ *     s[r] = dh[r] + a[r + 1] * s[r + 1] (+ dlast behind the last row),   dx[r] = (1 - a) * s[r],
+ *     dgate[r] = a * (1 - a) * (h[r - 1] - x[r]) * s[r],   dh0 = a * s at the first row (dlast if there is none; F32). */
+int tb200_gated_scan_grad(const void* d_dh, size_t dh_stride, const void* d_x, size_t x_stride, const void* d_gate,
+                          size_t gate_stride, const void* d_h, size_t h_stride, const void* d_h0, const void* d_dlast,
+                          const void* d_offsets, int offset_t, size_t batch, size_t n, size_t dim, int t, void* d_dx,
+                          void* d_dgate, void* d_dh0, tb200_stream_t stream);
+
+/* The recurrence for one token of each of n sequences whose states are kept in d_state (F32, pool x dim, packed): row i uses and
+ * replaces state d_slots[i] (NULL: i).  No slot may occur twice. */
+int tb200_gated_step(const void* d_x, size_t x_stride, const void* d_gate, size_t gate_stride, void* d_state,
+                     size_t pool, const void* d_slots, int slot_t, size_t n, size_t dim, int t, void* d_h,
+                     tb200_stream_t stream);
+
+/* Rows sent to experts: assignment i = token * choices + choice of n tokens goes to expert d_experts[i] < num_experts <= 1024
+ * (choices <= 32, n * choices < 2^30).  d_rows (n * choices of them) gets the tokens' rows by expert, those of an expert in the order of their
+ * assignments, zeros behind the last; d_slots[i] the place of assignment i, -1 if its id is none; d_sources[p] the
+ * assignment at place p, -1 behind the last; d_offsets (num_experts + 1) where the experts' rows begin, and how many there are. */
+int tb200_expert_dispatch(const void* d_x, size_t x_stride, const void* d_experts, int expert_t, size_t n,
+                          size_t choices, size_t num_experts, size_t dim, int t, void* d_rows, int* d_slots,
+                          int* d_sources, int* d_offsets, void* d_ws, size_t* ws_bytes, tb200_stream_t stream);
+
+/* Rows brought back: d_out[token] = the sum over its choices of d_weights[i] * d_rows[d_slots[i]] (F32 weights; NULL: all one),
+ * in the order of the choices, without those that have no place in [0, n * choices).  With NULL it is also the gradient of
+ * tb200_expert_dispatch. */
+int tb200_expert_combine(const void* d_rows, size_t rows_stride, const int* d_slots, const float* d_weights, size_t n,
+                         size_t choices, size_t dim, int t, void* d_out, tb200_stream_t stream);
+
+/* Its gradient: d_drows[d_slots[i]] = d_weights[i] * d_dout[token], d_dweights[i] = <d_dout[token], d_rows[d_slots[i]]> (0 without a
+ * place); rows from *d_kept (the last of d_offsets) on are zero. */
+int tb200_expert_combine_grad(const void* d_dout, size_t dout_stride, const void* d_rows, size_t rows_stride,
+                              const int* d_slots, const float* d_weights, const int* d_kept, size_t n, size_t choices,
+                              size_t dim, int t, void* d_drows, float* d_dweights, tb200_stream_t stream);
 
 #ifdef __cplusplus
 }

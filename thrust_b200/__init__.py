@@ -7,3 +7,4 @@ tests and the benchmark drive.
 from . import _lib  # noqa: F401
 from .api import *  # noqa: F401,F403
 from .api import Tb200Error, workspaces  # noqa: F401
+from .layers import *  # noqa: F401,F403

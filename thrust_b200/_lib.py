@@ -9,7 +9,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libthrust_b200.so")
 
-_vp, _sz, _i, _ll = C.c_void_p, C.c_size_t, C.c_int, C.c_longlong
+_vp, _sz, _i, _ll, _f = C.c_void_p, C.c_size_t, C.c_int, C.c_longlong, C.c_float
 _szp = C.POINTER(C.c_size_t)
 
 # name -> argtypes; every function returns int (cudaError_t)
@@ -55,6 +55,14 @@ PROTOTYPES = {
     "tb200_ipc_close_all": [],
     "tb200_sequence_u32": [_vp, _sz, _vp],
     "tb200_gather": [_vp, _vp, _vp, _sz, _i, _vp],
+    "tb200_embedding": [_vp, _sz, _sz, _vp, _i, _sz, _sz, _i, _f, _vp, _vp],
+    "tb200_embedding_grad": [_vp, _sz, _vp, _i, _sz, _sz, _sz, _i, _i, _f, _i, _vp, _vp, _szp, _vp],
+    "tb200_gated_scan": [_vp, _sz, _vp, _sz, _vp, _vp, _i, _sz, _sz, _sz, _i, _vp, _vp, _vp],
+    "tb200_gated_scan_grad": [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _i, _sz, _sz, _sz, _i, _vp, _vp, _vp, _vp],
+    "tb200_gated_step": [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _i, _sz, _sz, _i, _vp, _vp],
+    "tb200_expert_dispatch": [_vp, _sz, _vp, _i, _sz, _sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _szp, _vp],
+    "tb200_expert_combine": [_vp, _sz, _vp, _vp, _sz, _sz, _sz, _i, _vp, _vp],
+    "tb200_expert_combine_grad": [_vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _i, _vp, _vp, _vp],
     "tb200_kernel_timing": [_i],
     "tb200_kernel_timing_read": [_i, C.POINTER(C.c_int), C.POINTER(C.c_float), C.POINTER(C.c_int)],
 }
