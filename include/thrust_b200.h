@@ -374,7 +374,7 @@ int tb200_embedding_grad(const void* d_dout, size_t dout_stride, const void* d_t
  * NULL: n / batch rows each, which must divide.  Rows before the first and behind the last offset have h = 0. */
 int tb200_gated_scan(const void* d_x, size_t x_stride, const void* d_gate, size_t gate_stride, const void* d_h0,
                      const void* d_offsets, int offset_t, size_t batch, size_t n, size_t dim, int t, void* d_h,
-                     void* d_last, tb200_stream_t stream);
+                     void* d_last, void* d_ws, size_t* ws_bytes, tb200_stream_t stream);
 
 /* Its gradient.  d_h is what tb200_gated_scan returned; d_dh the gradient of h, d_dlast (F32, may be NULL: zero) that of d_last.
  *     s[r] = dh[r] + a[r + 1] * s[r + 1] (+ dlast behind the last row),   dx[r] = (1 - a) * s[r],
@@ -382,7 +382,7 @@ int tb200_gated_scan(const void* d_x, size_t x_stride, const void* d_gate, size_
 int tb200_gated_scan_grad(const void* d_dh, size_t dh_stride, const void* d_x, size_t x_stride, const void* d_gate,
                           size_t gate_stride, const void* d_h, size_t h_stride, const void* d_h0, const void* d_dlast,
                           const void* d_offsets, int offset_t, size_t batch, size_t n, size_t dim, int t, void* d_dx,
-                          void* d_dgate, void* d_dh0, tb200_stream_t stream);
+                          void* d_dgate, void* d_dh0, void* d_ws, size_t* ws_bytes, tb200_stream_t stream);
 
 /* The recurrence for one token of each of n sequences whose states are kept in d_state (F32, pool x dim, packed): row i uses and
  * replaces state d_slots[i] (NULL: i).  No slot may occur twice. */

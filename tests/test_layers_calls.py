@@ -22,20 +22,21 @@ def test_c_calls_refuse_wrong_arguments():
     lib, size = _lib.load(), ctypes.c_size_t(0)
     ref = ctypes.byref(size)
     f32, f64, i32, u8 = 8, 9, 4, 1
+    big = ctypes.byref(ctypes.c_size_t(1 << 20))
     # types
     assert lib.tb200_embedding(BUF, 4, 8, BUF, i32, 2, 8, f64, 1.0, BUF, None) == 801
     assert lib.tb200_embedding(BUF, 4, 8, BUF, u8, 2, 8, f32, 1.0, BUF, None) == 801
-    assert lib.tb200_gated_scan(BUF, 8, BUF, 8, None, BUF, u8, 1, 4, 8, f32, BUF, BUF, None) == 801
+    assert lib.tb200_gated_scan(BUF, 8, BUF, 8, None, BUF, u8, 1, 4, 8, f32, BUF, BUF, BUF, big, None) == 801
     assert lib.tb200_expert_dispatch(BUF, 8, BUF, f32, 2, 1, 4, 8, f32, BUF, BUF, BUF, BUF, None, ref, None) == 801
     # strides shorter than a row, missing buffers, sizes past their limits
     assert lib.tb200_embedding(BUF, 4, 7, BUF, i32, 2, 8, f32, 1.0, BUF, None) == 1
     assert lib.tb200_embedding(None, 4, 8, BUF, i32, 2, 8, f32, 1.0, BUF, None) == 1
     assert lib.tb200_embedding(BUF, 4, 8, BUF, i32, 1 << 31, 8, f32, 1.0, BUF, None) == 1
     assert lib.tb200_embedding_grad(BUF, 8, BUF, i32, 2, 1 << 31, 8, f32, f32, 1.0, 0, BUF, None, ref, None) == 1
-    assert lib.tb200_gated_scan(BUF, 7, BUF, 8, None, None, 0, 1, 4, 8, f32, BUF, BUF, None) == 1
-    assert lib.tb200_gated_scan(BUF, 8, BUF, 8, None, None, 0, 3, 4, 8, f32, BUF, BUF, None) == 1       # 4 rows are no 3 sequences
-    assert lib.tb200_gated_scan(BUF, 8, BUF, 8, None, None, 0, 1, 4, 8, f32, None, BUF, None) == 1
-    assert lib.tb200_gated_scan_grad(BUF, 8, BUF, 8, BUF, 8, BUF, 8, None, None, None, 0, 1, 4, 8, f32, BUF, BUF, None, None) == 1
+    assert lib.tb200_gated_scan(BUF, 7, BUF, 8, None, None, 0, 1, 4, 8, f32, BUF, BUF, BUF, big, None) == 1
+    assert lib.tb200_gated_scan(BUF, 8, BUF, 8, None, None, 0, 3, 4, 8, f32, BUF, BUF, BUF, big, None) == 1       # 4 rows are no 3 sequences
+    assert lib.tb200_gated_scan(BUF, 8, BUF, 8, None, None, 0, 1, 4, 8, f32, None, BUF, BUF, big, None) == 1
+    assert lib.tb200_gated_scan_grad(BUF, 8, BUF, 8, BUF, 8, BUF, 8, None, None, None, 0, 1, 4, 8, f32, BUF, BUF, None, BUF, big, None) == 1
     assert lib.tb200_gated_step(BUF, 8, BUF, 8, None, 3, BUF, i32, 2, 8, f32, BUF, None) == 1
     assert lib.tb200_expert_dispatch(BUF, 8, BUF, i32, 2, 1, 1025, 8, f32, BUF, BUF, BUF, BUF, None, ref, None) == 1
     assert lib.tb200_expert_dispatch(BUF, 8, BUF, i32, 1 << 30, 1, 4, 8, f32, BUF, BUF, BUF, BUF, None, ref, None) == 1
@@ -54,6 +55,11 @@ def test_c_calls_say_how_much_workspace_they_need():
         before = size.value
         size.value -= 1
         assert lib.tb200_embedding_grad(BUF, 8, BUF, 4, n, 1000, 8, 11, 8, 1.0, 0, BUF, BUF, ref, None) == 1
+    for offsets, need in ((None, 256), (BUF, 256 + 4 * 1000)):
+        assert lib.tb200_gated_scan(None, 8, None, 8, None, offsets, 4, 1, 1000, 8, 11, None, None, None, ref, None) == 0 and size.value >= need
+        assert lib.tb200_gated_scan_grad(None, 8, None, 8, None, 8, None, 8, None, None, offsets, 4, 1, 1000, 8, 11, None, None, None, None, ref, None) == 0 and size.value >= need
+        size.value -= 1
+        assert lib.tb200_gated_scan(BUF, 8, BUF, 8, None, offsets, 4, 1, 1000, 8, 11, BUF, BUF, BUF, ref, None) == 1
     for n in (0, 1, 1000, 1 << 20):
         assert lib.tb200_expert_dispatch(None, 8, None, 4, n, 8, 64, 8, 11, None, None, None, None, None, ref, None) == 0 and size.value >= 256
         size.value = 255
@@ -64,6 +70,6 @@ def test_c_calls_say_how_much_workspace_they_need():
 def test_nothing_to_do():
     lib = _lib.load()
     assert lib.tb200_embedding(None, 4, 8, None, 4, 0, 8, 8, 1.0, None, None) == 0
-    assert lib.tb200_gated_scan(None, 8, None, 8, None, None, 0, 0, 0, 8, 8, None, None, None) == 0
+    assert lib.tb200_gated_scan(None, 8, None, 8, None, None, 0, 0, 0, 8, 8, None, None, BUF, ctypes.byref(ctypes.c_size_t(1 << 20)), None) == 0
     assert lib.tb200_gated_step(None, 8, None, 8, None, 0, None, 4, 0, 8, 8, None, None) == 0
     assert lib.tb200_expert_combine(None, 8, None, None, 0, 2, 8, 8, None, None) == 0

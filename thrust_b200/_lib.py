@@ -57,8 +57,8 @@ PROTOTYPES = {
     "tb200_gather": [_vp, _vp, _vp, _sz, _i, _vp],
     "tb200_embedding": [_vp, _sz, _sz, _vp, _i, _sz, _sz, _i, _f, _vp, _vp],
     "tb200_embedding_grad": [_vp, _sz, _vp, _i, _sz, _sz, _sz, _i, _i, _f, _i, _vp, _vp, _szp, _vp],
-    "tb200_gated_scan": [_vp, _sz, _vp, _sz, _vp, _vp, _i, _sz, _sz, _sz, _i, _vp, _vp, _vp],
-    "tb200_gated_scan_grad": [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _i, _sz, _sz, _sz, _i, _vp, _vp, _vp, _vp],
+    "tb200_gated_scan": [_vp, _sz, _vp, _sz, _vp, _vp, _i, _sz, _sz, _sz, _i, _vp, _vp, _vp, _szp, _vp],
+    "tb200_gated_scan_grad": [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _i, _sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _szp, _vp],
     "tb200_gated_step": [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _i, _sz, _sz, _i, _vp, _vp],
     "tb200_expert_dispatch": [_vp, _sz, _vp, _i, _sz, _sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _szp, _vp],
     "tb200_expert_combine": [_vp, _sz, _vp, _vp, _sz, _sz, _sz, _i, _vp, _vp],

@@ -1,5 +1,9 @@
 // C ABI: tb200_gated_scan, tb200_gated_scan_grad and tb200_gated_step.
+#include <cuda.h>
+#include <type_traits>
+
 #include "abi_rows.cuh"
+#include "thrust_b200/bulk_copy.cuh"
 
 using namespace tb200_abi;
 using namespace tb200_rows;
@@ -18,61 +22,846 @@ __device__ __forceinline__ gate_pair open_gate(float g) {
   return p;
 }
 
-// Where the sequences lie: from offsets if there are any, else `batch` of equal length.  Offsets that point outside are cut off.
-template <class I> struct sequences {
-  const I* offsets;
-  size_t batch, n, length;
-  __device__ size_t begin(size_t s) const {
-    if (!offsets) return s * length;
-    const long long o = (long long)offsets[s];
-    return o < 0 ? 0 : (size_t)o > n ? n : (size_t)o;
-  }
-  __device__ size_t end(size_t s) const { return begin(s + 1); }
-};
+// ---------------------------------------------------------------------------------------------- scan by clusters
+// A chain of rows (a sequence; packed sequences are one chain that is cut at their ends) is walked in windows by a cluster of CTAs, one
+// chain and one slice of channels each.  A lane has V neighbouring channels and ROWS neighbouring positions of a window in registers:
+// position p is row p, or row length - 1 - p in the backward pass, so that both go the same way.  Over those positions a state q
+// becomes A q + B in each channel.  The warps' pairs meet in shared memory, the CTAs' in the shared memory of every CTA of the cluster, each
+// thread folds what comes before its rows onto the carry of the window, and only then walks its rows again.  So each
+// input is read once and each output written once; the rows of the next window are on their way meanwhile.  Pairs are
+// folded in the order of their positions: the same inputs give the same bits.
+//
+// A cut (a sequence begins there) makes a pair that forgets what came before: A is CUT instead of a product, and is selected on, not
+// multiplied with, so that NaNs and infinities of one sequence do not reach the next.
+constexpr float CUT = -1.f;
+constexpr int SCAN_WARPS = 8;
+constexpr int SCAN_BLOCK = SCAN_WARPS * 32;
 
-// a thread a channel of a sequence; the CTAs behind the last sequence's clear the rows that are in none
-template <class T, class I>
-__global__ void __launch_bounds__(BLOCK) gated_scan_kernel(const T* x, size_t xs, const T* gate, size_t gs, const float* h0, sequences<I> seq, size_t dim, T* h, float* last) {
-  const size_t c = (size_t)blockIdx.y * BLOCK + threadIdx.x, s = blockIdx.x;
-  if (c >= dim) return;
-  if (s == seq.batch) {
-    const size_t first = seq.begin(0), stop = seq.begin(seq.batch);
-    for (size_t r = 0; r < first; ++r) h[r * dim + c] = from_f32<T>(0.f);
-    for (size_t r = stop; r < seq.n; ++r) h[r * dim + c] = from_f32<T>(0.f);
-    return;
-  }
-  float state = h0 ? h0[s * dim + c] : 0.f;
-  const size_t end = seq.end(s);
-  for (size_t r = seq.begin(s); r < end; ++r) {
-    const gate_pair p = open_gate(to_f32(gate[r * gs + c]));
-    state = p.keep * state + p.give * to_f32(x[r * xs + c]);
-    h[r * dim + c] = from_f32<T>(state);
-  }
-  last[s * dim + c] = state;
+struct pair2 { float a, b; };
+template <bool CUTS> __device__ __forceinline__ float follow(float q, pair2 f) { return CUTS && f.a == CUT ? f.b : fmaf(f.a, q, f.b); }
+// first f, then g
+template <bool CUTS> __device__ __forceinline__ pair2 join(pair2 f, pair2 g) {
+  if (CUTS && g.a == CUT) return g;
+  pair2 r;
+  r.a = CUTS && f.a == CUT ? CUT : f.a * g.a;
+  r.b = fmaf(g.a, f.b, g.b);
+  return r;
 }
 
-template <class T, class I>
-__global__ void __launch_bounds__(BLOCK) gated_scan_grad_kernel(const T* dh, size_t ds, const T* x, size_t xs, const T* gate, size_t gs, const T* h, size_t hs, const float* h0,
-                                                              const float* dlast, sequences<I> seq, size_t dim, T* dx, T* dgate, float* dh0) {
-  const size_t c = (size_t)blockIdx.y * BLOCK + threadIdx.x, s = blockIdx.x;
-  if (c >= dim) return;
-  if (s == seq.batch) {
-    const size_t first = seq.begin(0), stop = seq.begin(seq.batch);
-    for (size_t r = 0; r < seq.n; ++r)
-      if (r < first || r >= stop) dx[r * dim + c] = dgate[r * dim + c] = from_f32<T>(0.f);
+template <int V> struct scan_shared {
+  pair2 warp[2][SCAN_WARPS][32 * V];
+  pair2 cta[2][tb200::CLUSTER_MAX_CTAS][32 * V];
+};
+
+// All threads: `own` are this thread's pairs.  Returns in `q` the state before its rows and brings `carry` from before the window to behind it.
+template <int V, bool CUTS>
+__device__ __forceinline__ void exchange(scan_shared<V>& sh, int parity, const pair2 (&own)[V], float (&carry)[V], float (&q)[V], unsigned rank, unsigned ctas) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+#pragma unroll
+  for (int v = 0; v < V; ++v) sh.warp[parity][warp][lane * V + v] = own[v];
+  __syncthreads();
+  if (ctas == 1) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float c = carry[v];
+      for (int w = 0; w < warps; ++w) {
+        if (w == warp) q[v] = c;
+        c = follow<CUTS>(c, sh.warp[parity][w][lane * V + v]);
+      }
+      carry[v] = c;
+    }
     return;
   }
-  float carry = dlast ? dlast[s * dim + c] : 0.f;
-  const size_t begin = seq.begin(s);
-  for (size_t r = seq.end(s); r-- > begin;) {
-    const gate_pair p = open_gate(to_f32(gate[r * gs + c]));
-    const float total = to_f32(dh[r * ds + c]) + carry;
-    const float before = r > begin ? to_f32(h[(r - 1) * hs + c]) : h0 ? h0[s * dim + c] : 0.f;
-    dx[r * dim + c] = from_f32<T>(p.give * total);
-    dgate[r * dim + c] = from_f32<T>(p.keep * p.give * (before - to_f32(x[r * xs + c])) * total);
-    carry = p.keep * total;
+  pair2 before[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    pair2 f = {1.f, 0.f};
+    for (int w = 0; w < warps; ++w) {
+      if (w == warp) before[v] = f;
+      f = join<CUTS>(f, sh.warp[parity][w][lane * V + v]);
+    }
+    // every warp has the CTA's pair: they take the cluster's CTAs in turn
+    for (unsigned c = warp; c < ctas; c += warps) tb200::cluster_store(tb200::cluster_addr(tb200::smem_addr(&sh.cta[parity][rank][lane * V + v]), c), f);
   }
-  dh0[s * dim + c] = carry;
+  tb200::cluster_barrier();
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float c = carry[v];
+    for (unsigned r = 0; r < ctas; ++r) {
+      if (r == rank) q[v] = follow<CUTS>(c, before[v]);
+      c = follow<CUTS>(c, sh.cta[parity][r][lane * V + v]);
+    }
+    carry[v] = c;
+  }
+}
+
+// What the ids of packed rows say about the positions of a warp, a bit each: ids[r] is the sequence of row r or -1.
+struct row_marks { unsigned inside, begins, ends; };
+// position p is row first + step * p; rows outside [0, n) are in no sequence
+__device__ __forceinline__ row_marks read_marks(const int* ids, long long row, int step, long long n) {
+  const int lane = threadIdx.x % 32;
+  const long long at = row + (long long)step * (lane - 1);      // lane i: position i - 1
+  const int id = at >= 0 && at < n ? ids[at] : -1;
+  const int before = __shfl_up_sync(tb200::FULL_MASK, id, 1), after = __shfl_down_sync(tb200::FULL_MASK, id, 1);
+  row_marks m;
+  m.inside = __ballot_sync(tb200::FULL_MASK, id >= 0) >> 1;
+  m.begins = __ballot_sync(tb200::FULL_MASK, id >= 0 && before != id) >> 1;
+  m.ends = __ballot_sync(tb200::FULL_MASK, id >= 0 && after != id) >> 1;
+  return m;
+}
+
+template <class T, int V, int ROWS, bool PACKED>
+__global__ void __launch_bounds__(SCAN_BLOCK, 2)
+gated_scan_kernel(const T* __restrict__ x, size_t xs, const T* __restrict__ gate, size_t gs, const float* __restrict__ h0, const int* __restrict__ ids, unsigned slices,
+                  size_t length, size_t dim, T* __restrict__ h, float* __restrict__ last) {
+  static_assert(ROWS <= 30, "a warp reads the ids of its positions and of their neighbours");
+  using P = words<T, V>;
+  __shared__ scan_shared<V> sh;
+  const unsigned ctas = tb200::cluster_size(), rank = tb200::cluster_rank();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+  const unsigned item = blockIdx.x / ctas;
+  const size_t chain = item / slices, c = ((size_t)(item % slices) * 32 + lane) * V, first = chain * length;
+  const bool there = c < dim;
+  const size_t window = (size_t)ctas * warps * ROWS;
+  const size_t windows = (length + window - 1) / window;
+  size_t p = ((size_t)rank * warps + warp) * ROWS;      // this thread's first position in the window
+  P xr[ROWS], gr[ROWS];
+  auto load = [&](size_t p) {
+    const T* xp = x + (first + p) * xs + c;
+    const T* gp = gate + (first + p) * gs + c;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i, xp += xs, gp += gs)
+      if (there && p + i < length) {
+        xr[i] = load_words<T, V>(xp);
+        gr[i] = load_words<T, V>(gp);
+      }
+  };
+  float carry[V], q[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) carry[v] = !PACKED && h0 && there ? h0[chain * dim + c + v] : 0.f;
+  load(p);
+  if (ctas > 1) tb200::cluster_barrier();      // all CTAs have begun: their shared memory may be written
+  for (size_t w = 0; w < windows; ++w, p += window) {
+    row_marks m = {~0u, 0u, 0u};
+    if constexpr (PACKED) m = read_marks(ids, (long long)p, 1, (long long)length);
+    float keep[ROWS][V], b[ROWS][V];
+    pair2 own[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) own[v] = {1.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const bool live = there && p + i < length;
+      float gv[V], xv[V];
+      channels(gr[i], gv);
+      channels(xr[i], xv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const gate_pair g = open_gate(gv[v]);
+        keep[i][v] = live ? g.keep : 1.f;
+        b[i][v] = live ? g.give * xv[v] : 0.f;
+      }
+      if constexpr (PACKED) {
+        if (!(m.inside >> i & 1)) {          // no sequence's: zero, and nothing of the inputs
+#pragma unroll
+          for (int v = 0; v < V; ++v) { keep[i][v] = 0.f; b[i][v] = 0.f; own[v] = {CUT, 0.f}; }
+          continue;
+        }
+        if (m.begins >> i & 1) {
+          const int s = ids[p + i];
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            if (h0 && there) b[i][v] = fmaf(keep[i][v], h0[(size_t)s * dim + c + v], b[i][v]);
+            own[v] = {CUT, b[i][v]};
+          }
+          continue;
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        own[v].b = fmaf(keep[i][v], own[v].b, b[i][v]);
+        own[v].a = PACKED && own[v].a == CUT ? CUT : own[v].a * keep[i][v];
+      }
+    }
+    if (w + 1 < windows) load(p + window);
+    exchange<V, PACKED>(sh, (int)(w & 1), own, carry, q, rank, ctas);
+    T* hp = h + (first + p) * dim + c;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const bool cut = PACKED && ((m.begins | ~m.inside) >> i & 1);
+        q[v] = cut ? b[i][v] : fmaf(keep[i][v], q[v], b[i][v]);
+      }
+      if (there && p + i < length) {
+        store_words<T, V>(hp + (size_t)i * dim, to_words<T, V>(q));
+        if (PACKED && (m.ends >> i & 1)) {
+          const int s = ids[p + i];
+#pragma unroll
+          for (int v = 0; v < V; ++v) last[(size_t)s * dim + c + v] = q[v];
+        }
+      }
+    }
+  }
+  if (!PACKED && rank == 0 && warp == 0 && there) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) last[chain * dim + c + v] = carry[v];
+  }
+}
+
+// The backward pass.  With q = a s handed from a row to the one before it: s = dh + q, q' = keep s, dx = give s,
+// dgate = keep give (h' - x) s, where h' is the state before the row.
+template <class T, int V, int ROWS, bool PACKED>
+__global__ void __launch_bounds__(SCAN_BLOCK, 2)
+gated_scan_grad_kernel(const T* __restrict__ dh, size_t ds, const T* __restrict__ x, size_t xs, const T* __restrict__ gate, size_t gs, const T* __restrict__ h, size_t hs,
+                       const float* __restrict__ h0, const float* __restrict__ dlast, const int* __restrict__ ids, unsigned slices, size_t length, size_t dim, T* __restrict__ dx,
+                       T* __restrict__ dgate, float* __restrict__ dh0) {
+  using P = words<T, V>;
+  __shared__ scan_shared<V> sh;
+  const unsigned ctas = tb200::cluster_size(), rank = tb200::cluster_rank();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+  const unsigned item = blockIdx.x / ctas;
+  const size_t chain = item / slices, c = ((size_t)(item % slices) * 32 + lane) * V, first = chain * length;
+  const bool there = c < dim;
+  const size_t window = (size_t)ctas * warps * ROWS;
+  const size_t windows = (length + window - 1) / window;
+  size_t p = ((size_t)rank * warps + warp) * ROWS;
+  P dr[ROWS], gr[ROWS], xr[ROWS], hr[ROWS];
+  auto load = [&](size_t p) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+      if (there && p + i < length) {
+        const size_t row = first + (length - 1 - (p + i));
+        dr[i] = load_words<T, V>(dh + row * ds + c);
+        gr[i] = load_words<T, V>(gate + row * gs + c);
+        xr[i] = load_words<T, V>(x + row * xs + c);
+        if (row > first) hr[i] = load_words<T, V>(h + (row - 1) * hs + c);
+      }
+  };
+  float carry[V], q[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) carry[v] = !PACKED && dlast && there ? dlast[chain * dim + c + v] : 0.f;
+  load(p);
+  if (ctas > 1) tb200::cluster_barrier();
+  for (size_t w = 0; w < windows; ++w, p += window) {
+    const long long row = (long long)length - 1 - (long long)p;       // of position p, inside the chain
+    row_marks m = {~0u, 0u, 0u};
+    if constexpr (PACKED) m = read_marks(ids, row, -1, (long long)length);
+    float keep[ROWS][V], give[ROWS][V], d[ROWS][V], diff[ROWS][V];
+    pair2 own[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) own[v] = {1.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const bool live = there && p + i < length;
+      const bool initial = PACKED ? (m.ends >> i & 1) != 0 : (size_t)i + p + 1 == length;      // the row before is none of this sequence
+      const int s = PACKED ? (live && (m.inside >> i & 1) ? ids[row - i] : 0) : (int)chain;
+      float gv[V], xv[V], dv[V], hv[V];
+      channels(gr[i], gv);
+      channels(xr[i], xv);
+      channels(dr[i], dv);
+      channels(hr[i], hv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const gate_pair g = open_gate(gv[v]);
+        keep[i][v] = live ? g.keep : 1.f;
+        give[i][v] = g.give;
+        d[i][v] = live ? dv[v] : 0.f;
+        const float before = initial ? (h0 && live ? h0[(size_t)s * dim + c + v] : 0.f) : hv[v];
+        diff[i][v] = before - xv[v];
+      }
+      if constexpr (PACKED) {
+        if (!(m.inside >> i & 1)) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) { keep[i][v] = give[i][v] = d[i][v] = diff[i][v] = 0.f; own[v] = {CUT, 0.f}; }
+          continue;
+        }
+        if (m.begins >> i & 1) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            if (dlast && live) d[i][v] += dlast[(size_t)s * dim + c + v];
+            own[v] = {CUT, keep[i][v] * d[i][v]};
+          }
+          continue;
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        own[v].b = keep[i][v] * (own[v].b + d[i][v]);
+        own[v].a = PACKED && own[v].a == CUT ? CUT : own[v].a * keep[i][v];
+      }
+    }
+    if (w + 1 < windows) load(p + window);
+    exchange<V, PACKED>(sh, (int)(w & 1), own, carry, q, rank, ctas);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      float ox[V], og[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const bool cut = PACKED && ((m.begins | ~m.inside) >> i & 1);
+        const float s = cut ? d[i][v] : d[i][v] + q[v];
+        q[v] = keep[i][v] * s;
+        const float in = give[i][v] * s;
+        ox[v] = in;
+        og[v] = keep[i][v] * diff[i][v] * in;
+      }
+      if (there && p + i < length) {
+        const size_t at = (first + (size_t)(row - i)) * dim + c;
+        store_words<T, V>(dx + at, to_words<T, V>(ox));
+        store_words<T, V>(dgate + at, to_words<T, V>(og));
+        if (PACKED && (m.ends >> i & 1)) {
+          const int s = ids[row - i];
+#pragma unroll
+          for (int v = 0; v < V; ++v) dh0[(size_t)s * dim + c + v] = q[v];
+        }
+      }
+    }
+  }
+  if (!PACKED && rank == 0 && warp == 0 && there) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) dh0[chain * dim + c + v] = carry[v];
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- the same from tiles in shared memory
+// Where rows are made of whole 16-byte pieces, the copy engine brings a CTA's tiles (WARPS * ROWS rows of 64 channels of each input) into a
+// ring of STAGES stages while earlier windows are worked on, and a lane takes its two channels of a row from there in one access.
+// Two channels go through the arithmetic side by side (f32x2).
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pack2(float x, float y) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ float2 unpack2(f2 a) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ float exp2_of(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float one_over(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+
+// two channels of a row
+template <class T> __device__ __forceinline__ float2 two_channels(const T* p) {
+  const words<T, 2> w = load_words<T, 2>(p);
+  return make_float2(channel<0>(w), channel<1>(w));
+}
+
+// open_gate for two channels: e = exp(-g), keep = 1 / (1 + e), give = e keep.  An e past the largest number makes keep 0 and e keep a NaN, for which
+// give is 1; a NaN gate makes keep a NaN.
+struct gates2 { f2 keep, give; };
+__device__ __forceinline__ gates2 open_gates(float2 g) {
+  constexpr float M = -1.4426950408889634f;
+  const float2 t = unpack2(mul2(pack2(g.x, g.y), pack2(M, M)));
+  const f2 e = pack2(exp2_of(t.x), exp2_of(t.y));
+  const float2 d = unpack2(add2(e, pack2(1.f, 1.f)));
+  gates2 r;
+  r.keep = pack2(one_over(d.x), one_over(d.y));
+  const float2 give = unpack2(mul2(e, r.keep));
+  r.give = pack2(fminf(give.x, 1.f), fminf(give.y, 1.f));
+  return r;
+}
+
+struct duo { f2 a, b; };       // pair2 of two channels
+template <bool CUTS> __device__ __forceinline__ f2 follow(f2 q, duo f) {
+  f2 r = fma2(f.a, q, f.b);
+  if (CUTS) {
+    const float2 a = unpack2(f.a), b = unpack2(f.b), s = unpack2(r);
+    r = pack2(a.x == CUT ? b.x : s.x, a.y == CUT ? b.y : s.y);
+  }
+  return r;
+}
+template <bool CUTS> __device__ __forceinline__ duo join(duo f, duo g) {
+  duo r = {mul2(f.a, g.a), fma2(g.a, f.b, g.b)};
+  if (CUTS) {
+    const float2 fa = unpack2(f.a), ga = unpack2(g.a), gb = unpack2(g.b), a = unpack2(r.a), b = unpack2(r.b);
+    r.a = pack2(fa.x == CUT || ga.x == CUT ? CUT : a.x, fa.y == CUT || ga.y == CUT ? CUT : a.y);
+    r.b = pack2(ga.x == CUT ? gb.x : b.x, ga.y == CUT ? gb.y : b.y);
+  }
+  return r;
+}
+
+constexpr int MOST_CTAS = tb200::CLUSTER_MAX_CTAS;
+constexpr int MEETINGS = 4;
+constexpr int TILE_CTAS = 4;        // a SM
+template <class T, int WARPS, int ROWS, int INPUTS, int STAGES> struct tiles_shared {
+  static constexpr int R = WARPS * ROWS;
+  alignas(128) T tile[STAGES][INPUTS][R][64];
+  duo warp[2][WARPS][32];
+  unsigned long long full[STAGES], met[MEETINGS];
+  // behind it, where there is more than one CTA: the CTAs' pairs, [MEETINGS][ctas][32]
+  static size_t bytes(unsigned ctas) { return tb200::align_up(sizeof(tiles_shared), 16) + (ctas > 1 ? MEETINGS * ctas * 32 * sizeof(duo) : 0); }
+  __device__ duo* pairs() { return reinterpret_cast<duo*>(reinterpret_cast<char*>(this) + (sizeof(tiles_shared) + 15) / 16 * 16); }
+};
+
+__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, int channel, int row, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(tb200::smem_addr(dst)), "l"(map), "r"(channel), "r"(row),
+               "r"(tb200::smem_addr(bar)) : "memory");
+}
+// by whole warps; false: the copies did not come within the limit
+__device__ __forceinline__ bool wait_tile(unsigned long long* bar, unsigned parity) {
+  bool came = false;
+  for (unsigned iter = 0; !came && iter < tb200::MBAR_SPIN_LIMIT; ++iter) came = tb200::mbar_try_wait(bar, parity);
+  return __all_sync(tb200::FULL_MASK, came);
+}
+// A 16-byte store into the shared memory of a CTA of the cluster, counted by the mbarrier there.  Unlike a barrier of the cluster it does not
+// wait for this CTA's stores to global memory.
+__device__ __forceinline__ void send_duo(unsigned to, const duo& d, unsigned bar) {
+  const float2 a = unpack2(d.a), b = unpack2(d.b);
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ bool wait_met(unsigned long long* bar, unsigned parity) {
+  unsigned came = 0;
+  for (unsigned iter = 0; !came && iter < tb200::MBAR_SPIN_LIMIT; ++iter)
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(came) : "r"(tb200::smem_addr(bar)), "r"(parity), "r"(1000u) : "memory");
+  return __all_sync(tb200::FULL_MASK, came != 0);
+}
+__device__ __forceinline__ f2 nan2() { return pack2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff)); }
+
+// The pairs of a warp's rows, once they are known, and the state before its rows, once that is.
+struct link { duo before, total; };       // of the CTA: what comes before this warp's rows, all of it
+
+// All threads of the CTA, with their warps' pairs of window w; `cut`: whether this warp's is one.  after_sync: run once every warp is done with
+// its tiles.  Also sends the CTA's pair to the cluster.
+template <class Shared, int WARPS, bool CUTS, class F>
+__device__ __forceinline__ link join_warps(Shared& sh, size_t w, const duo& own, bool cut, unsigned rank, unsigned ctas, F after_sync) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  sh.warp[w & 1][warp][lane] = own;
+  const bool some = CUTS ? __syncthreads_or(cut) != 0 : (__syncthreads(), false);
+  after_sync();
+  link l;
+  duo f = {pack2(1.f, 1.f), 0ull};
+  l.before = f;
+  if (CUTS && some) {
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      if (i == warp) l.before = f;
+      f = join<true>(f, sh.warp[w & 1][i][lane]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      if (i == warp) l.before = f;
+      f = join<false>(f, sh.warp[w & 1][i][lane]);
+    }
+  }
+  l.total = f;
+  if (ctas > 1) {
+    const int buffer = (int)(w % MEETINGS);
+    if (threadIdx.x == 0) tb200::mbar_arrive_expect(&sh.met[buffer], ctas * 32 * (unsigned)sizeof(duo));
+    const unsigned at = tb200::smem_addr(sh.pairs() + ((size_t)buffer * ctas + rank) * 32 + lane), bar = tb200::smem_addr(&sh.met[buffer]);
+    for (unsigned c = warp; c < ctas; c += WARPS) send_duo(tb200::cluster_addr(at, c), f, tb200::cluster_addr(bar, c));
+  }
+  return l;
+}
+// The state before this warp's rows of window w; `carry` goes from before the window to behind it.  false: the cluster's pairs did not come.
+// A CTA sends window w + 1 when it has everything of w - 1, which others sent when they were done with w - 3: four buffers.
+template <class Shared, bool CUTS>
+__device__ __forceinline__ bool join_ctas(Shared& sh, size_t w, const link& l, f2& carry, f2& q, unsigned rank, unsigned ctas) {
+  if (ctas == 1) {
+    q = follow<CUTS>(carry, l.before);
+    carry = follow<CUTS>(carry, l.total);
+    return true;
+  }
+  const bool met = wait_met(&sh.met[w % MEETINGS], (unsigned)(w / MEETINGS) & 1);
+  const duo* pairs = sh.pairs() + (w % MEETINGS) * ctas * 32 + threadIdx.x % 32;
+  f2 c = carry;
+  for (unsigned r0 = 0; r0 < ctas; r0 += 4) {
+    duo d[4];
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) if (r0 + j < ctas) d[j] = pairs[(r0 + j) * 32];
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j)
+      if (r0 + j < ctas) {
+        if (r0 + j == rank) q = follow<CUTS>(c, l.before);
+        c = follow<CUTS>(c, d[j]);
+      }
+  }
+  carry = c;
+  return met;
+}
+
+// Which of the ROWS positions of a warp lie in a sequence, begin one and end one (in the direction of the walk), a bit each.  From a table with
+// such bits for 32 rows an entry, read a window ahead.
+struct marks { unsigned inside, begins, ends; };
+struct row_table { const uint4* bits; const int* ids; };
+// Of the rows from `row` on, a word a lane: lanes 0 to 2 the entry of the first of them, 4 to 6 the one behind it.
+__device__ __forceinline__ unsigned read_marks(const row_table& t, long long row, long long length) {
+  const int lane = threadIdx.x % 32;
+  const long long k = (row >> 5) + (lane >> 2 & 1);
+  return lane < 8 && k >= 0 && k <= (length - 1) >> 5 ? reinterpret_cast<const unsigned*>(t.bits + k)[lane & 3] : 0u;
+}
+template <int ROWS, bool BACKWARD> __device__ __forceinline__ marks marks_of(unsigned word, long long row) {
+  auto cut_out = [&](int which) -> unsigned {
+    const unsigned bits = __funnelshift_r(__shfl_sync(tb200::FULL_MASK, word, which), __shfl_sync(tb200::FULL_MASK, word, which + 4), (unsigned)row & 31);
+    constexpr unsigned ALL = ROWS == 32 ? ~0u : (1u << (ROWS % 32)) - 1;
+    return (BACKWARD ? __brev(bits) >> (32 - ROWS) : bits) & ALL;
+  };
+  marks m;
+  m.inside = cut_out(0);
+  m.begins = cut_out(BACKWARD ? 2 : 1);
+  m.ends = cut_out(BACKWARD ? 1 : 2);
+  return m;
+}
+
+template <class T, int WARPS, int ROWS, int STAGES, bool PACKED>
+__global__ void __launch_bounds__(WARPS * 32, PACKED ? 3 : 4)
+gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap gate_map, const float* __restrict__ h0, row_table table, unsigned slices,
+                   size_t length, size_t dim, T* __restrict__ h, float* __restrict__ last, tb200::ws_header* hdr) {
+  static_assert(ROWS <= 32, "a lane holds the id of a position");
+  using Shared = tiles_shared<T, WARPS, ROWS, 2, STAGES>;
+  constexpr int R = Shared::R;
+  constexpr unsigned ALL = ROWS == 32 ? ~0u : (1u << ROWS) - 1;
+  extern __shared__ __align__(128) unsigned char raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(raw);
+  const unsigned ctas = tb200::cluster_size(), rank = tb200::cluster_rank();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const unsigned item = blockIdx.x / ctas;
+  const size_t chain = item / slices, c = (size_t)(item % slices) * 64 + lane * 2, first = chain * length;
+  const bool there = c < dim;
+  const size_t window = (size_t)ctas * R, windows = (length + window - 1) / window;
+  const size_t p0 = ((size_t)rank * WARPS + warp) * ROWS;       // this warp's first position in window 0
+  auto load = [&](size_t w) {       // the CTA's tiles of window w
+    const size_t row = w * window + (size_t)rank * R;
+    if (w >= windows || row >= length) return;
+    unsigned long long* const bar = &sh.full[w % STAGES];
+    tb200::mbar_arrive_expect(bar, 2 * R * 64 * (unsigned)sizeof(T));
+    load_tile(sh.tile[w % STAGES][0], &x_map, (int)(item % slices) * 64, (int)(first + row), bar);
+    load_tile(sh.tile[w % STAGES][1], &gate_map, (int)(item % slices) * 64, (int)(first + row), bar);
+  };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) tb200::mbar_init(&sh.full[i], 1);
+    for (int i = 0; i < MEETINGS; ++i) tb200::mbar_init(&sh.met[i], 1);
+    tb200::mbar_init_fence();
+    for (int i = 0; i < STAGES; ++i) load(i);
+  }
+  auto state_of = [&](size_t s) -> f2 {
+    if (!h0 || !there) return 0ull;
+    const float2 v = *reinterpret_cast<const float2*>(h0 + s * dim + c);
+    return pack2(v.x, v.y);
+  };
+  f2 carry = PACKED ? 0ull : state_of(chain);
+  unsigned coming = 0;              // marks of the next window
+  if constexpr (PACKED) coming = read_marks(table, (long long)p0, (long long)length);
+  __syncthreads();
+  if (ctas > 1) tb200::cluster_barrier();      // all CTAs have begun: their shared memory may be written
+  bool good = true;
+
+  struct held { f2 keep[ROWS], b[ROWS]; link l; unsigned cuts, ends; int id, rows; };
+  auto take = [&](held& s, size_t w) {
+    const size_t p = p0 + w * window;
+    const int stage = (int)(w % STAGES);
+    s.rows = p >= length ? 0 : length - p < (size_t)ROWS ? (int)(length - p) : ROWS;       // of this warp that there are
+    s.cuts = s.ends = 0;
+    unsigned begins = 0;
+    if constexpr (PACKED) {
+      const marks m = marks_of<ROWS, false>(coming, (long long)p);
+      s.cuts = m.begins | (~m.inside & ALL);
+      s.ends = m.ends;
+      begins = m.begins;
+      if (m.begins | m.ends) s.id = lane < ROWS && p + lane < length ? table.ids[p + lane] : 0;
+      coming = read_marks(table, (long long)(p + window), (long long)length);
+    }
+    if (w * window + (size_t)rank * R < length) good &= wait_tile(&sh.full[stage], (unsigned)(w / STAGES) & 1);
+    const T* const xt = &sh.tile[stage][0][warp * ROWS][lane * 2];
+    const T* const gt = &sh.tile[stage][1][warp * ROWS][lane * 2];
+    duo own = {pack2(1.f, 1.f), 0ull};
+    auto open = [&](int i) {
+      const gates2 g = open_gates(two_channels(gt + i * 64));
+      const float2 xv = two_channels(xt + i * 64);
+      s.keep[i] = g.keep;
+      s.b[i] = mul2(g.give, pack2(xv.x, xv.y));
+    };
+    // Rows first, without a branch between them (their chains of exponential and reciprocal overlap: with a test in each row a window took 1.6 us
+    // longer), then what is rare, then the pairs.
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) open(i);
+    if (!PACKED && s.rows < ROWS) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (i >= s.rows) { s.keep[i] = pack2(1.f, 1.f); s.b[i] = 0ull; }
+    }
+    if (PACKED && s.cuts) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (s.cuts >> i & 1) {
+          if (begins >> i & 1) {
+            s.b[i] = fma2(s.keep[i], state_of((size_t)__shfl_sync(tb200::FULL_MASK, s.id, i)), s.b[i]);
+          } else {
+            s.keep[i] = s.b[i] = 0ull;
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) own.b = s.cuts >> i & 1 ? s.b[i] : fma2(s.keep[i], own.b, s.b[i]);
+      own.a = pack2(CUT, CUT);
+    } else {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        own.b = fma2(s.keep[i], own.b, s.b[i]);
+        own.a = mul2(own.a, s.keep[i]);
+      }
+    }
+    if (!good) own = {pack2(1.f, 1.f), nan2()};
+    s.l = join_warps<Shared, WARPS, PACKED>(sh, w, own, s.cuts != 0, rank, ctas, [&] { if (threadIdx.x == 0) load(w + STAGES); });
+  };
+  auto give = [&](held& s, size_t w) {
+    f2 q = 0ull;
+    good &= join_ctas<Shared, PACKED>(sh, w, s.l, carry, q, rank, ctas);
+    if (!good) { q = nan2(); s.cuts = 0; }
+    T* hp = h + (first + p0 + w * window) * dim + c;
+    if (s.rows == ROWS && !(PACKED && (s.cuts | s.ends))) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i, hp += dim) {
+        q = fma2(s.keep[i], q, s.b[i]);
+        const float2 v = unpack2(q);
+        const float out[2] = {v.x, v.y};
+        if (there) store_words<T, 2>(hp, to_words<T, 2>(out));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i, hp += dim) {
+        q = PACKED && (s.cuts >> i & 1) ? s.b[i] : fma2(s.keep[i], q, s.b[i]);
+        const float2 v = unpack2(q);
+        const float out[2] = {v.x, v.y};
+        if (there && i < s.rows) store_words<T, 2>(hp, to_words<T, 2>(out));
+        if (PACKED && (s.ends >> i & 1)) {
+          const int seq = __shfl_sync(tb200::FULL_MASK, s.id, i);
+          if (there) *reinterpret_cast<float2*>(last + (size_t)seq * dim + c) = v;
+        }
+      }
+    }
+  };
+  held s;
+  for (size_t w = 0; w < windows; ++w) { take(s, w); give(s, w); }
+  if (ctas > 1) tb200::cluster_barrier();      // nobody leaves while something may still be sent there
+  if (!good && lane == 0) tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
+  if (!PACKED && rank == 0 && warp == 0 && there) *reinterpret_cast<float2*>(last + chain * dim + c) = unpack2(carry);
+}
+
+template <class T, int WARPS, int ROWS, int STAGES, bool PACKED>
+__global__ void __launch_bounds__(WARPS * 32, PACKED ? 3 : 4)
+gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_constant__ CUtensorMap gate_map, const __grid_constant__ CUtensorMap x_map,
+                        const __grid_constant__ CUtensorMap h_map, const float* __restrict__ h0, const float* __restrict__ dlast, row_table table, unsigned slices,
+                        size_t length, size_t dim, T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ dh0, tb200::ws_header* hdr) {
+  static_assert(ROWS <= 32, "a lane holds the id of a position");
+  using Shared = tiles_shared<T, WARPS, ROWS, 4, STAGES>;
+  constexpr int R = Shared::R;
+  constexpr unsigned ALL = ROWS == 32 ? ~0u : (1u << ROWS) - 1;
+  extern __shared__ __align__(128) unsigned char raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(raw);
+  const unsigned ctas = tb200::cluster_size(), rank = tb200::cluster_rank();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const unsigned item = blockIdx.x / ctas;
+  const size_t chain = item / slices, c = (size_t)(item % slices) * 64 + lane * 2, first = chain * length;
+  const bool there = c < dim;
+  const size_t window = (size_t)ctas * R, windows = (length + window - 1) / window;
+  const size_t p0 = ((size_t)rank * WARPS + warp) * ROWS;
+  auto load = [&](size_t w) {
+    const size_t p = w * window + (size_t)rank * R;      // the tile's position R - 1 is its first row, which may lie before the tensor
+    if (w >= windows || p >= length) return;
+    const int row = (int)((long long)first + (long long)length - (long long)p - R), channel = (int)(item % slices) * 64;
+    unsigned long long* const bar = &sh.full[w % STAGES];
+    tb200::mbar_arrive_expect(bar, 4 * R * 64 * (unsigned)sizeof(T));
+    load_tile(sh.tile[w % STAGES][0], &dh_map, channel, row, bar);
+    load_tile(sh.tile[w % STAGES][1], &gate_map, channel, row, bar);
+    load_tile(sh.tile[w % STAGES][2], &x_map, channel, row, bar);
+    load_tile(sh.tile[w % STAGES][3], &h_map, channel, row - 1, bar);
+  };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) tb200::mbar_init(&sh.full[i], 1);
+    for (int i = 0; i < MEETINGS; ++i) tb200::mbar_init(&sh.met[i], 1);
+    tb200::mbar_init_fence();
+    for (int i = 0; i < STAGES; ++i) load(i);
+  }
+  auto state_of = [&](const float* from, size_t s) -> f2 {
+    if (!from || !there) return 0ull;
+    const float2 v = *reinterpret_cast<const float2*>(from + s * dim + c);
+    return pack2(v.x, v.y);
+  };
+  f2 carry = PACKED ? 0ull : state_of(dlast, chain);
+  const f2 initial = PACKED ? 0ull : state_of(h0, chain);
+  unsigned coming = 0;
+  if constexpr (PACKED) coming = read_marks(table, (long long)length - (long long)p0 - ROWS, (long long)length);
+  __syncthreads();
+  if (ctas > 1) tb200::cluster_barrier();
+  bool good = true;
+
+  struct held { f2 keep[ROWS], give[ROWS], d[ROWS], slope[ROWS]; link l; unsigned cuts, ends; int id, rows; };
+  auto take = [&](held& s, size_t w) {
+    const size_t p = p0 + w * window;
+    const int stage = (int)(w % STAGES);
+    s.rows = p >= length ? 0 : length - p < (size_t)ROWS ? (int)(length - p) : ROWS;
+    s.cuts = s.ends = 0;
+    unsigned begins = 0;
+    if constexpr (PACKED) {
+      const long long row = (long long)length - (long long)p - ROWS;       // of the last position
+      const marks m = marks_of<ROWS, true>(coming, row);
+      s.cuts = m.begins | (~m.inside & ALL);
+      s.ends = m.ends;
+      begins = m.begins;
+      if (m.begins | m.ends) { const long long at = row + ROWS - 1 - lane; s.id = lane < ROWS && at >= 0 ? table.ids[at] : 0; }
+      coming = read_marks(table, row - (long long)window, (long long)length);
+    } else if (s.rows > 0 && p + s.rows == length) {
+      s.ends = 1u << (s.rows - 1);           // the sequence's first row
+    }
+    if (w * window + (size_t)rank * R < length) good &= wait_tile(&sh.full[stage], (unsigned)(w / STAGES) & 1);
+    const T* const dt = &sh.tile[stage][0][R - 1 - warp * ROWS][lane * 2];
+    const T* const gt = &sh.tile[stage][1][R - 1 - warp * ROWS][lane * 2];
+    const T* const xt = &sh.tile[stage][2][R - 1 - warp * ROWS][lane * 2];
+    const T* const ht = &sh.tile[stage][3][R - 1 - warp * ROWS][lane * 2];
+    const f2 minus = pack2(-1.f, -1.f);
+    duo own = {pack2(1.f, 1.f), 0ull};
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const gates2 g = open_gates(two_channels(gt - i * 64));
+      const float2 dv = two_channels(dt - i * 64), xv = two_channels(xt - i * 64), hv = two_channels(ht - i * 64);
+      s.keep[i] = g.keep;
+      s.give[i] = fma2(g.keep, 0ull, g.give);       // a NaN where the gate is one
+      s.d[i] = pack2(dv.x, dv.y);
+      s.slope[i] = mul2(mul2(g.keep, g.give), fma2(pack2(xv.x, xv.y), minus, pack2(hv.x, hv.y)));
+    }
+    if (s.ends) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (s.ends >> i & 1) {
+          const f2 from = PACKED ? state_of(h0, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, i)) : initial;
+          const float2 xv = two_channels(xt - i * 64);
+          s.slope[i] = mul2(mul2(s.keep[i], s.give[i]), fma2(pack2(xv.x, xv.y), minus, from));
+        }
+    }
+    if (!PACKED && s.rows < ROWS) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (i >= s.rows) { s.keep[i] = pack2(1.f, 1.f); s.give[i] = s.d[i] = s.slope[i] = 0ull; }
+    }
+    if (PACKED && s.cuts) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (s.cuts >> i & 1) {
+          if (begins >> i & 1) {
+            s.d[i] = add2(s.d[i], state_of(dlast, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, i)));
+          } else {
+            s.keep[i] = s.give[i] = s.d[i] = s.slope[i] = 0ull;
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) own.b = mul2(s.keep[i], s.cuts >> i & 1 ? s.d[i] : add2(own.b, s.d[i]));
+      own.a = pack2(CUT, CUT);
+    } else {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        own.b = mul2(s.keep[i], add2(own.b, s.d[i]));
+        own.a = mul2(own.a, s.keep[i]);
+      }
+    }
+    if (!good) own = {pack2(1.f, 1.f), nan2()};
+    s.l = join_warps<Shared, WARPS, PACKED>(sh, w, own, s.cuts != 0, rank, ctas, [&] { if (threadIdx.x == 0) load(w + STAGES); });
+  };
+  auto give = [&](held& s, size_t w) {
+    f2 q = 0ull;
+    good &= join_ctas<Shared, PACKED>(sh, w, s.l, carry, q, rank, ctas);
+    if (!good) { q = nan2(); s.cuts = 0; }
+    const long long at = ((long long)first + (long long)length - 1 - (long long)(p0 + w * window)) * (long long)dim + (long long)c;
+    T* xp = dx + at;
+    T* gp = dgate + at;
+    if (s.rows == ROWS && !(PACKED && (s.cuts | s.ends))) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i, xp -= dim, gp -= dim) {
+        const f2 sum = add2(s.d[i], q);
+        q = mul2(s.keep[i], sum);
+        const float2 a = unpack2(mul2(s.give[i], sum)), b = unpack2(mul2(s.slope[i], sum));
+        const float oa[2] = {a.x, a.y}, ob[2] = {b.x, b.y};
+        if (there) {
+          store_words<T, 2>(xp, to_words<T, 2>(oa));
+          store_words<T, 2>(gp, to_words<T, 2>(ob));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i, xp -= dim, gp -= dim) {
+        const f2 sum = PACKED && (s.cuts >> i & 1) ? s.d[i] : add2(s.d[i], q);
+        q = mul2(s.keep[i], sum);
+        const float2 a = unpack2(mul2(s.give[i], sum)), b = unpack2(mul2(s.slope[i], sum));
+        const float oa[2] = {a.x, a.y}, ob[2] = {b.x, b.y};
+        if (there && i < s.rows) {
+          store_words<T, 2>(xp, to_words<T, 2>(oa));
+          store_words<T, 2>(gp, to_words<T, 2>(ob));
+        }
+        if (PACKED && (s.ends >> i & 1)) {
+          const int seq = __shfl_sync(tb200::FULL_MASK, s.id, i);
+          if (there) *reinterpret_cast<float2*>(dh0 + (size_t)seq * dim + c) = unpack2(q);
+        }
+      }
+    }
+  };
+  held s;
+  for (size_t w = 0; w < windows; ++w) { take(s, w); give(s, w); }
+  if (ctas > 1) tb200::cluster_barrier();
+  if (!good && lane == 0) tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
+  if (!PACKED && rank == 0 && warp == 0 && there) *reinterpret_cast<float2*>(dh0 + chain * dim + c) = unpack2(carry);
+}
+
+// ids[r] = the sequence of row r, -1 if it is in none; bits[r / 32]: whether the rows are in one, begin one, end one.  A sequence without rows hands
+// its state (or its gradient) on.
+template <class I>
+__global__ void __launch_bounds__(256) row_table_kernel(const I* offsets, size_t batch, size_t n, int* ids, uint4* bits, const float* from, size_t dim, float* to) {
+  const size_t r = (size_t)blockIdx.x * 256 + threadIdx.x;
+  auto at = [&](size_t s) -> size_t { const long long o = (long long)offsets[s]; return o < 0 ? 0 : (size_t)o > n ? n : (size_t)o; };
+  bool inside = false, begins = false, ends = false;
+  if (r < n) {
+    size_t lo = 0, hi = batch + 1;          // how many of the offsets are at most r
+    while (lo < hi) { const size_t mid = (lo + hi) >> 1; if (at(mid) <= r) lo = mid + 1; else hi = mid; }
+    inside = lo > 0 && lo <= batch;
+    ids[r] = inside ? (int)(lo - 1) : -1;
+    begins = inside && at(lo - 1) == r;
+    ends = inside && at(lo) == r + 1;
+  }
+  const unsigned in = __ballot_sync(tb200::FULL_MASK, inside), first = __ballot_sync(tb200::FULL_MASK, begins), final = __ballot_sync(tb200::FULL_MASK, ends);
+  if (threadIdx.x % 32 == 0 && r < n) bits[r / 32] = make_uint4(in, first, final, 0);
+  for (size_t s = blockIdx.x; s < batch; s += gridDim.x)
+    if (at(s) >= at(s + 1))
+      for (size_t c = threadIdx.x; c < dim; c += 256) to[s * dim + c] = from ? from[s * dim + c] : 0.f;
+}
+
+// How many CTAs walk a chain together.  One, where the chains' slices fill the device by themselves: pairs that travel cost a window
+// about 0.6 us (256 slices of 4096 bf16 rows: one CTA each 79 us, two 98).  Else as many as make about 360 CTAs, but not more than nine: clusters of
+// more no longer all fit their GPCs (40 slices of 20011 rows: 9 CTAs 77 us, 7 93, 11 118; 16 slices of 65537 f32 rows: 9 204, 16 242), unless there are so few slices
+// that the device stays empty either way (2 slices of 65536 rows: 16 CTAs 112, 9 157).
+struct scan_shape { unsigned warps, ctas, slices; };
+inline scan_shape shape_of(size_t chains, size_t length, size_t slices, int rows, unsigned warps = 0) {
+  scan_shape s;
+  s.slices = (unsigned)slices;
+  s.warps = warps ? warps : 1;
+  while (!warps && s.warps < (unsigned)SCAN_WARPS && (size_t)s.warps * rows < length) s.warps *= 2;
+  const size_t items = chains * slices, tiles = (length + (size_t)s.warps * rows - 1) / ((size_t)s.warps * rows);
+  size_t ctas = items >= 200 ? 1 : items < 9 ? 16 : 360 / items < 9 ? 360 / items : 9;
+  if (ctas > tiles) ctas = tiles;
+  s.ctas = ctas < 1 ? 1 : (unsigned)ctas;
+  return s;
+}
+
+template <class... Params, class... Args>
+cudaError_t launch_chains(void (*kernel)(Params...), scan_shape s, size_t chains, size_t smem, cudaStream_t stream, Args... args) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3((unsigned)(chains * s.slices * s.ctas));
+  cfg.blockDim = dim3(s.warps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = s.ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (s.ctas > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+  if (s.ctas > 1 && tb200::launch_refused(e)) {      // no room for such a cluster: a CTA walks a chain alone
+    cfg.gridDim = dim3((unsigned)(chains * s.slices));
+    attr[0].val.clusterDim.x = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+  }
+  return e;
 }
 
 // one token of each sequence: state[slot] is read and written, and is the row's output too
@@ -94,42 +883,146 @@ __global__ void __launch_bounds__(BLOCK) gated_step_kernel(const T* x, size_t xs
 constexpr size_t MOST_CTAS_Y = 65535;
 }  // namespace
 
+namespace {
+// the workspace: header, then the rows' sequences where there are offsets
+size_t scan_workspace(const void* offsets, size_t n) { return sizeof(tb200::ws_header) + (offsets ? tb200::align_up(n * 4, 256) + tb200::align_up((n + 31) / 32 * 16, 256) : 0); }
+int* ids_of(void* d_ws) { return reinterpret_cast<int*>(static_cast<char*>(d_ws) + sizeof(tb200::ws_header)); }
+uint4* bits_of(void* d_ws, size_t n) { return reinterpret_cast<uint4*>(static_cast<char*>(d_ws) + sizeof(tb200::ws_header) + tb200::align_up(n * 4, 256)); }
+
+template <class I>
+cudaError_t find_ids(const void* offsets, size_t batch, size_t n, void* d_ws, const void* from, size_t dim, void* to, cudaStream_t stream) {
+  row_table_kernel<I><<<(unsigned)(n / 256 + 1), 256, 0, stream>>>(static_cast<const I*>(offsets), batch, n, ids_of(d_ws), bits_of(d_ws, n), static_cast<const float*>(from), dim, static_cast<float*>(to));
+  return cudaGetLastError();
+}
+
+// The rows as the copy engine takes tiles of `box` rows of 64 channels from them; false: it cannot.
+template <class T> bool tile_map(CUtensorMap& map, const void* p, size_t rows, size_t dim, size_t stride, unsigned box) {
+  using encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const encode call = []() -> encode {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+    return reinterpret_cast<encode>(f);
+  }();
+  const cuuint64_t dims[2] = {dim, rows}, strides[1] = {stride * sizeof(T)};
+  const cuuint32_t boxes[2] = {64, box}, steps[2] = {1, 1};
+  const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : std::is_same<T, f16>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return call && call(&map, type, 2, const_cast<void*>(p), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// a channel pair in one access where all rows allow it
+template <class T> bool in_pairs(const void* p, size_t dim, size_t stride) { return ((reinterpret_cast<uintptr_t>(p) | dim * sizeof(T) | stride * sizeof(T)) & (2 * sizeof(T) - 1)) == 0; }
+
+constexpr int NO_MAP = -1;        // the copy engine does not take these rows
+
+bool scan_sizes_fit(const void* offsets, size_t batch, size_t n, size_t dim) {
+  return batch < (1ull << 31) && n < (1ull << 40) && (offsets || (batch > 0 && n % batch == 0)) && (offsets ? 1 : batch) * ((dim + 31) / 32) * tb200::CLUSTER_MAX_CTAS < (1ull << 31) &&
+         n / 256 < (1ull << 31) - 1;
+}
+}  // namespace
+
 TB200_API int tb200_gated_scan(const void* d_x, size_t x_stride, const void* d_gate, size_t gate_stride, const void* d_h0, const void* d_offsets, int offset_t, size_t batch,
-                               size_t n, size_t dim, int t, void* d_h, void* d_last, tb200_stream_t stream) {
+                               size_t n, size_t dim, int t, void* d_h, void* d_last, void* d_ws, size_t* ws_bytes, tb200_stream_t stream) {
   return by_row_dtype(t, [&](auto tv) -> int {
     using T = decltype(tv);
     return by_index_dtype(d_offsets ? offset_t : TB200_I32, [&](auto iv) -> int {
       using I = decltype(iv);
+      int rc;
+      if (workspace_gate(d_ws, ws_bytes, scan_workspace(d_offsets, n), rc)) return rc;
       if (dim == 0 || (n == 0 && batch == 0)) return 0;
-      if ((n && (!d_x || !d_gate || !d_h)) || (batch && !d_last) || x_stride < dim || gate_stride < dim || batch >= 0x7fffffffull || (dim + BLOCK - 1) / BLOCK > MOST_CTAS_Y ||
-          (!d_offsets && (batch == 0 || n % batch)))
-        return ERR_INVALID;
-      const sequences<I> seq = {static_cast<const I*>(d_offsets), batch, n, d_offsets ? 0 : n / batch};
-      const dim3 grid((unsigned)(batch + (d_offsets ? 1 : 0)), (unsigned)((dim + BLOCK - 1) / BLOCK));
-      gated_scan_kernel<T, I><<<grid, BLOCK, 0, stream>>>(static_cast<const T*>(d_x), x_stride, static_cast<const T*>(d_gate), gate_stride, static_cast<const float*>(d_h0), seq, dim,
-                                                        static_cast<T*>(d_h), static_cast<float*>(d_last));
-      return (int)cudaGetLastError();
+      if ((n && (!d_x || !d_gate || !d_h)) || (batch && !d_last) || x_stride < dim || gate_stride < dim || !scan_sizes_fit(d_offsets, batch, n, dim)) return ERR_INVALID;
+      if (d_offsets) {
+        const cudaError_t e = find_ids<I>(d_offsets, batch, n, d_ws, d_h0, dim, d_last, stream);
+        if (e != cudaSuccess || n == 0) return (int)e;
+      }
+      const size_t chains = d_offsets ? 1 : batch, length = n / chains;
+      if (length > 32 && n < (1ull << 31) - 512 && in_16_bytes(d_x, dim, x_stride, sizeof(T)) && in_16_bytes(d_gate, dim, gate_stride, sizeof(T)) && in_16_bytes(d_h, dim, dim, sizeof(T)) &&
+          in_16_bytes(d_h0, dim, dim, 4) && in_16_bytes(d_last, dim, dim, 4)) {
+        auto tiled = [&](auto warps, auto rows, auto stages) -> int {
+          constexpr int WARPS = decltype(warps)::value, ROWS = decltype(rows)::value, STAGES = decltype(stages)::value;
+          using Shared = tiles_shared<T, WARPS, ROWS, 2, STAGES>;
+          CUtensorMap xm, gm;
+          if (!tile_map<T>(xm, d_x, n, dim, x_stride, WARPS * ROWS) || !tile_map<T>(gm, d_gate, n, dim, gate_stride, WARPS * ROWS)) return NO_MAP;
+          const scan_shape shape = shape_of(chains, length, (dim + 63) / 64, ROWS, WARPS);
+          auto with = [&](auto packed) -> int {
+            return (int)launch_chains(gated_tiles_kernel<T, WARPS, ROWS, STAGES, decltype(packed)::value>, shape, chains, Shared::bytes(shape.ctas), stream, xm, gm,
+                                      static_cast<const float*>(d_h0), row_table{bits_of(d_ws, n), ids_of(d_ws)}, shape.slices, length, dim, static_cast<T*>(d_h),
+                                      static_cast<float*>(d_last), static_cast<tb200::ws_header*>(d_ws));
+          };
+          return d_offsets ? with(std::true_type()) : with(std::false_type());
+        };
+        const int rc2 = tiled(std::integral_constant<int, 4>(), std::integral_constant<int, 16>(), std::integral_constant<int, 2>());
+        if (rc2 != NO_MAP) return rc2;
+      }
+      auto go = [&](auto v, auto packed) -> int {
+        constexpr int V = decltype(v)::value, ROWS = 16;
+        const scan_shape shape = shape_of(chains, length, (dim + 32 * V - 1) / (32 * V), ROWS);
+        return (int)launch_chains(gated_scan_kernel<T, V, ROWS, decltype(packed)::value>, shape, chains, 0, stream, static_cast<const T*>(d_x), x_stride, static_cast<const T*>(d_gate),
+                                  gate_stride, static_cast<const float*>(d_h0), ids_of(d_ws), shape.slices, length, dim, static_cast<T*>(d_h), static_cast<float*>(d_last));
+      };
+      const bool pairs = in_pairs<T>(d_x, dim, x_stride) && in_pairs<T>(d_gate, dim, gate_stride) && in_pairs<T>(d_h, dim, dim);
+      if constexpr (sizeof(T) == 2) {
+        if (pairs) return d_offsets ? go(std::integral_constant<int, 2>(), std::true_type()) : go(std::integral_constant<int, 2>(), std::false_type());
+      }
+      return d_offsets ? go(std::integral_constant<int, 1>(), std::true_type()) : go(std::integral_constant<int, 1>(), std::false_type());
     });
   });
 }
 
 TB200_API int tb200_gated_scan_grad(const void* d_dh, size_t dh_stride, const void* d_x, size_t x_stride, const void* d_gate, size_t gate_stride, const void* d_h, size_t h_stride,
                                     const void* d_h0, const void* d_dlast, const void* d_offsets, int offset_t, size_t batch, size_t n, size_t dim, int t, void* d_dx,
-                                    void* d_dgate, void* d_dh0, tb200_stream_t stream) {
+                                    void* d_dgate, void* d_dh0, void* d_ws, size_t* ws_bytes, tb200_stream_t stream) {
   return by_row_dtype(t, [&](auto tv) -> int {
     using T = decltype(tv);
     return by_index_dtype(d_offsets ? offset_t : TB200_I32, [&](auto iv) -> int {
       using I = decltype(iv);
+      int rc;
+      if (workspace_gate(d_ws, ws_bytes, scan_workspace(d_offsets, n), rc)) return rc;
       if (dim == 0 || (n == 0 && batch == 0)) return 0;
       if ((n && (!d_dh || !d_x || !d_gate || !d_h || !d_dx || !d_dgate)) || (batch && !d_dh0) || dh_stride < dim || x_stride < dim || gate_stride < dim || h_stride < dim ||
-          batch >= 0x7fffffffull || (dim + BLOCK - 1) / BLOCK > MOST_CTAS_Y || (!d_offsets && (batch == 0 || n % batch)))
+          !scan_sizes_fit(d_offsets, batch, n, dim))
         return ERR_INVALID;
-      const sequences<I> seq = {static_cast<const I*>(d_offsets), batch, n, d_offsets ? 0 : n / batch};
-      const dim3 grid((unsigned)(batch + (d_offsets ? 1 : 0)), (unsigned)((dim + BLOCK - 1) / BLOCK));
-      gated_scan_grad_kernel<T, I><<<grid, BLOCK, 0, stream>>>(static_cast<const T*>(d_dh), dh_stride, static_cast<const T*>(d_x), x_stride, static_cast<const T*>(d_gate), gate_stride,
-                                                             static_cast<const T*>(d_h), h_stride, static_cast<const float*>(d_h0), static_cast<const float*>(d_dlast), seq, dim,
-                                                             static_cast<T*>(d_dx), static_cast<T*>(d_dgate), static_cast<float*>(d_dh0));
-      return (int)cudaGetLastError();
+      if (d_offsets) {
+        const cudaError_t e = find_ids<I>(d_offsets, batch, n, d_ws, d_dlast, dim, d_dh0, stream);
+        if (e != cudaSuccess || n == 0) return (int)e;
+      }
+      const size_t chains = d_offsets ? 1 : batch, length = n / chains;
+      if (length > 32 && n < (1ull << 31) - 512 && in_16_bytes(d_dh, dim, dh_stride, sizeof(T)) && in_16_bytes(d_x, dim, x_stride, sizeof(T)) &&
+          in_16_bytes(d_gate, dim, gate_stride, sizeof(T)) && in_16_bytes(d_h, dim, h_stride, sizeof(T)) && in_16_bytes(d_dx, dim, dim, sizeof(T)) &&
+          in_16_bytes(d_dgate, dim, dim, sizeof(T)) && in_16_bytes(d_h0, dim, dim, 4) && in_16_bytes(d_dlast, dim, dim, 4) && in_16_bytes(d_dh0, dim, dim, 4)) {
+        auto tiled = [&](auto warps, auto rows, auto stages) -> int {
+          constexpr int WARPS = decltype(warps)::value, ROWS = decltype(rows)::value, STAGES = decltype(stages)::value;
+          using Shared = tiles_shared<T, WARPS, ROWS, 4, STAGES>;
+          CUtensorMap dm, gm, xm, hm;
+          if (!tile_map<T>(dm, d_dh, n, dim, dh_stride, WARPS * ROWS) || !tile_map<T>(gm, d_gate, n, dim, gate_stride, WARPS * ROWS) ||
+              !tile_map<T>(xm, d_x, n, dim, x_stride, WARPS * ROWS) || !tile_map<T>(hm, d_h, n, dim, h_stride, WARPS * ROWS))
+            return NO_MAP;
+          const scan_shape shape = shape_of(chains, length, (dim + 63) / 64, ROWS, WARPS);
+          auto with = [&](auto packed) -> int {
+            return (int)launch_chains(gated_tiles_grad_kernel<T, WARPS, ROWS, STAGES, decltype(packed)::value>, shape, chains, Shared::bytes(shape.ctas), stream, dm, gm, xm, hm,
+                                      static_cast<const float*>(d_h0), static_cast<const float*>(d_dlast), row_table{bits_of(d_ws, n), ids_of(d_ws)}, shape.slices, length, dim,
+                                      static_cast<T*>(d_dx), static_cast<T*>(d_dgate), static_cast<float*>(d_dh0), static_cast<tb200::ws_header*>(d_ws));
+          };
+          return d_offsets ? with(std::true_type()) : with(std::false_type());
+        };
+        const int rc2 = tiled(std::integral_constant<int, 4>(), std::integral_constant<int, 8>(), std::integral_constant<int, 2>());
+        if (rc2 != NO_MAP) return rc2;
+      }
+      auto go = [&](auto v, auto packed) -> int {
+        constexpr int V = decltype(v)::value, ROWS = 8;
+        const scan_shape shape = shape_of(chains, length, (dim + 32 * V - 1) / (32 * V), ROWS);
+        return (int)launch_chains(gated_scan_grad_kernel<T, V, ROWS, decltype(packed)::value>, shape, chains, 0, stream, static_cast<const T*>(d_dh), dh_stride, static_cast<const T*>(d_x),
+                                  x_stride, static_cast<const T*>(d_gate), gate_stride, static_cast<const T*>(d_h), h_stride, static_cast<const float*>(d_h0),
+                                  static_cast<const float*>(d_dlast), ids_of(d_ws), shape.slices, length, dim, static_cast<T*>(d_dx), static_cast<T*>(d_dgate), static_cast<float*>(d_dh0));
+      };
+      const bool pairs = in_pairs<T>(d_dh, dim, dh_stride) && in_pairs<T>(d_x, dim, x_stride) && in_pairs<T>(d_gate, dim, gate_stride) && in_pairs<T>(d_h, dim, h_stride) &&
+                         in_pairs<T>(d_dx, dim, dim) && in_pairs<T>(d_dgate, dim, dim);
+      if constexpr (sizeof(T) == 2) {
+        if (pairs) return d_offsets ? go(std::integral_constant<int, 2>(), std::true_type()) : go(std::integral_constant<int, 2>(), std::false_type());
+      }
+      return d_offsets ? go(std::integral_constant<int, 1>(), std::true_type()) : go(std::integral_constant<int, 1>(), std::false_type());
     });
   });
 }

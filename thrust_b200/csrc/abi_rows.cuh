@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "abi_common.cuh"
 
@@ -21,6 +22,54 @@ template <> __device__ __forceinline__ bf16 from_f32<bf16>(float x) { return __f
 
 // V neighbouring channels of a row, moved in one access.
 template <class T, int V> struct alignas(sizeof(T) * V) piece { T at[V]; };
+
+// The same as 32-bit words in registers: V * sizeof(T) is 2 (in the low half) or a multiple of 4.
+template <class T, int V> struct words {
+  static constexpr int BYTES = (int)sizeof(T) * V, N = BYTES < 4 ? 1 : BYTES / 4;
+  unsigned at[N];
+};
+template <class T, int V> __device__ __forceinline__ words<T, V> load_words(const T* p) {
+  words<T, V> w;
+  if constexpr (words<T, V>::BYTES == 2) w.at[0] = *reinterpret_cast<const unsigned short*>(p);
+  else if constexpr (words<T, V>::BYTES == 4) w.at[0] = *reinterpret_cast<const unsigned*>(p);
+  else if constexpr (words<T, V>::BYTES == 8) { const uint2 u = *reinterpret_cast<const uint2*>(p); w.at[0] = u.x; w.at[1] = u.y; }
+  else { const uint4 u = *reinterpret_cast<const uint4*>(p); w.at[0] = u.x; w.at[1] = u.y; w.at[2] = u.z; w.at[3] = u.w; }
+  return w;
+}
+template <class T, int V> __device__ __forceinline__ void store_words(T* p, const words<T, V>& w) {
+  if constexpr (words<T, V>::BYTES == 2) *reinterpret_cast<unsigned short*>(p) = (unsigned short)w.at[0];
+  else if constexpr (words<T, V>::BYTES == 4) *reinterpret_cast<unsigned*>(p) = w.at[0];
+  else if constexpr (words<T, V>::BYTES == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w.at[0], w.at[1]);
+  else *reinterpret_cast<uint4*>(p) = make_uint4(w.at[0], w.at[1], w.at[2], w.at[3]);
+}
+// channel v of them as a float; all of them from floats
+template <int v, class T, int V> __device__ __forceinline__ float channel(const words<T, V>& w) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w.at[v]);
+  else if constexpr (std::is_same<T, bf16>::value) return __uint_as_float(v % 2 ? w.at[v / 2] & 0xffff0000u : w.at[v / 2] << 16);
+  else return __half2float(__ushort_as_half((unsigned short)(v % 2 ? w.at[v / 2] >> 16 : w.at[v / 2])));
+}
+template <class T, int V> __device__ __forceinline__ words<T, V> to_words(const float (&f)[V]) {
+  words<T, V> w;
+#pragma unroll
+  for (int i = 0; i < words<T, V>::N; ++i) {
+    if constexpr (sizeof(T) == 4) w.at[i] = __float_as_uint(f[i]);
+    else if constexpr (V == 1) w.at[i] = std::is_same<T, bf16>::value ? (unsigned)__bfloat16_as_ushort(__float2bfloat16_rn(f[0])) : (unsigned)__half_as_ushort(__float2half_rn(f[0]));
+    else if constexpr (std::is_same<T, bf16>::value) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w.at[i] = *reinterpret_cast<const unsigned*>(&b);
+    } else {
+      const __half2 b = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w.at[i] = *reinterpret_cast<const unsigned*>(&b);
+    }
+  }
+  return w;
+}
+template <int N, class F> __device__ __forceinline__ void each(F f) {
+  if constexpr (N > 0) { each<N - 1>(f); f(std::integral_constant<int, N - 1>()); }
+}
+template <class T, int V> __device__ __forceinline__ void channels(const words<T, V>& w, float (&f)[V]) {
+  each<V>([&](auto v) { f[decltype(v)::value] = channel<decltype(v)::value>(w); });
+}
 
 // f(T()) for the type that a TB200_F32, TB200_F16 or TB200_BF16 names
 template <class F> int by_row_dtype(int t, F f) {

@@ -150,8 +150,8 @@ def gated_scan(x, gate, h0=None, offsets=None, out=None):
     batch, n, dim, offs, code = _sequences(x, offsets)
     h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
     last = torch.empty(batch, dim, dtype=torch.float32, device=x.device)
-    _check(_lib.load().tb200_gated_scan(x.data_ptr(), xs, gate.data_ptr(), gs, _maybe("h0", h0, torch.float32, (batch, dim)), offs, code, batch, n, dim, _ROW_CODE[x.dtype],
-                                        _packed("out", h, x.dtype, x.shape), last.data_ptr(), _stream()), "gated_scan")
+    _call_and_wait("gated", "gated_scan", "tb200_gated_scan", x.data_ptr(), xs, gate.data_ptr(), gs, _maybe("h0", h0, torch.float32, (batch, dim)), offs, code, batch, n, dim,
+                   _ROW_CODE[x.dtype], _packed("out", h, x.dtype, x.shape), last.data_ptr(), sync=False)
     return h, last
 
 
@@ -162,9 +162,9 @@ def gated_scan_grad(dh, x, gate, h, h0=None, dlast=None, offsets=None):
     batch, n, dim, offs, code = _sequences(x, offsets)
     dx, dgate = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dh0 = torch.empty(batch, dim, dtype=torch.float32, device=x.device)
-    _check(_lib.load().tb200_gated_scan_grad(dh.data_ptr(), ds, x.data_ptr(), xs, gate.data_ptr(), gs, h.data_ptr(), hs, _maybe("h0", h0, torch.float32, (batch, dim)),
-                                             _maybe("dlast", dlast, torch.float32, (batch, dim)), offs, code, batch, n, dim, _ROW_CODE[x.dtype], dx.data_ptr(),
-                                             dgate.data_ptr(), dh0.data_ptr(), _stream()), "gated_scan_grad")
+    _call_and_wait("gated", "gated_scan_grad", "tb200_gated_scan_grad", dh.data_ptr(), ds, x.data_ptr(), xs, gate.data_ptr(), gs, h.data_ptr(), hs,
+                   _maybe("h0", h0, torch.float32, (batch, dim)), _maybe("dlast", dlast, torch.float32, (batch, dim)), offs, code, batch, n, dim, _ROW_CODE[x.dtype],
+                   dx.data_ptr(), dgate.data_ptr(), dh0.data_ptr(), sync=False)
     return dx, dgate, dh0
 
 
