@@ -5,103 +5,249 @@ using namespace tb200_abi;
 using namespace tb200_rows;
 
 namespace {
-constexpr int BLOCK = 128;
 constexpr int MOST_EXPERTS = 1024;
 constexpr int MOST_CHOICES = 32;
+constexpr int DISPATCH_BLOCK = 1024;
+constexpr int SMALL_BLOCK = 256;
+constexpr unsigned COUNT_HERE = 8192;      // up to so many assignments every CTA counts them all itself
 
-// Stable counting sort of m ids by one CTA: counts, their prefixes, then 1024 ids at a time in order.
+template <class I> __device__ __forceinline__ unsigned expert_of(const I* ids, size_t i, unsigned experts) {      // `experts` for an id that is none
+  const long long e = (long long)ids[i];
+  return e >= 0 && e < (long long)experts ? (unsigned)e : experts;
+}
+
+// table[block][expert]: how many assignments of the block's tokens go there
 template <class I>
-__global__ void __launch_bounds__(1024) expert_places_kernel(const I* ids, unsigned m, unsigned experts, int* slots, int* sources, int* offsets) {
-  __shared__ unsigned next[MOST_EXPERTS];
-  __shared__ unsigned id_at[1024];
-  const unsigned t = threadIdx.x;
-  next[t] = 0;
+__global__ void __launch_bounds__(DISPATCH_BLOCK) expert_count_kernel(const I* ids, size_t n, unsigned choices, unsigned experts, unsigned* table) {
+  __shared__ unsigned count[MOST_EXPERTS];
+  for (unsigned e = threadIdx.x; e < experts; e += DISPATCH_BLOCK) count[e] = 0;
   __syncthreads();
-  for (unsigned i = t; i < m; i += 1024) {
-    const long long e = (long long)ids[i];
-    if (e >= 0 && e < (long long)experts) atomicAdd(&next[(unsigned)e], 1u);
-  }
-  __syncthreads();
-  if (t == 0) {
-    unsigned sum = 0;
-    for (unsigned e = 0; e < experts; ++e) { const unsigned c = next[e]; next[e] = sum; offsets[e] = (int)sum; sum += c; }
-    offsets[experts] = (int)sum;
+  const size_t per = (n + gridDim.x - 1) / gridDim.x, first = blockIdx.x * per < n ? blockIdx.x * per : n, stop = first + per < n ? first + per : n;
+  for (size_t i = first * choices + threadIdx.x; i < stop * choices; i += DISPATCH_BLOCK) {
+    const unsigned e = expert_of(ids, i, experts);
+    if (e < experts) atomicAdd(&count[e], 1u);
   }
   __syncthreads();
-  for (unsigned base = 0; base < m; base += 1024) {
-    const unsigned i = base + t;
-    const long long e = i < m ? (long long)ids[i] : -1;
-    const bool kept = e >= 0 && e < (long long)experts;
-    id_at[t] = kept ? (unsigned)e : ~0u;
-    __syncthreads();
-    unsigned before = 0, all = 0;
-    if (kept)
-      for (unsigned j = 0; j < 1024; ++j) { const bool same = id_at[j] == (unsigned)e; all += same; before += same && j < t; }
-    unsigned at = 0;
-    if (kept) at = next[(unsigned)e] + before;
-    __syncthreads();
-    if (kept) { slots[i] = (int)at; sources[at] = (int)i; if (before == 0) next[(unsigned)e] += all; }
-    else if (i < m) slots[i] = -1;
-    __syncthreads();
-  }
-  for (unsigned i = (unsigned)offsets[experts] + t; i < m; i += 1024) sources[i] = -1;
+  for (unsigned e = threadIdx.x; e < experts; e += DISPATCH_BLOCK) table[(size_t)blockIdx.x * experts + e] = count[e];
+  tb200::grid_dependents_launch();
 }
 
-// a CTA a row
-template <class T>
-__global__ void __launch_bounds__(BLOCK) expert_rows_kernel(const T* x, size_t xs, const int* sources, unsigned choices, size_t dim, T* rows) {
-  const int source = sources[blockIdx.x];
-  T* const to = rows + (size_t)blockIdx.x * dim;
-  for (size_t c = threadIdx.x; c < dim; c += BLOCK) to[c] = source < 0 ? from_f32<T>(0.f) : x[(size_t)((unsigned)source / choices) * xs + c];
+// lanes that take a row together: a power of two that covers its pieces
+inline __host__ __device__ unsigned lanes_for(size_t pieces) {
+  unsigned g = 1;
+  while (g < 32 && g < pieces) g *= 2;
+  return g;
 }
 
-// out[token] = sum of weights * rows over the token's choices that have a place; a CTA a token
-template <class T>
-__global__ void __launch_bounds__(BLOCK) expert_combine_kernel(const T* rows, size_t rs, size_t m, const int* slots, const float* weights, unsigned choices, size_t dim, T* out) {
-  const size_t token = blockIdx.x;
-  for (size_t c = threadIdx.x; c < dim; c += BLOCK) {
-    float sum = 0.f;
-    for (unsigned k = 0; k < choices; ++k) {
-      const int at = slots[token * choices + k];
-      if ((unsigned)at < m) sum += (weights ? weights[token * choices + k] : 1.f) * to_f32(rows[(size_t)at * rs + c]);
-    }
-    out[token * dim + c] = from_f32<T>(sum);
-  }
-}
-
-// drows[place] = weight * dout[token], dweight = <dout[token], rows[place]>; a CTA a token, and one more for each row without a source
-template <class T>
-__global__ void __launch_bounds__(BLOCK) expert_combine_grad_kernel(const T* dout, size_t ds, const T* rows, size_t rs, size_t m, const int* slots, const float* weights,
-                                                                  const int* end, size_t n, unsigned choices, size_t dim, T* drows, float* dweights) {
-  __shared__ float part[BLOCK / 32];
-  if (blockIdx.x >= n) {
-    const size_t row = blockIdx.x - n;
-    if ((long long)row < (long long)*end) return;
-    for (size_t c = threadIdx.x; c < dim; c += BLOCK) drows[row * dim + c] = from_f32<T>(0.f);
-    return;
-  }
-  const size_t token = blockIdx.x;
-  for (unsigned k = 0; k < choices; ++k) {
-    const int at = slots[token * choices + k];
-    const bool kept = (unsigned)at < m;
-    const float w = kept ? weights[token * choices + k] : 0.f;
-    float dot = 0.f;
-    if (kept)
-      for (size_t c = threadIdx.x; c < dim; c += BLOCK) {
-        const float d = to_f32(dout[token * ds + c]);
-        dot += d * to_f32(rows[(size_t)at * rs + c]);
-        drows[(size_t)at * dim + c] = from_f32<T>(w * d);
+// A stable counting sort of the assignments and the rows' way to their places, in one kernel.  A CTA has the assignments of neighbouring tokens.
+// It adds up, by expert, all assignments and those before its own (from the blocks' counts, or from the ids while they are few), ranks its own
+// ones warp by warp, and copies each of its tokens' rows to its places: a row is read once and written as often as it goes somewhere.
+// Bound by the bytes of the rows.
+template <class V, class I, bool COUNTED>
+__global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V* __restrict__ x, size_t xs, const I* __restrict__ ids, size_t n, unsigned choices, unsigned experts,
+                                                                       size_t pieces, V* __restrict__ rows, int* slots, int* sources, int* offsets,
+                                                                       const unsigned* __restrict__ table) {
+  extern __shared__ unsigned raw[];
+  const unsigned warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  unsigned* const total = raw;                    // [experts]
+  unsigned* const start = total + experts;        // [experts]: of this CTA's assignments, first how many come before them
+  unsigned* const at = start + experts;           // [warps][experts]
+  __shared__ unsigned kept;
+  const size_t m = n * choices;
+  const size_t per = (n + gridDim.x - 1) / gridDim.x, first = blockIdx.x * per < n ? blockIdx.x * per : n, stop = first + per < n ? first + per : n;
+  const size_t i0 = first * choices, i1 = stop * choices;
+  for (unsigned e = threadIdx.x; e < (2 + warps) * experts; e += blockDim.x) raw[e] = 0;
+  __syncthreads();
+  if (COUNTED) {
+    tb200::grid_dependency_wait();
+    const unsigned cells = gridDim.x * experts, mine = blockIdx.x * experts;
+    for (unsigned i = threadIdx.x; i < cells; i += blockDim.x) {
+      const unsigned c = table[i];
+      if (c) {
+        atomicAdd(&total[i % experts], c);
+        if (i < mine) atomicAdd(&start[i % experts], c);
       }
-    for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(tb200::FULL_MASK, dot, o);
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = dot;
-    __syncthreads();
-    if (threadIdx.x == 0) dweights[token * choices + k] = (part[0] + part[1]) + (part[2] + part[3]);
-    __syncthreads();
+    }
+  } else {
+    for (size_t i = threadIdx.x; i < m; i += blockDim.x) {
+      const unsigned e = expert_of(ids, i, experts);
+      if (e < experts) {
+        atomicAdd(&total[e], 1u);
+        if (i < i0) atomicAdd(&start[e], 1u);
+      }
+    }
   }
+  // this warp's assignments: neighbouring ones
+  const size_t share = ((i1 - i0 + warps - 1) / warps + 31) / 32 * 32;
+  const size_t w0 = i0 + warp * share < i1 ? i0 + warp * share : i1, w1 = w0 + share < i1 ? w0 + share : i1;
+  unsigned* const own = at + warp * experts;
+  for (size_t i = w0 + lane; i < w1; i += 32) {
+    const unsigned e = expert_of(ids, i, experts);
+    if (e < experts) atomicAdd(&own[e], 1u);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    unsigned sum = 0;
+    for (unsigned base = 0; base < experts; base += 32) {
+      const unsigned e = base + lane, c = e < experts ? total[e] : 0;
+      const unsigned inclusive = tb200::warp_inclusive_scan(c, tb200::plus_op());
+      if (e < experts) {
+        const unsigned o = sum + inclusive - c;
+        start[e] += o;
+        if (blockIdx.x == 0) offsets[e] = (int)o;
+      }
+      sum += __shfl_sync(tb200::FULL_MASK, inclusive, 31);
+    }
+    if (lane == 0) { kept = sum; if (blockIdx.x == 0) offsets[experts] = (int)sum; }
+  }
+  __syncthreads();
+  for (unsigned e = threadIdx.x; e < experts; e += blockDim.x) {
+    unsigned next = start[e];
+    for (unsigned w = 0; w < warps; ++w) { const unsigned c = at[w * experts + e]; at[w * experts + e] = next; next += c; }
+  }
+  __syncthreads();
+  for (size_t base = w0; base < w1; base += 32) {
+    const size_t i = base + lane;
+    const unsigned e = i < w1 ? expert_of(ids, i, experts) : experts;
+    const unsigned same = __match_any_sync(tb200::FULL_MASK, e);
+    const unsigned before = __popc(same & ((1u << lane) - 1));
+    unsigned place = 0;
+    if (e < experts) place = own[e] + before;
+    __syncwarp();
+    if (e < experts) {
+      if (before == 0) own[e] += __popc(same);
+      slots[i] = (int)place;
+      sources[place] = (int)i;
+    } else if (i < w1) {
+      slots[i] = -1;
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  constexpr int U = 8;
+  const unsigned g = lanes_for(pieces), group = threadIdx.x / g, groups = blockDim.x / g, in = threadIdx.x % g;
+  for (size_t token = first + group; token < stop; token += groups) {
+    const V* const from = x + token * xs;
+    for (size_t c0 = in; c0 < pieces; c0 += (size_t)g * U) {
+      V v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c0 + (size_t)u * g < pieces) v[u] = from[c0 + (size_t)u * g];
+      for (unsigned k = 0; k < choices; ++k) {
+        const int place = slots[token * choices + k];
+        if (place < 0) continue;
+        V* const to = rows + (size_t)place * pieces;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c0 + (size_t)u * g < pieces) to[c0 + (size_t)u * g] = v[u];
+      }
+    }
+  }
+  // rows that nothing goes to
+  for (size_t row = (size_t)kept + (size_t)blockIdx.x * groups + group; row < m; row += (size_t)gridDim.x * groups) {
+    if (in == 0) sources[row] = -1;
+    V* const to = rows + row * pieces;
+    for (size_t c = in; c < pieces; c += g) to[c] = V{};
+  }
+}
+
+// a thread a piece of a token's result; its rows' pieces are requested four at a time
+template <class T, int V, bool WEIGHTED>
+__global__ void __launch_bounds__(256) expert_combine_kernel(const T* __restrict__ rows, size_t rs, unsigned m, const int* __restrict__ slots, const float* __restrict__ weights,
+                                                             unsigned choices, unsigned pieces, size_t items, size_t dim, T* __restrict__ out) {
+  const size_t item = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (item >= items) return;
+  const size_t token = items <= 0xffffffffull ? (size_t)((unsigned)item / pieces) : item / pieces;
+  const size_t c = (item - token * pieces) * V;
+  const int* const at = slots + token * choices;
+  float sum[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum[v] = 0.f;
+  for (unsigned k0 = 0; k0 < choices; k0 += 4) {
+    words<T, V> r[4];
+    bool there[4];
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) {
+      const int place = k0 + j < choices ? at[k0 + j] : -1;
+      there[j] = (unsigned)place < m;
+      if (there[j]) r[j] = load_words<T, V>(rows + (size_t)place * rs + c);
+    }
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j)
+      if (there[j]) {
+        float f[V];
+        channels(r[j], f);
+        const float w = WEIGHTED ? weights[token * choices + k0 + j] : 1.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] = WEIGHTED ? fmaf(w, f[v], sum[v]) : sum[v] + f[v];
+      }
+  }
+  store_words<T, V>(out + token * dim + c, to_words<T, V>(sum));
+}
+
+// A warp a token: its row of dout stays in registers (while it fits) against the rows of all its choices, each read and written once.
+template <class T, int V>
+__global__ void __launch_bounds__(256) expert_combine_grad_kernel(const T* __restrict__ dout, size_t ds, const T* __restrict__ rows, size_t rs, size_t m, const int* __restrict__ slots,
+                                                                  const float* __restrict__ weights, const int* __restrict__ end, size_t n, unsigned choices, size_t pieces,
+                                                                  T* __restrict__ drows, float* __restrict__ dweights) {
+  constexpr int U = 8;
+  const int lane = threadIdx.x % 32;
+  const size_t warps = (size_t)gridDim.x * 8, index = (size_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const size_t dim = pieces * V;
+  for (size_t token = index; token < n; token += warps) {
+    const T* const d = dout + token * ds;
+    words<T, V> held[U];
+    auto take = [&](size_t c0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c0 + u * 32 < pieces) held[u] = load_words<T, V>(d + (c0 + u * 32) * V);
+    };
+    if (pieces <= U * 32) take(lane);
+    for (unsigned k = 0; k < choices; ++k) {
+      const int place = slots[token * choices + k];
+      float dot = 0.f;
+      if ((unsigned)place < m) {
+        const float w = weights[token * choices + k];
+        const T* const r = rows + (size_t)place * rs;
+        T* const to = drows + (size_t)place * dim;
+        for (size_t c0 = lane; c0 < pieces; c0 += U * 32) {
+          words<T, V> v[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (c0 + u * 32 < pieces) v[u] = load_words<T, V>(r + (c0 + u * 32) * V);
+          if (pieces > U * 32) take(c0);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (c0 + u * 32 < pieces) {
+              float a[V], b[V];
+              channels(held[u], a);
+              channels(v[u], b);
+#pragma unroll
+              for (int i = 0; i < V; ++i) { dot = fmaf(a[i], b[i], dot); a[i] *= w; }
+              store_words<T, V>(to + (c0 + u * 32) * V, to_words<T, V>(a));
+            }
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(tb200::FULL_MASK, dot, o);
+      }
+      if (lane == 0) dweights[token * choices + k] = dot;
+    }
+  }
+  float none[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) none[v] = 0.f;
+  const int kept = *end;
+  for (size_t row = (kept > 0 ? (size_t)kept : 0) + index; row < m; row += warps)
+    for (size_t c = lane; c < pieces; c += 32) store_words<T, V>(drows + row * dim + c * V, to_words<T, V>(none));
 }
 
 // what every one of these calls needs of its sizes: flat assignments and rows are counted in 31 bits
 bool sizes_fit(size_t n, size_t choices) { return choices >= 1 && choices <= (size_t)MOST_CHOICES && n <= 0x7fffffffull / choices / 2; }
+
+unsigned dispatch_grid(size_t n) { const size_t sms = (size_t)tb200::current_device_info().sm_count; return (unsigned)(n < sms ? (n ? n : 1) : sms); }
+size_t dispatch_workspace(size_t n, size_t choices, size_t experts) {
+  return sizeof(tb200::ws_header) + (n * choices > COUNT_HERE ? (size_t)dispatch_grid(n) * experts * 4 : 0);
+}
 }  // namespace
 
 TB200_API int tb200_expert_dispatch(const void* d_x, size_t x_stride, const void* d_experts, int expert_t, size_t n, size_t choices, size_t num_experts, size_t dim, int t,
@@ -112,12 +258,35 @@ TB200_API int tb200_expert_dispatch(const void* d_x, size_t x_stride, const void
       using I = decltype(iv);
       if (!sizes_fit(n, choices) || num_experts < 1 || num_experts > (size_t)MOST_EXPERTS) return ERR_INVALID;
       int rc;
-      if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header), rc)) return rc;
-      const unsigned m = (unsigned)(n * choices);
+      if (workspace_gate(d_ws, ws_bytes, dispatch_workspace(n, choices, num_experts), rc)) return rc;
+      const size_t m = n * choices;
       if (!d_offsets || (m && (!d_experts || !d_slots || !d_sources || (dim && (!d_x || !d_rows)))) || x_stride < dim) return ERR_INVALID;
-      expert_places_kernel<I><<<1, 1024, 0, stream>>>(static_cast<const I*>(d_experts), m, (unsigned)num_experts, d_slots, d_sources, d_offsets);
-      if (m && dim) expert_rows_kernel<T><<<m, BLOCK, 0, stream>>>(static_cast<const T*>(d_x), x_stride, d_sources, (unsigned)choices, dim, static_cast<T*>(d_rows));
-      return (int)cudaGetLastError();
+      const unsigned experts = (unsigned)num_experts, grid = dispatch_grid(n);
+      const bool counted = m > COUNT_HERE;
+      unsigned* const table = reinterpret_cast<unsigned*>(static_cast<char*>(d_ws) + sizeof(tb200::ws_header));
+      if (counted) expert_count_kernel<I><<<grid, DISPATCH_BLOCK, 0, stream>>>(static_cast<const I*>(d_experts), n, (unsigned)choices, experts, table);
+      auto go = [&](auto vv, auto cv) -> int {
+        using V = decltype(vv);
+        constexpr bool COUNTED = decltype(cv)::value;
+        const int block = COUNTED ? DISPATCH_BLOCK : SMALL_BLOCK;
+        const size_t smem = (2 + (size_t)block / 32) * experts * 4;
+        auto kernel = expert_dispatch_kernel<V, I, COUNTED>;
+        if (smem > 40 * 1024) {
+          const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+          if (e != cudaSuccess) return (int)e;
+        }
+        const size_t scale = sizeof(V) / sizeof(T);
+        if (COUNTED)      // begins while the blocks are still counted, and waits for that
+          return (int)tb200::launch_after(kernel, grid, block, smem, stream, static_cast<const V*>(d_x), x_stride / scale, static_cast<const I*>(d_experts), n, (unsigned)choices, experts,
+                                          dim / scale, static_cast<V*>(d_rows), d_slots, d_sources, d_offsets, table);
+        kernel<<<grid, block, smem, stream>>>(static_cast<const V*>(d_x), x_stride / scale, static_cast<const I*>(d_experts), n, (unsigned)choices, experts, dim / scale,
+                                              static_cast<V*>(d_rows), d_slots, d_sources, d_offsets, table);
+        return (int)cudaGetLastError();
+      };
+      auto with = [&](auto vv) -> int { return counted ? go(vv, std::true_type()) : go(vv, std::false_type()); };
+      if (in_16_bytes(d_x, dim, x_stride, sizeof(T)) && in_16_bytes(d_rows, dim, dim, sizeof(T))) return with(uint4());
+      if constexpr (sizeof(T) == 4) return with(unsigned());
+      else return with((unsigned short)0);
     });
   });
 }
@@ -129,8 +298,17 @@ TB200_API int tb200_expert_combine(const void* d_rows, size_t rows_stride, const
     if (!sizes_fit(n, choices)) return ERR_INVALID;
     if (n == 0 || dim == 0) return 0;
     if (!d_rows || !d_slots || !d_out || rows_stride < dim) return ERR_INVALID;
-    expert_combine_kernel<T><<<(unsigned)n, BLOCK, 0, stream>>>(static_cast<const T*>(d_rows), rows_stride, n * choices, d_slots, d_weights, (unsigned)choices, dim, static_cast<T*>(d_out));
-    return (int)cudaGetLastError();
+    auto go = [&](auto vv, auto wv) -> int {
+      constexpr int V = decltype(vv)::value;
+      const size_t pieces = dim / V, items = n * pieces, grid = (items + 255) / 256;
+      if (pieces > 0xffffffffull || grid > 0x7fffffffull) return ERR_INVALID;
+      expert_combine_kernel<T, V, decltype(wv)::value><<<(unsigned)grid, 256, 0, stream>>>(static_cast<const T*>(d_rows), rows_stride, (unsigned)(n * choices), d_slots, d_weights,
+                                                                                         (unsigned)choices, (unsigned)pieces, items, dim, static_cast<T*>(d_out));
+      return (int)cudaGetLastError();
+    };
+    auto with = [&](auto vv) -> int { return d_weights ? go(vv, std::true_type()) : go(vv, std::false_type()); };
+    if (in_16_bytes(d_rows, dim, rows_stride, sizeof(T)) && in_16_bytes(d_out, dim, dim, sizeof(T))) return with(std::integral_constant<int, 16 / sizeof(T)>());
+    return with(std::integral_constant<int, 1>());
   });
 }
 
@@ -141,9 +319,16 @@ TB200_API int tb200_expert_combine_grad(const void* d_dout, size_t dout_stride, 
     if (!sizes_fit(n, choices)) return ERR_INVALID;
     if (n == 0) return 0;
     if (!d_slots || !d_weights || !d_kept || !d_dweights || (dim && (!d_dout || !d_rows || !d_drows)) || dout_stride < dim || rows_stride < dim) return ERR_INVALID;
-    const size_t m = n * choices;
-    expert_combine_grad_kernel<T><<<(unsigned)(n + m), BLOCK, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, static_cast<const T*>(d_rows), rows_stride, m, d_slots, d_weights,
-                                                                         d_kept, n, (unsigned)choices, dim, static_cast<T*>(d_drows), d_dweights);
-    return (int)cudaGetLastError();
+    auto go = [&](auto vv) -> int {
+      constexpr int V = decltype(vv)::value;
+      const size_t most = (size_t)tb200::current_device_info().sm_count * 16, want = (n + 7) / 8;
+      expert_combine_grad_kernel<T, V><<<(unsigned)(want < most ? want : most), 256, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, static_cast<const T*>(d_rows), rows_stride,
+                                                                                              n * choices, d_slots, d_weights, d_kept, n, (unsigned)choices, dim / V,
+                                                                                              static_cast<T*>(d_drows), d_dweights);
+      return (int)cudaGetLastError();
+    };
+    if (in_16_bytes(d_dout, dim, dout_stride, sizeof(T)) && in_16_bytes(d_rows, dim, rows_stride, sizeof(T)) && in_16_bytes(d_drows, dim, dim, sizeof(T)))
+      return go(std::integral_constant<int, 16 / sizeof(T)>());
+    return go(std::integral_constant<int, 1>());
   });
 }
