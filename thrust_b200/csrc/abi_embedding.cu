@@ -6,23 +6,6 @@ using namespace tb200_abi;
 using namespace tb200_rows;
 
 namespace {
-// how many threads take a row's pieces side by side, as a power of two: enough to cover them, up to 2^most
-inline unsigned spread_of(size_t pieces, unsigned most) {
-  unsigned g = 0;
-  while (g < most && (size_t(1) << g) < pieces) ++g;
-  return g;
-}
-// which of the groups of 2^spread threads this thread is in is `part` of `parts` of item `at`
-struct share { size_t at; unsigned part, in; };
-__device__ __forceinline__ share share_of(size_t thread, unsigned spread, unsigned parts) {
-  const size_t group = thread >> spread;
-  share s;
-  s.at = parts == 1 ? group : group <= 0xffffffffull ? (size_t)((unsigned)group / parts) : group / parts;
-  s.part = (unsigned)(group - s.at * parts);
-  s.in = (unsigned)thread & ((1u << spread) - 1);
-  return s;
-}
-
 // out[i] = scale * weight[tokens[i]].  2^spread lanes take up to LOOKUP_U pieces each of a row (`parts` times that make a row): as many random reads
 // are in flight per thread.  Bound by the bytes of the rows.
 constexpr int LOOKUP_U = 4;
@@ -52,10 +35,11 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ we
     }
 }
 
-// keys: the token, or `rows` for one that is no row; positions 0, 1, ...
+// keys: the token, or `rows` for one that is no row; positions 0, 1, ...; and the list of long runs is empty
 template <class I>
-__global__ void __launch_bounds__(256) token_keys_kernel(const I* tokens, size_t n, unsigned rows, unsigned* keys, unsigned* positions) {
+__global__ void __launch_bounds__(256) token_keys_kernel(const I* tokens, size_t n, unsigned rows, unsigned* keys, unsigned* positions, unsigned* count) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i == 0) *count = 0;
   if (i >= n) return;
   const long long tok = (long long)tokens[i];
   keys[i] = tok >= 0 && tok < (long long)rows ? (unsigned)tok : rows;
@@ -77,15 +61,16 @@ __device__ __forceinline__ size_t warp_lower_bound(const unsigned* keys, size_t 
 }
 
 // The gradient, over the tokens' places in the order of the tokens.
-//   sums     A CTA takes a chunk of neighbouring places and a run of columns, a thread V of them: it adds up the rows of its chunk run by run (a run:
-//            places of the same token), GRAD_U rows requested ahead.  A run that lies in the chunk becomes a row of the result; what a run has in a chunk
-//            that it enters or leaves goes to two rows of 32-bit sums a chunk.
+//   sums     Some threads take a chunk of neighbouring places, V columns each, and add up its rows run by run (a run: places of the same token), GRAD_U
+//            rows requested ahead.  A run that begins in a chunk and ends in the next one at the latest is added up there, and the next chunk leaves it out;
+//            of a longer one each chunk adds up its own part, into one of two rows of 32-bit sums that it has.
 //   zeros    Further CTAs of the same launch clear the rows whose token does not occur, GRAD_ZERO rows each.
-//   joins    Where a run leaves the chunk in which it begins, its parts are added up, in order.
+//   joins    The parts of a long run are added up, in order.
 // So every row of dout is read once, every row of the result is written once, and the order of all sums is the places'.
 constexpr int GRAD_U = 8;
 constexpr int GRAD_BLOCK = 256;
-constexpr unsigned GRAD_ZERO = 32;
+constexpr unsigned GRAD_ZERO = 32, GRAD_CHUNK = 32;      // rows cleared by a CTA; most places of a chunk
+constexpr unsigned GRAD_SPREAD = 4;                        // at least 16 threads a chunk
 
 struct grad_shape {
   unsigned chunk;        // places of a chunk
@@ -94,16 +79,44 @@ struct grad_shape {
   unsigned parts;        // how many such groups take all columns
 };
 
-template <class O, int V> __device__ __forceinline__ void write_sum(O* to, const float (&sum)[V], float scale, bool accumulate) {
+// What a chunk has to do with the runs at its two ends.
+struct run_ends {
+  size_t end, stop;          // behind its last place; behind the last place that it may look at
+  unsigned first, last;      // the tokens at its ends
+  bool entered;              // its first run has begun in an earlier chunk,
+  bool skip;                 // and is added up there
+  bool extended;             // its last run goes on in the next chunk, and is added up here all the same
+  bool leaves;               // its last run begins here and has a part in at least two more chunks
+};
+__device__ __forceinline__ run_ends run_ends_of(const unsigned* keys, size_t n, size_t chunk, unsigned size) {
+  run_ends r;
+  const size_t begin = chunk * size;
+  r.end = begin + size < n ? begin + size : n;
+  const size_t next = r.end + size < n ? r.end + size : n;
+  r.first = keys[begin];
+  r.last = keys[r.end - 1];
+  const unsigned before = begin ? keys[begin - 1] : ~r.first, behind = r.end < n ? keys[r.end] : ~r.last;
+  const unsigned previous = begin ? keys[begin - size] : ~r.first, earlier = begin > size ? keys[begin - size - 1] : ~r.first;
+  const unsigned next_last = keys[next - 1], next_behind = next < n ? keys[next] : ~r.last;
+  r.entered = before == r.first;
+  const bool whole = r.entered && r.last == r.first;
+  r.skip = r.entered && !(r.last == r.first && behind == r.first) && !(previous == r.first && earlier == r.first);
+  const bool goes_on = behind == r.last && !whole, ends_next = !(next_last == r.last && next_behind == r.last);
+  r.extended = goes_on && ends_next;
+  r.leaves = goes_on && !ends_next;
+  r.stop = r.extended ? next : r.end;
+  return r;
+}
+
+// the chunks in which long runs begin
+struct long_runs { unsigned count, pad[63], chunks[1]; };
+
+// the sum becomes a row of the result, added to what is there (`old`) if that is wanted
+template <class O, int V, bool ADD> __device__ __forceinline__ void write_sum(O* to, const float (&sum)[V], float scale, const words<O, V>& old) {
   float f[V];
+  if (ADD) channels(old, f);
 #pragma unroll
-  for (int v = 0; v < V; ++v) f[v] = sum[v] * scale;
-  if (accumulate) {
-    float old[V];
-    channels(load_words<O, V>(to), old);
-#pragma unroll
-    for (int v = 0; v < V; ++v) f[v] += old[v];
-  }
+  for (int v = 0; v < V; ++v) f[v] = ADD ? fmaf(sum[v], scale, f[v]) : sum[v] * scale;
   store_words<O, V>(to, to_words<O, V>(f));
 }
 // rows of sums: in 16-byte pieces where V is a multiple of four (dim is one of V then)
@@ -129,28 +142,25 @@ template <int V> __device__ __forceinline__ void read_part(const float* from, fl
   }
 }
 
-template <class T, class O, int V>
-__global__ void __launch_bounds__(GRAD_BLOCK) embedding_grad_kernel(const T* __restrict__ dout, size_t stride, const unsigned* __restrict__ keys, const unsigned* __restrict__ positions,
-                                                                  size_t n, unsigned rows, unsigned pieces, grad_shape shape, float scale, bool accumulate, unsigned zero_blocks,
-                                                                  O* __restrict__ out, float* __restrict__ partial, const tb200::ws_header* hdr) {
+template <class T, class O, int V, bool ADD>
+__global__ void __launch_bounds__(GRAD_BLOCK, ADD ? 2 : 3) embedding_grad_kernel(const T* __restrict__ dout, size_t stride, const unsigned* __restrict__ keys, const unsigned* __restrict__ positions,
+                                                                  size_t n, unsigned rows, unsigned pieces, grad_shape shape, float scale, unsigned zero_blocks,
+                                                                  O* __restrict__ out, float* __restrict__ partial, long_runs* __restrict__ list, const tb200::ws_header* hdr) {
   const size_t dim = (size_t)pieces * V;
   if (hdr->error) {      // the sort's waits ran out
     for (size_t i = (size_t)blockIdx.x * GRAD_BLOCK + threadIdx.x; i < rows * dim; i += (size_t)gridDim.x * GRAD_BLOCK) out[i] = from_f32<O>(__int_as_float(0x7fffffff));
     return;
   }
-  if (blockIdx.x < zero_blocks) {
+  const unsigned sum_blocks = gridDim.x - zero_blocks;
+  if (blockIdx.x >= sum_blocks) {      // behind the sums, which take longer
     __shared__ unsigned present;
-    const unsigned first = blockIdx.x * GRAD_ZERO, count = rows - first < GRAD_ZERO ? rows - first : GRAD_ZERO;
-    if (threadIdx.x < 32) {
-      unsigned mine = 0;
-      bool more = true;
-      for (size_t i = warp_lower_bound(keys, n, first) + threadIdx.x; more; i += 32) {
-        const unsigned key = i < n ? keys[i] : ~0u;
-        if (key < first + count) mine |= 1u << (key - first);
-        more = __all_sync(tb200::FULL_MASK, key < first + count);
-      }
-      mine = __reduce_or_sync(tb200::FULL_MASK, mine);
-      if (threadIdx.x == 0) present = mine;
+    const unsigned first = (blockIdx.x - sum_blocks) * GRAD_ZERO, count = rows - first < GRAD_ZERO ? rows - first : GRAD_ZERO;
+    if (threadIdx.x < 32) {      // a lane a row: is there a place of its token among those of the rows?  (Walking them takes as long as a frequent token has places.)
+      const size_t from = warp_lower_bound(keys, n, first), to = warp_lower_bound(keys, n, first + count);
+      size_t lo = from, hi = to;
+      while (lo < hi) { const size_t mid = (lo + hi) >> 1; if (keys[mid] < first + threadIdx.x) lo = mid + 1; else hi = mid; }
+      const unsigned all = __ballot_sync(tb200::FULL_MASK, threadIdx.x < count && lo < to && keys[lo] == first + threadIdx.x);
+      if (threadIdx.x == 0) present = all;
     }
     __syncthreads();
     float none[V];
@@ -161,92 +171,147 @@ __global__ void __launch_bounds__(GRAD_BLOCK) embedding_grad_kernel(const T* __r
         for (unsigned c = threadIdx.x; c < pieces; c += GRAD_BLOCK) store_words<O, V>(out + (size_t)(first + r) * dim + (size_t)c * V, to_words<O, V>(none));
     return;
   }
-  const share mine = share_of((size_t)(blockIdx.x - zero_blocks) * GRAD_BLOCK + threadIdx.x, shape.spread, shape.parts);
-  const size_t chunk = mine.at;
-  const unsigned c = (mine.part << shape.spread) + mine.in;
-  if (chunk >= shape.chunks || c >= pieces) return;
-  const size_t begin = chunk * shape.chunk, end = begin + shape.chunk < n ? begin + shape.chunk : n;
-  const T* const from = dout + (size_t)c * V;
-  bool entered = begin > 0 && keys[begin - 1] == keys[begin];
-  unsigned key = keys[begin];
-  float sum[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) sum[v] = 0.f;
-  auto finish = [&](bool leaves) {
-    if (key < rows) {
-      if (entered) write_part<V>(partial + (2 * chunk) * dim + (size_t)c * V, sum);
-      else if (leaves) write_part<V>(partial + (2 * chunk + 1) * dim + (size_t)c * V, sum);
-      else write_sum<O, V>(out + (size_t)key * dim + (size_t)c * V, sum, scale, accumulate);
-    }
-    entered = false;
-#pragma unroll
-    for (int v = 0; v < V; ++v) sum[v] = 0.f;
-  };
-  for (size_t i0 = begin; i0 < end; i0 += GRAD_U) {
-    words<T, V> r[GRAD_U];
-    unsigned k[GRAD_U];
-#pragma unroll
-    for (int u = 0; u < GRAD_U; ++u) {
-      k[u] = i0 + u < end ? keys[i0 + u] : rows;
-      if (k[u] < rows) r[u] = load_words<T, V>(from + (size_t)positions[i0 + u] * stride);
-    }
-#pragma unroll
-    for (int u = 0; u < GRAD_U; ++u) {
-      if (i0 + u >= end) break;
-      if (k[u] != key) { finish(false); key = k[u]; }
-      if (key < rows) {
-        float f[V];
-        channels(r[u], f);
-#pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] += f[v];
-      }
-    }
-  }
-  finish(end < n && keys[end] == key);
-}
-
-template <class O, int V>
-__global__ void __launch_bounds__(GRAD_BLOCK) embedding_grad_join_kernel(const unsigned* __restrict__ keys, size_t n, unsigned rows, unsigned pieces, grad_shape shape, float scale,
-                                                                       bool accumulate, O* __restrict__ out, const float* __restrict__ partial, const tb200::ws_header* hdr) {
-  tb200::grid_dependency_wait();
-  if (hdr->error) return;
-  const size_t dim = (size_t)pieces * V;
   const share mine = share_of((size_t)blockIdx.x * GRAD_BLOCK + threadIdx.x, shape.spread, shape.parts);
   const size_t chunk = mine.at;
   const unsigned c = (mine.part << shape.spread) + mine.in;
-  if (chunk + 1 >= shape.chunks || c >= pieces) return;
-  const size_t begin = chunk * shape.chunk, end = begin + shape.chunk;
-  const unsigned key = keys[end - 1];
-  if (key >= rows || keys[end] != key) return;                                              // no run leaves this chunk
-  if (begin > 0 && keys[begin] == key && keys[begin - 1] == key) return;                    // one does that has begun earlier
-  size_t lo = chunk + 1, hi = shape.chunks;            // how many chunks begin with this token: those behind this one up to lo
-  while (lo < hi) { const size_t mid = (lo + hi) >> 1; if (keys[mid * shape.chunk] == key) lo = mid + 1; else hi = mid; }
-  float sum[V];
-  const float* p = partial + (size_t)c * V;
-  read_part<V>(p + (2 * chunk + 1) * dim, sum);
-  constexpr int AHEAD = V > 1 ? 4 : GRAD_U;
-  for (size_t q = chunk + 1; q < lo; q += AHEAD) {
-    float f[AHEAD][V];
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-      if (q + u < lo) read_part<V>(p + 2 * (q + u) * dim, f[u]);
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-      if (q + u < lo) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] += f[u][v];
-      }
+  // What there is to do, place by place, found once for all columns: the row of dout to add (NO_ROW: none), and what becomes of the sum behind it: 0
+  // nothing, 1 and 2 it is this chunk's part of a run that has begun earlier or goes on, 3 + v it is row v of the result.
+  constexpr unsigned MOST = 2 * GRAD_CHUNK, NO_ROW = ~0u;
+  __shared__ unsigned staged_keys[GRAD_BLOCK >> GRAD_SPREAD][MOST + 1];
+  __shared__ __align__(16) unsigned staged_rows[GRAD_BLOCK >> GRAD_SPREAD][MOST], staged_then[GRAD_BLOCK >> GRAD_SPREAD][MOST];
+  __shared__ unsigned staged_count[GRAD_BLOCK >> GRAD_SPREAD];
+  const unsigned group = threadIdx.x >> shape.spread, step = 1u << shape.spread;
+  unsigned* const its_keys = staged_keys[group];
+  unsigned* const its_rows = staged_rows[group];
+  unsigned* const its_then = staged_then[group];
+  const size_t begin = chunk * shape.chunk;
+  run_ends run = {};
+  if (chunk < shape.chunks) {
+    for (unsigned j = mine.in; j <= MOST; j += step) {
+      const bool there = j <= 2 * shape.chunk && begin + j < n;
+      its_keys[j] = there ? keys[begin + j] : ~0u;
+      if (j < MOST) its_rows[j] = there ? positions[begin + j] : NO_ROW;
+    }
+    run = run_ends_of(keys, n, chunk, shape.chunk);
+    if (run.leaves && run.last < rows && mine.part == 0 && mine.in == 0) list->chunks[atomicAdd(&list->count, 1u)] = (unsigned)chunk;
   }
-  write_sum<O, V>(out + (size_t)key * dim + (size_t)c * V, sum, scale, accumulate);
+  __syncthreads();
+  if (chunk < shape.chunks) {
+    const unsigned end = (unsigned)(run.end - begin), stop = (unsigned)(run.stop - begin);
+    for (unsigned j = mine.in; j < MOST; j += step) {
+      const unsigned key = its_keys[j];
+      const bool here = j < end || (j < stop && key == run.last), used = here && key < rows && !(run.skip && key == run.first);
+      const bool ends = its_keys[j + 1] != key, leaves = !ends && j + 1 == end && !run.extended;
+      if (!used) its_rows[j] = NO_ROW;
+      its_then[j] = !used || !(ends || leaves) ? 0u : run.entered && key == run.first ? 1u : leaves ? 2u : 3u + key;
+      if (here && (j + 1 == MOST || !(j + 1 < end || (j + 1 < stop && its_keys[j + 1] == run.last)))) staged_count[group] = j + 1;
+    }
+  }
+  __syncthreads();
+  if (chunk >= shape.chunks || c >= pieces) return;
+  const T* const from = dout + (size_t)c * V;
+  const unsigned count = staged_count[group];
+  float sum[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum[v] = 0.f;
+  for (unsigned j0 = 0; j0 < count; j0 += GRAD_U) {
+    words<T, V> r[GRAD_U] = {};
+    words<O, V> old[GRAD_U];
+    unsigned then[GRAD_U];
+#pragma unroll
+    for (int u = 0; u < GRAD_U; u += 4) {
+      const uint4 at = *reinterpret_cast<const uint4*>(its_rows + j0 + u), th = *reinterpret_cast<const uint4*>(its_then + j0 + u);
+      const unsigned row[4] = {at.x, at.y, at.z, at.w};
+      then[u] = th.x; then[u + 1] = th.y; then[u + 2] = th.z; then[u + 3] = th.w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (row[i] != NO_ROW) r[u + i] = load_words<T, V>(from + (size_t)row[i] * stride);
+        if (ADD && then[u + i] > 2) old[u + i] = load_words<O, V>(out + (size_t)(then[u + i] - 3) * dim + (size_t)c * V);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < GRAD_U; ++u) {
+      float f[V];
+      channels(r[u], f);
+#pragma unroll
+      for (int v = 0; v < V; ++v) sum[v] += f[v];
+      if (then[u]) {
+        if (then[u] > 2) write_sum<O, V, ADD>(out + (size_t)(then[u] - 3) * dim + (size_t)c * V, sum, scale, old[u]);
+        else write_part<V>(partial + (2 * chunk + then[u] - 1) * dim + (size_t)c * V, sum);
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] = 0.f;
+      }
+    }
+  }
 }
 
-// Chunks of 64 places, smaller ones (down to 8) while fewer than a thousand threads a SM would have work.
+// A CTA takes a listed run and 32 pieces of the columns at a time: its eight warps add up neighbouring parts each, and their sums are added up in
+// order.  (The order of the list is any; each run is by itself.)
+constexpr unsigned JOIN_WARPS = GRAD_BLOCK / 32;
+template <class O, int V, bool ADD>
+__global__ void __launch_bounds__(GRAD_BLOCK) embedding_grad_join_kernel(const unsigned* __restrict__ keys, unsigned pieces, grad_shape shape, float scale, O* __restrict__ out,
+                                                                       const float* __restrict__ partial, const long_runs* __restrict__ list, const tb200::ws_header* hdr) {
+  __shared__ size_t behind;            // the first chunk that has no part
+  __shared__ float sums[JOIN_WARPS][32][V];
+  tb200::grid_dependency_wait();
+  if (hdr->error) return;
+  const size_t dim = (size_t)pieces * V;
+  const unsigned columns = (pieces + 31) / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const unsigned long long items = (unsigned long long)list->count * columns;
+  for (unsigned long long item = blockIdx.x; item < items; item += gridDim.x) {
+    const unsigned nth = (unsigned)(item / columns), c = (unsigned)(item - (unsigned long long)nth * columns) * 32 + lane;
+    const size_t chunk = list->chunks[nth];
+    const unsigned key = keys[(chunk + 1) * shape.chunk];
+    if (warp == 0) {
+      size_t q = chunk + 1;
+      for (unsigned full = ~0u; full == ~0u; q += __popc(full)) full = __ballot_sync(tb200::FULL_MASK, q + lane < shape.chunks && keys[(q + lane) * shape.chunk] == key);
+      if (lane == 0) behind = q;
+    }
+    __syncthreads();
+    // parts 0, 1, ...: the second row of this chunk, the first rows of those behind it
+    const size_t parts = behind - chunk, share = (parts + JOIN_WARPS - 1) / JOIN_WARPS, from = warp * share, to = from + share < parts ? from + share : parts;
+    float sum[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum[v] = 0.f;
+    if (c < pieces) {
+      const float* const p = partial + 2 * chunk * dim + (size_t)c * V;
+      constexpr int AHEAD = 8;
+      for (size_t i = from; i < to; i += AHEAD) {
+        float f[AHEAD][V];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+          if (i + u < to) read_part<V>(p + (i + u ? 2 * (i + u) : 1) * dim, f[u]);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+          if (i + u < to) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum[v] += f[u][v];
+          }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) sums[warp][lane][v] = sum[v];
+    __syncthreads();
+    if (warp == 0 && c < pieces) {
+      O* const at = out + (size_t)key * dim + (size_t)c * V;
+      words<O, V> old;
+      if (ADD) old = load_words<O, V>(at);
+      for (unsigned w = 1; w < JOIN_WARPS && w * share < parts; ++w)
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] += sums[w][lane][v];
+      write_sum<O, V, ADD>(at, sum, scale, old);
+    }
+    __syncthreads();
+  }
+}
+
+// Chunks of GRAD_CHUNK places, smaller ones (down to 8) while fewer than a thousand threads a SM would have work.
 constexpr size_t GRAD_THREADS = 148 * 1024;
 grad_shape grad_shape_of(size_t n, size_t pieces) {
   grad_shape s;
-  s.spread = spread_of(pieces, 8);
+  s.spread = spread_of(pieces, 8) < GRAD_SPREAD ? GRAD_SPREAD : spread_of(pieces, 8);
   s.parts = (unsigned)((pieces + (size_t(1) << s.spread) - 1) >> s.spread);
-  s.chunk = 64;
+  s.chunk = GRAD_CHUNK;
   while (s.chunk > 8 && ((n + s.chunk - 1) / s.chunk * s.parts << s.spread) < GRAD_THREADS) s.chunk /= 2;
   s.chunks = (n + s.chunk - 1) / s.chunk;
   return s;
@@ -254,14 +319,15 @@ grad_shape grad_shape_of(size_t n, size_t pieces) {
 
 // the workspace: the sort's, then keys, positions and the sort's other halves, then the chunks' sums
 struct grad_layout {
-  size_t array, sort, partial, need;
+  size_t array, sort, list, partial, need;
   grad_layout(size_t n, size_t dim) {
     array = tb200::align_up(n * 4, 256);
     sort = tb200::align_up(tb200::radix_workspace_bytes<4, 4>(n), 256);
-    partial = sort + 4 * array;
-    // as many chunks as there can be, whatever the pieces: of 8 places, or 64 and, where they are smaller, at most GRAD_THREADS to the half of them
+    // as many chunks as there can be, whatever the pieces: of 8 places, or GRAD_CHUNK and, where they are smaller, at most GRAD_THREADS to the half of them
     const grad_shape s = grad_shape_of(n, (dim + 7) / 8);
-    const size_t most = n / 64 + 2 * GRAD_THREADS / ((size_t)s.parts << s.spread) + 2, chunks = (n + 7) / 8 < most ? (n + 7) / 8 : most;
+    const size_t most = n / GRAD_CHUNK + 2 * GRAD_THREADS / ((size_t)s.parts << s.spread) + 2, chunks = (n + 7) / 8 < most ? (n + 7) / 8 : most;
+    list = sort + 4 * array;
+    partial = list + tb200::align_up(256 + chunks * 4, 256);
     need = partial + 2 * chunks * dim * 4;
   }
 };
@@ -308,7 +374,8 @@ TB200_API int tb200_embedding_grad(const void* d_dout, size_t dout_stride, const
         unsigned* const keys = reinterpret_cast<unsigned*>(base + lay.sort);
         unsigned* const positions = reinterpret_cast<unsigned*>(base + lay.sort + 2 * lay.array);
         float* const partial = reinterpret_cast<float*>(base + lay.partial);
-        if (n) token_keys_kernel<I><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(static_cast<const I*>(d_tokens), n, (unsigned)rows, keys, positions);
+        long_runs* const list = reinterpret_cast<long_runs*>(base + lay.list);
+        if (n) token_keys_kernel<I><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(static_cast<const I*>(d_tokens), n, (unsigned)rows, keys, positions, &list->count);
         tb200::key_coding coding;
         coding.kind = tb200::KEY_UNSIGNED;
         coding.descending = 0;
@@ -316,26 +383,29 @@ TB200_API int tb200_embedding_grad(const void* d_dout, size_t dout_stride, const
         while (bits < 32 && (rows >> bits)) bits += 8;      // the largest key is `rows`
         const cudaError_t e = tb200::radix_sort_async<uint32_t, uint32_t, true>(keys, keys + lay.array / 4, positions, positions + lay.array / 4, n, coding, 0, bits, d_ws, stream);
         if (e != cudaSuccess) return (int)e;
-        auto go = [&](auto vv) -> int {
-          constexpr int V = decltype(vv)::value;
-          const unsigned pieces = (unsigned)(dim / V);
+        auto go = [&](auto vv, auto av) -> int {
+          constexpr int V = decltype(vv)::value, JOIN_V = V < 4 ? V : 4;
+          constexpr bool ADD = decltype(av)::value;
+          const unsigned pieces = (unsigned)(dim / V), join_pieces = (unsigned)(dim / JOIN_V);
           const grad_shape shape = grad_shape_of(n, pieces);
           const tb200::ws_header* hdr = static_cast<const tb200::ws_header*>(d_ws);
-          const unsigned zero_blocks = accumulate ? 0u : (unsigned)((rows + GRAD_ZERO - 1) / GRAD_ZERO);
+          const unsigned zero_blocks = ADD ? 0u : (unsigned)((rows + GRAD_ZERO - 1) / GRAD_ZERO);
           const size_t grid = ((shape.chunks * shape.parts << shape.spread) + GRAD_BLOCK - 1) / GRAD_BLOCK;
           if (grid + zero_blocks > 0x7fffffffull) return ERR_INVALID;
           if (grid + zero_blocks == 0) return 0;
-          embedding_grad_kernel<T, O, V><<<(unsigned)(grid + zero_blocks), GRAD_BLOCK, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, keys, positions, n, (unsigned)rows, pieces,
-                                                                                                shape, scale, accumulate != 0, zero_blocks, static_cast<O*>(d_out), partial, hdr);
+          embedding_grad_kernel<T, O, V, ADD><<<(unsigned)(grid + zero_blocks), GRAD_BLOCK, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, keys, positions, n, (unsigned)rows, pieces,
+                                                                                                     shape, scale, zero_blocks, static_cast<O*>(d_out), partial, list, hdr);
           const cudaError_t e = cudaGetLastError();
-          if (e != cudaSuccess || shape.chunks < 2) return (int)e;
-          return (int)tb200::launch_after(embedding_grad_join_kernel<O, V>, grid, GRAD_BLOCK, 0, stream, keys, n, (unsigned)rows, pieces, shape, scale, accumulate != 0,
-                                          static_cast<O*>(d_out), partial, hdr);
+          if (e != cudaSuccess || shape.chunks < 3) return (int)e;
+          const size_t items = (join_pieces + 31) / 32 * shape.chunks / 2, most = (size_t)tb200::current_device_info().sm_count * 3;
+          return (int)tb200::launch_after(embedding_grad_join_kernel<O, JOIN_V, ADD>, items < most ? items : most, GRAD_BLOCK, 0, stream, keys, join_pieces, shape, scale,
+                                          static_cast<O*>(d_out), partial, list, hdr);
         };
+        auto with = [&](auto vv) -> int { return accumulate ? go(vv, std::true_type()) : go(vv, std::false_type()); };
         // pieces of 16 bytes of the wider of the two types, at most 8 channels: both sides are aligned to theirs then
         constexpr int WIDE = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
-        if (in_16_bytes(d_dout, dim, dout_stride, sizeof(T)) && in_16_bytes(d_out, dim, dim, sizeof(O))) return go(std::integral_constant<int, WIDE>());
-        return go(std::integral_constant<int, 1>());
+        if (in_16_bytes(d_dout, dim, dout_stride, sizeof(T)) && in_16_bytes(d_out, dim, dim, sizeof(O))) return with(std::integral_constant<int, WIDE>());
+        return with(std::integral_constant<int, 1>());
       });
     });
   });

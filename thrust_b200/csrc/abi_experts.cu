@@ -32,20 +32,13 @@ __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_count_kernel(const I* i
   tb200::grid_dependents_launch();
 }
 
-// lanes that take a row together: a power of two that covers its pieces
-inline __host__ __device__ unsigned lanes_for(size_t pieces) {
-  unsigned g = 1;
-  while (g < 32 && g < pieces) g *= 2;
-  return g;
-}
-
 // A stable counting sort of the assignments and the rows' way to their places, in one kernel.  A CTA has the assignments of neighbouring tokens.
 // It adds up, by expert, all assignments and those before its own (from the blocks' counts, or from the ids while they are few), ranks its own
 // ones warp by warp, and copies each of its tokens' rows to its places: a row is read once and written as often as it goes somewhere.
 // Bound by the bytes of the rows.
 template <class V, class I, bool COUNTED>
 __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V* __restrict__ x, size_t xs, const I* __restrict__ ids, size_t n, unsigned choices, unsigned experts,
-                                                                       size_t pieces, V* __restrict__ rows, int* slots, int* sources, int* offsets,
+                                                                       size_t pieces, unsigned spread, V* __restrict__ rows, int* slots, int* sources, int* offsets,
                                                                        const unsigned* __restrict__ table) {
   extern __shared__ unsigned raw[];
   const unsigned warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -125,7 +118,7 @@ __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V
   }
   __syncthreads();
   constexpr int U = 8;
-  const unsigned g = lanes_for(pieces), group = threadIdx.x / g, groups = blockDim.x / g, in = threadIdx.x % g;
+  const unsigned g = 1u << spread, group = threadIdx.x / g, groups = blockDim.x / g, in = threadIdx.x % g;
   for (size_t token = first + group; token < stop; token += groups) {
     const V* const from = x + token * xs;
     for (size_t c0 = in; c0 < pieces; c0 += (size_t)g * U) {
@@ -151,38 +144,51 @@ __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V
   }
 }
 
-// a thread a piece of a token's result; its rows' pieces are requested four at a time
+// A thread has up to COMBINE_U pieces of a token's result; the pieces of two of its rows are requested at a time, so that eight reads are in flight
+// (one piece a thread and four rows at a time: 44 us for 8191 x 2 f16 rows of 4096, for which the bytes need 31).
+constexpr int COMBINE_U = 4, COMBINE_K = 2;
 template <class T, int V, bool WEIGHTED>
 __global__ void __launch_bounds__(256) expert_combine_kernel(const T* __restrict__ rows, size_t rs, unsigned m, const int* __restrict__ slots, const float* __restrict__ weights,
-                                                             unsigned choices, unsigned pieces, size_t items, size_t dim, T* __restrict__ out) {
-  const size_t item = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (item >= items) return;
-  const size_t token = items <= 0xffffffffull ? (size_t)((unsigned)item / pieces) : item / pieces;
-  const size_t c = (item - token * pieces) * V;
+                                                             size_t n, unsigned choices, unsigned pieces, unsigned spread, unsigned parts, T* __restrict__ out) {
+  const share s = share_of((size_t)blockIdx.x * 256 + threadIdx.x, spread, parts);
+  const size_t token = s.at;
+  if (token >= n) return;
+  const unsigned lanes = 1u << spread, c0 = s.part * lanes * COMBINE_U + s.in;
   const int* const at = slots + token * choices;
-  float sum[V];
+  float sum[COMBINE_U][V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) sum[v] = 0.f;
-  for (unsigned k0 = 0; k0 < choices; k0 += 4) {
-    words<T, V> r[4];
-    bool there[4];
+  for (int u = 0; u < COMBINE_U; ++u)
 #pragma unroll
-    for (unsigned j = 0; j < 4; ++j) {
+    for (int v = 0; v < V; ++v) sum[u][v] = 0.f;
+  for (unsigned k0 = 0; k0 < choices; k0 += COMBINE_K) {
+    words<T, V> r[COMBINE_K][COMBINE_U];
+    bool there[COMBINE_K];
+#pragma unroll
+    for (unsigned j = 0; j < COMBINE_K; ++j) {
       const int place = k0 + j < choices ? at[k0 + j] : -1;
       there[j] = (unsigned)place < m;
-      if (there[j]) r[j] = load_words<T, V>(rows + (size_t)place * rs + c);
+      const T* const from = rows + (there[j] ? (size_t)place * rs : 0);
+#pragma unroll
+      for (int u = 0; u < COMBINE_U; ++u)
+        if (there[j] && c0 + u * lanes < pieces) r[j][u] = load_words<T, V>(from + (size_t)(c0 + u * lanes) * V);
     }
 #pragma unroll
-    for (unsigned j = 0; j < 4; ++j)
+    for (unsigned j = 0; j < COMBINE_K; ++j)
       if (there[j]) {
-        float f[V];
-        channels(r[j], f);
         const float w = WEIGHTED ? weights[token * choices + k0 + j] : 1.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] = WEIGHTED ? fmaf(w, f[v], sum[v]) : sum[v] + f[v];
+        for (int u = 0; u < COMBINE_U; ++u) {
+          float f[V];
+          channels(r[j][u], f);
+#pragma unroll
+          for (int v = 0; v < V; ++v) sum[u][v] = WEIGHTED ? fmaf(w, f[v], sum[u][v]) : sum[u][v] + f[v];
+        }
       }
   }
-  store_words<T, V>(out + token * dim + c, to_words<T, V>(sum));
+  T* const to = out + token * pieces * V;
+#pragma unroll
+  for (int u = 0; u < COMBINE_U; ++u)
+    if (c0 + u * lanes < pieces) store_words<T, V>(to + (size_t)(c0 + u * lanes) * V, to_words<T, V>(sum[u]));
 }
 
 // A warp a token: its row of dout stays in registers (while it fits) against the rows of all its choices, each read and written once.
@@ -278,9 +284,9 @@ TB200_API int tb200_expert_dispatch(const void* d_x, size_t x_stride, const void
         const size_t scale = sizeof(V) / sizeof(T);
         if (COUNTED)      // begins while the blocks are still counted, and waits for that
           return (int)tb200::launch_after(kernel, grid, block, smem, stream, static_cast<const V*>(d_x), x_stride / scale, static_cast<const I*>(d_experts), n, (unsigned)choices, experts,
-                                          dim / scale, static_cast<V*>(d_rows), d_slots, d_sources, d_offsets, table);
+                                          dim / scale, spread_of(dim / scale, 5), static_cast<V*>(d_rows), d_slots, d_sources, d_offsets, table);
         kernel<<<grid, block, smem, stream>>>(static_cast<const V*>(d_x), x_stride / scale, static_cast<const I*>(d_experts), n, (unsigned)choices, experts, dim / scale,
-                                              static_cast<V*>(d_rows), d_slots, d_sources, d_offsets, table);
+                                              spread_of(dim / scale, 5), static_cast<V*>(d_rows), d_slots, d_sources, d_offsets, table);
         return (int)cudaGetLastError();
       };
       auto with = [&](auto vv) -> int { return counted ? go(vv, std::true_type()) : go(vv, std::false_type()); };
@@ -300,10 +306,13 @@ TB200_API int tb200_expert_combine(const void* d_rows, size_t rows_stride, const
     if (!d_rows || !d_slots || !d_out || rows_stride < dim) return ERR_INVALID;
     auto go = [&](auto vv, auto wv) -> int {
       constexpr int V = decltype(vv)::value;
-      const size_t pieces = dim / V, items = n * pieces, grid = (items + 255) / 256;
-      if (pieces > 0xffffffffull || grid > 0x7fffffffull) return ERR_INVALID;
-      expert_combine_kernel<T, V, decltype(wv)::value><<<(unsigned)grid, 256, 0, stream>>>(static_cast<const T*>(d_rows), rows_stride, (unsigned)(n * choices), d_slots, d_weights,
-                                                                                         (unsigned)choices, (unsigned)pieces, items, dim, static_cast<T*>(d_out));
+      if (dim >= (1ull << 31)) return ERR_INVALID;
+      const unsigned pieces = (unsigned)(dim / V), spread = spread_of((pieces + COMBINE_U - 1) / COMBINE_U, 5);
+      const unsigned parts = (unsigned)(((size_t)pieces + (COMBINE_U << spread) - 1) / (COMBINE_U << spread));
+      const size_t grid = (((n * parts) << spread) + 255) / 256;
+      if (grid > 0x7fffffffull) return ERR_INVALID;
+      expert_combine_kernel<T, V, decltype(wv)::value><<<(unsigned)grid, 256, 0, stream>>>(static_cast<const T*>(d_rows), rows_stride, (unsigned)(n * choices), d_slots, d_weights, n,
+                                                                                         (unsigned)choices, pieces, spread, parts, static_cast<T*>(d_out));
       return (int)cudaGetLastError();
     };
     auto with = [&](auto vv) -> int { return d_weights ? go(vv, std::true_type()) : go(vv, std::false_type()); };

@@ -71,6 +71,23 @@ template <class T, int V> __device__ __forceinline__ void channels(const words<T
   each<V>([&](auto v) { f[decltype(v)::value] = channel<decltype(v)::value>(w); });
 }
 
+// how many threads take a row's pieces side by side, as a power of two: enough to cover them, up to 2^most
+inline unsigned spread_of(size_t pieces, unsigned most) {
+  unsigned g = 0;
+  while (g < most && (size_t(1) << g) < pieces) ++g;
+  return g;
+}
+// which of the groups of 2^spread threads this thread is in is `part` of `parts` of item `at`
+struct share { size_t at; unsigned part, in; };
+__device__ __forceinline__ share share_of(size_t thread, unsigned spread, unsigned parts) {
+  const size_t group = thread >> spread;
+  share s;
+  s.at = parts == 1 ? group : group <= 0xffffffffull ? (size_t)((unsigned)group / parts) : group / parts;
+  s.part = (unsigned)(group - s.at * parts);
+  s.in = (unsigned)thread & ((1u << spread) - 1);
+  return s;
+}
+
 // f(T()) for the type that a TB200_F32, TB200_F16 or TB200_BF16 names
 template <class F> int by_row_dtype(int t, F f) {
   switch (t) {
