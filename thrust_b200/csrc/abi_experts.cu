@@ -53,13 +53,18 @@ __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V
   __syncthreads();
   if (COUNTED) {
     tb200::grid_dependency_wait();
-    const unsigned cells = gridDim.x * experts, mine = blockIdx.x * experts;
-    for (unsigned i = threadIdx.x; i < cells; i += blockDim.x) {
-      const unsigned c = table[i];
-      if (c) {
-        atomicAdd(&total[i % experts], c);
-        if (i < mine) atomicAdd(&start[i % experts], c);
+    // a column of the table is one thread's, or several threads' that take its rows in turn
+    const unsigned turns = blockDim.x / experts > 0 ? blockDim.x / experts : 1, e = threadIdx.x % experts, turn = threadIdx.x / experts;
+    if (turn < turns && threadIdx.x < turns * experts) {
+      unsigned all = 0, before = 0;
+#pragma unroll 8
+      for (unsigned r = turn; r < gridDim.x; r += turns) {
+        const unsigned c = table[(size_t)r * experts + e];
+        all += c;
+        before += r < blockIdx.x ? c : 0;
       }
+      if (all) atomicAdd(&total[e], all);
+      if (before) atomicAdd(&start[e], before);
     }
   } else {
     for (size_t i = threadIdx.x; i < m; i += blockDim.x) {
@@ -144,51 +149,60 @@ __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V
   }
 }
 
-// A thread has up to COMBINE_U pieces of a token's result; the pieces of two of its rows are requested at a time, so that eight reads are in flight
-// (one piece a thread and four rows at a time: 44 us for 8191 x 2 f16 rows of 4096, for which the bytes need 31).
-constexpr int COMBINE_U = 4, COMBINE_K = 2;
-template <class T, int V, bool WEIGHTED>
+// A thread has up to U pieces of a token's result, and requests those of K of its rows at a time.  ALL: K rows are all there are, so that no sums have
+// to be held while rows are on their way: few registers, many reads in flight.
+template <class T, int V, bool WEIGHTED, int K, int U, bool ALL>
 __global__ void __launch_bounds__(256) expert_combine_kernel(const T* __restrict__ rows, size_t rs, unsigned m, const int* __restrict__ slots, const float* __restrict__ weights,
                                                              size_t n, unsigned choices, unsigned pieces, unsigned spread, unsigned parts, T* __restrict__ out) {
   const share s = share_of((size_t)blockIdx.x * 256 + threadIdx.x, spread, parts);
   const size_t token = s.at;
   if (token >= n) return;
-  const unsigned lanes = 1u << spread, c0 = s.part * lanes * COMBINE_U + s.in;
+  const unsigned lanes = 1u << spread, c0 = s.part * lanes * U + s.in;
   const int* const at = slots + token * choices;
-  float sum[COMBINE_U][V];
+  T* const to = out + token * pieces * V;
+  float sum[ALL ? 1 : U][V];
 #pragma unroll
-  for (int u = 0; u < COMBINE_U; ++u)
+  for (int u = 0; u < (ALL ? 1 : U); ++u)
 #pragma unroll
     for (int v = 0; v < V; ++v) sum[u][v] = 0.f;
-  for (unsigned k0 = 0; k0 < choices; k0 += COMBINE_K) {
-    words<T, V> r[COMBINE_K][COMBINE_U];
-    bool there[COMBINE_K];
+  for (unsigned k0 = 0; k0 < (ALL ? 1 : choices); k0 += K) {
+    words<T, V> r[K][U];
+    bool there[K];
 #pragma unroll
-    for (unsigned j = 0; j < COMBINE_K; ++j) {
+    for (unsigned j = 0; j < K; ++j) {
       const int place = k0 + j < choices ? at[k0 + j] : -1;
       there[j] = (unsigned)place < m;
       const T* const from = rows + (there[j] ? (size_t)place * rs : 0);
 #pragma unroll
-      for (int u = 0; u < COMBINE_U; ++u)
+      for (int u = 0; u < U; ++u)
         if (there[j] && c0 + u * lanes < pieces) r[j][u] = load_words<T, V>(from + (size_t)(c0 + u * lanes) * V);
     }
+    float w[K];
 #pragma unroll
-    for (unsigned j = 0; j < COMBINE_K; ++j)
-      if (there[j]) {
-        const float w = WEIGHTED ? weights[token * choices + k0 + j] : 1.f;
+    for (unsigned j = 0; j < K; ++j) w[j] = WEIGHTED && there[j] ? weights[token * choices + k0 + j] : 1.f;
 #pragma unroll
-        for (int u = 0; u < COMBINE_U; ++u) {
+    for (int u = 0; u < U; ++u) {
+      float (&t)[V] = sum[ALL ? 0 : u];
+      if (ALL) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) t[v] = 0.f;
+      }
+#pragma unroll
+      for (unsigned j = 0; j < K; ++j)
+        if (there[j]) {
           float f[V];
           channels(r[j][u], f);
 #pragma unroll
-          for (int v = 0; v < V; ++v) sum[u][v] = WEIGHTED ? fmaf(w, f[v], sum[u][v]) : sum[u][v] + f[v];
+          for (int v = 0; v < V; ++v) t[v] = WEIGHTED ? fmaf(w[j], f[v], t[v]) : t[v] + f[v];
         }
-      }
+      if (ALL && c0 + u * lanes < pieces) store_words<T, V>(to + (size_t)(c0 + u * lanes) * V, to_words<T, V>(t));
+    }
   }
-  T* const to = out + token * pieces * V;
+  if (!ALL) {
 #pragma unroll
-  for (int u = 0; u < COMBINE_U; ++u)
-    if (c0 + u * lanes < pieces) store_words<T, V>(to + (size_t)(c0 + u * lanes) * V, to_words<T, V>(sum[u]));
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * lanes < pieces) store_words<T, V>(to + (size_t)(c0 + u * lanes) * V, to_words<T, V>(sum[ALL ? 0 : u]));
+  }
 }
 
 // A warp a token: its row of dout stays in registers (while it fits) against the rows of all its choices, each read and written once.
@@ -307,13 +321,29 @@ TB200_API int tb200_expert_combine(const void* d_rows, size_t rows_stride, const
     auto go = [&](auto vv, auto wv) -> int {
       constexpr int V = decltype(vv)::value;
       if (dim >= (1ull << 31)) return ERR_INVALID;
-      const unsigned pieces = (unsigned)(dim / V), spread = spread_of((pieces + COMBINE_U - 1) / COMBINE_U, 5);
-      const unsigned parts = (unsigned)(((size_t)pieces + (COMBINE_U << spread) - 1) / (COMBINE_U << spread));
-      const size_t grid = (((n * parts) << spread) + 255) / 256;
-      if (grid > 0x7fffffffull) return ERR_INVALID;
-      expert_combine_kernel<T, V, decltype(wv)::value><<<(unsigned)grid, 256, 0, stream>>>(static_cast<const T*>(d_rows), rows_stride, (unsigned)(n * choices), d_slots, d_weights, n,
-                                                                                         (unsigned)choices, pieces, spread, parts, static_cast<T*>(d_out));
-      return (int)cudaGetLastError();
+      const unsigned pieces = (unsigned)(dim / V);
+      auto run = [&](auto kk, auto uu, auto all) -> int {
+        constexpr int K = decltype(kk)::value, U = decltype(uu)::value;
+        const unsigned spread = spread_of((pieces + U - 1) / U, 5), parts = (unsigned)(((size_t)pieces + (U << spread) - 1) / (U << spread));
+        const size_t grid = (((n * parts) << spread) + 255) / 256;
+        if (grid > 0x7fffffffull) return ERR_INVALID;
+        expert_combine_kernel<T, V, decltype(wv)::value, K, U, decltype(all)::value><<<(unsigned)grid, 256, 0, stream>>>(
+            static_cast<const T*>(d_rows), rows_stride, (unsigned)(n * choices), d_slots, d_weights, n, (unsigned)choices, pieces, spread, parts, static_cast<T*>(d_out));
+        return (int)cudaGetLastError();
+      };
+      using std::integral_constant;
+      // 16-byte pieces, four to eight reads a thread.  8191 x 2 f16 rows of 4096: 34 us (two rows at a time with their sums held: 39, eight reads with four sums: 45);
+      // 8192 x 8 bf16 rows of 2048: 50 (two at a time: 52); 16384 x 1 of 4096: 45 (62).  Channel by channel two of eight rows at a time are faster than all of
+      // them: 8192 x 4 bf16 rows of 1501: 44 us against 72.
+      if constexpr (V > 1) {
+        if (choices == 1) return run(integral_constant<int, 1>(), integral_constant<int, 4>(), std::true_type());
+        if (choices == 2) return run(integral_constant<int, 2>(), integral_constant<int, 2>(), std::true_type());
+        if (choices <= 4) return run(integral_constant<int, 4>(), integral_constant<int, 2>(), std::true_type());
+        if (choices <= 8) return run(integral_constant<int, 8>(), integral_constant<int, 1>(), std::true_type());
+        return run(integral_constant<int, 2>(), integral_constant<int, 2>(), std::false_type());
+      } else {
+        return run(integral_constant<int, 2>(), integral_constant<int, 4>(), std::false_type());
+      }
     };
     auto with = [&](auto vv) -> int { return d_weights ? go(vv, std::true_type()) : go(vv, std::false_type()); };
     if (in_16_bytes(d_rows, dim, rows_stride, sizeof(T)) && in_16_bytes(d_out, dim, dim, sizeof(T))) return with(std::integral_constant<int, 16 / sizeof(T)>());
