@@ -416,12 +416,14 @@ __device__ __forceinline__ bool wait_met(unsigned long long* bar, unsigned parit
 __device__ __forceinline__ f2 nan2() { return pack2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff)); }
 
 // The pairs of a warp's rows, once they are known, and the state before its rows, once that is.
+// where the shared memory of the CTAs lies that this warp sends to: every fourth one
+struct peers { static constexpr int N = MOST_CTAS / 4; unsigned base[N]; };
 struct link { duo before, total; };       // of the CTA: what comes before this warp's rows, all of it
 
 // All threads of the CTA, with their warps' pairs of window w; `cut`: whether this warp's is one.  after_sync: run once every warp is done with
 // its tiles.  Also sends the CTA's pair to the cluster.
 template <class Shared, int WARPS, bool CUTS>
-__device__ __forceinline__ link join_warps(Shared& sh, size_t w, const duo& own, bool cut, unsigned rank, unsigned ctas) {
+__device__ __forceinline__ link join_warps(Shared& sh, unsigned w, const duo& own, bool cut, unsigned rank, unsigned ctas, const peers& to) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   sh.warp[w & 1][warp][lane] = own;
   const bool some = CUTS ? __syncthreads_or(cut) != 0 : (__syncthreads(), false);
@@ -443,10 +445,12 @@ __device__ __forceinline__ link join_warps(Shared& sh, size_t w, const duo& own,
   }
   l.total = f;
   if (ctas > 1) {
-    const int buffer = (int)(w % MEETINGS);
+    const unsigned buffer = w % MEETINGS;
     if (threadIdx.x == 0) tb200::mbar_arrive_expect(&sh.met[buffer], ctas * 32 * (unsigned)sizeof(duo));
-    const unsigned at = tb200::smem_addr(sh.pairs() + ((size_t)buffer * pair_slots(ctas) + rank) * 32 + lane), bar = tb200::smem_addr(&sh.met[buffer]);
-    for (unsigned c = warp; c < ctas; c += WARPS) send_duo(tb200::cluster_addr(at, c), f, tb200::cluster_addr(bar, c));
+    const unsigned base = tb200::smem_addr(&sh), at = tb200::smem_addr(sh.pairs() + (buffer * pair_slots(ctas) + rank) * 32 + lane) - base, bar = tb200::smem_addr(&sh.met[buffer]) - base;
+#pragma unroll
+    for (int k = 0; k < peers::N; ++k)
+      if (warp + k * WARPS < (int)ctas) send_duo(to.base[k] + at, f, to.base[k] + bar);
   }
   return l;
 }
@@ -459,7 +463,7 @@ template <class Shared> __device__ __forceinline__ void no_pairs_behind(Shared& 
 // The state before this warp's rows of window w; `carry` goes from before the window to behind it.  false: the cluster's pairs did not come.
 // A CTA sends window w + 1 when it has everything of w - 1, which others sent when they were done with w - 3: four buffers.
 template <class Shared, bool CUTS>
-__device__ __forceinline__ bool join_ctas(Shared& sh, size_t w, const link& l, f2& carry, f2& q, unsigned rank, unsigned ctas) {
+__device__ __forceinline__ bool join_ctas(Shared& sh, unsigned w, const link& l, f2& carry, f2& q, unsigned rank, unsigned ctas) {
   if (ctas == 1) {
     q = follow<CUTS>(carry, l.before);
     carry = follow<CUTS>(carry, l.total);
@@ -526,21 +530,25 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
   const unsigned item = blockIdx.x / ctas;
   const size_t chain = item / slices, c = (size_t)(item % slices) * 64 + lane * 2, first = chain * length;
   const bool there = c < dim;
-  const size_t window = (size_t)ctas * R, windows = (length + window - 1) / window;
+  const size_t window = (size_t)ctas * R;
+  const unsigned windows = (unsigned)((length + window - 1) / window);
   const size_t p0 = ((size_t)rank * WARPS + warp) * ROWS;       // this warp's first position in window 0
-  auto load = [&](size_t w) {       // the CTA's tiles of window w
-    const size_t row = w * window + (size_t)rank * R;
-    if (w >= windows || row >= length) return;
+  // the CTA has a tile in `tiles` windows
+  const unsigned tiles = length > (size_t)rank * R ? (unsigned)((length - (size_t)rank * R + window - 1) / window) : 0;
+  const int row0 = (int)(first + (size_t)rank * R), row_step = (int)window, channel0 = (int)(item % slices) * 64;
+  auto load = [&](unsigned w) {
+    if (w >= tiles) return;
     unsigned long long* const bar = &sh.full[w % STAGES];
+    const int row = row0 + (int)w * row_step;
     tb200::mbar_arrive_expect(bar, 2 * R * 64 * (unsigned)sizeof(T));
-    load_tile(sh.tile[w % STAGES][0], &x_map, (int)(item % slices) * 64, (int)(first + row), bar);
-    load_tile(sh.tile[w % STAGES][1], &gate_map, (int)(item % slices) * 64, (int)(first + row), bar);
+    load_tile(sh.tile[w % STAGES][0], &x_map, channel0, row, bar);
+    load_tile(sh.tile[w % STAGES][1], &gate_map, channel0, row, bar);
   };
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) tb200::mbar_init(&sh.full[i], 1);
     for (int i = 0; i < MEETINGS; ++i) tb200::mbar_init(&sh.met[i], 1);
     tb200::mbar_init_fence();
-    for (int i = 0; i < STAGES; ++i) load(i);
+    for (unsigned i = 0; i < (unsigned)STAGES; ++i) load(i);
   }
   auto state_of = [&](size_t s) -> f2 {
     if (!h0 || !there) return 0ull;
@@ -554,9 +562,13 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
   __syncthreads();
   if (ctas > 1) tb200::cluster_barrier();      // all CTAs have begun: their shared memory may be written
   bool good = true;
+  static_assert(WARPS == 4, "peers");
+  peers to;
+#pragma unroll
+  for (int k = 0; k < peers::N; ++k) to.base[k] = warp + k * WARPS < (int)ctas ? tb200::cluster_addr(tb200::smem_addr(&sh), warp + k * WARPS) : 0;
 
   struct held { f2 keep[ROWS], b[ROWS]; link l; unsigned cuts, ends; int id, rows; };
-  auto take = [&](held& s, size_t w) {
+  auto take = [&](held& s, unsigned w) {
     const size_t p = p0 + w * window;
     const int stage = (int)(w % STAGES);
     s.rows = p >= length ? 0 : length - p < (size_t)ROWS ? (int)(length - p) : ROWS;       // of this warp that there are
@@ -570,7 +582,7 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
       if (m.begins | m.ends) s.id = lane < ROWS && p + lane < length ? table.ids[p + lane] : 0;
       coming = read_marks(table, (long long)(p + window), (long long)length);
     }
-    if (w * window + (size_t)rank * R < length) good &= wait_tile(&sh.full[stage], (unsigned)(w / STAGES) & 1);
+    if (w < tiles) good &= wait_tile(&sh.full[stage], (unsigned)(w / STAGES) & 1);
     const T* const xt = &sh.tile[stage][0][warp * ROWS][lane * 2];
     const T* const gt = &sh.tile[stage][1][warp * ROWS][lane * 2];
     duo own = {pack2(1.f, 1.f), 0ull};
@@ -610,10 +622,10 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
       }
     }
     if (!good) own = {pack2(1.f, 1.f), nan2()};
-    s.l = join_warps<Shared, WARPS, PACKED>(sh, w, own, s.cuts != 0, rank, ctas);
+    s.l = join_warps<Shared, WARPS, PACKED>(sh, w, own, s.cuts != 0, rank, ctas, to);
     if (threadIdx.x == 0) load(w + STAGES);      // every warp has taken its rows from the tiles
   };
-  auto give = [&](held& s, size_t w) {
+  auto give = [&](held& s, unsigned w) {
     f2 q = 0ull;
     good &= join_ctas<Shared, PACKED>(sh, w, s.l, carry, q, rank, ctas);
     if (!good) { q = nan2(); s.cuts = 0; }
@@ -641,7 +653,7 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
     }
   };
   held s;
-  for (size_t w = 0; w < windows; ++w) { take(s, w); give(s, w); }
+  for (unsigned w = 0; w < windows; ++w) { take(s, w); give(s, w); }
   if (ctas > 1) tb200::cluster_barrier();      // nobody leaves while something may still be sent there
   if (!good && lane == 0) tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
   if (!PACKED && rank == 0 && warp == 0 && there) *reinterpret_cast<float2*>(last + chain * dim + c) = unpack2(carry);
@@ -663,24 +675,27 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
   const unsigned item = blockIdx.x / ctas;
   const size_t chain = item / slices, c = (size_t)(item % slices) * 64 + lane * 2, first = chain * length;
   const bool there = c < dim;
-  const size_t window = (size_t)ctas * R, windows = (length + window - 1) / window;
+  const size_t window = (size_t)ctas * R;
+  const unsigned windows = (unsigned)((length + window - 1) / window);
   const size_t p0 = ((size_t)rank * WARPS + warp) * ROWS;
-  auto load = [&](size_t w) {
-    const size_t p = w * window + (size_t)rank * R;      // the tile's position R - 1 is its first row, which may lie before the tensor
-    if (w >= windows || p >= length) return;
-    const int row = (int)((long long)first + (long long)length - (long long)p - R), channel = (int)(item % slices) * 64;
+  // the CTA has a tile in `tiles` windows; its position R - 1 is its first row, which may lie before the tensor
+  const unsigned tiles = length > (size_t)rank * R ? (unsigned)((length - (size_t)rank * R + window - 1) / window) : 0;
+  const int row0 = (int)((long long)first + (long long)length - (long long)rank * R - R), row_step = (int)window, channel0 = (int)(item % slices) * 64;
+  auto load = [&](unsigned w) {
+    if (w >= tiles) return;
     unsigned long long* const bar = &sh.full[w % STAGES];
+    const int row = row0 - (int)w * row_step;
     tb200::mbar_arrive_expect(bar, 4 * R * 64 * (unsigned)sizeof(T));
-    load_tile(sh.tile[w % STAGES][0], &dh_map, channel, row, bar);
-    load_tile(sh.tile[w % STAGES][1], &gate_map, channel, row, bar);
-    load_tile(sh.tile[w % STAGES][2], &x_map, channel, row, bar);
-    load_tile(sh.tile[w % STAGES][3], &h_map, channel, row - 1, bar);
+    load_tile(sh.tile[w % STAGES][0], &dh_map, channel0, row, bar);
+    load_tile(sh.tile[w % STAGES][1], &gate_map, channel0, row, bar);
+    load_tile(sh.tile[w % STAGES][2], &x_map, channel0, row, bar);
+    load_tile(sh.tile[w % STAGES][3], &h_map, channel0, row - 1, bar);
   };
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) tb200::mbar_init(&sh.full[i], 1);
     for (int i = 0; i < MEETINGS; ++i) tb200::mbar_init(&sh.met[i], 1);
     tb200::mbar_init_fence();
-    for (int i = 0; i < STAGES; ++i) load(i);
+    for (unsigned i = 0; i < (unsigned)STAGES; ++i) load(i);
   }
   auto state_of = [&](const float* from, size_t s) -> f2 {
     if (!from || !there) return 0ull;
@@ -695,9 +710,13 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
   __syncthreads();
   if (ctas > 1) tb200::cluster_barrier();
   bool good = true;
+  static_assert(WARPS == 4, "peers");
+  peers to;
+#pragma unroll
+  for (int k = 0; k < peers::N; ++k) to.base[k] = warp + k * WARPS < (int)ctas ? tb200::cluster_addr(tb200::smem_addr(&sh), warp + k * WARPS) : 0;
 
   struct held { f2 keep[ROWS], give[ROWS], d[ROWS], slope[ROWS]; link l; unsigned cuts, ends; int id, rows; };
-  auto take = [&](held& s, size_t w) {
+  auto take = [&](held& s, unsigned w) {
     const size_t p = p0 + w * window;
     const int stage = (int)(w % STAGES);
     s.rows = p >= length ? 0 : length - p < (size_t)ROWS ? (int)(length - p) : ROWS;
@@ -714,7 +733,7 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
     } else if (s.rows > 0 && p + s.rows == length) {
       s.ends = 1u << (s.rows - 1);           // the sequence's first row
     }
-    if (w * window + (size_t)rank * R < length) good &= wait_tile(&sh.full[stage], (unsigned)(w / STAGES) & 1);
+    if (w < tiles) good &= wait_tile(&sh.full[stage], (unsigned)(w / STAGES) & 1);
     const T* const dt = &sh.tile[stage][0][R - 1 - warp * ROWS][lane * 2];
     const T* const gt = &sh.tile[stage][1][R - 1 - warp * ROWS][lane * 2];
     const T* const xt = &sh.tile[stage][2][R - 1 - warp * ROWS][lane * 2];
@@ -765,10 +784,10 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
       }
     }
     if (!good) own = {pack2(1.f, 1.f), nan2()};
-    s.l = join_warps<Shared, WARPS, PACKED>(sh, w, own, s.cuts != 0, rank, ctas);
+    s.l = join_warps<Shared, WARPS, PACKED>(sh, w, own, s.cuts != 0, rank, ctas, to);
     if (threadIdx.x == 0) load(w + STAGES);      // every warp has taken its rows from the tiles
   };
-  auto give = [&](held& s, size_t w) {
+  auto give = [&](held& s, unsigned w) {
     f2 q = 0ull;
     good &= join_ctas<Shared, PACKED>(sh, w, s.l, carry, q, rank, ctas);
     if (!good) { q = nan2(); s.cuts = 0; }
@@ -806,7 +825,7 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
     }
   };
   held s;
-  for (size_t w = 0; w < windows; ++w) { take(s, w); give(s, w); }
+  for (unsigned w = 0; w < windows; ++w) { take(s, w); give(s, w); }
   if (ctas > 1) tb200::cluster_barrier();
   if (!good && lane == 0) tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
   if (!PACKED && rank == 0 && warp == 0 && there) *reinterpret_cast<float2*>(dh0 + chain * dim + c) = unpack2(carry);
