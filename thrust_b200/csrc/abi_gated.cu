@@ -556,8 +556,10 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
     return pack2(v.x, v.y);
   };
   f2 carry = PACKED ? 0ull : state_of(chain);
-  unsigned coming = 0;              // marks of the next window
-  if constexpr (PACKED) coming = read_marks(table, (long long)p0, (long long)length);
+  unsigned coming = 0;              // marks of the next window, and the ids of its rows, a lane a row
+  int next_id = 0;
+  auto id_at = [&](size_t p) -> int { return lane < ROWS && p + lane < length ? table.ids[p + lane] : 0; };
+  if constexpr (PACKED) { coming = read_marks(table, (long long)p0, (long long)length); next_id = id_at(p0); }
   if (ctas > 1) no_pairs_behind(sh, ctas);
   __syncthreads();
   if (ctas > 1) tb200::cluster_barrier();      // all CTAs have begun: their shared memory may be written
@@ -574,13 +576,16 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
     s.rows = p >= length ? 0 : length - p < (size_t)ROWS ? (int)(length - p) : ROWS;       // of this warp that there are
     s.cuts = s.ends = 0;
     unsigned begins = 0;
+    f2 start = 0ull;
     if constexpr (PACKED) {
       const marks m = marks_of<ROWS, false>(coming, (long long)p);
       s.cuts = m.begins | (~m.inside & ALL);
       s.ends = m.ends;
       begins = m.begins;
-      if (m.begins | m.ends) s.id = lane < ROWS && p + lane < length ? table.ids[p + lane] : 0;
+      s.id = next_id;
+      if (begins) start = state_of((size_t)__shfl_sync(tb200::FULL_MASK, s.id, __ffs(begins) - 1));      // on its way while the gates are worked out
       coming = read_marks(table, (long long)(p + window), (long long)length);
+      next_id = id_at(p + window);
     }
     if (w < tiles) good &= wait_tile(&sh.full[stage], (unsigned)(w / STAGES) & 1);
     const T* const xt = &sh.tile[stage][0][warp * ROWS][lane * 2];
@@ -606,7 +611,8 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
       for (int i = 0; i < ROWS; ++i)
         if (s.cuts >> i & 1) {
           if (begins >> i & 1) {
-            s.b[i] = fma2(s.keep[i], state_of((size_t)__shfl_sync(tb200::FULL_MASK, s.id, i)), s.b[i]);
+            if (begins & ((1u << i) - 1)) start = state_of((size_t)__shfl_sync(tb200::FULL_MASK, s.id, i));
+            s.b[i] = fma2(s.keep[i], start, s.b[i]);
           } else {
             s.keep[i] = s.b[i] = 0ull;
           }
@@ -705,7 +711,13 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
   f2 carry = PACKED ? 0ull : state_of(dlast, chain);
   const f2 initial = PACKED ? 0ull : state_of(h0, chain);
   unsigned coming = 0;
-  if constexpr (PACKED) coming = read_marks(table, (long long)length - (long long)p0 - ROWS, (long long)length);
+  int next_id = 0;
+  auto id_at = [&](long long row) -> int { const long long at = row + ROWS - 1 - lane; return lane < ROWS && at >= 0 && at < (long long)length ? table.ids[at] : 0; };
+  if constexpr (PACKED) {
+    const long long row = (long long)length - (long long)p0 - ROWS;
+    coming = read_marks(table, row, (long long)length);
+    next_id = id_at(row);
+  }
   if (ctas > 1) no_pairs_behind(sh, ctas);
   __syncthreads();
   if (ctas > 1) tb200::cluster_barrier();
@@ -722,14 +734,18 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
     s.rows = p >= length ? 0 : length - p < (size_t)ROWS ? (int)(length - p) : ROWS;
     s.cuts = s.ends = 0;
     unsigned begins = 0;
+    f2 start = 0ull, from = initial;
     if constexpr (PACKED) {
       const long long row = (long long)length - (long long)p - ROWS;       // of the last position
       const marks m = marks_of<ROWS, true>(coming, row);
       s.cuts = m.begins | (~m.inside & ALL);
       s.ends = m.ends;
       begins = m.begins;
-      if (m.begins | m.ends) { const long long at = row + ROWS - 1 - lane; s.id = lane < ROWS && at >= 0 ? table.ids[at] : 0; }
+      s.id = next_id;
+      if (begins) start = state_of(dlast, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, __ffs(begins) - 1));
+      if (s.ends) from = state_of(h0, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, __ffs(s.ends) - 1));
       coming = read_marks(table, row - (long long)window, (long long)length);
+      next_id = id_at(row - (long long)window);
     } else if (s.rows > 0 && p + s.rows == length) {
       s.ends = 1u << (s.rows - 1);           // the sequence's first row
     }
@@ -753,7 +769,7 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
 #pragma unroll
       for (int i = 0; i < ROWS; ++i)
         if (s.ends >> i & 1) {
-          const f2 from = PACKED ? state_of(h0, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, i)) : initial;
+          if (s.ends & ((1u << i) - 1)) from = state_of(h0, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, i));
           const float2 xv = two_channels(xt - i * 64);
           s.slope[i] = mul2(mul2(s.keep[i], s.give[i]), fma2(pack2(xv.x, xv.y), minus, from));
         }
@@ -768,7 +784,8 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
       for (int i = 0; i < ROWS; ++i)
         if (s.cuts >> i & 1) {
           if (begins >> i & 1) {
-            s.d[i] = add2(s.d[i], state_of(dlast, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, i)));
+            if (begins & ((1u << i) - 1)) start = state_of(dlast, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, i));
+            s.d[i] = add2(s.d[i], start);
           } else {
             s.keep[i] = s.give[i] = s.d[i] = s.slope[i] = 0ull;
           }
