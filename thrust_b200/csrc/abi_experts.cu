@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_count_kernel(const I* i
 template <class V, class I, bool COUNTED>
 __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V* __restrict__ x, size_t xs, const I* __restrict__ ids, size_t n, unsigned choices, unsigned experts,
                                                                        size_t pieces, unsigned spread, V* __restrict__ rows, int* slots, int* sources, int* offsets,
-                                                                       const unsigned* __restrict__ table) {
+                                                                       const unsigned* __restrict__ table, tb200::ws_header* hdr) {
   extern __shared__ unsigned raw[];
   const unsigned warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   unsigned* const total = raw;                    // [experts]
@@ -96,7 +96,10 @@ __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V
       }
       sum += __shfl_sync(tb200::FULL_MASK, inclusive, 31);
     }
-    if (lane == 0) { kept = sum; if (blockIdx.x == 0) offsets[experts] = (int)sum; }
+    if (lane == 0) {
+      kept = sum;
+      if (blockIdx.x == 0) { offsets[experts] = (int)sum; hdr->error = 0; }      // nothing here waits
+    }
   }
   __syncthreads();
   for (unsigned e = threadIdx.x; e < experts; e += blockDim.x) {
@@ -298,9 +301,10 @@ TB200_API int tb200_expert_dispatch(const void* d_x, size_t x_stride, const void
         const size_t scale = sizeof(V) / sizeof(T);
         if (COUNTED)      // begins while the blocks are still counted, and waits for that
           return (int)tb200::launch_after(kernel, grid, block, smem, stream, static_cast<const V*>(d_x), x_stride / scale, static_cast<const I*>(d_experts), n, (unsigned)choices, experts,
-                                          dim / scale, spread_of(dim / scale, 5), static_cast<V*>(d_rows), d_slots, d_sources, d_offsets, table);
+                                          dim / scale, spread_of(dim / scale, 5), static_cast<V*>(d_rows), d_slots, d_sources, d_offsets, table,
+                                          static_cast<tb200::ws_header*>(d_ws));
         kernel<<<grid, block, smem, stream>>>(static_cast<const V*>(d_x), x_stride / scale, static_cast<const I*>(d_experts), n, (unsigned)choices, experts, dim / scale,
-                                              spread_of(dim / scale, 5), static_cast<V*>(d_rows), d_slots, d_sources, d_offsets, table);
+                                              spread_of(dim / scale, 5), static_cast<V*>(d_rows), d_slots, d_sources, d_offsets, table, static_cast<tb200::ws_header*>(d_ws));
         return (int)cudaGetLastError();
       };
       auto with = [&](auto vv) -> int { return counted ? go(vv, std::true_type()) : go(vv, std::false_type()); };

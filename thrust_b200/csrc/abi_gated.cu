@@ -24,308 +24,27 @@ __device__ __forceinline__ gate_pair open_gate(float g) {
 
 // ---------------------------------------------------------------------------------------------- scan by clusters
 // A chain of rows (a sequence; packed sequences are one chain that is cut at their ends) is walked in windows by a cluster of CTAs, one
-// chain and one slice of channels each.  A lane has V neighbouring channels and ROWS neighbouring positions of a window in registers:
+// chain and one slice of 64 channels each.  A lane has two neighbouring channels and ROWS neighbouring positions of a window in registers:
 // position p is row p, or row length - 1 - p in the backward pass, so that both go the same way.  Over those positions a state q
-// becomes A q + B in each channel.  The warps' pairs meet in shared memory, the CTAs' in the shared memory of every CTA of the cluster, each
+// becomes A q + B in each channel.  The warps' pairs (A, B) meet in shared memory, the CTAs' in the shared memory of every CTA of the cluster, each
 // thread folds what comes before its rows onto the carry of the window, and only then walks its rows again.  So each
-// input is read once and each output written once; the rows of the next window are on their way meanwhile.  Pairs are
-// folded in the order of their positions: the same inputs give the same bits.
+// input is read once and each output written once.  Pairs are folded in the order of their positions: the same inputs give the same bits.
+// States, pairs and sums are 32 bits; h, dx and dgate are rounded to the rows' type where they are stored, and nowhere before.
 //
 // A cut (a sequence begins there) makes a pair that forgets what came before: A is CUT instead of a product, and is selected on, not
 // multiplied with, so that NaNs and infinities of one sequence do not reach the next.
-constexpr float CUT = -1.f;
-constexpr int SCAN_WARPS = 8;
-constexpr int SCAN_BLOCK = SCAN_WARPS * 32;
-
-struct pair2 { float a, b; };
-template <bool CUTS> __device__ __forceinline__ float follow(float q, pair2 f) { return CUTS && f.a == CUT ? f.b : fmaf(f.a, q, f.b); }
-// first f, then g
-template <bool CUTS> __device__ __forceinline__ pair2 join(pair2 f, pair2 g) {
-  if (CUTS && g.a == CUT) return g;
-  pair2 r;
-  r.a = CUTS && f.a == CUT ? CUT : f.a * g.a;
-  r.b = fmaf(g.a, f.b, g.b);
-  return r;
-}
-
-template <int V> struct scan_shared {
-  pair2 warp[2][SCAN_WARPS][32 * V];
-  pair2 cta[2][tb200::CLUSTER_MAX_CTAS][32 * V];
-};
-
-// All threads: `own` are this thread's pairs.  Returns in `q` the state before its rows and brings `carry` from before the window to behind it.
-template <int V, bool CUTS>
-__device__ __forceinline__ void exchange(scan_shared<V>& sh, int parity, const pair2 (&own)[V], float (&carry)[V], float (&q)[V], unsigned rank, unsigned ctas) {
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
-#pragma unroll
-  for (int v = 0; v < V; ++v) sh.warp[parity][warp][lane * V + v] = own[v];
-  __syncthreads();
-  if (ctas == 1) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float c = carry[v];
-      for (int w = 0; w < warps; ++w) {
-        if (w == warp) q[v] = c;
-        c = follow<CUTS>(c, sh.warp[parity][w][lane * V + v]);
-      }
-      carry[v] = c;
-    }
-    return;
-  }
-  pair2 before[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    pair2 f = {1.f, 0.f};
-    for (int w = 0; w < warps; ++w) {
-      if (w == warp) before[v] = f;
-      f = join<CUTS>(f, sh.warp[parity][w][lane * V + v]);
-    }
-    // every warp has the CTA's pair: they take the cluster's CTAs in turn
-    for (unsigned c = warp; c < ctas; c += warps) tb200::cluster_store(tb200::cluster_addr(tb200::smem_addr(&sh.cta[parity][rank][lane * V + v]), c), f);
-  }
-  tb200::cluster_barrier();
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float c = carry[v];
-    for (unsigned r = 0; r < ctas; ++r) {
-      if (r == rank) q[v] = follow<CUTS>(c, before[v]);
-      c = follow<CUTS>(c, sh.cta[parity][r][lane * V + v]);
-    }
-    carry[v] = c;
-  }
-}
-
-// What the ids of packed rows say about the positions of a warp, a bit each: ids[r] is the sequence of row r or -1.
-struct row_marks { unsigned inside, begins, ends; };
-// position p is row first + step * p; rows outside [0, n) are in no sequence
-__device__ __forceinline__ row_marks read_marks(const int* ids, long long row, int step, long long n) {
-  const int lane = threadIdx.x % 32;
-  const long long at = row + (long long)step * (lane - 1);      // lane i: position i - 1
-  const int id = at >= 0 && at < n ? ids[at] : -1;
-  const int before = __shfl_up_sync(tb200::FULL_MASK, id, 1), after = __shfl_down_sync(tb200::FULL_MASK, id, 1);
-  row_marks m;
-  m.inside = __ballot_sync(tb200::FULL_MASK, id >= 0) >> 1;
-  m.begins = __ballot_sync(tb200::FULL_MASK, id >= 0 && before != id) >> 1;
-  m.ends = __ballot_sync(tb200::FULL_MASK, id >= 0 && after != id) >> 1;
-  return m;
-}
-
-template <class T, int V, int ROWS, bool PACKED>
-__global__ void __launch_bounds__(SCAN_BLOCK, 2)
-gated_scan_kernel(const T* __restrict__ x, size_t xs, const T* __restrict__ gate, size_t gs, const float* __restrict__ h0, const int* __restrict__ ids, unsigned slices,
-                  size_t length, size_t dim, T* __restrict__ h, float* __restrict__ last) {
-  static_assert(ROWS <= 30, "a warp reads the ids of its positions and of their neighbours");
-  using P = words<T, V>;
-  __shared__ scan_shared<V> sh;
-  const unsigned ctas = tb200::cluster_size(), rank = tb200::cluster_rank();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
-  const unsigned item = blockIdx.x / ctas;
-  const size_t chain = item / slices, c = ((size_t)(item % slices) * 32 + lane) * V, first = chain * length;
-  const bool there = c < dim;
-  const size_t window = (size_t)ctas * warps * ROWS;
-  const size_t windows = (length + window - 1) / window;
-  size_t p = ((size_t)rank * warps + warp) * ROWS;      // this thread's first position in the window
-  P xr[ROWS], gr[ROWS];
-  auto load = [&](size_t p) {
-    const T* xp = x + (first + p) * xs + c;
-    const T* gp = gate + (first + p) * gs + c;
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i, xp += xs, gp += gs)
-      if (there && p + i < length) {
-        xr[i] = load_words<T, V>(xp);
-        gr[i] = load_words<T, V>(gp);
-      }
-  };
-  float carry[V], q[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) carry[v] = !PACKED && h0 && there ? h0[chain * dim + c + v] : 0.f;
-  load(p);
-  if (ctas > 1) tb200::cluster_barrier();      // all CTAs have begun: their shared memory may be written
-  for (size_t w = 0; w < windows; ++w, p += window) {
-    row_marks m = {~0u, 0u, 0u};
-    if constexpr (PACKED) m = read_marks(ids, (long long)p, 1, (long long)length);
-    float keep[ROWS][V], b[ROWS][V];
-    pair2 own[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) own[v] = {1.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const bool live = there && p + i < length;
-      float gv[V], xv[V];
-      channels(gr[i], gv);
-      channels(xr[i], xv);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const gate_pair g = open_gate(gv[v]);
-        keep[i][v] = live ? g.keep : 1.f;
-        b[i][v] = live ? g.give * xv[v] : 0.f;
-      }
-      if constexpr (PACKED) {
-        if (!(m.inside >> i & 1)) {          // no sequence's: zero, and nothing of the inputs
-#pragma unroll
-          for (int v = 0; v < V; ++v) { keep[i][v] = 0.f; b[i][v] = 0.f; own[v] = {CUT, 0.f}; }
-          continue;
-        }
-        if (m.begins >> i & 1) {
-          const int s = ids[p + i];
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            if (h0 && there) b[i][v] = fmaf(keep[i][v], h0[(size_t)s * dim + c + v], b[i][v]);
-            own[v] = {CUT, b[i][v]};
-          }
-          continue;
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        own[v].b = fmaf(keep[i][v], own[v].b, b[i][v]);
-        own[v].a = PACKED && own[v].a == CUT ? CUT : own[v].a * keep[i][v];
-      }
-    }
-    if (w + 1 < windows) load(p + window);
-    exchange<V, PACKED>(sh, (int)(w & 1), own, carry, q, rank, ctas);
-    T* hp = h + (first + p) * dim + c;
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const bool cut = PACKED && ((m.begins | ~m.inside) >> i & 1);
-        q[v] = cut ? b[i][v] : fmaf(keep[i][v], q[v], b[i][v]);
-      }
-      if (there && p + i < length) {
-        store_words<T, V>(hp + (size_t)i * dim, to_words<T, V>(q));
-        if (PACKED && (m.ends >> i & 1)) {
-          const int s = ids[p + i];
-#pragma unroll
-          for (int v = 0; v < V; ++v) last[(size_t)s * dim + c + v] = q[v];
-        }
-      }
-    }
-  }
-  if (!PACKED && rank == 0 && warp == 0 && there) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) last[chain * dim + c + v] = carry[v];
-  }
-}
-
-// The backward pass.  With q = a s handed from a row to the one before it: s = dh + q, q' = keep s, dx = give s,
-// dgate = keep give (h' - x) s, where h' is the state before the row.
-template <class T, int V, int ROWS, bool PACKED>
-__global__ void __launch_bounds__(SCAN_BLOCK, 2)
-gated_scan_grad_kernel(const T* __restrict__ dh, size_t ds, const T* __restrict__ x, size_t xs, const T* __restrict__ gate, size_t gs, const T* __restrict__ h, size_t hs,
-                       const float* __restrict__ h0, const float* __restrict__ dlast, const int* __restrict__ ids, unsigned slices, size_t length, size_t dim, T* __restrict__ dx,
-                       T* __restrict__ dgate, float* __restrict__ dh0) {
-  using P = words<T, V>;
-  __shared__ scan_shared<V> sh;
-  const unsigned ctas = tb200::cluster_size(), rank = tb200::cluster_rank();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
-  const unsigned item = blockIdx.x / ctas;
-  const size_t chain = item / slices, c = ((size_t)(item % slices) * 32 + lane) * V, first = chain * length;
-  const bool there = c < dim;
-  const size_t window = (size_t)ctas * warps * ROWS;
-  const size_t windows = (length + window - 1) / window;
-  size_t p = ((size_t)rank * warps + warp) * ROWS;
-  P dr[ROWS], gr[ROWS], xr[ROWS], hr[ROWS];
-  auto load = [&](size_t p) {
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-      if (there && p + i < length) {
-        const size_t row = first + (length - 1 - (p + i));
-        dr[i] = load_words<T, V>(dh + row * ds + c);
-        gr[i] = load_words<T, V>(gate + row * gs + c);
-        xr[i] = load_words<T, V>(x + row * xs + c);
-        if (row > first) hr[i] = load_words<T, V>(h + (row - 1) * hs + c);
-      }
-  };
-  float carry[V], q[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) carry[v] = !PACKED && dlast && there ? dlast[chain * dim + c + v] : 0.f;
-  load(p);
-  if (ctas > 1) tb200::cluster_barrier();
-  for (size_t w = 0; w < windows; ++w, p += window) {
-    const long long row = (long long)length - 1 - (long long)p;       // of position p, inside the chain
-    row_marks m = {~0u, 0u, 0u};
-    if constexpr (PACKED) m = read_marks(ids, row, -1, (long long)length);
-    float keep[ROWS][V], give[ROWS][V], d[ROWS][V], diff[ROWS][V];
-    pair2 own[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) own[v] = {1.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const bool live = there && p + i < length;
-      const bool initial = PACKED ? (m.ends >> i & 1) != 0 : (size_t)i + p + 1 == length;      // the row before is none of this sequence
-      const int s = PACKED ? (live && (m.inside >> i & 1) ? ids[row - i] : 0) : (int)chain;
-      float gv[V], xv[V], dv[V], hv[V];
-      channels(gr[i], gv);
-      channels(xr[i], xv);
-      channels(dr[i], dv);
-      channels(hr[i], hv);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const gate_pair g = open_gate(gv[v]);
-        keep[i][v] = live ? g.keep : 1.f;
-        give[i][v] = g.give;
-        d[i][v] = live ? dv[v] : 0.f;
-        const float before = initial ? (h0 && live ? h0[(size_t)s * dim + c + v] : 0.f) : hv[v];
-        diff[i][v] = before - xv[v];
-      }
-      if constexpr (PACKED) {
-        if (!(m.inside >> i & 1)) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) { keep[i][v] = give[i][v] = d[i][v] = diff[i][v] = 0.f; own[v] = {CUT, 0.f}; }
-          continue;
-        }
-        if (m.begins >> i & 1) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            if (dlast && live) d[i][v] += dlast[(size_t)s * dim + c + v];
-            own[v] = {CUT, keep[i][v] * d[i][v]};
-          }
-          continue;
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        own[v].b = keep[i][v] * (own[v].b + d[i][v]);
-        own[v].a = PACKED && own[v].a == CUT ? CUT : own[v].a * keep[i][v];
-      }
-    }
-    if (w + 1 < windows) load(p + window);
-    exchange<V, PACKED>(sh, (int)(w & 1), own, carry, q, rank, ctas);
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      float ox[V], og[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const bool cut = PACKED && ((m.begins | ~m.inside) >> i & 1);
-        const float s = cut ? d[i][v] : d[i][v] + q[v];
-        q[v] = keep[i][v] * s;
-        const float in = give[i][v] * s;
-        ox[v] = in;
-        og[v] = keep[i][v] * diff[i][v] * in;
-      }
-      if (there && p + i < length) {
-        const size_t at = (first + (size_t)(row - i)) * dim + c;
-        store_words<T, V>(dx + at, to_words<T, V>(ox));
-        store_words<T, V>(dgate + at, to_words<T, V>(og));
-        if (PACKED && (m.ends >> i & 1)) {
-          const int s = ids[row - i];
-#pragma unroll
-          for (int v = 0; v < V; ++v) dh0[(size_t)s * dim + c + v] = q[v];
-        }
-      }
-    }
-  }
-  if (!PACKED && rank == 0 && warp == 0 && there) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) dh0[chain * dim + c + v] = carry[v];
-  }
-}
-
-// ---------------------------------------------------------------------------------------------- the same from tiles in shared memory
+//
 // Where rows are made of whole 16-byte pieces, the copy engine brings a CTA's tiles (WARPS * ROWS rows of 64 channels of each input) into a
-// ring of STAGES stages while earlier windows are worked on, and a lane takes its two channels of a row from there in one access.
-// Two channels go through the arithmetic side by side (f32x2).
+// ring of STAGES stages while earlier windows are worked on, and a lane takes its two channels of a row from there in one access.  Other rows (STAGES
+// = 0) are read channel by channel where they are needed.  Two channels go through the arithmetic side by side (f32x2).
+//
+// What bounds it: with one CTA a chain the bytes (8 x 4096 bf16 rows of 2048: 81 us, 4960 GB/s; their gradient 142 us, 5670 GB/s).  Where a cluster
+// shares a chain, the length of a window: the gates 860 cycles (two exponentials or reciprocals an element: the unit takes eight cycles for a warp's), the
+// pairs' way through the warps 330, to the other CTAs and back 400, the rows 350, of which two CTAs a SM hide a part of one another's (one sequence of 20011
+// bf16 rows of 2560 71 us, of 65537 f32 rows of 1024 171 us).  Taking the next window's gates before this one's pairs have come needs twice the
+// registers, and the CTA that has no room for them costs more than it saves (119 us and 196).
+constexpr float CUT = -1.f;
+
 using f2 = unsigned long long;
 __device__ __forceinline__ f2 pack2(float x, float y) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
 __device__ __forceinline__ float2 unpack2(f2 a) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a)); return r; }
@@ -335,10 +54,55 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1,
 __device__ __forceinline__ float exp2_of(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 __device__ __forceinline__ float one_over(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
-// two channels of a row
+// two channels of a row, in a tile
 template <class T> __device__ __forceinline__ float2 two_channels(const T* p) {
   const words<T, 2> w = load_words<T, 2>(p);
   return make_float2(channel<0>(w), channel<1>(w));
+}
+
+template <class T> struct rows_of { const T* at; size_t stride; };
+// A lane's channels of up to ROWS rows, channel by channel.  Channels past the last are read as the last, rows that are not there as nothing in
+// particular: no lane has a test of its own.
+template <class T, int ROWS, bool EMPTY> struct direct_rows {
+  T at[ROWS][2];
+  __device__ __forceinline__ void request(const rows_of<T>& from, size_t row, int rows, int step, size_t c, size_t dim) {
+    const size_t c0 = c < dim ? c : dim - 1;
+    const unsigned next = c + 1 < dim ? 1 : 0;
+    const T* q = from.at + row * from.stride + c0;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      if (i < rows) { at[i][0] = q[0]; at[i][1] = q[next]; }
+      q = step > 0 ? q + from.stride : q - from.stride;
+    }
+  }
+  __device__ __forceinline__ float2 get(int i) const { return make_float2(to_f32(at[i][0]), to_f32(at[i][1])); }
+};
+template <class T, int ROWS> struct direct_rows<T, ROWS, true> {};
+// a lane's part of a row of states or of a result; PAIRS: both channels are there or none, and lie on a boundary of two
+template <bool PAIRS> __device__ __forceinline__ f2 read_state(const float* p, bool first, bool second) {
+  if constexpr (PAIRS) {
+    if (!first) return 0ull;
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    return pack2(v.x, v.y);
+  } else {
+    return pack2(first ? p[0] : 0.f, second ? p[1] : 0.f);
+  }
+}
+template <bool PAIRS> __device__ __forceinline__ void write_state(float* p, float2 v, bool first, bool second) {
+  if constexpr (PAIRS) {
+    if (first) *reinterpret_cast<float2*>(p) = v;
+  } else {
+    if (first) p[0] = v.x;
+    if (second) p[1] = v.y;
+  }
+}
+template <bool PAIRS, class T> __device__ __forceinline__ void write_pair(T* p, const float (&v)[2], bool first, bool second) {
+  if constexpr (PAIRS) {
+    if (first) store_words<T, 2>(p, to_words<T, 2>(v));
+  } else {
+    if (first) p[0] = from_f32<T>(v[0]);
+    if (second) p[1] = from_f32<T>(v[1]);
+  }
 }
 
 // open_gate for two channels: e = exp(-g), keep = 1 / (1 + e), give = e keep.  An e past the largest number makes keep 0 and e keep a NaN, for which
@@ -356,7 +120,7 @@ __device__ __forceinline__ gates2 open_gates(float2 g) {
   return r;
 }
 
-struct duo { f2 a, b; };       // pair2 of two channels
+struct duo { f2 a, b; };       // q becomes a q + b, in two channels
 template <bool CUTS> __device__ __forceinline__ f2 follow(f2 q, duo f) {
   f2 r = fma2(f.a, q, f.b);
   if (CUTS) {
@@ -365,6 +129,7 @@ template <bool CUTS> __device__ __forceinline__ f2 follow(f2 q, duo f) {
   }
   return r;
 }
+// first f, then g
 template <bool CUTS> __device__ __forceinline__ duo join(duo f, duo g) {
   duo r = {mul2(f.a, g.a), fma2(g.a, f.b, g.b)};
   if (CUTS) {
@@ -379,12 +144,12 @@ constexpr int MOST_CTAS = tb200::CLUSTER_MAX_CTAS;
 constexpr int MEETINGS = 4;
 constexpr unsigned FEW_CTAS = 9;
 inline __host__ __device__ unsigned pair_slots(unsigned ctas) { return ctas > FEW_CTAS ? MOST_CTAS : FEW_CTAS; }
-constexpr int TILE_CTAS = 4;        // a SM
 template <class T, int WARPS, int ROWS, int INPUTS, int STAGES> struct tiles_shared {
   static constexpr int R = WARPS * ROWS;
-  alignas(128) T tile[STAGES][INPUTS][R][64];
+  static constexpr bool TILES = STAGES > 0;
+  alignas(128) T tile[TILES ? STAGES : 1][TILES ? INPUTS : 1][TILES ? R : 1][64];
   duo warp[2][WARPS][32];
-  unsigned long long full[STAGES], met[MEETINGS];
+  unsigned long long full[TILES ? STAGES : 1], met[MEETINGS];
   // behind it, where there is more than one CTA: the CTAs' pairs, [MEETINGS][pair_slots][32]
   static size_t bytes(unsigned ctas) { return tb200::align_up(sizeof(tiles_shared), 16) + (ctas > 1 ? MEETINGS * pair_slots(ctas) * 32 * sizeof(duo) : 0); }
   __device__ duo* pairs() { return reinterpret_cast<duo*>(reinterpret_cast<char*>(this) + (sizeof(tiles_shared) + 15) / 16 * 16); }
@@ -415,15 +180,14 @@ __device__ __forceinline__ bool wait_met(unsigned long long* bar, unsigned parit
 }
 __device__ __forceinline__ f2 nan2() { return pack2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff)); }
 
-// The pairs of a warp's rows, once they are known, and the state before its rows, once that is.
-// where the shared memory of the CTAs lies that this warp sends to: every fourth one
-struct peers { static constexpr int N = MOST_CTAS / 4; unsigned base[N]; };
+// where the shared memory of the CTAs lies that this warp sends to: one in WARPS (a single warp is a CTA that has no others)
+template <int WARPS> struct peers { static constexpr int N = WARPS == 1 ? 1 : MOST_CTAS / WARPS; unsigned base[N]; };
 struct link { duo before, total; };       // of the CTA: what comes before this warp's rows, all of it
 
-// All threads of the CTA, with their warps' pairs of window w; `cut`: whether this warp's is one.  after_sync: run once every warp is done with
-// its tiles.  Also sends the CTA's pair to the cluster.
+// All threads of the CTA, with their warps' pairs of window w; `cut`: whether this warp's is one.  Behind it every warp is done with its tiles.
+// Also sends the CTA's pair to the cluster.
 template <class Shared, int WARPS, bool CUTS>
-__device__ __forceinline__ link join_warps(Shared& sh, unsigned w, const duo& own, bool cut, unsigned rank, unsigned ctas, const peers& to) {
+__device__ __forceinline__ link join_warps(Shared& sh, unsigned w, const duo& own, bool cut, unsigned rank, unsigned ctas, const peers<WARPS>& to) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   sh.warp[w & 1][warp][lane] = own;
   const bool some = CUTS ? __syncthreads_or(cut) != 0 : (__syncthreads(), false);
@@ -449,7 +213,7 @@ __device__ __forceinline__ link join_warps(Shared& sh, unsigned w, const duo& ow
     if (threadIdx.x == 0) tb200::mbar_arrive_expect(&sh.met[buffer], ctas * 32 * (unsigned)sizeof(duo));
     const unsigned base = tb200::smem_addr(&sh), at = tb200::smem_addr(sh.pairs() + (buffer * pair_slots(ctas) + rank) * 32 + lane) - base, bar = tb200::smem_addr(&sh.met[buffer]) - base;
 #pragma unroll
-    for (int k = 0; k < peers::N; ++k)
+    for (int k = 0; k < peers<WARPS>::N; ++k)
       if (warp + k * WARPS < (int)ctas) send_duo(to.base[k] + at, f, to.base[k] + bar);
   }
   return l;
@@ -516,8 +280,8 @@ template <int ROWS, bool BACKWARD> __device__ __forceinline__ marks marks_of(uns
 }
 
 template <class T, int WARPS, int ROWS, int STAGES, bool PACKED>
-__global__ void __launch_bounds__(WARPS * 32, PACKED ? 3 : 4)
-gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap gate_map, const float* __restrict__ h0, row_table table, unsigned slices,
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 1 ? 10 : STAGES == 0 ? 2 : PACKED ? 3 : 4)
+gated_scan_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap gate_map, rows_of<T> x, rows_of<T> gate, const float* __restrict__ h0, row_table table, unsigned slices,
                    size_t length, size_t dim, T* __restrict__ h, float* __restrict__ last, tb200::ws_header* hdr) {
   static_assert(ROWS <= 32, "a lane holds the id of a position");
   using Shared = tiles_shared<T, WARPS, ROWS, 2, STAGES>;
@@ -529,7 +293,8 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const unsigned item = blockIdx.x / ctas;
   const size_t chain = item / slices, c = (size_t)(item % slices) * 64 + lane * 2, first = chain * length;
-  const bool there = c < dim;
+  constexpr bool TILES = STAGES > 0;
+  const bool there = c < dim, both = TILES ? there : c + 1 < dim;      // its channels
   const size_t window = (size_t)ctas * R;
   const unsigned windows = (unsigned)((length + window - 1) / window);
   const size_t p0 = ((size_t)rank * WARPS + warp) * ROWS;       // this warp's first position in window 0
@@ -537,24 +302,23 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
   const unsigned tiles = length > (size_t)rank * R ? (unsigned)((length - (size_t)rank * R + window - 1) / window) : 0;
   const int row0 = (int)(first + (size_t)rank * R), row_step = (int)window, channel0 = (int)(item % slices) * 64;
   auto load = [&](unsigned w) {
+    if constexpr (!TILES) return;
+    constexpr unsigned S = TILES ? STAGES : 1;
     if (w >= tiles) return;
-    unsigned long long* const bar = &sh.full[w % STAGES];
+    unsigned long long* const bar = &sh.full[w % S];
     const int row = row0 + (int)w * row_step;
     tb200::mbar_arrive_expect(bar, 2 * R * 64 * (unsigned)sizeof(T));
-    load_tile(sh.tile[w % STAGES][0], &x_map, channel0, row, bar);
-    load_tile(sh.tile[w % STAGES][1], &gate_map, channel0, row, bar);
+    load_tile(sh.tile[w % S][0], &x_map, channel0, row, bar);
+    load_tile(sh.tile[w % S][1], &gate_map, channel0, row, bar);
   };
   if (threadIdx.x == 0) {
+    if (blockIdx.x == 0) hdr->error = 0;      // a wait that runs out does so long after this
     for (int i = 0; i < STAGES; ++i) tb200::mbar_init(&sh.full[i], 1);
     for (int i = 0; i < MEETINGS; ++i) tb200::mbar_init(&sh.met[i], 1);
     tb200::mbar_init_fence();
     for (unsigned i = 0; i < (unsigned)STAGES; ++i) load(i);
   }
-  auto state_of = [&](size_t s) -> f2 {
-    if (!h0 || !there) return 0ull;
-    const float2 v = *reinterpret_cast<const float2*>(h0 + s * dim + c);
-    return pack2(v.x, v.y);
-  };
+  auto state_of = [&](size_t s) -> f2 { return h0 ? read_state<TILES>(h0 + s * dim + c, there, both) : 0ull; };
   f2 carry = PACKED ? 0ull : state_of(chain);
   unsigned coming = 0;              // marks of the next window, and the ids of its rows, a lane a row
   int next_id = 0;
@@ -564,15 +328,15 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
   __syncthreads();
   if (ctas > 1) tb200::cluster_barrier();      // all CTAs have begun: their shared memory may be written
   bool good = true;
-  static_assert(WARPS == 4, "peers");
-  peers to;
+  peers<WARPS> to;
 #pragma unroll
-  for (int k = 0; k < peers::N; ++k) to.base[k] = warp + k * WARPS < (int)ctas ? tb200::cluster_addr(tb200::smem_addr(&sh), warp + k * WARPS) : 0;
+  for (int k = 0; k < peers<WARPS>::N; ++k) to.base[k] = warp + k * WARPS < (int)ctas ? tb200::cluster_addr(tb200::smem_addr(&sh), warp + k * WARPS) : 0;
 
   struct held { f2 keep[ROWS], b[ROWS]; link l; unsigned cuts, ends; int id, rows; };
   auto take = [&](held& s, unsigned w) {
     const size_t p = p0 + w * window;
-    const int stage = (int)(w % STAGES);
+    constexpr unsigned S = TILES ? STAGES : 1;
+    const unsigned stage = w % S;
     s.rows = p >= length ? 0 : length - p < (size_t)ROWS ? (int)(length - p) : ROWS;       // of this warp that there are
     s.cuts = s.ends = 0;
     unsigned begins = 0;
@@ -587,13 +351,21 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
       coming = read_marks(table, (long long)(p + window), (long long)length);
       next_id = id_at(p + window);
     }
-    if (w < tiles) good &= wait_tile(&sh.full[stage], (unsigned)(w / STAGES) & 1);
-    const T* const xt = &sh.tile[stage][0][warp * ROWS][lane * 2];
-    const T* const gt = &sh.tile[stage][1][warp * ROWS][lane * 2];
+    if (TILES && w < tiles) good &= wait_tile(&sh.full[stage], w / S & 1);
+    // the warp's rows of an input: in its tile, or all requested from where they lie
+    direct_rows<T, ROWS, TILES> rx, rg;
+    if constexpr (!TILES) {
+      rx.request(x, first + p, s.rows, 1, c, dim);
+      rg.request(gate, first + p, s.rows, 1, c, dim);
+    }
+    auto in = [&](int which, const direct_rows<T, ROWS, TILES>& from, int i) -> float2 {
+      if constexpr (TILES) return two_channels(&sh.tile[stage][which][warp * ROWS + i][lane * 2]);
+      else return from.get(i);
+    };
     duo own = {pack2(1.f, 1.f), 0ull};
     auto open = [&](int i) {
-      const gates2 g = open_gates(two_channels(gt + i * 64));
-      const float2 xv = two_channels(xt + i * 64);
+      const gates2 g = open_gates(in(1, rg, i));
+      const float2 xv = in(0, rx, i);
       s.keep[i] = g.keep;
       s.b[i] = mul2(g.give, pack2(xv.x, xv.y));
     };
@@ -642,7 +414,7 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
         q = fma2(s.keep[i], q, s.b[i]);
         const float2 v = unpack2(q);
         const float out[2] = {v.x, v.y};
-        if (there) store_words<T, 2>(hp, to_words<T, 2>(out));
+        write_pair<TILES>(hp, out, there, both);
       }
     } else {
 #pragma unroll
@@ -650,10 +422,10 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
         q = PACKED && (s.cuts >> i & 1) ? s.b[i] : fma2(s.keep[i], q, s.b[i]);
         const float2 v = unpack2(q);
         const float out[2] = {v.x, v.y};
-        if (there && i < s.rows) store_words<T, 2>(hp, to_words<T, 2>(out));
+        write_pair<TILES>(hp, out, there && i < s.rows, both && i < s.rows);
         if (PACKED && (s.ends >> i & 1)) {
           const int seq = __shfl_sync(tb200::FULL_MASK, s.id, i);
-          if (there) *reinterpret_cast<float2*>(last + (size_t)seq * dim + c) = v;
+          write_state<TILES>(last + (size_t)seq * dim + c, v, there, both);
         }
       }
     }
@@ -662,13 +434,13 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_const
   for (unsigned w = 0; w < windows; ++w) { take(s, w); give(s, w); }
   if (ctas > 1) tb200::cluster_barrier();      // nobody leaves while something may still be sent there
   if (!good && lane == 0) tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
-  if (!PACKED && rank == 0 && warp == 0 && there) *reinterpret_cast<float2*>(last + chain * dim + c) = unpack2(carry);
+  if (!PACKED && rank == 0 && warp == 0) write_state<TILES>(last + chain * dim + c, unpack2(carry), there, both);
 }
 
 template <class T, int WARPS, int ROWS, int STAGES, bool PACKED>
-__global__ void __launch_bounds__(WARPS * 32, PACKED ? 3 : 4)
-gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_constant__ CUtensorMap gate_map, const __grid_constant__ CUtensorMap x_map,
-                        const __grid_constant__ CUtensorMap h_map, const float* __restrict__ h0, const float* __restrict__ dlast, row_table table, unsigned slices,
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 1 ? 10 : STAGES == 0 ? 2 : PACKED ? 3 : 4)
+gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_constant__ CUtensorMap gate_map, const __grid_constant__ CUtensorMap x_map,
+                       const __grid_constant__ CUtensorMap h_map, rows_of<T> dh, rows_of<T> gate, rows_of<T> x, rows_of<T> h, const float* __restrict__ h0, const float* __restrict__ dlast, row_table table, unsigned slices,
                         size_t length, size_t dim, T* __restrict__ dx, T* __restrict__ dgate, float* __restrict__ dh0, tb200::ws_header* hdr) {
   static_assert(ROWS <= 32, "a lane holds the id of a position");
   using Shared = tiles_shared<T, WARPS, ROWS, 4, STAGES>;
@@ -680,7 +452,8 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const unsigned item = blockIdx.x / ctas;
   const size_t chain = item / slices, c = (size_t)(item % slices) * 64 + lane * 2, first = chain * length;
-  const bool there = c < dim;
+  constexpr bool TILES = STAGES > 0;
+  const bool there = c < dim, both = TILES ? there : c + 1 < dim;      // its channels
   const size_t window = (size_t)ctas * R;
   const unsigned windows = (unsigned)((length + window - 1) / window);
   const size_t p0 = ((size_t)rank * WARPS + warp) * ROWS;
@@ -688,26 +461,25 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
   const unsigned tiles = length > (size_t)rank * R ? (unsigned)((length - (size_t)rank * R + window - 1) / window) : 0;
   const int row0 = (int)((long long)first + (long long)length - (long long)rank * R - R), row_step = (int)window, channel0 = (int)(item % slices) * 64;
   auto load = [&](unsigned w) {
+    if constexpr (!TILES) return;
+    constexpr unsigned S = TILES ? STAGES : 1;
     if (w >= tiles) return;
-    unsigned long long* const bar = &sh.full[w % STAGES];
+    unsigned long long* const bar = &sh.full[w % S];
     const int row = row0 - (int)w * row_step;
     tb200::mbar_arrive_expect(bar, 4 * R * 64 * (unsigned)sizeof(T));
-    load_tile(sh.tile[w % STAGES][0], &dh_map, channel0, row, bar);
-    load_tile(sh.tile[w % STAGES][1], &gate_map, channel0, row, bar);
-    load_tile(sh.tile[w % STAGES][2], &x_map, channel0, row, bar);
-    load_tile(sh.tile[w % STAGES][3], &h_map, channel0, row - 1, bar);
+    load_tile(sh.tile[w % S][0], &dh_map, channel0, row, bar);
+    load_tile(sh.tile[w % S][1], &gate_map, channel0, row, bar);
+    load_tile(sh.tile[w % S][2], &x_map, channel0, row, bar);
+    load_tile(sh.tile[w % S][3], &h_map, channel0, row - 1, bar);
   };
   if (threadIdx.x == 0) {
+    if (blockIdx.x == 0) hdr->error = 0;      // a wait that runs out does so long after this
     for (int i = 0; i < STAGES; ++i) tb200::mbar_init(&sh.full[i], 1);
     for (int i = 0; i < MEETINGS; ++i) tb200::mbar_init(&sh.met[i], 1);
     tb200::mbar_init_fence();
     for (unsigned i = 0; i < (unsigned)STAGES; ++i) load(i);
   }
-  auto state_of = [&](const float* from, size_t s) -> f2 {
-    if (!from || !there) return 0ull;
-    const float2 v = *reinterpret_cast<const float2*>(from + s * dim + c);
-    return pack2(v.x, v.y);
-  };
+  auto state_of = [&](const float* from, size_t s) -> f2 { return from ? read_state<TILES>(from + s * dim + c, there, both) : 0ull; };
   f2 carry = PACKED ? 0ull : state_of(dlast, chain);
   const f2 initial = PACKED ? 0ull : state_of(h0, chain);
   unsigned coming = 0;
@@ -722,15 +494,15 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
   __syncthreads();
   if (ctas > 1) tb200::cluster_barrier();
   bool good = true;
-  static_assert(WARPS == 4, "peers");
-  peers to;
+  peers<WARPS> to;
 #pragma unroll
-  for (int k = 0; k < peers::N; ++k) to.base[k] = warp + k * WARPS < (int)ctas ? tb200::cluster_addr(tb200::smem_addr(&sh), warp + k * WARPS) : 0;
+  for (int k = 0; k < peers<WARPS>::N; ++k) to.base[k] = warp + k * WARPS < (int)ctas ? tb200::cluster_addr(tb200::smem_addr(&sh), warp + k * WARPS) : 0;
 
   struct held { f2 keep[ROWS], give[ROWS], d[ROWS], slope[ROWS]; link l; unsigned cuts, ends; int id, rows; };
   auto take = [&](held& s, unsigned w) {
     const size_t p = p0 + w * window;
-    const int stage = (int)(w % STAGES);
+    constexpr unsigned S = TILES ? STAGES : 1;
+    const unsigned stage = w % S;
     s.rows = p >= length ? 0 : length - p < (size_t)ROWS ? (int)(length - p) : ROWS;
     s.cuts = s.ends = 0;
     unsigned begins = 0;
@@ -749,17 +521,25 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
     } else if (s.rows > 0 && p + s.rows == length) {
       s.ends = 1u << (s.rows - 1);           // the sequence's first row
     }
-    if (w < tiles) good &= wait_tile(&sh.full[stage], (unsigned)(w / STAGES) & 1);
-    const T* const dt = &sh.tile[stage][0][R - 1 - warp * ROWS][lane * 2];
-    const T* const gt = &sh.tile[stage][1][R - 1 - warp * ROWS][lane * 2];
-    const T* const xt = &sh.tile[stage][2][R - 1 - warp * ROWS][lane * 2];
-    const T* const ht = &sh.tile[stage][3][R - 1 - warp * ROWS][lane * 2];
+    if (TILES && w < tiles) good &= wait_tile(&sh.full[stage], w / S & 1);
+    direct_rows<T, ROWS, TILES> rd, rg, rx, rh;
+    if constexpr (!TILES) {
+      const size_t row = first + (length - 1 - (s.rows ? p : 0));
+      rd.request(dh, row, s.rows, -1, c, dim);
+      rg.request(gate, row, s.rows, -1, c, dim);
+      rx.request(x, row, s.rows, -1, c, dim);
+      rh.request(h, row - 1, s.rows - (s.rows > 0 && p + s.rows == length), -1, c, dim);      // the state before the chain's first row is not among them
+    }
+    auto in = [&](int which, const direct_rows<T, ROWS, TILES>& from, int i) -> float2 {
+      if constexpr (TILES) return two_channels(&sh.tile[stage][which][R - 1 - warp * ROWS - i][lane * 2]);
+      else return from.get(i);
+    };
     const f2 minus = pack2(-1.f, -1.f);
     duo own = {pack2(1.f, 1.f), 0ull};
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const gates2 g = open_gates(two_channels(gt - i * 64));
-      const float2 dv = two_channels(dt - i * 64), xv = two_channels(xt - i * 64), hv = two_channels(ht - i * 64);
+      const gates2 g = open_gates(in(1, rg, i));
+      const float2 dv = in(0, rd, i), xv = in(2, rx, i), hv = in(3, rh, i);
       s.keep[i] = g.keep;
       s.give[i] = fma2(g.keep, 0ull, g.give);       // a NaN where the gate is one
       s.d[i] = pack2(dv.x, dv.y);
@@ -770,7 +550,7 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
       for (int i = 0; i < ROWS; ++i)
         if (s.ends >> i & 1) {
           if (s.ends & ((1u << i) - 1)) from = state_of(h0, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, i));
-          const float2 xv = two_channels(xt - i * 64);
+          const float2 xv = in(2, rx, i);
           s.slope[i] = mul2(mul2(s.keep[i], s.give[i]), fma2(pack2(xv.x, xv.y), minus, from));
         }
     }
@@ -818,10 +598,8 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
         q = mul2(s.keep[i], sum);
         const float2 a = unpack2(mul2(s.give[i], sum)), b = unpack2(mul2(s.slope[i], sum));
         const float oa[2] = {a.x, a.y}, ob[2] = {b.x, b.y};
-        if (there) {
-          store_words<T, 2>(xp, to_words<T, 2>(oa));
-          store_words<T, 2>(gp, to_words<T, 2>(ob));
-        }
+        write_pair<TILES>(xp, oa, there, both);
+        write_pair<TILES>(gp, ob, there, both);
       }
     } else {
 #pragma unroll
@@ -830,13 +608,11 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
         q = mul2(s.keep[i], sum);
         const float2 a = unpack2(mul2(s.give[i], sum)), b = unpack2(mul2(s.slope[i], sum));
         const float oa[2] = {a.x, a.y}, ob[2] = {b.x, b.y};
-        if (there && i < s.rows) {
-          store_words<T, 2>(xp, to_words<T, 2>(oa));
-          store_words<T, 2>(gp, to_words<T, 2>(ob));
-        }
+        write_pair<TILES>(xp, oa, there && i < s.rows, both && i < s.rows);
+        write_pair<TILES>(gp, ob, there && i < s.rows, both && i < s.rows);
         if (PACKED && (s.ends >> i & 1)) {
           const int seq = __shfl_sync(tb200::FULL_MASK, s.id, i);
-          if (there) *reinterpret_cast<float2*>(dh0 + (size_t)seq * dim + c) = unpack2(q);
+          write_state<TILES>(dh0 + (size_t)seq * dim + c, unpack2(q), there, both);
         }
       }
     }
@@ -845,13 +621,14 @@ gated_tiles_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid
   for (unsigned w = 0; w < windows; ++w) { take(s, w); give(s, w); }
   if (ctas > 1) tb200::cluster_barrier();
   if (!good && lane == 0) tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
-  if (!PACKED && rank == 0 && warp == 0 && there) *reinterpret_cast<float2*>(dh0 + chain * dim + c) = unpack2(carry);
+  if (!PACKED && rank == 0 && warp == 0) write_state<TILES>(dh0 + chain * dim + c, unpack2(carry), there, both);
 }
 
 // ids[r] = the sequence of row r, -1 if it is in none; bits[r / 32]: whether the rows are in one, begin one, end one.  A sequence without rows hands
 // its state (or its gradient) on.
 template <class I>
-__global__ void __launch_bounds__(256) row_table_kernel(const I* offsets, size_t batch, size_t n, int* ids, uint4* bits, const float* from, size_t dim, float* to) {
+__global__ void __launch_bounds__(256) row_table_kernel(const I* offsets, size_t batch, size_t n, int* ids, uint4* bits, const float* from, size_t dim, float* to, tb200::ws_header* hdr) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) hdr->error = 0;
   const size_t r = (size_t)blockIdx.x * 256 + threadIdx.x;
   auto at = [&](size_t s) -> size_t { const long long o = (long long)offsets[s]; return o < 0 ? 0 : (size_t)o > n ? n : (size_t)o; };
   bool inside = false, begins = false, ends = false;
@@ -875,13 +652,12 @@ __global__ void __launch_bounds__(256) row_table_kernel(const I* offsets, size_t
 // more no longer all fit their GPCs (40 slices of 20011 rows: 9 CTAs 77 us, 7 93, 11 118; 16 slices of 65537 f32 rows: 9 204, 16 242), unless there are so few slices
 // that the device stays empty either way (2 slices of 65536 rows: 16 CTAs 112, 9 157).
 struct scan_shape { unsigned warps, ctas, slices; };
-inline scan_shape shape_of(size_t chains, size_t length, size_t slices, int rows, unsigned warps = 0) {
+inline scan_shape shape_of(size_t chains, size_t length, size_t dim, unsigned warps, unsigned rows) {
   scan_shape s;
-  s.slices = (unsigned)slices;
-  s.warps = warps ? warps : 1;
-  while (!warps && s.warps < (unsigned)SCAN_WARPS && (size_t)s.warps * rows < length) s.warps *= 2;
-  const size_t items = chains * slices, tiles = (length + (size_t)s.warps * rows - 1) / ((size_t)s.warps * rows);
-  size_t ctas = items >= 200 ? 1 : items < 9 ? 16 : 360 / items < 9 ? 360 / items : 9;
+  s.warps = warps;
+  s.slices = (unsigned)((dim + 63) / 64);
+  const size_t items = chains * s.slices, tiles = (length + (size_t)warps * rows - 1) / ((size_t)warps * rows);
+  size_t ctas = items >= 200 || warps == 1 ? 1 : items < 9 ? MOST_CTAS : 360 / items < FEW_CTAS ? 360 / items : FEW_CTAS;
   if (ctas > tiles) ctas = tiles;
   s.ctas = ctas < 1 ? 1 : (unsigned)ctas;
   return s;
@@ -933,9 +709,6 @@ __global__ void __launch_bounds__(BLOCK) gated_step_kernel(const T* x, size_t xs
 }
 
 constexpr size_t MOST_CTAS_Y = 65535;
-}  // namespace
-
-namespace {
 // the workspace: header, then the rows' sequences where there are offsets
 size_t scan_workspace(const void* offsets, size_t n) { return sizeof(tb200::ws_header) + (offsets ? tb200::align_up(n * 4, 256) + tb200::align_up((n + 31) / 32 * 16, 256) : 0); }
 int* ids_of(void* d_ws) { return reinterpret_cast<int*>(static_cast<char*>(d_ws) + sizeof(tb200::ws_header)); }
@@ -943,7 +716,8 @@ uint4* bits_of(void* d_ws, size_t n) { return reinterpret_cast<uint4*>(static_ca
 
 template <class I>
 cudaError_t find_ids(const void* offsets, size_t batch, size_t n, void* d_ws, const void* from, size_t dim, void* to, cudaStream_t stream) {
-  row_table_kernel<I><<<(unsigned)(n / 256 + 1), 256, 0, stream>>>(static_cast<const I*>(offsets), batch, n, ids_of(d_ws), bits_of(d_ws, n), static_cast<const float*>(from), dim, static_cast<float*>(to));
+  row_table_kernel<I><<<(unsigned)(n / 256 + 1), 256, 0, stream>>>(static_cast<const I*>(offsets), batch, n, ids_of(d_ws), bits_of(d_ws, n), static_cast<const float*>(from), dim, static_cast<float*>(to),
+                                                               static_cast<tb200::ws_header*>(d_ws));
   return cudaGetLastError();
 }
 
@@ -957,6 +731,7 @@ template <class T> bool tile_map(CUtensorMap& map, const void* p, size_t rows, s
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
     return reinterpret_cast<encode>(f);
   }();
+  if (!in_16_bytes(p, dim, stride, sizeof(T)) || rows >= (1ull << 31) - 512) return false;
   const cuuint64_t dims[2] = {dim, rows}, strides[1] = {stride * sizeof(T)};
   const cuuint32_t boxes[2] = {64, box}, steps[2] = {1, 1};
   const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : std::is_same<T, f16>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -964,13 +739,17 @@ template <class T> bool tile_map(CUtensorMap& map, const void* p, size_t rows, s
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// a channel pair in one access where all rows allow it
-template <class T> bool in_pairs(const void* p, size_t dim, size_t stride) { return ((reinterpret_cast<uintptr_t>(p) | dim * sizeof(T) | stride * sizeof(T)) & (2 * sizeof(T) - 1)) == 0; }
-
-constexpr int NO_MAP = -1;        // the copy engine does not take these rows
+// Four warps of 16 rows (backward: of 8), one warp where a chain is no longer than 16.  Two stages leave room for four CTAs a SM; a CTA that walks a chain
+// alone gains from a third (gradient of 8 x 4096 bf16 rows of 2048: 142 us against 151; five: 144).
+constexpr int SCAN_WARPS = 4, SCAN_ROWS = 16, GRAD_ROWS = 8, SHORT = 16;
+using few_warps = std::integral_constant<int, SCAN_WARPS>;
+using one_warp = std::integral_constant<int, 1>;
+using no_stages = std::integral_constant<int, 0>;
+using stages_shared = std::integral_constant<int, 2>;
+using stages_alone = std::integral_constant<int, 3>;
 
 bool scan_sizes_fit(const void* offsets, size_t batch, size_t n, size_t dim) {
-  return batch < (1ull << 31) && n < (1ull << 40) && (offsets || (batch > 0 && n % batch == 0)) && (offsets ? 1 : batch) * ((dim + 31) / 32) * tb200::CLUSTER_MAX_CTAS < (1ull << 31) &&
+  return batch < (1ull << 31) && n < (1ull << 40) && (offsets || (batch > 0 && n % batch == 0)) && n / 16 < (1ull << 31) - 1 && (offsets ? 1 : batch) * ((dim + 63) / 64) * MOST_CTAS < (1ull << 31) &&
          n / 256 < (1ull << 31) - 1;
 }
 }  // namespace
@@ -990,35 +769,25 @@ TB200_API int tb200_gated_scan(const void* d_x, size_t x_stride, const void* d_g
         if (e != cudaSuccess || n == 0) return (int)e;
       }
       const size_t chains = d_offsets ? 1 : batch, length = n / chains;
-      if (length > 32 && n < (1ull << 31) - 512 && in_16_bytes(d_x, dim, x_stride, sizeof(T)) && in_16_bytes(d_gate, dim, gate_stride, sizeof(T)) && in_16_bytes(d_h, dim, dim, sizeof(T)) &&
-          in_16_bytes(d_h0, dim, dim, 4) && in_16_bytes(d_last, dim, dim, 4)) {
-        auto tiled = [&](auto warps, auto rows, auto stages) -> int {
-          constexpr int WARPS = decltype(warps)::value, ROWS = decltype(rows)::value, STAGES = decltype(stages)::value;
-          using Shared = tiles_shared<T, WARPS, ROWS, 2, STAGES>;
-          CUtensorMap xm, gm;
-          if (!tile_map<T>(xm, d_x, n, dim, x_stride, WARPS * ROWS) || !tile_map<T>(gm, d_gate, n, dim, gate_stride, WARPS * ROWS)) return NO_MAP;
-          const scan_shape shape = shape_of(chains, length, (dim + 63) / 64, ROWS, WARPS);
-          auto with = [&](auto packed) -> int {
-            return (int)launch_chains(gated_tiles_kernel<T, WARPS, ROWS, STAGES, decltype(packed)::value>, shape, chains, Shared::bytes(shape.ctas), stream, xm, gm,
-                                      static_cast<const float*>(d_h0), row_table{bits_of(d_ws, n), ids_of(d_ws)}, shape.slices, length, dim, static_cast<T*>(d_h),
-                                      static_cast<float*>(d_last), static_cast<tb200::ws_header*>(d_ws));
-          };
-          return d_offsets ? with(std::true_type()) : with(std::false_type());
+      auto go = [&](auto warps, auto stages, const CUtensorMap& xm, const CUtensorMap& gm) -> int {
+        constexpr int WARPS = decltype(warps)::value, STAGES = decltype(stages)::value;
+        const scan_shape shape = shape_of(chains, length, dim, WARPS, SCAN_ROWS);
+        auto with = [&](auto packed) -> int {
+          return (int)launch_chains(gated_scan_kernel<T, WARPS, SCAN_ROWS, STAGES, decltype(packed)::value>, shape, chains,
+                                    tiles_shared<T, WARPS, SCAN_ROWS, 2, STAGES>::bytes(shape.ctas), stream, xm, gm, rows_of<T>{static_cast<const T*>(d_x), x_stride},
+                                    rows_of<T>{static_cast<const T*>(d_gate), gate_stride}, static_cast<const float*>(d_h0), row_table{bits_of(d_ws, n), ids_of(d_ws)}, shape.slices,
+                                    length, dim, static_cast<T*>(d_h), static_cast<float*>(d_last), static_cast<tb200::ws_header*>(d_ws));
         };
-        const int rc2 = tiled(std::integral_constant<int, 4>(), std::integral_constant<int, 16>(), std::integral_constant<int, 2>());
-        if (rc2 != NO_MAP) return rc2;
-      }
-      auto go = [&](auto v, auto packed) -> int {
-        constexpr int V = decltype(v)::value, ROWS = 16;
-        const scan_shape shape = shape_of(chains, length, (dim + 32 * V - 1) / (32 * V), ROWS);
-        return (int)launch_chains(gated_scan_kernel<T, V, ROWS, decltype(packed)::value>, shape, chains, 0, stream, static_cast<const T*>(d_x), x_stride, static_cast<const T*>(d_gate),
-                                  gate_stride, static_cast<const float*>(d_h0), ids_of(d_ws), shape.slices, length, dim, static_cast<T*>(d_h), static_cast<float*>(d_last));
+        return d_offsets ? with(std::true_type()) : with(std::false_type());
       };
-      const bool pairs = in_pairs<T>(d_x, dim, x_stride) && in_pairs<T>(d_gate, dim, gate_stride) && in_pairs<T>(d_h, dim, dim);
-      if constexpr (sizeof(T) == 2) {
-        if (pairs) return d_offsets ? go(std::integral_constant<int, 2>(), std::true_type()) : go(std::integral_constant<int, 2>(), std::false_type());
+      CUtensorMap xm = {}, gm = {};
+      constexpr unsigned BOX = SCAN_WARPS * SCAN_ROWS;
+      if (length > SHORT && in_16_bytes(d_h, dim, dim, sizeof(T)) && in_16_bytes(d_h0, dim, dim, 4) && in_16_bytes(d_last, dim, dim, 4) && tile_map<T>(xm, d_x, n, dim, x_stride, BOX) &&
+          tile_map<T>(gm, d_gate, n, dim, gate_stride, BOX)) {
+        if (shape_of(chains, length, dim, SCAN_WARPS, SCAN_ROWS).ctas == 1) return go(few_warps(), stages_alone(), xm, gm);
+        return go(few_warps(), stages_shared(), xm, gm);
       }
-      return d_offsets ? go(std::integral_constant<int, 1>(), std::true_type()) : go(std::integral_constant<int, 1>(), std::false_type());
+      return length > SHORT ? go(few_warps(), no_stages(), xm, gm) : go(one_warp(), no_stages(), xm, gm);
     });
   });
 }
@@ -1041,40 +810,27 @@ TB200_API int tb200_gated_scan_grad(const void* d_dh, size_t dh_stride, const vo
         if (e != cudaSuccess || n == 0) return (int)e;
       }
       const size_t chains = d_offsets ? 1 : batch, length = n / chains;
-      if (length > 32 && n < (1ull << 31) - 512 && in_16_bytes(d_dh, dim, dh_stride, sizeof(T)) && in_16_bytes(d_x, dim, x_stride, sizeof(T)) &&
-          in_16_bytes(d_gate, dim, gate_stride, sizeof(T)) && in_16_bytes(d_h, dim, h_stride, sizeof(T)) && in_16_bytes(d_dx, dim, dim, sizeof(T)) &&
-          in_16_bytes(d_dgate, dim, dim, sizeof(T)) && in_16_bytes(d_h0, dim, dim, 4) && in_16_bytes(d_dlast, dim, dim, 4) && in_16_bytes(d_dh0, dim, dim, 4)) {
-        auto tiled = [&](auto warps, auto rows, auto stages) -> int {
-          constexpr int WARPS = decltype(warps)::value, ROWS = decltype(rows)::value, STAGES = decltype(stages)::value;
-          using Shared = tiles_shared<T, WARPS, ROWS, 4, STAGES>;
-          CUtensorMap dm, gm, xm, hm;
-          if (!tile_map<T>(dm, d_dh, n, dim, dh_stride, WARPS * ROWS) || !tile_map<T>(gm, d_gate, n, dim, gate_stride, WARPS * ROWS) ||
-              !tile_map<T>(xm, d_x, n, dim, x_stride, WARPS * ROWS) || !tile_map<T>(hm, d_h, n, dim, h_stride, WARPS * ROWS))
-            return NO_MAP;
-          const scan_shape shape = shape_of(chains, length, (dim + 63) / 64, ROWS, WARPS);
-          auto with = [&](auto packed) -> int {
-            return (int)launch_chains(gated_tiles_grad_kernel<T, WARPS, ROWS, STAGES, decltype(packed)::value>, shape, chains, Shared::bytes(shape.ctas), stream, dm, gm, xm, hm,
-                                      static_cast<const float*>(d_h0), static_cast<const float*>(d_dlast), row_table{bits_of(d_ws, n), ids_of(d_ws)}, shape.slices, length, dim,
-                                      static_cast<T*>(d_dx), static_cast<T*>(d_dgate), static_cast<float*>(d_dh0), static_cast<tb200::ws_header*>(d_ws));
-          };
-          return d_offsets ? with(std::true_type()) : with(std::false_type());
+      auto go = [&](auto warps, auto stages, const CUtensorMap& dm, const CUtensorMap& gm, const CUtensorMap& xm, const CUtensorMap& hm) -> int {
+        constexpr int WARPS = decltype(warps)::value, STAGES = decltype(stages)::value, ROWS = GRAD_ROWS;
+        const scan_shape shape = shape_of(chains, length, dim, WARPS, ROWS);
+        auto with = [&](auto packed) -> int {
+          return (int)launch_chains(gated_scan_grad_kernel<T, WARPS, ROWS, STAGES, decltype(packed)::value>, shape, chains, tiles_shared<T, WARPS, ROWS, 4, STAGES>::bytes(shape.ctas),
+                                    stream, dm, gm, xm, hm, rows_of<T>{static_cast<const T*>(d_dh), dh_stride}, rows_of<T>{static_cast<const T*>(d_gate), gate_stride},
+                                    rows_of<T>{static_cast<const T*>(d_x), x_stride}, rows_of<T>{static_cast<const T*>(d_h), h_stride}, static_cast<const float*>(d_h0),
+                                    static_cast<const float*>(d_dlast), row_table{bits_of(d_ws, n), ids_of(d_ws)}, shape.slices, length, dim, static_cast<T*>(d_dx),
+                                    static_cast<T*>(d_dgate), static_cast<float*>(d_dh0), static_cast<tb200::ws_header*>(d_ws));
         };
-        const int rc2 = tiled(std::integral_constant<int, 4>(), std::integral_constant<int, 8>(), std::integral_constant<int, 2>());
-        if (rc2 != NO_MAP) return rc2;
-      }
-      auto go = [&](auto v, auto packed) -> int {
-        constexpr int V = decltype(v)::value, ROWS = 8;
-        const scan_shape shape = shape_of(chains, length, (dim + 32 * V - 1) / (32 * V), ROWS);
-        return (int)launch_chains(gated_scan_grad_kernel<T, V, ROWS, decltype(packed)::value>, shape, chains, 0, stream, static_cast<const T*>(d_dh), dh_stride, static_cast<const T*>(d_x),
-                                  x_stride, static_cast<const T*>(d_gate), gate_stride, static_cast<const T*>(d_h), h_stride, static_cast<const float*>(d_h0),
-                                  static_cast<const float*>(d_dlast), ids_of(d_ws), shape.slices, length, dim, static_cast<T*>(d_dx), static_cast<T*>(d_dgate), static_cast<float*>(d_dh0));
+        return d_offsets ? with(std::true_type()) : with(std::false_type());
       };
-      const bool pairs = in_pairs<T>(d_dh, dim, dh_stride) && in_pairs<T>(d_x, dim, x_stride) && in_pairs<T>(d_gate, dim, gate_stride) && in_pairs<T>(d_h, dim, h_stride) &&
-                         in_pairs<T>(d_dx, dim, dim) && in_pairs<T>(d_dgate, dim, dim);
-      if constexpr (sizeof(T) == 2) {
-        if (pairs) return d_offsets ? go(std::integral_constant<int, 2>(), std::true_type()) : go(std::integral_constant<int, 2>(), std::false_type());
+      CUtensorMap dm = {}, gm = {}, xm = {}, hm = {};
+      constexpr unsigned BOX = SCAN_WARPS * GRAD_ROWS;
+      if (length > SHORT && in_16_bytes(d_dx, dim, dim, sizeof(T)) && in_16_bytes(d_dgate, dim, dim, sizeof(T)) && in_16_bytes(d_h0, dim, dim, 4) && in_16_bytes(d_dlast, dim, dim, 4) &&
+          in_16_bytes(d_dh0, dim, dim, 4) && tile_map<T>(dm, d_dh, n, dim, dh_stride, BOX) && tile_map<T>(gm, d_gate, n, dim, gate_stride, BOX) &&
+          tile_map<T>(xm, d_x, n, dim, x_stride, BOX) && tile_map<T>(hm, d_h, n, dim, h_stride, BOX)) {
+        if (shape_of(chains, length, dim, SCAN_WARPS, GRAD_ROWS).ctas == 1) return go(few_warps(), stages_alone(), dm, gm, xm, hm);
+        return go(few_warps(), stages_shared(), dm, gm, xm, hm);
       }
-      return d_offsets ? go(std::integral_constant<int, 1>(), std::true_type()) : go(std::integral_constant<int, 1>(), std::false_type());
+      return length > SHORT ? go(few_warps(), no_stages(), dm, gm, xm, hm) : go(one_warp(), no_stages(), dm, gm, xm, hm);
     });
   });
 }
