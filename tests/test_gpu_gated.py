@@ -275,3 +275,22 @@ def test_refusals(tb):
                  lambda: tb.gated_step(flat[:2], flat[:2], h0, at.float()), lambda: tb.gated_step(flat[:2], flat[:2], h0[:, :4], at)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_copies_that_never_come(tmp_path):
+    """tests/cpp/gated_waits_test.cu, built here with the test hooks and short waits: the wait runs out, the kernel ends, the results are NaNs and the
+    status says so; the next call is right again."""
+    import os
+    import shutil
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.isfile(nvcc):
+        pytest.skip("nvcc is not available on this machine")
+    exe = str(tmp_path / "gated_waits_test")
+    r = subprocess.run([nvcc, "-std=c++17", "-O2", "-gencode", "arch=compute_100a,code=sm_100a", "-DTB200_TEST_HOOKS", "-DTB200_SPIN_LIMIT=65536",
+                        "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "thrust_b200", "csrc"), os.path.join(root, "tests", "cpp", "gated_waits_test.cu"), "-o", exe],
+                       capture_output=True, text=True, timeout=900)
+    assert r.returncode == 0, r.stdout + r.stderr
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr

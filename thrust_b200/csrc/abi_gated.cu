@@ -45,6 +45,14 @@ __device__ __forceinline__ gate_pair open_gate(float g) {
 // registers, and the CTA that has no room for them costs more than it saves (119 us and 196).
 constexpr float CUT = -1.f;
 
+#ifdef TB200_TEST_HOOKS
+// Test builds only (tests/cpp/gated_waits_test.cu): the copies of window 1 of a cluster's first CTA are announced and not made.
+__device__ unsigned withhold_copies;
+__device__ __forceinline__ bool withheld(unsigned w, unsigned rank) { return withhold_copies && w == 1 && rank == 0; }
+#else
+__device__ __forceinline__ bool withheld(unsigned, unsigned) { return false; }
+#endif
+
 using f2 = unsigned long long;
 __device__ __forceinline__ f2 pack2(float x, float y) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
 __device__ __forceinline__ float2 unpack2(f2 a) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a)); return r; }
@@ -165,6 +173,11 @@ __device__ __forceinline__ bool wait_tile(unsigned long long* bar, unsigned pari
   for (unsigned iter = 0; !came && iter < tb200::MBAR_SPIN_LIMIT; ++iter) came = tb200::mbar_try_wait(bar, parity);
   return __all_sync(tb200::FULL_MASK, came);
 }
+// a CTA that gives up: copies that were requested beyond the windows reached are not left in flight
+template <int STAGES> __device__ __forceinline__ void wait_for_copies(unsigned long long* full, unsigned reached, unsigned tiles) {
+  constexpr unsigned S = STAGES > 0 ? STAGES : 1;
+  for (unsigned w = reached; w < tiles && w < reached + S; ++w) wait_tile(&full[w % S], w / S & 1);
+}
 // A 16-byte store into the shared memory of a CTA of the cluster, counted by the mbarrier there.  Unlike a barrier of the cluster it does not
 // wait for this CTA's stores to global memory.
 __device__ __forceinline__ void send_duo(unsigned to, const duo& d, unsigned bar) {
@@ -187,7 +200,7 @@ struct link { duo before, total; };       // of the CTA: what comes before this 
 // All threads of the CTA, with their warps' pairs of window w; `cut`: whether this warp's is one.  Behind it every warp is done with its tiles.
 // Also sends the CTA's pair to the cluster.
 template <class Shared, int WARPS, bool CUTS>
-__device__ __forceinline__ link join_warps(Shared& sh, unsigned w, const duo& own, bool cut, unsigned rank, unsigned ctas, const peers<WARPS>& to) {
+__device__ __forceinline__ link join_warps(Shared& sh, unsigned w, const duo& own, bool cut, unsigned rank, unsigned ctas, const peers<WARPS>& to, bool good) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   sh.warp[w & 1][warp][lane] = own;
   const bool some = CUTS ? __syncthreads_or(cut) != 0 : (__syncthreads(), false);
@@ -210,7 +223,7 @@ __device__ __forceinline__ link join_warps(Shared& sh, unsigned w, const duo& ow
   l.total = f;
   if (ctas > 1) {
     const unsigned buffer = w % MEETINGS;
-    if (threadIdx.x == 0) tb200::mbar_arrive_expect(&sh.met[buffer], ctas * 32 * (unsigned)sizeof(duo));
+    if (threadIdx.x == 0 && good) tb200::mbar_arrive_expect(&sh.met[buffer], ctas * 32 * (unsigned)sizeof(duo));
     const unsigned base = tb200::smem_addr(&sh), at = tb200::smem_addr(sh.pairs() + (buffer * pair_slots(ctas) + rank) * 32 + lane) - base, bar = tb200::smem_addr(&sh.met[buffer]) - base;
 #pragma unroll
     for (int k = 0; k < peers<WARPS>::N; ++k)
@@ -227,13 +240,13 @@ template <class Shared> __device__ __forceinline__ void no_pairs_behind(Shared& 
 // The state before this warp's rows of window w; `carry` goes from before the window to behind it.  false: the cluster's pairs did not come.
 // A CTA sends window w + 1 when it has everything of w - 1, which others sent when they were done with w - 3: four buffers.
 template <class Shared, bool CUTS>
-__device__ __forceinline__ bool join_ctas(Shared& sh, unsigned w, const link& l, f2& carry, f2& q, unsigned rank, unsigned ctas) {
+__device__ __forceinline__ bool join_ctas(Shared& sh, unsigned w, const link& l, f2& carry, f2& q, unsigned rank, unsigned ctas, bool good) {
   if (ctas == 1) {
     q = follow<CUTS>(carry, l.before);
     carry = follow<CUTS>(carry, l.total);
     return true;
   }
-  const bool met = wait_met(&sh.met[w % MEETINGS], (unsigned)(w / MEETINGS) & 1);
+  const bool met = good && wait_met(&sh.met[w % MEETINGS], w / MEETINGS & 1);
   // all steps the same, without a branch between them, so that the pairs are fetched together (behind the last CTA's there are pairs that change nothing):
   // nine steps with a test in each took 640 cycles of a window's 2900
   const duo* pairs = sh.pairs() + (w % MEETINGS) * pair_slots(ctas) * 32 + threadIdx.x % 32;
@@ -308,6 +321,7 @@ gated_scan_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
     unsigned long long* const bar = &sh.full[w % S];
     const int row = row0 + (int)w * row_step;
     tb200::mbar_arrive_expect(bar, 2 * R * 64 * (unsigned)sizeof(T));
+    if (withheld(w, rank)) return;
     load_tile(sh.tile[w % S][0], &x_map, channel0, row, bar);
     load_tile(sh.tile[w % S][1], &gate_map, channel0, row, bar);
   };
@@ -316,7 +330,7 @@ gated_scan_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
     for (int i = 0; i < STAGES; ++i) tb200::mbar_init(&sh.full[i], 1);
     for (int i = 0; i < MEETINGS; ++i) tb200::mbar_init(&sh.met[i], 1);
     tb200::mbar_init_fence();
-    for (unsigned i = 0; i < (unsigned)STAGES; ++i) load(i);
+    for (int i = 0; i < STAGES; ++i) load((unsigned)i);
   }
   auto state_of = [&](size_t s) -> f2 { return h0 ? read_state<TILES>(h0 + s * dim + c, there, both) : 0ull; };
   f2 carry = PACKED ? 0ull : state_of(chain);
@@ -327,7 +341,9 @@ gated_scan_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
   if (ctas > 1) no_pairs_behind(sh, ctas);
   __syncthreads();
   if (ctas > 1) tb200::cluster_barrier();      // all CTAs have begun: their shared memory may be written
+  // Once a wait has run out nothing more is waited for, requested or announced; the results are NaNs from there on, and the kernel ends.
   bool good = true;
+  unsigned reached = 0;        // windows whose tiles have come
   peers<WARPS> to;
 #pragma unroll
   for (int k = 0; k < peers<WARPS>::N; ++k) to.base[k] = warp + k * WARPS < (int)ctas ? tb200::cluster_addr(tb200::smem_addr(&sh), warp + k * WARPS) : 0;
@@ -351,7 +367,8 @@ gated_scan_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
       coming = read_marks(table, (long long)(p + window), (long long)length);
       next_id = id_at(p + window);
     }
-    if (TILES && w < tiles) good &= wait_tile(&sh.full[stage], w / S & 1);
+    if (TILES && w < tiles && good) good = wait_tile(&sh.full[stage], w / S & 1);
+    if (good) reached = w + 1;
     // the warp's rows of an input: in its tile, or all requested from where they lie
     direct_rows<T, ROWS, TILES> rx, rg;
     if constexpr (!TILES) {
@@ -400,12 +417,12 @@ gated_scan_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
       }
     }
     if (!good) own = {pack2(1.f, 1.f), nan2()};
-    s.l = join_warps<Shared, WARPS, PACKED>(sh, w, own, s.cuts != 0, rank, ctas, to);
-    if (threadIdx.x == 0) load(w + STAGES);      // every warp has taken its rows from the tiles
+    s.l = join_warps<Shared, WARPS, PACKED>(sh, w, own, s.cuts != 0, rank, ctas, to, good);
+    if (threadIdx.x == 0 && good) load(w + STAGES);      // every warp has taken its rows from the tiles
   };
   auto give = [&](held& s, unsigned w) {
     f2 q = 0ull;
-    good &= join_ctas<Shared, PACKED>(sh, w, s.l, carry, q, rank, ctas);
+    good &= join_ctas<Shared, PACKED>(sh, w, s.l, carry, q, rank, ctas, good);
     if (!good) { q = nan2(); s.cuts = 0; }
     T* hp = h + (first + p0 + w * window) * dim + c;
     if (s.rows == ROWS && !(PACKED && (s.cuts | s.ends))) {
@@ -432,6 +449,7 @@ gated_scan_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
   };
   held s;
   for (unsigned w = 0; w < windows; ++w) { take(s, w); give(s, w); }
+  if (TILES && !good && warp == 0) wait_for_copies<STAGES>(sh.full, reached, tiles);
   if (ctas > 1) tb200::cluster_barrier();      // nobody leaves while something may still be sent there
   if (!good && lane == 0) tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
   if (!PACKED && rank == 0 && warp == 0) write_state<TILES>(last + chain * dim + c, unpack2(carry), there, both);
@@ -467,6 +485,7 @@ gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_
     unsigned long long* const bar = &sh.full[w % S];
     const int row = row0 - (int)w * row_step;
     tb200::mbar_arrive_expect(bar, 4 * R * 64 * (unsigned)sizeof(T));
+    if (withheld(w, rank)) return;
     load_tile(sh.tile[w % S][0], &dh_map, channel0, row, bar);
     load_tile(sh.tile[w % S][1], &gate_map, channel0, row, bar);
     load_tile(sh.tile[w % S][2], &x_map, channel0, row, bar);
@@ -477,7 +496,7 @@ gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_
     for (int i = 0; i < STAGES; ++i) tb200::mbar_init(&sh.full[i], 1);
     for (int i = 0; i < MEETINGS; ++i) tb200::mbar_init(&sh.met[i], 1);
     tb200::mbar_init_fence();
-    for (unsigned i = 0; i < (unsigned)STAGES; ++i) load(i);
+    for (int i = 0; i < STAGES; ++i) load((unsigned)i);
   }
   auto state_of = [&](const float* from, size_t s) -> f2 { return from ? read_state<TILES>(from + s * dim + c, there, both) : 0ull; };
   f2 carry = PACKED ? 0ull : state_of(dlast, chain);
@@ -494,6 +513,7 @@ gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_
   __syncthreads();
   if (ctas > 1) tb200::cluster_barrier();
   bool good = true;
+  unsigned reached = 0;
   peers<WARPS> to;
 #pragma unroll
   for (int k = 0; k < peers<WARPS>::N; ++k) to.base[k] = warp + k * WARPS < (int)ctas ? tb200::cluster_addr(tb200::smem_addr(&sh), warp + k * WARPS) : 0;
@@ -521,7 +541,8 @@ gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_
     } else if (s.rows > 0 && p + s.rows == length) {
       s.ends = 1u << (s.rows - 1);           // the sequence's first row
     }
-    if (TILES && w < tiles) good &= wait_tile(&sh.full[stage], w / S & 1);
+    if (TILES && w < tiles && good) good = wait_tile(&sh.full[stage], w / S & 1);
+    if (good) reached = w + 1;
     direct_rows<T, ROWS, TILES> rd, rg, rx, rh;
     if constexpr (!TILES) {
       const size_t row = first + (length - 1 - (s.rows ? p : 0));
@@ -581,12 +602,12 @@ gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_
       }
     }
     if (!good) own = {pack2(1.f, 1.f), nan2()};
-    s.l = join_warps<Shared, WARPS, PACKED>(sh, w, own, s.cuts != 0, rank, ctas, to);
-    if (threadIdx.x == 0) load(w + STAGES);      // every warp has taken its rows from the tiles
+    s.l = join_warps<Shared, WARPS, PACKED>(sh, w, own, s.cuts != 0, rank, ctas, to, good);
+    if (threadIdx.x == 0 && good) load(w + STAGES);      // every warp has taken its rows from the tiles
   };
   auto give = [&](held& s, unsigned w) {
     f2 q = 0ull;
-    good &= join_ctas<Shared, PACKED>(sh, w, s.l, carry, q, rank, ctas);
+    good &= join_ctas<Shared, PACKED>(sh, w, s.l, carry, q, rank, ctas, good);
     if (!good) { q = nan2(); s.cuts = 0; }
     const long long at = ((long long)first + (long long)length - 1 - (long long)(p0 + w * window)) * (long long)dim + (long long)c;
     T* xp = dx + at;
@@ -619,6 +640,7 @@ gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_
   };
   held s;
   for (unsigned w = 0; w < windows; ++w) { take(s, w); give(s, w); }
+  if (TILES && !good && warp == 0) wait_for_copies<STAGES>(sh.full, reached, tiles);
   if (ctas > 1) tb200::cluster_barrier();
   if (!good && lane == 0) tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
   if (!PACKED && rank == 0 && warp == 0) write_state<TILES>(dh0 + chain * dim + c, unpack2(carry), there, both);
