@@ -59,6 +59,7 @@ __device__ __forceinline__ float2 unpack2(f2 a) { float2 r; asm("mov.b64 {%0, %1
 __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 __device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 choose(bool c, f2 a, f2 b) { const float2 x = unpack2(a), y = unpack2(b); return pack2(c ? x.x : y.x, c ? x.y : y.y); }
 __device__ __forceinline__ float exp2_of(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 __device__ __forceinline__ float one_over(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
@@ -396,18 +397,24 @@ gated_scan_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
         if (i >= s.rows) { s.keep[i] = pack2(1.f, 1.f); s.b[i] = 0ull; }
     }
     if (PACKED && s.cuts) {
+      if (s.cuts == begins && (begins & (begins - 1)) == 0) {      // one beginning, as a rule: without a branch in each row
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i)
-        if (s.cuts >> i & 1) {
-          if (begins >> i & 1) {
-            if (begins & ((1u << i) - 1)) start = state_of((size_t)__shfl_sync(tb200::FULL_MASK, s.id, i));
-            s.b[i] = fma2(s.keep[i], start, s.b[i]);
-          } else {
-            s.keep[i] = s.b[i] = 0ull;
+        for (int i = 0; i < ROWS; ++i)
+          s.b[i] = choose(begins >> i & 1, fma2(s.keep[i], start, s.b[i]), s.b[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+          if (s.cuts >> i & 1) {
+            if (begins >> i & 1) {
+              if (begins & ((1u << i) - 1)) start = state_of((size_t)__shfl_sync(tb200::FULL_MASK, s.id, i));
+              s.b[i] = fma2(s.keep[i], start, s.b[i]);
+            } else {
+              s.keep[i] = s.b[i] = 0ull;
+            }
           }
-        }
+      }
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i) own.b = s.cuts >> i & 1 ? s.b[i] : fma2(s.keep[i], own.b, s.b[i]);
+      for (int i = 0; i < ROWS; ++i) own.b = choose(s.cuts >> i & 1, s.b[i], fma2(s.keep[i], own.b, s.b[i]));
       own.a = pack2(CUT, CUT);
     } else {
 #pragma unroll
@@ -432,6 +439,20 @@ gated_scan_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
         const float2 v = unpack2(q);
         const float out[2] = {v.x, v.y};
         write_pair<TILES>(hp, out, there, both);
+      }
+    } else if (PACKED && s.rows == ROWS && (s.ends & (s.ends - 1)) == 0) {      // one end at most
+      f2 end = 0ull;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i, hp += dim) {
+        q = choose(s.cuts >> i & 1, s.b[i], fma2(s.keep[i], q, s.b[i]));
+        end = choose(s.ends >> i & 1, q, end);
+        const float2 v = unpack2(q);
+        const float out[2] = {v.x, v.y};
+        write_pair<TILES>(hp, out, there, both);
+      }
+      if (s.ends) {
+        const int seq = __shfl_sync(tb200::FULL_MASK, s.id, __ffs(s.ends) - 1);
+        write_state<TILES>(last + (size_t)seq * dim + c, unpack2(end), there, both);
       }
     } else {
 #pragma unroll
@@ -566,7 +587,13 @@ gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_
       s.d[i] = pack2(dv.x, dv.y);
       s.slope[i] = mul2(mul2(g.keep, g.give), fma2(pack2(xv.x, xv.y), minus, pack2(hv.x, hv.y)));
     }
-    if (s.ends) {
+    if (s.ends && (s.ends & (s.ends - 1)) == 0) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const float2 xv = in(2, rx, i);
+        s.slope[i] = choose(s.ends >> i & 1, mul2(mul2(s.keep[i], s.give[i]), fma2(pack2(xv.x, xv.y), minus, from)), s.slope[i]);
+      }
+    } else if (s.ends) {
 #pragma unroll
       for (int i = 0; i < ROWS; ++i)
         if (s.ends >> i & 1) {
@@ -581,18 +608,23 @@ gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_
         if (i >= s.rows) { s.keep[i] = pack2(1.f, 1.f); s.give[i] = s.d[i] = s.slope[i] = 0ull; }
     }
     if (PACKED && s.cuts) {
+      if (s.cuts == begins && (begins & (begins - 1)) == 0) {
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i)
-        if (s.cuts >> i & 1) {
-          if (begins >> i & 1) {
-            if (begins & ((1u << i) - 1)) start = state_of(dlast, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, i));
-            s.d[i] = add2(s.d[i], start);
-          } else {
-            s.keep[i] = s.give[i] = s.d[i] = s.slope[i] = 0ull;
+        for (int i = 0; i < ROWS; ++i) s.d[i] = choose(begins >> i & 1, add2(s.d[i], start), s.d[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+          if (s.cuts >> i & 1) {
+            if (begins >> i & 1) {
+              if (begins & ((1u << i) - 1)) start = state_of(dlast, (size_t)__shfl_sync(tb200::FULL_MASK, s.id, i));
+              s.d[i] = add2(s.d[i], start);
+            } else {
+              s.keep[i] = s.give[i] = s.d[i] = s.slope[i] = 0ull;
+            }
           }
-        }
+      }
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i) own.b = mul2(s.keep[i], s.cuts >> i & 1 ? s.d[i] : add2(own.b, s.d[i]));
+      for (int i = 0; i < ROWS; ++i) own.b = mul2(s.keep[i], choose(s.cuts >> i & 1, s.d[i], add2(own.b, s.d[i])));
       own.a = pack2(CUT, CUT);
     } else {
 #pragma unroll
@@ -621,6 +653,22 @@ gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_
         const float oa[2] = {a.x, a.y}, ob[2] = {b.x, b.y};
         write_pair<TILES>(xp, oa, there, both);
         write_pair<TILES>(gp, ob, there, both);
+      }
+    } else if (PACKED && s.rows == ROWS && (s.ends & (s.ends - 1)) == 0) {
+      f2 end = 0ull;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i, xp -= dim, gp -= dim) {
+        const f2 sum = choose(s.cuts >> i & 1, s.d[i], add2(s.d[i], q));
+        q = mul2(s.keep[i], sum);
+        end = choose(s.ends >> i & 1, q, end);
+        const float2 a = unpack2(mul2(s.give[i], sum)), b = unpack2(mul2(s.slope[i], sum));
+        const float oa[2] = {a.x, a.y}, ob[2] = {b.x, b.y};
+        write_pair<TILES>(xp, oa, there, both);
+        write_pair<TILES>(gp, ob, there, both);
+      }
+      if (s.ends) {
+        const int seq = __shfl_sync(tb200::FULL_MASK, s.id, __ffs(s.ends) - 1);
+        write_state<TILES>(dh0 + (size_t)seq * dim + c, unpack2(end), there, both);
       }
     } else {
 #pragma unroll
