@@ -717,45 +717,68 @@ __global__ void __launch_bounds__(256) row_table_kernel(const I* offsets, size_t
       for (size_t c = threadIdx.x; c < dim; c += 256) to[s * dim + c] = from ? from[s * dim + c] : 0.f;
 }
 
-// How many CTAs walk a chain together.  One, where the chains' slices fill the device by themselves: pairs that travel cost a window
-// about 0.6 us (256 slices of 4096 bf16 rows: one CTA each 79 us, two 98).  Else as many as make about 360 CTAs, but not more than nine: clusters of
-// more no longer all fit their GPCs (40 slices of 20011 rows: 9 CTAs 77 us, 7 93, 11 118; 16 slices of 65537 f32 rows: 9 204, 16 242), unless there are so few slices
-// that the device stays empty either way (2 slices of 65536 rows: 16 CTAs 112, 9 157).
-struct scan_shape { unsigned warps, ctas, slices; };
-inline scan_shape shape_of(size_t chains, size_t length, size_t dim, unsigned warps, unsigned rows) {
-  scan_shape s;
-  s.warps = warps;
-  s.slices = (unsigned)((dim + 63) / 64);
-  const size_t items = chains * s.slices, tiles = (length + (size_t)warps * rows - 1) / ((size_t)warps * rows);
-  size_t ctas = items >= 200 || warps == 1 ? 1 : items < 9 ? MOST_CTAS : 360 / items < FEW_CTAS ? 360 / items : FEW_CTAS;
-  if (ctas > tiles) ctas = tiles;
-  s.ctas = ctas < 1 ? 1 : (unsigned)ctas;
-  return s;
+// How many clusters of each size the device holds at once, for a kernel: asked once a kernel, device and host thread.
+struct cluster_room { const void* kernel = nullptr; int device = -1; int clusters[MOST_CTAS + 1]; };
+template <class... Params> const cluster_room& room_for(void (*kernel)(Params...), int block, size_t smem_few, size_t smem_most) {
+  constexpr int KEPT = 32;
+  static thread_local cluster_room kept[KEPT];
+  static thread_local int next = 0;
+  int device = 0;
+  cudaGetDevice(&device);
+  for (const cluster_room& r : kept) if (r.kernel == (const void*)kernel && r.device == device) return r;
+  cluster_room& r = kept[next++ % KEPT];
+  r.kernel = (const void*)kernel;
+  r.device = device;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_most) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    cudaGetLastError();
+  for (int c = 2; c <= MOST_CTAS; ++c) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)c);
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = (unsigned)c > FEW_CTAS ? smem_most : smem_few;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)c; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&r.clusters[c], kernel, &cfg) != cudaSuccess) { cudaGetLastError(); r.clusters[c] = 0; }
+  }
+  return r;
 }
 
-template <class... Params, class... Args>
-cudaError_t launch_chains(void (*kernel)(Params...), scan_shape s, size_t chains, size_t smem, cudaStream_t stream, Args... args) {
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
+// Whether the chains' slices fill the device by themselves: then one CTA walks a chain, and no pairs travel.
+inline bool walked_alone(size_t chains, size_t dim) { return chains * ((dim + 63) / 64) >= 200; }
+
+// Launches `kernel` on all chains and slices.  How many CTAs walk a chain together: as many as there are tiles, but no more than let all clusters run at
+// once, since a second round costs more than any window saved (40 slices of 20011 bf16 rows: 9 CTAs 71 us, 7 88, 12 109, of which not all fit; 16 slices of 65537 f32
+// rows: 12 CTAs 150, 9 176, 14 230; 256 slices of 4096 bf16 rows, their gradient: one CTA each 141 us, two 162).
+template <class Shared, class... Params, class... Args>
+cudaError_t launch_chains(void (*kernel)(Params...), unsigned warps, bool alone, size_t chains, size_t length, size_t dim, cudaStream_t stream, Args... args) {
+  const size_t items = chains * ((dim + 63) / 64), tiles = (length + Shared::R - 1) / Shared::R;
+  unsigned ctas = 1;
+  if (!alone && tiles > 1) {
+    const cluster_room& room = room_for(kernel, (int)warps * 32, Shared::bytes(2), Shared::bytes(MOST_CTAS));
+    ctas = tiles < (size_t)MOST_CTAS ? (unsigned)tiles : MOST_CTAS;
+    while (ctas > 1 && (size_t)room.clusters[ctas] < items) --ctas;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.dynamicSmemBytes = smem;
-  cfg.gridDim = dim3((unsigned)(chains * s.slices * s.ctas));
-  cfg.blockDim = dim3(s.warps * 32);
+  cfg.dynamicSmemBytes = Shared::bytes(ctas);
+  if (cfg.dynamicSmemBytes > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shared::bytes(MOST_CTAS));
+    if (e != cudaSuccess) return e;
+  }
+  cfg.gridDim = dim3((unsigned)(items * ctas));
+  cfg.blockDim = dim3(warps * 32);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = s.ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (s.ctas > 8) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
-  if (s.ctas > 1 && tb200::launch_refused(e)) {      // no room for such a cluster: a CTA walks a chain alone
-    cfg.gridDim = dim3((unsigned)(chains * s.slices));
+  if (ctas > 1 && tb200::launch_refused(e)) {      // no room for such a cluster after all: a CTA walks a chain alone
+    cfg.gridDim = dim3((unsigned)items);
     attr[0].val.clusterDim.x = 1;
     e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
   }
@@ -839,25 +862,26 @@ TB200_API int tb200_gated_scan(const void* d_x, size_t x_stride, const void* d_g
         if (e != cudaSuccess || n == 0) return (int)e;
       }
       const size_t chains = d_offsets ? 1 : batch, length = n / chains;
+      const unsigned slices = (unsigned)((dim + 63) / 64);
+      const bool alone = length <= SHORT || walked_alone(chains, dim);
       auto go = [&](auto warps, auto stages, const CUtensorMap& xm, const CUtensorMap& gm) -> int {
         constexpr int WARPS = decltype(warps)::value, STAGES = decltype(stages)::value;
-        const scan_shape shape = shape_of(chains, length, dim, WARPS, SCAN_ROWS);
         auto with = [&](auto packed) -> int {
-          return (int)launch_chains(gated_scan_kernel<T, WARPS, SCAN_ROWS, STAGES, decltype(packed)::value>, shape, chains,
-                                    tiles_shared<T, WARPS, SCAN_ROWS, 2, STAGES>::bytes(shape.ctas), stream, xm, gm, rows_of<T>{static_cast<const T*>(d_x), x_stride},
-                                    rows_of<T>{static_cast<const T*>(d_gate), gate_stride}, static_cast<const float*>(d_h0), row_table{bits_of(d_ws, n), ids_of(d_ws)}, shape.slices,
-                                    length, dim, static_cast<T*>(d_h), static_cast<float*>(d_last), static_cast<tb200::ws_header*>(d_ws));
+          return (int)launch_chains<tiles_shared<T, WARPS, SCAN_ROWS, 2, STAGES>>(gated_scan_kernel<T, WARPS, SCAN_ROWS, STAGES, decltype(packed)::value>, WARPS, alone, chains, length, dim,
+                                                                               stream, xm, gm, rows_of<T>{static_cast<const T*>(d_x), x_stride},
+                                                                               rows_of<T>{static_cast<const T*>(d_gate), gate_stride}, static_cast<const float*>(d_h0),
+                                                                               row_table{bits_of(d_ws, n), ids_of(d_ws)}, slices, length, dim, static_cast<T*>(d_h),
+                                                                               static_cast<float*>(d_last), static_cast<tb200::ws_header*>(d_ws));
         };
         return d_offsets ? with(std::true_type()) : with(std::false_type());
       };
       CUtensorMap xm = {}, gm = {};
       constexpr unsigned BOX = SCAN_WARPS * SCAN_ROWS;
-      if (length > SHORT && in_16_bytes(d_h, dim, dim, sizeof(T)) && in_16_bytes(d_h0, dim, dim, 4) && in_16_bytes(d_last, dim, dim, 4) && tile_map<T>(xm, d_x, n, dim, x_stride, BOX) &&
-          tile_map<T>(gm, d_gate, n, dim, gate_stride, BOX)) {
-        if (shape_of(chains, length, dim, SCAN_WARPS, SCAN_ROWS).ctas == 1) return go(few_warps(), stages_alone(), xm, gm);
-        return go(few_warps(), stages_shared(), xm, gm);
-      }
-      return length > SHORT ? go(few_warps(), no_stages(), xm, gm) : go(one_warp(), no_stages(), xm, gm);
+      if (length <= SHORT) return go(one_warp(), no_stages(), xm, gm);
+      if (in_16_bytes(d_h, dim, dim, sizeof(T)) && in_16_bytes(d_h0, dim, dim, 4) && in_16_bytes(d_last, dim, dim, 4) && tile_map<T>(xm, d_x, n, dim, x_stride, BOX) &&
+          tile_map<T>(gm, d_gate, n, dim, gate_stride, BOX))
+        return alone ? go(few_warps(), stages_alone(), xm, gm) : go(few_warps(), stages_shared(), xm, gm);
+      return go(few_warps(), no_stages(), xm, gm);
     });
   });
 }
@@ -880,27 +904,27 @@ TB200_API int tb200_gated_scan_grad(const void* d_dh, size_t dh_stride, const vo
         if (e != cudaSuccess || n == 0) return (int)e;
       }
       const size_t chains = d_offsets ? 1 : batch, length = n / chains;
+      const unsigned slices = (unsigned)((dim + 63) / 64);
+      const bool alone = length <= SHORT || walked_alone(chains, dim);
       auto go = [&](auto warps, auto stages, const CUtensorMap& dm, const CUtensorMap& gm, const CUtensorMap& xm, const CUtensorMap& hm) -> int {
-        constexpr int WARPS = decltype(warps)::value, STAGES = decltype(stages)::value, ROWS = GRAD_ROWS;
-        const scan_shape shape = shape_of(chains, length, dim, WARPS, ROWS);
+        constexpr int WARPS = decltype(warps)::value, STAGES = decltype(stages)::value;
         auto with = [&](auto packed) -> int {
-          return (int)launch_chains(gated_scan_grad_kernel<T, WARPS, ROWS, STAGES, decltype(packed)::value>, shape, chains, tiles_shared<T, WARPS, ROWS, 4, STAGES>::bytes(shape.ctas),
-                                    stream, dm, gm, xm, hm, rows_of<T>{static_cast<const T*>(d_dh), dh_stride}, rows_of<T>{static_cast<const T*>(d_gate), gate_stride},
-                                    rows_of<T>{static_cast<const T*>(d_x), x_stride}, rows_of<T>{static_cast<const T*>(d_h), h_stride}, static_cast<const float*>(d_h0),
-                                    static_cast<const float*>(d_dlast), row_table{bits_of(d_ws, n), ids_of(d_ws)}, shape.slices, length, dim, static_cast<T*>(d_dx),
-                                    static_cast<T*>(d_dgate), static_cast<float*>(d_dh0), static_cast<tb200::ws_header*>(d_ws));
+          return (int)launch_chains<tiles_shared<T, WARPS, GRAD_ROWS, 4, STAGES>>(
+              gated_scan_grad_kernel<T, WARPS, GRAD_ROWS, STAGES, decltype(packed)::value>, WARPS, alone, chains, length, dim, stream, dm, gm, xm, hm,
+              rows_of<T>{static_cast<const T*>(d_dh), dh_stride}, rows_of<T>{static_cast<const T*>(d_gate), gate_stride}, rows_of<T>{static_cast<const T*>(d_x), x_stride},
+              rows_of<T>{static_cast<const T*>(d_h), h_stride}, static_cast<const float*>(d_h0), static_cast<const float*>(d_dlast), row_table{bits_of(d_ws, n), ids_of(d_ws)}, slices,
+              length, dim, static_cast<T*>(d_dx), static_cast<T*>(d_dgate), static_cast<float*>(d_dh0), static_cast<tb200::ws_header*>(d_ws));
         };
         return d_offsets ? with(std::true_type()) : with(std::false_type());
       };
       CUtensorMap dm = {}, gm = {}, xm = {}, hm = {};
       constexpr unsigned BOX = SCAN_WARPS * GRAD_ROWS;
-      if (length > SHORT && in_16_bytes(d_dx, dim, dim, sizeof(T)) && in_16_bytes(d_dgate, dim, dim, sizeof(T)) && in_16_bytes(d_h0, dim, dim, 4) && in_16_bytes(d_dlast, dim, dim, 4) &&
+      if (length <= SHORT) return go(one_warp(), no_stages(), dm, gm, xm, hm);
+      if (in_16_bytes(d_dx, dim, dim, sizeof(T)) && in_16_bytes(d_dgate, dim, dim, sizeof(T)) && in_16_bytes(d_h0, dim, dim, 4) && in_16_bytes(d_dlast, dim, dim, 4) &&
           in_16_bytes(d_dh0, dim, dim, 4) && tile_map<T>(dm, d_dh, n, dim, dh_stride, BOX) && tile_map<T>(gm, d_gate, n, dim, gate_stride, BOX) &&
-          tile_map<T>(xm, d_x, n, dim, x_stride, BOX) && tile_map<T>(hm, d_h, n, dim, h_stride, BOX)) {
-        if (shape_of(chains, length, dim, SCAN_WARPS, GRAD_ROWS).ctas == 1) return go(few_warps(), stages_alone(), dm, gm, xm, hm);
-        return go(few_warps(), stages_shared(), dm, gm, xm, hm);
-      }
-      return length > SHORT ? go(few_warps(), no_stages(), dm, gm, xm, hm) : go(one_warp(), no_stages(), dm, gm, xm, hm);
+          tile_map<T>(xm, d_x, n, dim, x_stride, BOX) && tile_map<T>(hm, d_h, n, dim, h_stride, BOX))
+        return alone ? go(few_warps(), stages_alone(), dm, gm, xm, hm) : go(few_warps(), stages_shared(), dm, gm, xm, hm);
+      return go(few_warps(), no_stages(), dm, gm, xm, hm);
     });
   });
 }
