@@ -785,23 +785,53 @@ cudaError_t launch_chains(void (*kernel)(Params...), unsigned warps, bool alone,
   return e;
 }
 
-// one token of each sequence: state[slot] is read and written, and is the row's output too
-template <class T, class I>
-__global__ void __launch_bounds__(BLOCK) gated_step_kernel(const T* x, size_t xs, const T* gate, size_t gs, float* state, size_t pool, const I* slots, size_t dim, T* h) {
-  const size_t c = (size_t)blockIdx.y * BLOCK + threadIdx.x, r = blockIdx.x;
-  if (c >= dim) return;
+// One token of each sequence: state[slot] is read and written, and is the row's output too.  A thread has up to STEP_U pieces of V channels of a row; bound by the
+// bytes of states and rows.
+constexpr int STEP_U = 2;
+template <class T, int V, class I>
+__global__ void __launch_bounds__(BLOCK) gated_step_kernel(const T* __restrict__ x, size_t xs, const T* __restrict__ gate, size_t gs, float* state, size_t pool, const I* __restrict__ slots,
+                                                         size_t n, unsigned pieces, unsigned spread, unsigned parts, T* __restrict__ h) {
+  const share s = share_of((size_t)blockIdx.x * BLOCK + threadIdx.x, spread, parts);
+  const size_t r = s.at;
+  if (r >= n) return;
+  const unsigned lanes = 1u << spread, c0 = s.part * lanes * STEP_U + s.in;
   const long long slot = slots ? (long long)slots[r] : (long long)r;
-  float v = 0.f;
-  if (slot >= 0 && (size_t)slot < pool) {
-    const gate_pair p = open_gate(to_f32(gate[r * gs + c]));
-    float* const at = state + (size_t)slot * dim + c;
-    v = p.keep * *at + p.give * to_f32(x[r * xs + c]);
-    *at = v;
+  const bool there = slot >= 0 && (size_t)slot < pool;
+  float* const at = state + (there ? (size_t)slot * pieces * V : 0);
+  words<T, V> xw[STEP_U], gw[STEP_U];
+  words<float, V> old[STEP_U];
+#pragma unroll
+  for (int u = 0; u < STEP_U; ++u) {
+    const size_t c = (size_t)(c0 + u * lanes) * V;
+    if (there && c0 + u * lanes < pieces) {
+      xw[u] = load_words<T, V>(x + r * xs + c);
+      gw[u] = load_words<T, V>(gate + r * gs + c);
+      old[u] = load_words<float, V>(at + c);
+    }
   }
-  h[r * dim + c] = from_f32<T>(v);
+#pragma unroll
+  for (int u = 0; u < STEP_U; ++u) {
+    if (c0 + u * lanes >= pieces) break;
+    const size_t c = (size_t)(c0 + u * lanes) * V;
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.f;
+    if (there) {
+      float xv[V], gv[V];
+      channels(xw[u], xv);
+      channels(gw[u], gv);
+      channels(old[u], v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const gate_pair p = open_gate(gv[i]);
+        v[i] = fmaf(p.keep, v[i], p.give * xv[i]);
+      }
+      store_words<float, V>(at + c, to_words<float, V>(v));
+    }
+    store_words<T, V>(h + r * pieces * V + c, to_words<T, V>(v));
+  }
 }
 
-constexpr size_t MOST_CTAS_Y = 65535;
 // the workspace: header, then the rows' sequences where there are offsets
 size_t scan_workspace(const void* offsets, size_t n) { return sizeof(tb200::ws_header) + (offsets ? tb200::align_up(n * 4, 256) + tb200::align_up((n + 31) / 32 * 16, 256) : 0); }
 int* ids_of(void* d_ws) { return reinterpret_cast<int*>(static_cast<char*>(d_ws) + sizeof(tb200::ws_header)); }
@@ -936,12 +966,19 @@ TB200_API int tb200_gated_step(const void* d_x, size_t x_stride, const void* d_g
     return by_index_dtype(d_slots ? slot_t : TB200_I32, [&](auto iv) -> int {
       using I = decltype(iv);
       if (n == 0 || dim == 0) return 0;
-      if (!d_x || !d_gate || !d_h || (pool && !d_state) || x_stride < dim || gate_stride < dim || n > 0x7fffffffull || (dim + BLOCK - 1) / BLOCK > MOST_CTAS_Y)
-        return ERR_INVALID;
-      const dim3 grid((unsigned)n, (unsigned)((dim + BLOCK - 1) / BLOCK));
-      gated_step_kernel<T, I><<<grid, BLOCK, 0, stream>>>(static_cast<const T*>(d_x), x_stride, static_cast<const T*>(d_gate), gate_stride, static_cast<float*>(d_state), pool,
-                                                        static_cast<const I*>(d_slots), dim, static_cast<T*>(d_h));
-      return (int)cudaGetLastError();
+      if (!d_x || !d_gate || !d_h || (pool && !d_state) || x_stride < dim || gate_stride < dim || n > 0x7fffffffull || dim >= (1ull << 31)) return ERR_INVALID;
+      auto go = [&](auto vv) -> int {
+        constexpr int V = decltype(vv)::value;
+        const unsigned pieces = (unsigned)(dim / V), spread = spread_of((pieces + STEP_U - 1) / STEP_U, 5), parts = (unsigned)(((size_t)pieces + (STEP_U << spread) - 1) / (STEP_U << spread));
+        const size_t grid = (((n * parts) << spread) + BLOCK - 1) / BLOCK;
+        if (grid > 0x7fffffffull) return ERR_INVALID;
+        gated_step_kernel<T, V, I><<<(unsigned)grid, BLOCK, 0, stream>>>(static_cast<const T*>(d_x), x_stride, static_cast<const T*>(d_gate), gate_stride, static_cast<float*>(d_state), pool,
+                                                                       static_cast<const I*>(d_slots), n, pieces, spread, parts, static_cast<T*>(d_h));
+        return (int)cudaGetLastError();
+      };
+      if (in_16_bytes(d_x, dim, x_stride, sizeof(T)) && in_16_bytes(d_gate, dim, gate_stride, sizeof(T)) && in_16_bytes(d_h, dim, dim, sizeof(T)) && in_16_bytes(d_state, dim, dim, 4))
+        return go(std::integral_constant<int, 4>());
+      return go(std::integral_constant<int, 1>());
     });
   });
 }
