@@ -35,11 +35,11 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ we
     }
 }
 
-// keys: the token, or `rows` for one that is no row; positions 0, 1, ...; and the list of long runs is empty
+// keys: the token, or `rows` for one that is no row; positions 0, 1, ...; and the lists of long runs are empty
 template <class I>
-__global__ void __launch_bounds__(256) token_keys_kernel(const I* tokens, size_t n, unsigned rows, unsigned* keys, unsigned* positions, unsigned* count) {
+__global__ void __launch_bounds__(256) token_keys_kernel(const I* tokens, size_t n, unsigned rows, unsigned* keys, unsigned* positions, unsigned* counts) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i == 0) *count = 0;
+  if (i < 2) counts[i] = 0;
   if (i >= n) return;
   const long long tok = (long long)tokens[i];
   keys[i] = tok >= 0 && tok < (long long)rows ? (unsigned)tok : rows;
@@ -108,8 +108,9 @@ __device__ __forceinline__ run_ends run_ends_of(const unsigned* keys, size_t n, 
   return r;
 }
 
-// the chunks in which long runs begin
-struct long_runs { unsigned count, pad[63], chunks[1]; };
+// The chunks in which long runs begin: those of up to MANY_PARTS parts from the front of the list, the others from its back.
+constexpr unsigned MANY_PARTS = 32;
+struct long_runs { unsigned few, many, pad[62], chunks[1]; };
 
 // the sum becomes a row of the result, added to what is there (`old`) if that is wanted
 template <class O, int V, bool ADD> __device__ __forceinline__ void write_sum(O* to, const float (&sum)[V], float scale, const words<O, V>& old) {
@@ -146,6 +147,7 @@ template <class T, class O, int V, bool ADD>
 __global__ void __launch_bounds__(GRAD_BLOCK, ADD ? 2 : 3) embedding_grad_kernel(const T* __restrict__ dout, size_t stride, const unsigned* __restrict__ keys, const unsigned* __restrict__ positions,
                                                                   size_t n, unsigned rows, unsigned pieces, grad_shape shape, float scale, unsigned zero_blocks,
                                                                   O* __restrict__ out, float* __restrict__ partial, long_runs* __restrict__ list, const tb200::ws_header* hdr) {
+  tb200::grid_dependents_launch();      // the join may take its place
   const size_t dim = (size_t)pieces * V;
   if (hdr->error) {      // the sort's waits ran out
     for (size_t i = (size_t)blockIdx.x * GRAD_BLOCK + threadIdx.x; i < rows * dim; i += (size_t)gridDim.x * GRAD_BLOCK) out[i] = from_f32<O>(__int_as_float(0x7fffffff));
@@ -193,7 +195,11 @@ __global__ void __launch_bounds__(GRAD_BLOCK, ADD ? 2 : 3) embedding_grad_kernel
       if (j < MOST) its_rows[j] = there ? positions[begin + j] : NO_ROW;
     }
     run = run_ends_of(keys, n, chunk, shape.chunk);
-    if (run.leaves && run.last < rows && mine.part == 0 && mine.in == 0) list->chunks[atomicAdd(&list->count, 1u)] = (unsigned)chunk;
+    if (run.leaves && run.last < rows && mine.part == 0 && mine.in == 0) {
+      const size_t far = (chunk + MANY_PARTS) * shape.chunk;      // a place of the part behind so many
+      if (far < n && keys[far] == run.last) list->chunks[shape.chunks - 1 - atomicAdd(&list->many, 1u)] = (unsigned)chunk;
+      else list->chunks[atomicAdd(&list->few, 1u)] = (unsigned)chunk;
+    }
   }
   __syncthreads();
   if (chunk < shape.chunks) {
@@ -245,8 +251,8 @@ __global__ void __launch_bounds__(GRAD_BLOCK, ADD ? 2 : 3) embedding_grad_kernel
   }
 }
 
-// A CTA takes a listed run and 32 pieces of the columns at a time: its eight warps add up neighbouring parts each, and their sums are added up in
-// order.  (The order of the list is any; each run is by itself.)
+// Runs of few parts: a warp takes one, 32 pieces of the columns at a time.  Of the others a CTA's eight warps add up neighbouring parts each, and their sums
+// are added up in order.  (The order of the list is any; each run is by itself.)
 constexpr unsigned JOIN_WARPS = GRAD_BLOCK / 32;
 template <class O, int V, bool ADD>
 __global__ void __launch_bounds__(GRAD_BLOCK) embedding_grad_join_kernel(const unsigned* __restrict__ keys, unsigned pieces, grad_shape shape, float scale, O* __restrict__ out,
@@ -255,12 +261,41 @@ __global__ void __launch_bounds__(GRAD_BLOCK) embedding_grad_join_kernel(const u
   __shared__ float sums[JOIN_WARPS][32][V];
   tb200::grid_dependency_wait();
   if (hdr->error) return;
+  constexpr int AHEAD = 8;
   const size_t dim = (size_t)pieces * V;
-  const unsigned columns = (pieces + 31) / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const unsigned long long items = (unsigned long long)list->count * columns;
-  for (unsigned long long item = blockIdx.x; item < items; item += gridDim.x) {
+  const unsigned columns = (pieces + 31) / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32, few = list->few, many = list->many;
+  for (unsigned long long item = (unsigned long long)blockIdx.x * JOIN_WARPS + warp; item < (unsigned long long)few * columns; item += (unsigned long long)gridDim.x * JOIN_WARPS) {
     const unsigned nth = (unsigned)(item / columns), c = (unsigned)(item - (unsigned long long)nth * columns) * 32 + lane;
     const size_t chunk = list->chunks[nth];
+    const unsigned key = keys[(chunk + 1) * shape.chunk];
+    const bool its = chunk + 1 + lane < shape.chunks && keys[(chunk + 1 + lane) * shape.chunk] == key;
+    const unsigned parts = 1 + __popc(__ballot_sync(tb200::FULL_MASK, its));
+    if (c < pieces) {
+      const float* const p = partial + 2 * chunk * dim + (size_t)c * V;
+      O* const at = out + (size_t)key * dim + (size_t)c * V;
+      words<O, V> old;
+      if (ADD) old = load_words<O, V>(at);
+      float sum[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) sum[v] = 0.f;
+      for (unsigned i = 0; i < parts; i += AHEAD) {
+        float f[AHEAD][V];
+#pragma unroll
+        for (unsigned u = 0; u < AHEAD; ++u)
+          if (i + u < parts) read_part<V>(p + (i + u ? 2 * (size_t)(i + u) : 1) * dim, f[u]);
+#pragma unroll
+        for (unsigned u = 0; u < AHEAD; ++u)
+          if (i + u < parts) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum[v] += f[u][v];
+          }
+      }
+      write_sum<O, V, ADD>(at, sum, scale, old);
+    }
+  }
+  for (unsigned long long item = blockIdx.x; item < (unsigned long long)many * columns; item += gridDim.x) {
+    const unsigned nth = (unsigned)(item / columns), c = (unsigned)(item - (unsigned long long)nth * columns) * 32 + lane;
+    const size_t chunk = list->chunks[shape.chunks - 1 - nth];
     const unsigned key = keys[(chunk + 1) * shape.chunk];
     if (warp == 0) {
       size_t q = chunk + 1;
@@ -275,7 +310,6 @@ __global__ void __launch_bounds__(GRAD_BLOCK) embedding_grad_join_kernel(const u
     for (int v = 0; v < V; ++v) sum[v] = 0.f;
     if (c < pieces) {
       const float* const p = partial + 2 * chunk * dim + (size_t)c * V;
-      constexpr int AHEAD = 8;
       for (size_t i = from; i < to; i += AHEAD) {
         float f[AHEAD][V];
 #pragma unroll
@@ -375,7 +409,7 @@ TB200_API int tb200_embedding_grad(const void* d_dout, size_t dout_stride, const
         unsigned* const positions = reinterpret_cast<unsigned*>(base + lay.sort + 2 * lay.array);
         float* const partial = reinterpret_cast<float*>(base + lay.partial);
         long_runs* const list = reinterpret_cast<long_runs*>(base + lay.list);
-        if (n) token_keys_kernel<I><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(static_cast<const I*>(d_tokens), n, (unsigned)rows, keys, positions, &list->count);
+        if (n) token_keys_kernel<I><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(static_cast<const I*>(d_tokens), n, (unsigned)rows, keys, positions, &list->few);
         tb200::key_coding coding;
         coding.kind = tb200::KEY_UNSIGNED;
         coding.descending = 0;
