@@ -82,6 +82,20 @@ def test_gradient(tb, dtype, out, accumulate, n, rows, dim):
     lu.near(got, want, error)
 
 
+@pytest.mark.parametrize("n", [1, 31, 32, 33, 34, 66, 99, 32 * 33, 33 * 33, 33 * 33 + 1, 33 * 33 * 2, 33 * 66, 33 * 33 * 33])
+@pytest.mark.parametrize("shift", [0, 31])
+def test_each_row_is_summed_or_cleared(tb, n, shift):
+    """Tokens that all differ, so that each row of the result is one row of dout or zero: whether a row occurs is searched for 33 parts at a time, and
+    these numbers of places are where such a search comes out even."""
+    rows = n + 70
+    tokens = torch.randperm(n, generator=torch.Generator(device="cuda").manual_seed(n), device="cuda") + shift
+    dout = 1.0 + torch.rand(n, 8, generator=torch.Generator(device="cuda").manual_seed(n + 1), device="cuda")
+    want = torch.zeros(rows, 8, device="cuda")
+    want[tokens] = dout
+    for _ in range(3):
+        assert torch.equal(tb.embedding_grad(dout, tokens, rows), want)
+
+
 @pytest.mark.parametrize("n,rows,dim", [(20000, 50, 320), (3001, 3001, 72)])
 def test_gradient_gives_the_same_bits(tb, n, rows, dim):
     dout, tokens = _normal((n, dim), torch.float32, 9), _tokens(n, rows, 10)
