@@ -208,60 +208,64 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const T* __restrict
   }
 }
 
-// A warp a token: its row of dout stays in registers (while it fits) against the rows of all its choices, each read and written once.
-template <class T, int V>
+// 2^spread lanes a token (WARP: 32, known beforehand, where the rows are long enough): its row of dout stays in registers (while it fits) against the rows of all its choices, each
+// read and written once.
+template <class T, int V, bool WARP>
 __global__ void __launch_bounds__(256) expert_combine_grad_kernel(const T* __restrict__ dout, size_t ds, const T* __restrict__ rows, size_t rs, size_t m, const int* __restrict__ slots,
                                                                   const float* __restrict__ weights, const int* __restrict__ end, size_t n, unsigned choices, size_t pieces,
-                                                                  T* __restrict__ drows, float* __restrict__ dweights) {
+                                                                  unsigned lanes_log, T* __restrict__ drows, float* __restrict__ dweights) {
   constexpr int U = 8;
-  const int lane = threadIdx.x % 32;
-  const size_t warps = (size_t)gridDim.x * 8, index = (size_t)blockIdx.x * 8 + threadIdx.x / 32;
-  const size_t dim = pieces * V;
-  for (size_t token = index; token < n; token += warps) {
-    const T* const d = dout + token * ds;
+  const unsigned spread = WARP ? 5 : lanes_log, lanes = 1u << spread, in = threadIdx.x & (lanes - 1);
+  const size_t groups = ((size_t)gridDim.x * 256) >> spread, index = ((size_t)blockIdx.x * 256 + threadIdx.x) >> spread;
+  const size_t dim = pieces * V, rounds = (n + groups - 1) / groups;
+  for (size_t round = 0; round < rounds; ++round) {      // the same for all groups of a warp
+    const size_t token = index + round * groups;
+    const bool there = token < n;
+    const T* const d = dout + (there ? token : 0) * ds;
     words<T, V> held[U];
     auto take = [&](size_t c0) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (c0 + u * 32 < pieces) held[u] = load_words<T, V>(d + (c0 + u * 32) * V);
+        if (c0 + u * lanes < pieces) held[u] = load_words<T, V>(d + (c0 + u * lanes) * V);
     };
-    if (pieces <= U * 32) take(lane);
+    if (there && pieces <= (size_t)U * lanes) take(in);
     for (unsigned k = 0; k < choices; ++k) {
-      const int place = slots[token * choices + k];
+      const int place = there ? slots[token * choices + k] : -1;
       float dot = 0.f;
       if ((unsigned)place < m) {
         const float w = weights[token * choices + k];
         const T* const r = rows + (size_t)place * rs;
         T* const to = drows + (size_t)place * dim;
-        for (size_t c0 = lane; c0 < pieces; c0 += U * 32) {
+        for (size_t c0 = in; c0 < pieces; c0 += (size_t)U * lanes) {
           words<T, V> v[U];
 #pragma unroll
           for (int u = 0; u < U; ++u)
-            if (c0 + u * 32 < pieces) v[u] = load_words<T, V>(r + (c0 + u * 32) * V);
-          if (pieces > U * 32) take(c0);
+            if (c0 + u * lanes < pieces) v[u] = load_words<T, V>(r + (c0 + u * lanes) * V);
+          if (pieces > (size_t)U * lanes) take(c0);
 #pragma unroll
           for (int u = 0; u < U; ++u)
-            if (c0 + u * 32 < pieces) {
+            if (c0 + u * lanes < pieces) {
               float a[V], b[V];
               channels(held[u], a);
               channels(v[u], b);
 #pragma unroll
               for (int i = 0; i < V; ++i) { dot = fmaf(a[i], b[i], dot); a[i] *= w; }
-              store_words<T, V>(to + (c0 + u * 32) * V, to_words<T, V>(a));
+              store_words<T, V>(to + (c0 + u * lanes) * V, to_words<T, V>(a));
             }
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(tb200::FULL_MASK, dot, o);
       }
-      if (lane == 0) dweights[token * choices + k] = dot;
+#pragma unroll
+      for (unsigned o = 16; o; o >>= 1)
+        if (WARP || o < lanes) dot += __shfl_xor_sync(tb200::FULL_MASK, dot, o);
+      if (there && in == 0) dweights[token * choices + k] = dot;
     }
   }
   float none[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) none[v] = 0.f;
   const int kept = *end;
-  for (size_t row = (kept > 0 ? (size_t)kept : 0) + index; row < m; row += warps)
-    for (size_t c = lane; c < pieces; c += 32) store_words<T, V>(drows + row * dim + c * V, to_words<T, V>(none));
+  for (size_t row = (kept > 0 ? (size_t)kept : 0) + index; row < m; row += groups)
+    for (size_t c = in; c < pieces; c += lanes) store_words<T, V>(drows + row * dim + c * V, to_words<T, V>(none));
 }
 
 // what every one of these calls needs of its sizes: flat assignments and rows are counted in 31 bits
@@ -364,9 +368,10 @@ TB200_API int tb200_expert_combine_grad(const void* d_dout, size_t dout_stride, 
     if (!d_slots || !d_weights || !d_kept || !d_dweights || (dim && (!d_dout || !d_rows || !d_drows)) || dout_stride < dim || rows_stride < dim) return ERR_INVALID;
     auto go = [&](auto vv) -> int {
       constexpr int V = decltype(vv)::value;
-      const size_t most = (size_t)tb200::current_device_info().sm_count * 16, want = (n + 7) / 8;
-      expert_combine_grad_kernel<T, V><<<(unsigned)(want < most ? want : most), 256, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, static_cast<const T*>(d_rows), rows_stride,
-                                                                                              n * choices, d_slots, d_weights, d_kept, n, (unsigned)choices, dim / V,
+      const unsigned spread = spread_of(dim / V, 5);
+      const size_t most = (size_t)tb200::current_device_info().sm_count * 16, want = ((n << spread) + 255) / 256;
+      (spread == 5 ? expert_combine_grad_kernel<T, V, true> : expert_combine_grad_kernel<T, V, false>)<<<(unsigned)(want < most ? want : most), 256, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, static_cast<const T*>(d_rows), rows_stride,
+                                                                                              n * choices, d_slots, d_weights, d_kept, n, (unsigned)choices, dim / V, spread,
                                                                                               static_cast<T*>(d_drows), d_dweights);
       return (int)cudaGetLastError();
     };
