@@ -8,10 +8,12 @@ using namespace tb200_rows;
 namespace {
 // out[i] = scale * weight[tokens[i]].  2^spread lanes take up to LOOKUP_U pieces each of a row (`parts` times that make a row): as many random reads
 // are in flight per thread.  Bound by the bytes of the rows.
-constexpr int LOOKUP_U = 4;
+// channel by channel 16 reads of 32 bits (16391 rows of 2049: 44 us, with four 55) or eight of 16 (with 16 57, with four 53)
+constexpr int lookup_u(int v, size_t bytes) { return v > 1 ? 4 : bytes == 4 ? 16 : 8; }
 template <class T, int V, class I>
 __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ weight, size_t rows, size_t stride, const I* __restrict__ tokens, size_t n, unsigned pieces, unsigned parts,
                                                         unsigned spread, float scale, T* __restrict__ out) {
+  constexpr int LOOKUP_U = lookup_u(V, sizeof(T));
   const share s = share_of((size_t)blockIdx.x * 256 + threadIdx.x, spread, parts);
   const size_t i = s.at;
   if (i >= n) return;
@@ -400,6 +402,7 @@ TB200_API int tb200_embedding(const void* d_weight, size_t rows, size_t weight_s
       if (!d_tokens || !d_out || (rows && !d_weight) || weight_stride < dim || n >= (1ull << 31) || dim >= (1ull << 31)) return ERR_INVALID;
       auto go = [&](auto vv) -> int {
         constexpr int V = decltype(vv)::value;
+        constexpr int LOOKUP_U = lookup_u(V, sizeof(T));
         const unsigned pieces = (unsigned)(dim / V), spread = spread_of((pieces + LOOKUP_U - 1) / LOOKUP_U, 5), parts = (unsigned)(((size_t)pieces + (LOOKUP_U << spread) - 1) / (LOOKUP_U << spread));
         const size_t grid = (((n * parts) << spread) + 255) / 256;
         if (grid > 0x7fffffffull) return ERR_INVALID;

@@ -342,7 +342,7 @@ TB200_API int tb200_expert_combine(const void* d_rows, size_t rows_stride, const
       using std::integral_constant;
       // 16-byte pieces, four to eight reads a thread.  8191 x 2 f16 rows of 4096: 34 us (two rows at a time with their sums held: 39, eight reads with four sums: 45);
       // 8192 x 8 bf16 rows of 2048: 50 (two at a time: 52); 16384 x 1 of 4096: 45 (62).  Channel by channel two of eight rows at a time are faster than all of
-      // them: 8192 x 4 bf16 rows of 1501: 44 us against 72.
+      // them: 8192 x 4 bf16 rows of 1501: 42 us against 72 (eight pieces a thread; four: 52).
       if constexpr (V > 1) {
         if (choices == 1) return run(integral_constant<int, 1>(), integral_constant<int, 4>(), std::true_type());
         if (choices == 2) return run(integral_constant<int, 2>(), integral_constant<int, 2>(), std::true_type());
@@ -350,7 +350,7 @@ TB200_API int tb200_expert_combine(const void* d_rows, size_t rows_stride, const
         if (choices <= 8) return run(integral_constant<int, 8>(), integral_constant<int, 1>(), std::true_type());
         return run(integral_constant<int, 2>(), integral_constant<int, 2>(), std::false_type());
       } else {
-        return run(integral_constant<int, 2>(), integral_constant<int, 4>(), std::false_type());
+        return run(integral_constant<int, 2>(), integral_constant<int, 8>(), std::false_type());
       }
     };
     auto with = [&](auto vv) -> int { return d_weights ? go(vv, std::true_type()) : go(vv, std::false_type()); };
