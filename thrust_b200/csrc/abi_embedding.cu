@@ -163,6 +163,7 @@ template <class T, class O, int V, bool ADD>
 __global__ void __launch_bounds__(GRAD_BLOCK, ADD ? 2 : 3) embedding_grad_kernel(const T* __restrict__ dout, size_t stride, const unsigned* __restrict__ keys, const unsigned* __restrict__ positions,
                                                                   size_t n, unsigned rows, unsigned pieces, grad_shape shape, float scale, unsigned zero_blocks,
                                                                   O* __restrict__ out, float* __restrict__ partial, long_runs* __restrict__ list, const tb200::ws_header* hdr) {
+  tb200::grid_dependency_wait();        // the places are sorted
   tb200::grid_dependents_launch();      // the join may take its place
   const size_t dim = (size_t)pieces * V;
   if (hdr->error) {      // the sort's waits ran out
@@ -453,9 +454,8 @@ TB200_API int tb200_embedding_grad(const void* d_dout, size_t dout_stride, const
           const size_t grid = ((shape.chunks * shape.parts << shape.spread) + GRAD_BLOCK - 1) / GRAD_BLOCK;
           if (grid + zero_blocks > 0x7fffffffull) return ERR_INVALID;
           if (grid + zero_blocks == 0) return 0;
-          embedding_grad_kernel<T, O, V, ADD><<<(unsigned)(grid + zero_blocks), GRAD_BLOCK, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, keys, positions, n, (unsigned)rows, pieces,
-                                                                                                     shape, scale, zero_blocks, static_cast<O*>(d_out), partial, list, hdr);
-          const cudaError_t e = cudaGetLastError();
+          const cudaError_t e = tb200::launch_after(embedding_grad_kernel<T, O, V, ADD>, grid + zero_blocks, GRAD_BLOCK, 0, stream, static_cast<const T*>(d_dout), dout_stride, keys, positions, n,
+                                                    (unsigned)rows, pieces, shape, scale, zero_blocks, static_cast<O*>(d_out), partial, list, hdr);
           if (e != cudaSuccess || shape.chunks < 3) return (int)e;
           const size_t items = (join_pieces + 31) / 32 * shape.chunks / 2, most = (size_t)tb200::current_device_info().sm_count * 3;
           return (int)tb200::launch_after(embedding_grad_join_kernel<O, JOIN_V, ADD>, items < most ? items : most, GRAD_BLOCK, 0, stream, keys, join_pieces, shape, scale,
