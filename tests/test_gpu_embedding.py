@@ -96,6 +96,21 @@ def test_each_row_is_summed_or_cleared(tb, n, shift):
         assert torch.equal(tb.embedding_grad(dout, tokens, rows), want)
 
 
+@pytest.mark.parametrize("n", [2, 31, 33, 127, 129, 4095, 4736, 4737, 6001, 8191, 8192, 8193])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_places_of_a_token_are_added_in_their_order(tb, n, index):
+    """Each token occurs four times or so and some are no rows: the sums of so few are taken one after another in 32 bits, so that any other order shows."""
+    rows = n // 4 + 1
+    g = torch.Generator(device="cuda").manual_seed(n)
+    tokens = ((torch.randperm(n, generator=g, device="cuda") % (rows + 3)) - 1).to(index)      # -1 and some behind the last row
+    dout = _normal((n, 12), torch.float32, n + 1)
+    on_host, want = dout.cpu(), torch.zeros(rows, 12)
+    for i, token in enumerate(tokens.tolist()):
+        if 0 <= token < rows:
+            want[token] += on_host[i]
+    assert torch.equal(tb.embedding_grad(dout, tokens, rows).cpu(), want)
+
+
 @pytest.mark.parametrize("n,rows,dim", [(20000, 50, 320), (3001, 3001, 72)])
 def test_gradient_gives_the_same_bits(tb, n, rows, dim):
     dout, tokens = _normal((n, dim), torch.float32, 9), _tokens(n, rows, 10)

@@ -48,6 +48,73 @@ __global__ void __launch_bounds__(256) token_keys_kernel(const I* tokens, size_t
   positions[i] = (unsigned)i;
 }
 
+// The same places, sorted, where there are few: the rank of a place is the number of places whose key is smaller, or the same and further in front.  A CTA has
+// all keys in shared memory, its lanes P places each and its warps a share of the keys each: P = 1 while that makes a CTA a SM at most, so that no SM has twice
+// the others' work.  Bound by n * n additions; one kernel instead of the sort's two.  A whole gradient (bf16 rows of 1000 added to f32) takes 18 us instead of 26
+// for 4099 places and 30 instead of 33 for 8192; for 10000 it would take 40 instead of 34.
+constexpr unsigned PLACE_MOST = 8192, PLACE_BLOCK = 1024;
+// count + (not_key's key < limit): the sum limit + ~key carries then
+__device__ __forceinline__ unsigned count_below(unsigned count, unsigned not_key, unsigned limit) {
+  asm("{.reg .u32 t; add.cc.u32 t, %1, %2; addc.u32 %0, %0, 0;}" : "+r"(count) : "r"(limit), "r"(not_key));
+  return count;
+}
+template <int P, class I>
+__global__ void __launch_bounds__(PLACE_BLOCK) place_kernel(const I* tokens, unsigned n, unsigned rows, unsigned* keys, unsigned* positions, unsigned* counts, tb200::ws_header* hdr) {
+  __shared__ uint4 all[PLACE_MOST / 4];
+  __shared__ unsigned rank[32 * P];
+  tb200::grid_dependents_launch();
+  if (blockIdx.x == 0 && threadIdx.x < 2) counts[threadIdx.x] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) hdr->error = 0;
+  if (threadIdx.x < 32 * P) rank[threadIdx.x] = 0;
+  constexpr unsigned WARPS = PLACE_BLOCK / 32;
+  const unsigned fours = (n + 3) / 4, share = (fours + WARPS - 1) / WARPS;      // of each warp
+  unsigned* const not_key = reinterpret_cast<unsigned*>(all);
+#pragma unroll 4
+  for (unsigned i = threadIdx.x; i < fours * 4; i += PLACE_BLOCK) {
+    const long long tok = i < n ? (long long)tokens[i] : -1;
+    not_key[i] = ~(tok >= 0 && tok < (long long)rows ? (unsigned)tok : i < n ? rows : ~0u);      // the largest behind the last one
+  }
+  __syncthreads();
+  const unsigned lane = threadIdx.x % 32, first = blockIdx.x * 32 * P;
+  const unsigned from = threadIdx.x / 32 * share, to = from + share < fours ? from + share : fours;
+  unsigned mine[P], below[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const unsigned i = first + p * 32 + lane;
+    mine[p] = i < n ? ~not_key[i] : 0;
+    below[p] = 0;
+  }
+  auto count = [&](unsigned a, unsigned b, unsigned more) {
+#pragma unroll 4
+    for (unsigned j = a; j < b; ++j) {
+      const uint4 k = all[j];
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const unsigned limit = mine[p] + more;
+        below[p] = count_below(count_below(count_below(count_below(below[p], k.x, limit), k.y, limit), k.z, limit), k.w, limit);
+      }
+    }
+  };
+  const unsigned here = first / 4, behind = here + 8 * P;      // the fours of this CTA's own places
+  count(from, to < here ? to : here, 1);
+  for (unsigned j = from > here ? from : here; j < to && j < behind; ++j)
+#pragma unroll
+    for (unsigned u = 0; u < 4; ++u)
+#pragma unroll
+      for (int p = 0; p < P; ++p) below[p] = count_below(below[p], not_key[j * 4 + u], mine[p] + (j * 4 + u < first + p * 32 + lane));
+  count(from > behind ? from : behind, to, 0);
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    if (from < to) atomicAdd(&rank[p * 32 + lane], below[p]);
+  __syncthreads();
+  const unsigned i = first + threadIdx.x;
+  if (threadIdx.x < 32 * P && i < n) {
+    const unsigned at = rank[threadIdx.x];
+    keys[at] = ~not_key[i];
+    positions[at] = i;
+  }
+}
+
 // how many of keys[0, n) are below `key`, by a whole warp: 32 probes a round trip
 __device__ __forceinline__ size_t warp_lower_bound(const unsigned* keys, size_t n, unsigned key) {
   size_t lo = 0, hi = n;
@@ -436,13 +503,25 @@ TB200_API int tb200_embedding_grad(const void* d_dout, size_t dout_stride, const
         unsigned* const positions = reinterpret_cast<unsigned*>(base + lay.sort + 2 * lay.array);
         float* const partial = reinterpret_cast<float*>(base + lay.partial);
         long_runs* const list = reinterpret_cast<long_runs*>(base + lay.list);
-        if (n) token_keys_kernel<I><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(static_cast<const I*>(d_tokens), n, (unsigned)rows, keys, positions, &list->few);
-        tb200::key_coding coding;
-        coding.kind = tb200::KEY_UNSIGNED;
-        coding.descending = 0;
-        int bits = 8;
-        while (bits < 32 && (rows >> bits)) bits += 8;      // the largest key is `rows`
-        const cudaError_t e = tb200::radix_sort_async<uint32_t, uint32_t, true>(keys, keys + lay.array / 4, positions, positions + lay.array / 4, n, coding, 0, bits, d_ws, stream);
+        cudaError_t e;
+        if (n && n <= PLACE_MOST) {
+          auto place = [&](auto pv) {
+            constexpr int P = decltype(pv)::value;
+            place_kernel<P, I><<<(unsigned)((n + 32 * P - 1) / (32 * P)), PLACE_BLOCK, 0, stream>>>(static_cast<const I*>(d_tokens), (unsigned)n, (unsigned)rows, keys, positions, &list->few,
+                                                                                                  static_cast<tb200::ws_header*>(d_ws));
+          };
+          if (n <= 32u * (unsigned)tb200::current_device_info().sm_count) place(std::integral_constant<int, 1>());
+          else place(std::integral_constant<int, 2>());
+          e = cudaGetLastError();
+        } else {
+          if (n) token_keys_kernel<I><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(static_cast<const I*>(d_tokens), n, (unsigned)rows, keys, positions, &list->few);
+          tb200::key_coding coding;
+          coding.kind = tb200::KEY_UNSIGNED;
+          coding.descending = 0;
+          int bits = 8;
+          while (bits < 32 && (rows >> bits)) bits += 8;      // the largest key is `rows`
+          e = tb200::radix_sort_async<uint32_t, uint32_t, true>(keys, keys + lay.array / 4, positions, positions + lay.array / 4, n, coding, 0, bits, d_ws, stream);
+        }
         if (e != cudaSuccess) return (int)e;
         auto go = [&](auto vv, auto av) -> int {
           constexpr int V = decltype(vv)::value, JOIN_V = V < 4 ? V : 4;
