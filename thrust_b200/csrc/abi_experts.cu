@@ -35,7 +35,8 @@ __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_count_kernel(const I* i
 // A stable counting sort of the assignments and the rows' way to their places, in one kernel.  A CTA has the assignments of neighbouring tokens.
 // It adds up, by expert, all assignments and those before its own (from the blocks' counts, or from the ids while they are few), ranks its own
 // ones warp by warp, and copies each of its tokens' rows to its places: a row is read once and written as often as it goes somewhere.
-// Bound by the bytes of the rows.
+// Bound by the bytes of the rows, most of them scattered writes: 16384 bf16 rows of 2048 to 8 of 128 experts take 123 us (4900 GB/s), of which counting and
+// ranking are the first 9.  Rows in the order of their places, gathered by their sources, take 144: each is read eight times then.
 template <class V, class I, bool COUNTED>
 __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V* __restrict__ x, size_t xs, const I* __restrict__ ids, size_t n, unsigned choices, unsigned experts,
                                                                        size_t pieces, unsigned spread, V* __restrict__ rows, int* slots, int* sources, int* offsets,
@@ -153,7 +154,8 @@ __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V
 }
 
 // A thread has up to U pieces of a token's result, and requests those of K of its rows at a time.  ALL: K rows are all there are, so that no sums have
-// to be held while rows are on their way: few registers, many reads in flight.
+// to be held while rows are on their way: few registers, many reads in flight.  Bound by the bytes of the rows: 8191 f16 rows of 4096, the sums of two, take
+// 33 us, of which 31 are bytes.
 template <class T, int V, bool WEIGHTED, int K, int U, bool ALL>
 __global__ void __launch_bounds__(256) expert_combine_kernel(const T* __restrict__ rows, size_t rs, unsigned m, const int* __restrict__ slots, const float* __restrict__ weights,
                                                              size_t n, unsigned choices, unsigned pieces, unsigned spread, unsigned parts, T* __restrict__ out) {
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const T* __restrict
 }
 
 // 2^spread lanes a token (WARP: 32, known beforehand, where the rows are long enough): its row of dout stays in registers (while it fits) against the rows of all its choices, each
-// read and written once.
+// read and written once.  Bound by the bytes of the rows: 16384 bf16 rows of 2048 with six choices take 135 us, of which 131 are bytes.
 template <class T, int V, bool WARP>
 __global__ void __launch_bounds__(256) expert_combine_grad_kernel(const T* __restrict__ dout, size_t ds, const T* __restrict__ rows, size_t rs, size_t m, const int* __restrict__ slots,
                                                                   const float* __restrict__ weights, const int* __restrict__ end, size_t n, unsigned choices, size_t pieces,
