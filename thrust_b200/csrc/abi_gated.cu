@@ -114,18 +114,18 @@ template <bool PAIRS, class T> __device__ __forceinline__ void write_pair(T* p, 
   }
 }
 
-// open_gate for two channels: e = exp(-g), keep = 1 / (1 + e), give = e keep.  An e past the largest number makes keep 0 and e keep a NaN, for which
-// give is 1; a NaN gate makes keep a NaN.
+// open_gate for two channels: e = exp(-g), keep = 1 / (1 + e), give = e keep.  From e = 2^25 on give is 1 to 32 bits and is not made from keep, which the
+// reciprocal takes as zero where e is above 2^126; a NaN gate makes keep a NaN.
 struct gates2 { f2 keep, give; };
 __device__ __forceinline__ gates2 open_gates(float2 g) {
-  constexpr float M = -1.4426950408889634f;
+  constexpr float M = -1.4426950408889634f, ALL = 25.f;
   const float2 t = unpack2(mul2(pack2(g.x, g.y), pack2(M, M)));
   const f2 e = pack2(exp2_of(t.x), exp2_of(t.y));
   const float2 d = unpack2(add2(e, pack2(1.f, 1.f)));
   gates2 r;
   r.keep = pack2(one_over(d.x), one_over(d.y));
   const float2 give = unpack2(mul2(e, r.keep));
-  r.give = pack2(fminf(give.x, 1.f), fminf(give.y, 1.f));
+  r.give = pack2(t.x < ALL ? give.x : 1.f, t.y < ALL ? give.y : 1.f);
   return r;
 }
 
