@@ -46,11 +46,14 @@ __device__ __forceinline__ gate_pair open_gate(float g) {
 constexpr float CUT = -1.f;
 
 #ifdef TB200_TEST_HOOKS
-// Test builds only (tests/cpp/gated_waits_test.cu): the copies of window 1 of a cluster's first CTA are announced and not made.
-__device__ unsigned withhold_copies;
+// Test builds only (tests/cpp/gated_waits_test.cu, gated_waits_states_test.cu): the copies of window 1 of a cluster's first CTA are announced and not
+// made; the pairs of window 1 of its last CTA are not sent.
+__device__ unsigned withhold_copies, withhold_pairs;
 __device__ __forceinline__ bool withheld(unsigned w, unsigned rank) { return withhold_copies && w == 1 && rank == 0; }
+__device__ __forceinline__ bool pair_withheld(unsigned w, unsigned rank, unsigned ctas) { return withhold_pairs && w == 1 && rank == ctas - 1; }
 #else
 __device__ __forceinline__ bool withheld(unsigned, unsigned) { return false; }
+__device__ __forceinline__ bool pair_withheld(unsigned, unsigned, unsigned) { return false; }
 #endif
 
 using f2 = unsigned long long;
@@ -228,7 +231,7 @@ __device__ __forceinline__ link join_warps(Shared& sh, unsigned w, const duo& ow
     const unsigned base = tb200::smem_addr(&sh), at = tb200::smem_addr(sh.pairs() + (buffer * pair_slots(ctas) + rank) * 32 + lane) - base, bar = tb200::smem_addr(&sh.met[buffer]) - base;
 #pragma unroll
     for (int k = 0; k < peers<WARPS>::N; ++k)
-      if (warp + k * WARPS < (int)ctas) send_duo(to.base[k] + at, f, to.base[k] + bar);
+      if (warp + k * WARPS < (int)ctas && !pair_withheld(w, rank, ctas)) send_duo(to.base[k] + at, f, to.base[k] + bar);
   }
   return l;
 }
@@ -430,7 +433,7 @@ gated_scan_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
   auto give = [&](held& s, unsigned w) {
     f2 q = 0ull;
     good &= join_ctas<Shared, PACKED>(sh, w, s.l, carry, q, rank, ctas, good);
-    if (!good) { q = nan2(); s.cuts = 0; }
+    if (!good) { q = carry = nan2(); s.cuts = 0; }      // what was folded may be anything
     T* hp = h + (first + p0 + w * window) * dim + c;
     if (s.rows == ROWS && !(PACKED && (s.cuts | s.ends))) {
 #pragma unroll
@@ -640,7 +643,7 @@ gated_scan_grad_kernel(const __grid_constant__ CUtensorMap dh_map, const __grid_
   auto give = [&](held& s, unsigned w) {
     f2 q = 0ull;
     good &= join_ctas<Shared, PACKED>(sh, w, s.l, carry, q, rank, ctas, good);
-    if (!good) { q = nan2(); s.cuts = 0; }
+    if (!good) { q = carry = nan2(); s.cuts = 0; }      // what was folded may be anything
     const long long at = ((long long)first + (long long)length - 1 - (long long)(p0 + w * window)) * (long long)dim + (long long)c;
     T* xp = dx + at;
     T* gp = dgate + at;
