@@ -495,7 +495,7 @@ TB200_API int tb200_embedding_grad(const void* d_dout, size_t dout_stride, const
       return by_index_dtype(token_t, [&](auto iv) -> int {
         using I = decltype(iv);
         if (n >= (1ull << 31) || rows >= (1ull << 31)) return ERR_INVALID;
-        const grad_layout lay(n, dim);
+        const grad_layout lay(n, dim ? dim : 1);      // (no channels: nothing is done below, but the size may be asked for)
         int rc;
         if (workspace_gate(d_ws, ws_bytes, lay.need, rc)) return rc;
         if (rows == 0 || dim == 0) return 0;
