@@ -168,6 +168,13 @@ template <int KB, int VB> struct onesweep_tuning {
 template <class UK, class UV, bool IS_FLOAT> struct radix_pass_policy {
   static constexpr int BITS = RADIX_BITS;       // ballots per key
   UK* dst; UV* vdst; int shift; unsigned dmask;
+  radix_ctrl* ctrl; int pass;
+  // A wait ran out: this pass leaves some places of dst as they were, so that its counts are no longer those that were taken beforehand, by which the
+  // later ones place their items.  They are left out.
+  __device__ __forceinline__ void gave_up() const {
+#pragma unroll 1
+    for (int q = pass + 1; q < (int)sizeof(UK); ++q) ctrl->skip[q] = 1;
+  }
   __device__ __forceinline__ unsigned digit(UK k) const { return key_digit<IS_FLOAT>(k, shift, dmask); }
   __device__ __forceinline__ UK* keys_of(unsigned) const { return dst; }
   __device__ __forceinline__ UV* vals_of(unsigned) const { return vdst; }
@@ -202,6 +209,7 @@ template <class UK, class UV> struct bucket_policy {
   key_coding coding; int buckets;
   const UK* split_code;      // shared memory: buckets - 1 codes, ascending
   UK* const* dst_k; UV* const* dst_v;   // shared memory tables of destination pointers
+  __device__ __forceinline__ void gave_up() const {}
   __device__ __forceinline__ unsigned digit(UK k) const {
     return bucket_of(key_code(k, coding), split_code, buckets);
   }
@@ -321,6 +329,9 @@ __device__ __forceinline__ void onesweep_tile(sweep_regs<UK, UV, HAS_V, IPT>& r,
     for (int w = 0; w < NWARPS; ++w) { first_of[w] = run; run += warp_hist[w * RADIX_BINS + threadIdx.x]; }
     my_count = run;
     if (!FULL && threadIdx.x == PAD_DIGIT) my_count -= (unsigned)TILE - tile_n;
+#ifdef TB200_TEST_HOOKS
+    if (tile || !(reinterpret_cast<const ws_header*>(err)->flags & 1u))      // err points at the header's first word
+#endif
     *reinterpret_cast<volatile LB*>(slot) = (tile == 0 ? (F_VALID | F_INC) : F_VALID) | (LB)my_count;
     const unsigned incl = warp_inclusive_scan(run, plus_op());
     if (lane == 31) s_scan[warp] = incl;
@@ -383,7 +394,7 @@ __device__ __forceinline__ void onesweep_tile(sweep_regs<UK, UV, HAS_V, IPT>& r,
         }
         t -= taken;
         if (taken == 0) {
-          if (++iter > SPIN_LIMIT) { record_error(err, ERR_LOOKBACK_TIMEOUT); break; }
+          if (++iter > SPIN_LIMIT) { record_error(err, ERR_LOOKBACK_TIMEOUT); policy.gave_up(); break; }
           backoff(iter);
         } else {
           iter = 0;
@@ -460,7 +471,7 @@ onesweep_kernel(UK* buf_a, UK* buf_b, UV* val_a, UV* val_b, unsigned n, key_codi
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const int shift = pass * RADIX_BITS;
   using Policy = radix_pass_policy<UK, UV, IS_FLOAT>;
-  const Policy policy{dst, vdst, shift, digit_mask<UK>(coding, shift)};
+  const Policy policy{dst, vdst, shift, digit_mask<UK>(coding, shift), ctrl, pass};
   const unsigned my_bin_base = threadIdx.x < RADIX_BINS ? (unsigned)ctrl->hist[pass][threadIdx.x] : 0u;
   sweep_tiles<UK, UV, HAS_V, Policy, LB, IPT>(src, vsrc, n, &ctrl->tickets[pass], policy, my_bin_base, lookback, &rep->error, smem_raw);
 }
@@ -670,6 +681,7 @@ template <class UK, class UV> struct exchange_policy {
   key_coding coding; int shift;
   const unsigned char* lut;              // shared memory, 4096 entries
   UK* const* dst_k; UV* const* dst_v;    // shared memory tables of destination pointers
+  __device__ __forceinline__ void gave_up() const {}
   __device__ __forceinline__ unsigned digit(UK k) const { return lut[(unsigned)(key_code(k, coding) >> shift) & (EXCH_BINS - 1)]; }
   __device__ __forceinline__ UK* keys_of(unsigned d) const { return dst_k[d]; }
   __device__ __forceinline__ UV* vals_of(unsigned d) const { return dst_v[d]; }
@@ -777,6 +789,9 @@ cudaError_t radix_sort_async(UK* keys_a, UK* keys_b, UV* vals_a, UV* vals_b, siz
   radix_ctrl* ctrl = reinterpret_cast<radix_ctrl*>(base + sizeof(ws_header));
   char* lb0 = base + sizeof(ws_header) + sizeof(radix_ctrl);
   cudaError_t e = cudaMemsetAsync(base, 0, (size_t)(lb0 - base) + lb_bytes * num_passes, stream);
+#ifdef TB200_TEST_HOOKS
+  if (e == cudaSuccess) e = cudaMemsetAsync(&hdr->flags, (int)(test_hook_flags() & 1u), 1, stream);
+#endif
   if (e != cudaSuccess) return e;
 
   const device_info& di = current_device_info();
