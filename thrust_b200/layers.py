@@ -142,6 +142,8 @@ def embedding_grad(dout, tokens, num_rows, scale=1.0, dtype=None, out=None, accu
     out = torch.empty(num_rows, dim, dtype=dtype, device=dout.device) if out is None else out
     args = (dout.data_ptr(), step, tokens.data_ptr(), code, tokens.numel(), num_rows, dim, _ROW_CODE[dout.dtype], _ROW_CODE[dtype], scale, int(accumulate),
             _packed("out", out, dtype, (num_rows, dim), dev))
+    if out.numel() == 0:      # nothing to write: no kernel runs, and the workspace says nothing of this call
+        return out
     if sync:
         _call_and_wait("embedding_grad", "embedding_grad", "tb200_embedding_grad", *args)
     else:
