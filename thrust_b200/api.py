@@ -62,21 +62,39 @@ _HEADER = struct.Struct("<IIQ")
 _HEADER_RESULT, _HEADER_BYTES = 32, 256
 
 
+_stream_captures = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
+
+
 class _Kept:
-    """One kept buffer: the tensor, its address and size as the C ABI takes them, its lock (re-entrant), and where its
-    header is read to."""
-    __slots__ = ("lock", "buf", "ptr", "size", "size_ref", "head")
+    """One kept buffer: the tensor, its address and size as the C ABI takes them, its lock (re-entrant), where its
+    header is read to, and whether a graph uses it; with the smaller ones before it that graphs go on using."""
+    __slots__ = ("lock", "buf", "ptr", "size", "size_ref", "head", "no_graph", "of_graphs")
 
     def __init__(self):
         self.lock = threading.RLock()
         self.head = C.create_string_buffer(_HEADER_BYTES)
-        self.keep(None)
+        self.clear()
 
     def keep(self, buf):
+        if self.buf is not None and self.buf.is_cuda and not self.no_graph:
+            self.of_graphs.append(self.buf)
+        self._set(buf)
+
+    def clear(self):
+        self.of_graphs = []
+        self._set(None)
+
+    def _set(self, buf):
         self.buf = buf
         self.ptr = None if buf is None else buf.data_ptr()
         self.size = C.c_size_t(0 if buf is None else buf.numel())
         self.size_ref = C.byref(self.size)
+        self.no_graph = buf is not None and buf.is_cuda
+
+    def used(self):
+        """A call that is not waited for has been enqueued with the buffer.  If it was captured, the graph will use the buffer whenever it is replayed."""
+        if self.no_graph and _stream_captures():
+            self.no_graph = False
 
 
 class _Workspaces:
@@ -84,7 +102,10 @@ class _Workspaces:
     the reference's per-call temporary_array (thrust/system/cuda/detail/reduce.h:959).
 
     Threads that share a stream share its buffers too, and a call's status, count or result lies in one until it
-    is read back; a call therefore holds the buffer's lock from its first launch to that read-back."""
+    is read back; a call therefore holds the buffer's lock from its first launch to that read-back.
+
+    A buffer that a captured call was given is kept when a larger one replaces it, until clear(): call that when no
+    graph is left that holds calls of this library."""
 
     def __init__(self):
         self._kept = {}
@@ -107,7 +128,7 @@ class _Workspaces:
     def clear(self):
         for kept in list(self._kept.values()):
             with kept.lock:
-                kept.keep(None)
+                kept.clear()
 
 
 workspaces = _Workspaces()
@@ -176,6 +197,7 @@ def _call_with_ws(tag, fn, *args):
     kept = workspaces.at(key)
     with kept.lock:
         _enqueue(key, kept, fn, args)
+        kept.used()
         return kept.buf
 
 
@@ -185,7 +207,10 @@ def _call_and_wait(tag, what, fn, *args, sync=True, key=None):
     key = key or workspaces.key(tag)
     kept = workspaces.at(key)
     with kept.lock:
-        return _enqueue_and_read(key, kept, what, fn, args) if sync else _enqueue(key, kept, fn, args)
+        if sync:
+            return _enqueue_and_read(key, kept, what, fn, args)
+        _enqueue(key, kept, fn, args)
+        kept.used()
 
 
 def _sync_and_check(ws, what):
@@ -266,6 +291,10 @@ def _sort_impl(keys, vals, descending, begin_bit, end_bit, sync=True):
         valt = None if vals is None else workspaces.get("sort_vals_alt", n * vb, key[:2] + ("sort_vals_alt",))
         _call_and_wait("sort", "sort", "tb200_sort_by_key", _ptr(keys), _ptr(kalt), _ptr(vals), _ptr(valt), n,
                        DTYPE_CODE[keys.dtype], vb, int(descending), begin_bit, end_bit, sync=sync, key=key[:2] + ("sort",))
+        if not sync:
+            workspaces.at(key).used()
+            if vals is not None:
+                workspaces.at(key[:2] + ("sort_vals_alt",)).used()
 
 
 def sort(keys, descending=False, sync=True):

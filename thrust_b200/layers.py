@@ -16,7 +16,7 @@ from collections import namedtuple
 import torch
 
 from . import _lib, api
-from .api import _call_and_wait, _check, _raw_stream
+from .api import _call_and_wait, _check, _raw_stream, _stream_captures
 
 __all__ = ["ExpertPlan", "embedding", "embedding_grad", "gated_scan", "gated_scan_grad", "gated_step", "expert_dispatch", "expert_combine",
            "expert_combine_grad", "expert_dispatch_grad"]
@@ -99,6 +99,8 @@ def _enqueue(tag, what, fn, dev, *args):
         if kept.ptr is not None:
             rc = getattr(_lib.load(), fn)(*args, kept.ptr, kept.size_ref, key[1])
             if rc != 1:      # cudaErrorInvalidValue: too small, perhaps
+                if kept.no_graph and _stream_captures():      # _Kept.used
+                    kept.no_graph = False
                 return _check(rc, what)
         _call_and_wait(tag, what, fn, *args, sync=False, key=key)      # made, or made larger, or the error raised
 
