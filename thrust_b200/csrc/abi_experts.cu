@@ -9,6 +9,7 @@ constexpr int MOST_EXPERTS = 1024;
 constexpr int MOST_CHOICES = 32;
 constexpr int DISPATCH_BLOCK = 1024;
 constexpr int SMALL_BLOCK = 256;
+static_assert((2 + SMALL_BLOCK / 32) * MOST_EXPERTS * 4 <= 40 * 1024, "the small block's dynamic shared memory, beside what it has besides");
 constexpr unsigned COUNT_HERE = 8192;      // up to so many assignments every CTA counts them all itself
 
 template <class I> __device__ __forceinline__ unsigned expert_of(const I* ids, size_t i, unsigned experts) {      // `experts` for an id that is none
@@ -293,16 +294,17 @@ TB200_API int tb200_expert_dispatch(const void* d_x, size_t x_stride, const void
       const unsigned experts = (unsigned)num_experts, grid = dispatch_grid(n);
       const bool counted = m > COUNT_HERE;
       unsigned* const table = reinterpret_cast<unsigned*>(static_cast<char*>(d_ws) + sizeof(tb200::ws_header));
-      if (counted) expert_count_kernel<I><<<grid, DISPATCH_BLOCK, 0, stream>>>(static_cast<const I*>(d_experts), n, (unsigned)choices, experts, table);
       auto go = [&](auto vv, auto cv) -> int {
         using V = decltype(vv);
         constexpr bool COUNTED = decltype(cv)::value;
         const int block = COUNTED ? DISPATCH_BLOCK : SMALL_BLOCK;
         const size_t smem = (2 + (size_t)block / 32) * experts * 4;
         auto kernel = expert_dispatch_kernel<V, I, COUNTED>;
-        if (smem > 40 * 1024) {
-          const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (COUNTED) {      // (the smaller block needs no more than any kernel may have)
+          // the most that any call needs: the limit is the kernel's, and calls in other threads may lie between this line and the launch
+          const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 + DISPATCH_BLOCK / 32) * MOST_EXPERTS * 4);
           if (e != cudaSuccess) return (int)e;
+          expert_count_kernel<I><<<grid, DISPATCH_BLOCK, 0, stream>>>(static_cast<const I*>(d_experts), n, (unsigned)choices, experts, table);
         }
         const size_t scale = sizeof(V) / sizeof(T);
         if (COUNTED)      // begins while the blocks are still counted, and waits for that
