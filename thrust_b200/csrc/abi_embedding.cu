@@ -228,8 +228,10 @@ template <int V> __device__ __forceinline__ void read_part(const float* from, fl
   }
 }
 
+// (keys, positions, partial and list are written by the kernels before this one and the join, while they may already be resident: not __restrict__, which would
+// allow loads that are for data that does not change.)
 template <class T, class O, int V, bool ADD>
-__global__ void __launch_bounds__(GRAD_BLOCK, ADD ? 2 : 3) embedding_grad_kernel(const T* __restrict__ dout, size_t stride, const unsigned* __restrict__ keys, const unsigned* __restrict__ positions,
+__global__ void __launch_bounds__(GRAD_BLOCK, ADD ? 2 : 3) embedding_grad_kernel(const T* __restrict__ dout, size_t stride, const unsigned* keys, const unsigned* positions,
                                                                   size_t n, unsigned rows, unsigned pieces, grad_shape shape, float scale, unsigned zero_blocks,
                                                                   O* __restrict__ out, float* __restrict__ partial, long_runs* __restrict__ list, const tb200::ws_header* hdr) {
   tb200::grid_dependency_wait();        // the places are sorted
@@ -353,8 +355,8 @@ __global__ void __launch_bounds__(GRAD_BLOCK, ADD ? 2 : 3) embedding_grad_kernel
 // are added up in order.  (The order of the list is any; each run is by itself.)  About 10 us of those 163, mostly the way to the first part and back.
 constexpr unsigned JOIN_WARPS = GRAD_BLOCK / 32;
 template <class O, int V, bool ADD>
-__global__ void __launch_bounds__(GRAD_BLOCK) embedding_grad_join_kernel(const unsigned* __restrict__ keys, unsigned pieces, grad_shape shape, float scale, O* __restrict__ out,
-                                                                       const float* __restrict__ partial, const long_runs* __restrict__ list, const tb200::ws_header* hdr) {
+__global__ void __launch_bounds__(GRAD_BLOCK) embedding_grad_join_kernel(const unsigned* keys, unsigned pieces, grad_shape shape, float scale, O* __restrict__ out,
+                                                                       const float* partial, const long_runs* list, const tb200::ws_header* hdr) {
   __shared__ size_t behind;            // the first chunk that has no part
   __shared__ float sums[JOIN_WARPS][32][V];
   tb200::grid_dependency_wait();

@@ -38,10 +38,11 @@ __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_count_kernel(const I* i
 // ones warp by warp, and copies each of its tokens' rows to its places: a row is read once and written as often as it goes somewhere.
 // Bound by the bytes of the rows, most of them scattered writes: 16384 bf16 rows of 2048 to 8 of 128 experts take 123 us (4900 GB/s), of which counting and
 // ranking are the first 9.  Rows in the order of their places, gathered by their sources, take 144: each is read eight times then.
+// (table is written while this kernel may already be resident: not __restrict__, which would allow loads that are for data that does not change.)
 template <class V, class I, bool COUNTED>
 __global__ void __launch_bounds__(DISPATCH_BLOCK) expert_dispatch_kernel(const V* __restrict__ x, size_t xs, const I* __restrict__ ids, size_t n, unsigned choices, unsigned experts,
                                                                        size_t pieces, unsigned spread, V* __restrict__ rows, int* slots, int* sources, int* offsets,
-                                                                       const unsigned* __restrict__ table, tb200::ws_header* hdr) {
+                                                                       const unsigned* table, tb200::ws_header* hdr) {
   extern __shared__ unsigned raw[];
   const unsigned warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   unsigned* const total = raw;                    // [experts]
