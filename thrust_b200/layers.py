@@ -279,6 +279,8 @@ def expert_combine_grad(dout, rows, plan, weights):
     dev, n, choices, dim, step, slots = _planned(rows, plan)
     if dout.shape != (n, dim) or dout.dtype != rows.dtype:
         raise ValueError("dout: shape %s and type %s are needed" % ((n, dim), rows.dtype))
+    if weights is None:
+        raise ValueError("weights: expert_combine's are needed (ones, if it was called without)")
     offsets = plan.offsets
     if offsets.dim() != 1 or offsets.numel() < 2:
         raise ValueError("plan.offsets: one more than there are experts")
