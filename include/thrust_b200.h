@@ -352,8 +352,9 @@ int tb200_ipc_close_all(void);
  *
  * Rows hold `dim` neighbouring elements of type t (F32, F16 or BF16); row i of an input begins at i * stride elements
  * (stride >= dim; outputs are packed).  Arithmetic is in 32 bits, rounded once, to nearest, where a result is stored.  Ids are I32 or I64; an
- * id outside its range names nothing: its row of a result is zero and nothing that belongs to it is read.
- * Outputs must not overlap inputs.  The same inputs give the same bits.  None of these has a counterpart in the reference. */
+ * id outside its range names nothing: its row of a result is zero and nothing that belongs to it, NaNs included, reaches a result.
+ * Outputs must not overlap inputs.  The same inputs give the same bits.  A call with nothing to write launches nothing and leaves d_ws, and the
+ * status in it, as they were.  None of these has a counterpart in the reference. */
 
 /* d_out[i] = scale * d_weight[d_tokens[i]] for i < n (n < 2^31); zero where the token is outside [0, rows). */
 int tb200_embedding(const void* d_weight, size_t rows, size_t weight_stride, const void* d_tokens, int token_t,
@@ -372,7 +373,9 @@ int tb200_embedding_grad(const void* d_dout, size_t dout_stride, const void* d_t
  * begun from d_h0[s] (F32, batch x dim, packed; NULL: zero); d_last[s] (F32) is the state behind the sequence's last row, unrounded, or
  * d_h0[s] if it has none.  Sequence s has rows [d_offsets[s], d_offsets[s + 1]) (batch + 1 of type offset_t, not decreasing); d_offsets ==
  * NULL: n / batch rows each, which must divide.  Rows before the first and behind the last offset have h = 0; offsets outside
- * [0, n] are cut off.  The waits between a sequence's CTAs are bounded: one that ran out leaves NaNs from there on and status 1. */
+ * [0, n] are cut off.  The larger of a and 1 - a is good to a few units in its last place, the smaller one to (8 + 1.2 |gate|) 2^-23 of itself; below
+ * 2^-126 it may be zero.  A state that is not finite leaves no later one of its sequence finite; whether those are infinite or NaN is not said.
+ * The waits between a sequence's CTAs are bounded: one that ran out leaves NaNs from there on, in d_last too, and status 1. */
 int tb200_gated_scan(const void* d_x, size_t x_stride, const void* d_gate, size_t gate_stride, const void* d_h0,
                      const void* d_offsets, int offset_t, size_t batch, size_t n, size_t dim, int t, void* d_h,
                      void* d_last, void* d_ws, size_t* ws_bytes, tb200_stream_t stream);

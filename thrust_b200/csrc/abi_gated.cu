@@ -11,8 +11,9 @@ using namespace tb200_rows;
 namespace {
 constexpr int BLOCK = 128;
 
-// keep = 1 / (1 + exp(-g)) and give = 1 - keep, each to a few units in its last place: from e = exp(-|g|), which cannot overflow, so
-// that the smaller of the two is e / (1 + e) and no difference of nearly equal numbers.
+// keep = 1 / (1 + exp(-g)) and give = 1 - keep, from e = exp(-|g|), which cannot overflow, so that the smaller of the two is e / (1 + e) and no difference
+// of nearly equal numbers.  The larger one is good to a few units in its last place, the smaller one to (8 + 1.2 |g|) of 2^-23: the exponential multiplies
+// g by log2 e in 32 bits, and the fast exponential and reciprocal are what the scan's windows have time for (its gates are the longest part of a window).
 struct gate_pair { float keep, give; };
 __device__ __forceinline__ gate_pair open_gate(float g) {
   const float e = __expf(-fabsf(g)), r = __fdividef(1.f, 1.f + e), s = e * r;
@@ -38,11 +39,12 @@ __device__ __forceinline__ gate_pair open_gate(float g) {
 // ring of STAGES stages while earlier windows are worked on, and a lane takes its two channels of a row from there in one access.  Other rows (STAGES
 // = 0) are read channel by channel where they are needed.  Two channels go through the arithmetic side by side (f32x2).
 //
-// What bounds it: with one CTA a chain the bytes (8 x 4096 bf16 rows of 2048: 81 us, 4960 GB/s; their gradient 142 us, 5670 GB/s).  Where a cluster
-// shares a chain, the length of a window: the gates 860 cycles (two exponentials or reciprocals an element: the unit takes eight cycles for a warp's), the
-// pairs' way through the warps 330, to the other CTAs and back 400, the rows 350, of which two CTAs a SM hide a part of one another's (one sequence of 20011
-// bf16 rows of 2560 71 us, of 65537 f32 rows of 1024 142 us).  Taking the next window's gates before this one's pairs have come needs twice the
-// registers, and the CTA that has no room for them costs more than it saves (119 us and 196 when they took 71 and 171).
+// What bounds it: with one CTA a chain the bytes (8 x 4096 bf16 rows of 2048: 82 us, 4910 GB/s; their gradient 143 us, 5620 GB/s, and 153 among other
+// calls).  Where a cluster shares a chain, the length of a window: the gates about 860 cycles (two exponentials or reciprocals an element: the unit takes eight
+// cycles for a warp's), the pairs' way through the warps 330, to the other CTAs and back 400, the rows 350, of which two CTAs a SM hide a part of one another's
+// (one sequence of 20011 bf16 rows of 2560 76 us, its gradient 123, packed 101 and 165; of 65537 f32 rows of 1024 143 us).  Taking the next window's gates
+// before this one's pairs have come needs twice the registers, and the CTA that has no room for them costs more than it saves (119 us and 196 when they took
+// 71 and 171).  A chain has at most 16 CTAs for 64 channels: few channels leave SMs idle, however long the chain is.
 constexpr float CUT = -1.f;
 
 #ifdef TB200_TEST_HOOKS
@@ -153,7 +155,10 @@ template <bool CUTS> __device__ __forceinline__ duo join(duo f, duo g) {
 }
 
 constexpr int MOST_CTAS = tb200::CLUSTER_MAX_CTAS;
-constexpr int MEETINGS = 4;
+constexpr int MEETINGS = 4;       // buffers of pairs; two are needed (join_ctas)
+// Clusters of up to so many CTAs have room for no more pairs, and fold no more.  With room for 16 in all of them fewer clusters fit a SM's shared memory (20011 bf16
+// rows: 60 slices get 9 CTAs each, 92 us and 168 with the gradient, or 6, 115 and 190; 150 slices 3, 242 and 455, or 2, 295 and 524; only the
+// gradient of 100 slices, 5 or 4, is the faster for it, 274 against 295).  Larger clusters fold 16 either way.
 constexpr unsigned FEW_CTAS = 9;
 inline __host__ __device__ unsigned pair_slots(unsigned ctas) { return ctas > FEW_CTAS ? MOST_CTAS : FEW_CTAS; }
 template <class T, int WARPS, int ROWS, int INPUTS, int STAGES> struct tiles_shared {
@@ -242,7 +247,7 @@ template <class Shared> __device__ __forceinline__ void no_pairs_behind(Shared& 
   for (unsigned i = threadIdx.x; i < MEETINGS * spare; i += blockDim.x) sh.pairs()[(i / spare * slots + ctas) * 32 + i % spare] = none;
 }
 // The state before this warp's rows of window w; `carry` goes from before the window to behind it.  false: the cluster's pairs did not come.
-// A CTA sends window w + 1 when it has everything of w - 1, which others sent when they were done with w - 3: four buffers.
+// A CTA sends window w + 1 when it has everything of w, which others sent when all their warps were done with w - 1: two buffers would do.
 template <class Shared, bool CUTS>
 __device__ __forceinline__ bool join_ctas(Shared& sh, unsigned w, const link& l, f2& carry, f2& q, unsigned rank, unsigned ctas, bool good) {
   if (ctas == 1) {
@@ -750,12 +755,13 @@ template <class... Params> const cluster_room& room_for(void (*kernel)(Params...
   return r;
 }
 
-// Whether the chains' slices fill the device by themselves: then one CTA walks a chain, and no pairs travel.
+// Whether the chains' slices fill the device by themselves: then one CTA walks a chain, and no pairs travel.  Sequences of 4096 bf16 rows of 2048, alone / shared:
+// 192 slices 82 / 68 us (gradient 141 / 115), 224 slices 82 / 82 (143 / 138), 256 slices 82 / 84 (143 / 158), 320 slices 107 / 104 (201 / 184).
 inline bool walked_alone(size_t chains, size_t dim) { return chains * ((dim + 63) / 64) >= 200; }
 
 // Launches `kernel` on all chains and slices.  How many CTAs walk a chain together: as many as there are tiles, but no more than let all clusters run at
-// once, since a second round costs more than any window saved (40 slices of 20011 bf16 rows: 9 CTAs 71 us, 7 88, 12 109, of which not all fit; 16 slices of 65537 f32
-// rows: 12 CTAs 150, 9 176, 14 230; 256 slices of 4096 bf16 rows, their gradient: one CTA each 141 us, two 162).
+// once, since a second round costs more than any window saved (40 slices of 20011 bf16 rows: 10 CTAs 76 us, 9 76, 8 83, 7 91, and 11, of which not all fit, 109; 16
+// slices of 65537 f32 rows: 13 CTAs 143, 12 152, 9 178, 14 229).
 template <class Shared, class... Params, class... Args>
 cudaError_t launch_chains(void (*kernel)(Params...), unsigned warps, bool alone, size_t chains, size_t length, size_t dim, cudaStream_t stream, Args... args) {
   const size_t items = chains * ((dim + 63) / 64), tiles = (length + Shared::R - 1) / Shared::R;
@@ -866,7 +872,7 @@ template <class T> bool tile_map(CUtensorMap& map, const void* p, size_t rows, s
 }
 
 // Four warps of 16 rows (backward: of 8), one warp where a chain is no longer than 16.  Two stages leave room for four CTAs a SM; a CTA that walks a chain
-// alone gains from a third (gradient of 8 x 4096 bf16 rows of 2048: 142 us against 151; five: 144).
+// alone gains from a third (8 x 4096 bf16 rows of 2048: 82 us against 88, gradient 143 against 156; five: 83 and 148).
 constexpr int SCAN_WARPS = 4, SCAN_ROWS = 16, GRAD_ROWS = 8, SHORT = 16;
 using few_warps = std::integral_constant<int, SCAN_WARPS>;
 using one_warp = std::integral_constant<int, 1>;

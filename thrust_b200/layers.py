@@ -7,7 +7,7 @@ expert and back, with both gradients (expert_dispatch, expert_combine, expert_co
 Tensors live on the current CUDA device.  Rows are float32, float16 or bfloat16, their channels next to one another; the rows of an
 input may lie further apart than they are long, evenly (one half of a fused projection, say), everything else is contiguous.
 Arithmetic is in 32 bits and rounded once where a result is stored.  Ids are int32 or int64; an id outside its range names
-nothing: its result is zero, and what belongs to it, NaNs included, is not read.
+nothing: its result is zero, and what belongs to it, NaNs included, reaches no result.  Outputs must not overlap inputs.
 
 Every call only enqueues work on the current stream, like reduce_to_device.  There is no fallback path.
 """
@@ -128,7 +128,7 @@ def embedding_grad(dout, tokens, num_rows, scale=1.0, dtype=None, out=None, accu
     """The gradient of embedding's weight: [num_rows, dim] of type dtype (dout's by default), row v = scale * the sum of dout over the
     places of token v.  accumulate: added to `out` (a gradient that several micro-batches share; float32 as a rule).  The order of the
     sums is fixed, so the same inputs give the same bits.  sync: waits for the result and raises if the sort's waits ran out; without
-    it such a failure shows as NaNs."""
+    it such a failure shows as NaNs.  A result without elements is not waited for."""
     dev = _device_of("dout", dout)
     step, code = _row_step("dout", dout, dev), _ids("tokens", tokens, dev)
     dim = dout.shape[-1]
@@ -172,7 +172,8 @@ def gated_scan(x, gate, h0=None, offsets=None, out=None):
     """h[t] = a[t] h[t-1] + (1 - a[t]) x[t] with a = sigmoid(gate), in every channel of every sequence, from h0 (zeros by default).
 
     x, gate: [batch, length, dim], or [rows, dim]: one sequence, or those that `offsets` (ids [sequences + 1], not decreasing) cut the rows
-    into, empty ones among them; rows outside [offsets[0], offsets[-1]) belong to none and have h = 0.  h0: float32 [sequences, dim].
+    into, empty ones among them; rows outside [offsets[0], offsets[-1]) belong to none and have h = 0.  h0: float32 [sequences, dim].  A state that is
+    not finite leaves no later one of its sequence finite.
     Returns (h, last): h as x, last float32 [sequences, dim], the unrounded state behind each sequence (h0's where that is empty)."""
     dev = _device_of("x", x)
     xs, gs = _row_step("x", x, dev), _same("gate", gate, x, dev)
