@@ -45,7 +45,8 @@ struct radix_ctrl {
   unsigned long long hist[RADIX_MAX_PASSES][RADIX_BINS];   // counts, then exclusive bases
   unsigned skip[RADIX_MAX_PASSES];                         // 1: every key shares this digit
   unsigned tickets[RADIX_MAX_PASSES];
-  unsigned pad[48];
+  unsigned gave_up;                                        // a wait of a pass ran out
+  unsigned pad[47];
 };
 
 // ---------------------------------------------------------------- 1. histograms of all digit places
@@ -170,8 +171,10 @@ template <class UK, class UV, bool IS_FLOAT> struct radix_pass_policy {
   UK* dst; UV* vdst; int shift; unsigned dmask;
   radix_ctrl* ctrl; int pass;
   // A wait ran out: this pass leaves some places of dst as they were, so that its counts are no longer those that were taken beforehand, by which the
-  // later ones place their items.  They are left out.
+  // later ones place their items.  They are left out, and so is the copy back: the caller's arrays hold items of the input then (what the passes before
+  // have left there, and perhaps some that this one has moved), the alternate ones may hold anything.
   __device__ __forceinline__ void gave_up() const {
+    ctrl->gave_up = 1;
 #pragma unroll 1
     for (int q = pass + 1; q < (int)sizeof(UK); ++q) ctrl->skip[q] = 1;
   }
@@ -738,7 +741,7 @@ radix_copy_back_kernel(UK* buf_a, const UK* buf_b, UV* val_a, const UV* val_b, s
   grid_dependency_wait();
   int active = 0;
   for (int q = first_pass; q < first_pass + num_passes; ++q) active += ctrl->skip[q] ? 0 : 1;
-  if (!(active & 1)) return;
+  if (!(active & 1) || ctrl->gave_up) return;
   copy_array(buf_a, buf_b, n);
   if constexpr (HAS_V) copy_array(val_a, val_b, n);
 }

@@ -1,5 +1,6 @@
-// The general sort where tile 0 of the digit passes never publishes its counts: the wait for them runs out, status 1 is left, and no pass writes outside the
-// arrays, whatever lay in the alternate buffers; the next call on the same workspace sorts.  Compiled with -DTB200_TEST_HOOKS and a limit of 65536 polls.
+// The general sort where tile 0 of the digit passes never publishes its counts: the wait for them runs out, status 1 is left, no pass writes outside the
+// arrays, and what they hold are items of the input, whatever lay in the alternate buffers; the next call on the same workspace sorts.  Compiled with
+// -DTB200_TEST_HOOKS and a limit of 65536 polls.
 // Every array has as much room again on both sides as it is long, so that what should not be written can be looked at.
 #include <cstdint>
 #include <cstdio>
@@ -47,6 +48,13 @@ template <class UK, class UV, bool HAS_V> static void sorts(size_t n) {
     CHECK(cudaDeviceSynchronize() == cudaSuccess && cudaMemcpy(&status, ws, 4, cudaMemcpyDeviceToHost) == cudaSuccess);
     CHECK(status == (withheld ? tb200::ERR_LOOKBACK_TIMEOUT : tb200::ERR_NONE));
     CHECK(ka.kept() && kb.kept() && va.kept() && vb.kept());
+    if (withheld) {      // some items twice, others not at all, but none that is no item: what a caller looks up by them is there
+      const std::vector<UK> k = ka.back();
+      const std::vector<UV> o = va.back();
+      size_t odd = 0;
+      for (size_t i = 0; i < n; ++i) odd += HAS_V ? o[n + i] >= n || k[n + i] != h[o[n + i]] : k[n + i] == (UK)~(UK)0;
+      CHECK(odd == 0);
+    }
   }
   std::vector<UV> order = v;
   std::stable_sort(order.begin(), order.end(), [&](UV a, UV b) { return h[a] < h[b]; });
