@@ -372,7 +372,7 @@ int tb200_embedding_grad(const void* d_dout, size_t dout_stride, const void* d_t
  *     a = 1 / (1 + exp(-gate[r])),   h[r] = a * h[r - 1] + (1 - a) * x[r],
  * begun from d_h0[s] (F32, batch x dim, packed; NULL: zero); d_last[s] (F32) is the state behind the sequence's last row, unrounded, or
  * d_h0[s] if it has none.  Sequence s has rows [d_offsets[s], d_offsets[s + 1]) (batch + 1 of type offset_t, not decreasing); d_offsets ==
- * NULL: n / batch rows each, which must divide.  Rows before the first and behind the last offset have h = 0; offsets outside
+ * NULL: n / batch rows each, which must divide, batch * ceil(dim / 64) < 2^27.  Rows before the first and behind the last offset have h = 0; offsets outside
  * [0, n] are cut off.  The larger of a and 1 - a is good to a few units in its last place, the smaller one to (8 + 1.2 |gate|) 2^-23 of itself; below
  * 2^-126 it may be zero.  A state that is not finite leaves no later one of its sequence finite; whether those are infinite or NaN is not said.
  * The waits between a sequence's CTAs are bounded: one that ran out leaves NaNs from there on, in d_last too, and status 1. */
