@@ -414,6 +414,62 @@ int tb200_expert_combine_grad(const void* d_dout, size_t dout_stride, const void
                               const int* d_slots, const float* d_weights, const int* d_kept, size_t n, size_t choices,
                               size_t dim, int t, void* d_drows, float* d_dweights, tb200_stream_t stream);
 
+/* How a router scores its experts. */
+enum tb200_scores { TB200_SOFTMAX = 0, TB200_SIGMOID = 1 };
+
+/* Which experts a token goes to, and with what weights: of row i of d_logits (num_experts <= 1024 of type t, logits_stride apart) the `choices` <= 32
+ * best by score + bias, best first, the lower index before an equal one; d_experts[i * choices + c] (-1 where there is none) and d_weights (F32),
+ * scale times the score (without the bias), divided by the sum of the chosen ones' scores if renormalize != 0.
+ *   scores   TB200_SOFTMAX: over the row's open experts; TB200_SIGMOID: 1 / (1 + exp(-logit)).
+ *   d_bias   F32, num_experts; NULL: the order is the logits'.
+ *   open     are experts whose logit, and logit's score + bias, is neither NaN nor -infinity; the others are never chosen.  A row without open experts
+ *            has -1 and weights of zero throughout.
+ *   groups   <= 32, dividing num_experts: only the group_choices best of the groups of neighbouring experts take part, by the sum of the group_best (1 or 2)
+ *            best score + bias of their open experts.
+ * Scores are compared as 64-bit numbers.  Quotients are good where the scores vanish in 32 bits too.  n * choices < 2^30. */
+int tb200_expert_route(const void* d_logits, size_t logits_stride, size_t n, size_t num_experts, int t, const float* d_bias,
+                       size_t choices, int scores, size_t groups, size_t group_choices, int group_best,
+                       int renormalize, float scale, int* d_experts, float* d_weights, tb200_stream_t stream);
+
+/* Its gradient: d_dlogits (packed) from that of d_weights and the chosen d_experts; the choice itself has none, nor has the bias.  A choice outside
+ * [0, num_experts), or of an expert that is not open, has no part; choices of the same expert add up. */
+int tb200_expert_route_grad(const float* d_dweights, const int* d_experts, const void* d_logits, size_t logits_stride,
+                            size_t n, size_t num_experts, size_t choices, int t, int scores, int renormalize,
+                            float scale, void* d_dlogits, tb200_stream_t stream);
+
+/* Activations of an expert's product: silu(x) = x / (1 + exp(-x)); gelu(x) = x times the normal distribution function of x; gated: the outputs are two halves
+ * [a | b], and act(a) * b is what comes of them. */
+enum tb200_activation { TB200_ACT_NONE = 0, TB200_ACT_SILU = 1, TB200_ACT_GELU = 2, TB200_ACT_GATED = 4 /* | SILU or GELU */ };
+
+/* Each expert's rows times its matrix: with expert e's rows in [d_offsets[e], d_offsets[e + 1]) (num_experts + 1 <= 1025 of type offset_t, not
+ * decreasing, cut off at [0, n]),
+ *     before[i] = d_rows[i] W[e] + d_bias[e],   d_out[i] = act(before[i]) + d_residual[i].
+ * W is in x out; element (i, o) of expert e's is at e * expert_stride + i * weight_stride + o, or with inputs_inside != 0 at e * expert_stride + o * weight_stride
+ * + i (experts' matrices must not overlap).  d_bias (packed, num_experts x out) and d_residual may be NULL, and so may d_before (n x out), which a gradient
+ * needs.  d_out is n x out, gated n x out / 2.  Rows that are no expert's are zero in d_out and d_before.  All are of type t; in, out < 2^24, n < 2^31 - 1024.
+ * The size of the workspace depends on all arguments but d_ws: operands that are not made of 16-byte pieces are laid out anew there.
+ * Waits inside a CTA are bounded: one that ran out leaves NaNs and status 1. */
+int tb200_expert_product(const void* d_rows, size_t rows_stride, const void* d_offsets, int offset_t, const void* d_weight,
+                         size_t expert_stride, size_t weight_stride, int inputs_inside, const void* d_bias,
+                         const void* d_residual, size_t residual_stride, int activation, size_t n, size_t num_experts,
+                         size_t in, size_t out, int t, void* d_out, void* d_before, void* d_ws, size_t* ws_bytes,
+                         tb200_stream_t stream);
+
+/* The gradient of `before`, n x width (gated n x 2 width, two halves), from that of act(before); width and dout_stride are d_dout's. */
+int tb200_expert_activation_grad(const void* d_dout, size_t dout_stride, const void* d_before, int activation, size_t n,
+                                 size_t width, int t, void* d_dbefore, tb200_stream_t stream);
+
+/* The gradients of the product: from that of `before` (d_dout, n x out)
+ *     d_drows[i] = d_dout[i] W[e]^T,   d_dweight[e] = the sum over its rows of d_rows[i]^T d_dout[i],   d_dbias[e] = the sum of d_dout[i].
+ * d_dweight is packed, its elements in the order of W's (inputs_inside), of type grad_t (t or F32); with accumulate != 0 the sums are added to it.
+ * d_dbias (F32, num_experts x out) may be NULL.  Rows that are no expert's have d_drows zero and reach no sum; an expert without rows has sums of zero.
+ * The order of the sums is fixed.  The rest as tb200_expert_product. */
+int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, const void* d_rows, size_t rows_stride,
+                              const void* d_offsets, int offset_t, const void* d_weight, size_t expert_stride,
+                              size_t weight_stride, int inputs_inside, size_t n, size_t num_experts, size_t in, size_t out,
+                              int t, int grad_t, int accumulate, void* d_drows, void* d_dweight, float* d_dbias,
+                              void* d_ws, size_t* ws_bytes, tb200_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

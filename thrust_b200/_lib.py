@@ -63,6 +63,11 @@ PROTOTYPES = {
     "tb200_expert_dispatch": [_vp, _sz, _vp, _i, _sz, _sz, _sz, _sz, _i, _vp, _vp, _vp, _vp, _vp, _szp, _vp],
     "tb200_expert_combine": [_vp, _sz, _vp, _vp, _sz, _sz, _sz, _i, _vp, _vp],
     "tb200_expert_combine_grad": [_vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _i, _vp, _vp, _vp],
+    "tb200_expert_route": [_vp, _sz, _sz, _sz, _i, _vp, _sz, _i, _sz, _sz, _i, _i, _f, _vp, _vp, _vp],
+    "tb200_expert_route_grad": [_vp, _vp, _vp, _sz, _sz, _sz, _sz, _i, _i, _i, _f, _vp, _vp],
+    "tb200_expert_product": [_vp, _sz, _vp, _i, _vp, _sz, _sz, _i, _vp, _vp, _sz, _i, _sz, _sz, _sz, _sz, _i, _vp, _vp, _vp, _szp, _vp],
+    "tb200_expert_activation_grad": [_vp, _sz, _vp, _i, _sz, _sz, _i, _vp, _vp],
+    "tb200_expert_product_grad": [_vp, _sz, _vp, _sz, _vp, _i, _vp, _sz, _sz, _i, _sz, _sz, _sz, _sz, _i, _i, _i, _vp, _vp, _vp, _vp, _szp, _vp],
     "tb200_kernel_timing": [_i],
     "tb200_kernel_timing_read": [_i, C.POINTER(C.c_int), C.POINTER(C.c_float), C.POINTER(C.c_int)],
 }

@@ -1,0 +1,865 @@
+// C ABI: tb200_expert_product, tb200_expert_product_grad and tb200_expert_activation_grad.
+#include <cuda.h>
+#include <type_traits>
+
+#include "abi_rows.cuh"
+#include "tensor_core.cuh"
+
+using namespace tb200_abi;
+using namespace tb200_rows;
+
+namespace {
+constexpr int MOST_EXPERTS = 1024;
+constexpr size_t MOST_ROWS = (1ull << 31) - 1024, MOST_CHANNELS = 1ull << 24;
+
+// ---------------------------------------------------------------------------------------------- activations
+// silu(x) = x s(x) with s(x) = 1 / (1 + exp(-x)); gelu(x) = x P(x) with P the normal distribution.  s and 1 - s are made of exp(-|x|), which cannot overflow
+// and keeps the smaller of the two good where it is tiny; P comes from erfc, which does not cancel where P is small.  FAST: s is good to a few 2^-22 (and
+// 2^-24 |x| for the exponential's argument) of itself, for results that are rounded to 16 bits.
+enum : int { ACT_NONE = TB200_ACT_NONE, ACT_SILU = TB200_ACT_SILU, ACT_GELU = TB200_ACT_GELU, ACT_GATED = TB200_ACT_GATED };
+struct sigmoid_pair { float s, other; };
+template <bool FAST> __device__ __forceinline__ sigmoid_pair sigmoid(float x) {
+  float e, r;
+  if (FAST) {
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * fabsf(x)));      // (not .ftz: exp(-88) is not zero)
+    r = __fdividef(1.f, 1.f + e);
+  } else {
+    e = expf(-fabsf(x));
+    r = 1.f / (1.f + e);
+  }
+  sigmoid_pair p;
+  p.s = x >= 0.f ? r : e * r;
+  p.other = x >= 0.f ? e * r : r;
+  return p;
+}
+__device__ __forceinline__ float normal_below(float x) { return 0.5f * erfcf(-0.70710678118654752f * x); }
+template <bool FAST> __device__ __forceinline__ float activated(float x, int kind) { return kind == ACT_SILU ? x * sigmoid<FAST>(x).s : kind == ACT_GELU ? x * normal_below(x) : x; }
+// and its slope
+template <bool FAST> __device__ __forceinline__ float slope(float x, int kind) {
+  if (kind == ACT_SILU) { const sigmoid_pair p = sigmoid<FAST>(x); return p.s * fmaf(x, p.other, 1.f); }
+  return fmaf(x * 0.39894228040143268f, expf(-0.5f * x * x), normal_below(x));
+}
+
+// ---------------------------------------------------------------------------------------------- where the experts' rows are
+// The offsets, cut off at the rows there are, and before each expert how many tiles of up to `tall` rows the experts before it have.
+struct spans { int* at; int* tiles; };
+__device__ __forceinline__ int read_offset(const void* offsets, bool wide, unsigned i, int m) {
+  const long long o = wide ? static_cast<const long long*>(offsets)[i] : (long long)static_cast<const int*>(offsets)[i];
+  return o < 0 ? 0 : o > m ? m : (int)o;
+}
+__device__ __forceinline__ int rows_of(const spans& s, unsigned e) { const int n = s.at[e + 1] - s.at[e]; return n > 0 ? n : 0; }
+__device__ __forceinline__ void read_spans(spans s, const void* offsets, bool wide, unsigned experts, int m, int tall) {
+  for (unsigned e = threadIdx.x; e <= experts; e += blockDim.x) s.at[e] = read_offset(offsets, wide, e, m);
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int sum = 0;
+    for (unsigned base = 0; base < experts; base += 32) {
+      const unsigned e = base + threadIdx.x;
+      const int own = e < experts ? (rows_of(s, e) + tall - 1) / tall : 0;
+      const int upto = tb200::warp_inclusive_scan(own, tb200::plus_op());
+      if (e < experts) s.tiles[e] = sum + upto - own;
+      sum += __shfl_sync(tb200::FULL_MASK, upto, 31);
+    }
+    if (threadIdx.x == 0) s.tiles[experts] = sum;
+  }
+  __syncthreads();
+}
+
+// What one product is made of.  Features are what the lanes of a result's tile stand for, neighbours in memory; `others` what its columns stand for.
+//   BY_ROWS: results are rows, a feature is an output, the contraction goes over k inputs.  BY_EXPERTS: a result is an expert's matrix, others x
+//   features, and the contraction goes over the expert's rows.
+enum : int { BY_ROWS, BY_EXPERTS };
+template <class T> struct product_plan {
+  const void* offsets;
+  bool wide;
+  unsigned experts;
+  int m, k, features, others;
+  int second;                 // gated: where the second half of the features begins in A
+  bool a_mn;                  // A's features are neighbours (else its k)
+  int box;                    // rows in a box of B
+  const T *bias, *residual;
+  size_t residual_stride;
+  T *out, *before;
+  int activation;
+  void* matrix;
+  bool accumulate, first;     // first: of the call's kernels, the one that clears the status
+  tb200::ws_header* hdr;
+};
+struct product_tile { unsigned e; int row, rows, feature, other, depth; };
+
+// Tile t.  By rows: an expert's rows in tiles of equal height (multiples of 16), all features of one before the next.  `e`: the expert of the
+// last tile asked for, from which the search goes on.
+template <int MODE, int WIDE, int BN, class T> __device__ __forceinline__ product_tile tile_at(const product_plan<T>& p, const spans& s, unsigned t, unsigned& e) {
+  product_tile r;
+  const unsigned across = (unsigned)(p.features + WIDE - 1) / WIDE;
+  if (MODE == BY_ROWS) {
+    const unsigned index = t / across;
+    while (index >= (unsigned)s.tiles[e + 1]) ++e;
+    const int n = rows_of(s, e), parts = (n + BN - 1) / BN, tall = ((n + parts - 1) / parts + 15) / 16 * 16, part = (int)(index - s.tiles[e]);
+    r.e = e;
+    r.feature = (int)(t - index * across) * WIDE;
+    r.row = s.at[e] + part * tall;
+    r.rows = n - part * tall < tall ? n - part * tall : tall;
+    r.other = 0;
+    r.depth = p.k;
+  } else {
+    const unsigned down = (unsigned)(p.others + BN - 1) / BN, each = across * down;
+    r.e = t / each;
+    const unsigned in = t - r.e * each, o = in / across;
+    r.feature = (int)(in - o * across) * WIDE;
+    r.other = (int)o * BN;
+    r.rows = p.others - r.other < BN ? p.others - r.other : BN;
+    r.row = s.at[r.e];
+    r.depth = rows_of(s, r.e);
+  }
+  return r;
+}
+template <int MODE, int WIDE, int BN, class T> __device__ __forceinline__ unsigned tiles_of(const product_plan<T>& p, const spans& s) {
+  const unsigned across = (unsigned)(p.features + WIDE - 1) / WIDE;
+  return MODE == BY_ROWS ? across * (unsigned)s.tiles[p.experts] : across * (unsigned)((p.others + BN - 1) / BN) * p.experts;
+}
+
+// rows [first, last) of `width` packed elements are zeros
+template <class T> __device__ __forceinline__ void clear_rows(T* to, size_t first, size_t last, size_t width, size_t thread, size_t threads) {
+  char* const begin = reinterpret_cast<char*>(to + first * width);
+  char* const end = reinterpret_cast<char*>(to + last * width);
+  char* const a = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(begin) + 15) & ~(uintptr_t)15);
+  char* const b = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(end) & ~(uintptr_t)15);
+  if (a >= b) {
+    for (T* q = reinterpret_cast<T*>(begin) + thread; q < reinterpret_cast<T*>(end); q += threads) *q = from_f32<T>(0.f);
+    return;
+  }
+  for (T* q = reinterpret_cast<T*>(begin) + thread; q < reinterpret_cast<T*>(a); q += threads) *q = from_f32<T>(0.f);
+  for (T* q = reinterpret_cast<T*>(b) + thread; q < reinterpret_cast<T*>(end); q += threads) *q = from_f32<T>(0.f);
+  for (uint4* q = reinterpret_cast<uint4*>(a) + thread; q < reinterpret_cast<uint4*>(b); q += threads) *q = make_uint4(0, 0, 0, 0);
+}
+// the rows that are no expert's
+template <class T> __device__ __forceinline__ void clear_others(const product_plan<T>& p, const spans& s, size_t thread, size_t threads) {
+  const size_t first = s.at[0], last = s.at[p.experts] > s.at[0] ? s.at[p.experts] : s.at[0], width = p.features, m = p.m;
+  clear_rows(p.out, 0, first, width, thread, threads);
+  clear_rows(p.out, last, m, width, thread, threads);
+  if (p.before) {
+    const size_t both = p.activation & ACT_GATED ? 2 * width : width;
+    clear_rows(p.before, 0, first, both, thread, threads);
+    clear_rows(p.before, last, m, both, thread, threads);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- 16 bits: tensor cores
+#ifdef TB200_TEST_HOOKS
+// Test builds only: the copies of the first CTA's second tile are announced and not made.
+__device__ unsigned withhold_boxes;
+__device__ __forceinline__ bool withheld(unsigned t) { return withhold_boxes && blockIdx.x == 0 && t == gridDim.x; }
+#else
+__device__ __forceinline__ bool withheld(unsigned) { return false; }
+#endif
+
+constexpr int DEEP = 64;                      // of the contraction, a stage: 128 bytes
+constexpr int TC_THREADS = 192;               // warps 0 to 3 write results, 4 brings operands, 5 multiplies
+constexpr unsigned BOX64 = 64 * DEEP * 2;     // a box of 64 x 64
+
+template <bool GATED, int BN, int STAGES> struct tc_shared {
+  static constexpr unsigned A = 128 * DEEP * 2, STAGE = A * (GATED ? 2 : 1) + BN * DEEP * 2;
+  static constexpr unsigned COLUMNS = 2 * BN * (GATED ? 2 : 1);
+  static_assert(COLUMNS <= 512, "two sets of sums in tensor memory");
+  unsigned long long full[STAGES], empty[STAGES], made[2], taken[2], done;
+  unsigned tmem;
+  int dead;
+  static size_t bytes(unsigned experts) { return 1024 + (size_t)STAGES * STAGE + sizeof(tc_shared) + (2 * (size_t)experts + 2) * 4; }
+};
+// false: it did not come within the limit, or another warp has given up
+__device__ __forceinline__ bool await(unsigned long long* bar, unsigned parity, int* dead, tb200::ws_header* hdr) {
+  for (unsigned iter = 0; iter < tb200::MBAR_SPIN_LIMIT; ++iter) {
+    if (tb200::mbar_try_wait(bar, parity)) return true;
+    if (*(volatile int*)dead) return false;
+  }
+  *(volatile int*)dead = 1;
+  tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
+  return false;
+}
+// at the end, dead or not: what was asked for is not left on its way
+__device__ __forceinline__ void outlast(unsigned long long* bar, unsigned parity) {
+  for (unsigned iter = 0; iter < tb200::MBAR_SPIN_LIMIT && !tb200::mbar_try_wait(bar, parity); ++iter) {}
+}
+
+// results of 32 columns in a lane's registers go to p, p + stride, ...: the warp writes 32 neighbouring features at a time
+template <class O> __device__ __forceinline__ void put_column(O* p, size_t stride, int count, const float (&v)[32]) {
+  if (count >= 32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) p[(size_t)j * stride] = from_f32<O>(v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < count) p[(size_t)j * stride] = from_f32<O>(v[j]);
+  }
+}
+template <class O> __device__ __forceinline__ void get_column(const O* p, size_t stride, int count, O (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j < count) v[j] = p[(size_t)j * stride];
+}
+
+// D^T = A B^T by tiles of 128 features (gated: 128 of each half) x up to BN rows, one CTA a SM, which goes from tile to tile.  Features are the lanes of tensor
+// memory and rows its columns, so that a tile that has few rows takes a narrower instruction and no more time than they need: experts have as many rows as they have.
+//
+// One warp keeps STAGES boxes of A and B on their way by the copy engine, one issues the matrix instructions as they come, four take the sums of the last
+// tile from tensor memory, while the next one's are made in its other half, and write them.  Sums are 32 bits from first to last; they
+// are rounded once, where they are stored, after bias, activation and residual.
+//
+// By experts the contraction ends where the expert's rows do, in the middle of a box: what the box has of the next rows is cleared in shared memory, up to
+// the next 16, where the instructions end.
+template <class T, class O, int MODE, bool GATED, int BN, int STAGES>
+__global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const product_plan<T> p) {
+  using Shared = tc_shared<GATED, BN, STAGES>;
+  extern __shared__ char raw[];
+  char* const stages = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  Shared& sh = *reinterpret_cast<Shared*>(stages + STAGES * Shared::STAGE);
+  spans s;
+  s.at = reinterpret_cast<int*>(&sh + 1);
+  s.tiles = s.at + p.experts + 1;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    if (blockIdx.x == 0 && p.first) p.hdr->error = 0;      // a wait that runs out does so long after this
+    for (int i = 0; i < STAGES; ++i) { tb200::mbar_init(&sh.full[i], 1); tb200::mbar_init(&sh.empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { tb200::mbar_init(&sh.made[i], 1); tb200::mbar_init(&sh.taken[i], 4); }
+    tb200::mbar_init(&sh.done, 1);
+    sh.dead = 0;
+    tb200::mbar_init_fence();
+  }
+  if (warp == 5) tb200_tc::tmem_alloc(&sh.tmem, Shared::COLUMNS);
+  tb200_tc::fence_before_sync();
+  read_spans(s, p.offsets, p.wide, p.experts, p.m, BN);
+  tb200_tc::fence_after_sync();
+  const unsigned tmem = sh.tmem, tiles = tiles_of<MODE, 128, BN>(p, s);
+  constexpr unsigned SETS = GATED ? 2 : 1;
+
+  if (warp == 4) {
+    if (lane == 0) {
+      const unsigned base = tb200::smem_addr(stages);
+      unsigned count = 0, e = 0;      // stages filled so far
+      bool good = true;
+      for (unsigned t = blockIdx.x; good && t < tiles; t += gridDim.x) {
+        const product_tile tile = tile_at<MODE, 128, BN>(p, s, t, e);
+        const int boxes = (tile.rows + p.box - 1) / p.box;
+        const unsigned bytes = Shared::A * SETS + (MODE == BY_ROWS ? boxes * p.box * DEEP * 2 : boxes * BOX64);
+        for (int k = 0; k < tile.depth; k += DEEP, ++count) {
+          const unsigned stage = count % STAGES, to = base + stage * Shared::STAGE;
+          if (!await(&sh.empty[stage], (count / STAGES & 1) ^ 1, &sh.dead, p.hdr)) { good = false; break; }
+          unsigned long long* const bar = &sh.full[stage];
+          tb200::mbar_arrive_expect(bar, bytes);
+          if (withheld(t)) continue;
+          if (MODE == BY_ROWS) {
+            for (unsigned h = 0; h < SETS; ++h) {
+              const int f = tile.feature + (h ? p.second : 0);
+              if (p.a_mn) {
+                tb200_tc::load_box(to + h * Shared::A, &map_a, f, k, tile.e, bar);
+                tb200_tc::load_box(to + h * Shared::A + BOX64, &map_a, f + 64, k, tile.e, bar);
+              } else {
+                tb200_tc::load_box(to + h * Shared::A, &map_a, k, f, tile.e, bar);
+              }
+            }
+            for (int b = 0; b < boxes; ++b) tb200_tc::load_box(to + SETS * Shared::A + b * p.box * DEEP * 2, &map_b, k, tile.row + b * p.box, bar);
+          } else {
+            tb200_tc::load_box(to, &map_a, tile.feature, tile.row + k, bar);
+            tb200_tc::load_box(to + BOX64, &map_a, tile.feature + 64, tile.row + k, bar);
+            for (int b = 0; b < boxes; ++b) tb200_tc::load_box(to + Shared::A + b * BOX64, &map_b, tile.other + b * 64, tile.row + k, bar);
+          }
+        }
+      }
+      // the last of each stage: brought, and no longer needed
+      for (unsigned i = 0; i < STAGES && i < count; ++i) {
+        const unsigned c = count - 1 - i;
+        outlast(&sh.full[c % STAGES], c / STAGES & 1);
+        if (good && !*(volatile int*)&sh.dead) outlast(&sh.empty[c % STAGES], c / STAGES & 1);
+      }
+    }
+  } else if (warp == 5) {
+    const unsigned base = tb200::smem_addr(stages);
+    unsigned count = 0, made = 0, e = 0;
+    bool good = true;
+    const bool a_mn = MODE == BY_EXPERTS || p.a_mn;
+    constexpr bool b_mn = MODE == BY_EXPERTS;
+    const unsigned a_step = tb200_tc::step_of(a_mn), b_step = tb200_tc::step_of(b_mn);
+    for (unsigned t = blockIdx.x; good && t < tiles; t += gridDim.x) {
+      const product_tile tile = tile_at<MODE, 128, BN>(p, s, t, e);
+      if (tile.depth == 0) continue;
+      const unsigned set = made & 1, d = tmem + set * SETS * BN;
+      good = __all_sync(tb200::FULL_MASK, await(&sh.taken[set], (made / 2 & 1) ^ 1, &sh.dead, p.hdr));
+      if (!good) break;
+      ++made;
+      tb200_tc::fence_after_sync();
+      const unsigned what = tb200_tc::instruction(std::is_same<T, bf16>::value, a_mn, b_mn, (tile.rows + 15) / 16 * 16);
+      for (int k = 0; k < tile.depth; k += DEEP, ++count) {
+        const unsigned stage = count % STAGES, from = base + stage * Shared::STAGE;
+        good = __all_sync(tb200::FULL_MASK, await(&sh.full[stage], count / STAGES & 1, &sh.dead, p.hdr));
+        if (!good) break;
+        const int valid = tile.depth - k < DEEP ? tile.depth - k : DEEP, steps = (valid + 15) / 16;
+        if (MODE == BY_EXPERTS && valid < steps * 16) {
+          const int pieces = (steps * 16 - valid) * 8, boxes = 2 + (tile.rows + 63) / 64;
+          for (int i = lane; i < pieces * boxes; i += 32)
+            *reinterpret_cast<uint4*>(stages + stage * Shared::STAGE + i / pieces * BOX64 + valid * 128 + i % pieces * 16) = make_uint4(0, 0, 0, 0);
+          tb200::fence_async_smem();
+          __syncwarp();
+        }
+        tb200_tc::fence_after_sync();
+        if (lane == 0) {
+          unsigned long long a = tb200_tc::operand(from, a_mn, BOX64), b = tb200_tc::operand(from + SETS * Shared::A, b_mn, BOX64);
+          for (int i = 0; i < steps; ++i, a += a_step, b += b_step) {
+            tb200_tc::multiply(d, a, b, what, k > 0 || i > 0);
+            if (GATED) tb200_tc::multiply(d + BN, a + (Shared::A >> 4), b, what, k > 0 || i > 0);
+          }
+          tb200_tc::commit(&sh.empty[stage]);
+        }
+        __syncwarp();
+      }
+      if (good && lane == 0) tb200_tc::commit(&sh.made[set]);
+      __syncwarp();
+    }
+    if (lane == 0) { tb200_tc::commit(&sh.done); outlast(&sh.done, 0); }
+    __syncwarp();
+  } else {
+    unsigned made = 0, e = 0;
+    bool good = true;
+    const bool gated = GATED;
+    const int kind = p.activation & ~ACT_GATED;
+    for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
+      const product_tile tile = tile_at<MODE, 128, BN>(p, s, t, e);
+      const unsigned set = made & 1, d = tmem + (warp * 32u << 16) + set * SETS * BN;
+      if (tile.depth) {
+        if (good) good = __all_sync(tb200::FULL_MASK, await(&sh.made[set], made / 2 & 1, &sh.dead, p.hdr));
+        ++made;
+        tb200_tc::fence_after_sync();
+      }
+      const int f = tile.feature + warp * 32 + lane;
+      const bool there = f < p.features;
+      float b0 = 0.f, b1 = 0.f;
+      if (MODE == BY_ROWS && p.bias && there) {
+        const T* const b = p.bias + (size_t)tile.e * p.features * (gated ? 2 : 1) + f;
+        b0 = to_f32(b[0]);
+        if (gated) b1 = to_f32(b[p.features]);
+      }
+      for (int c = 0; c < tile.rows; c += 32) {
+        float v[32], u[32];
+        if (tile.depth && good) {
+          tb200_tc::tmem_load(v, d + c);
+          if (GATED) tb200_tc::tmem_load(u, d + BN + c);
+          tb200_tc::tmem_load_wait();
+          if (c + 32 >= tile.rows) {      // the last of them: the next sums may be made there
+            tb200_tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tb200::mbar_arrive(&sh.taken[set]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = u[j] = good ? 0.f : __int_as_float(0x7fffffff);
+        }
+        if (!there) continue;
+        const int count = tile.rows - c;
+        if (MODE == BY_ROWS) {
+          const size_t row = (size_t)tile.row + c, width = p.features;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) { v[j] += b0; if (GATED) u[j] += b1; }
+          if (p.before) {
+            T* const q = p.before + row * width * SETS + f;
+            put_column(q, width * SETS, count, v);
+            if (GATED) put_column(q + width, width * SETS, count, u);
+          }
+          if (kind == ACT_SILU) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = activated<true>(v[j], ACT_SILU);
+          } else if (kind == ACT_GELU) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = activated<true>(v[j], ACT_GELU);
+          }
+          if (GATED) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= u[j];
+          }
+          if (p.residual) {
+            T r[32];
+            get_column(p.residual + row * p.residual_stride + f, p.residual_stride, count, r);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < count) v[j] += to_f32(r[j]);
+          }
+          put_column(p.out + row * width + f, width, count, v);
+        } else {
+          O* const q = static_cast<O*>(p.matrix) + ((size_t)tile.e * p.others + tile.other + c) * p.features + f;
+          if (p.accumulate) {
+            if (tile.depth == 0 && good) continue;      // nothing is added
+            O old[32];
+            get_column(q, p.features, count, old);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < count) v[j] += to_f32(old[j]);
+          }
+          put_column(q, p.features, count, v);
+        }
+      }
+    }
+    if (MODE == BY_ROWS) clear_others(p, s, (size_t)blockIdx.x * 128 + threadIdx.x, (size_t)gridDim.x * 128);
+    tb200_tc::fence_before_sync();
+  }
+  __syncthreads();
+  if (warp == 5) {
+    tb200_tc::fence_after_sync();
+    tb200_tc::tmem_free(tmem, Shared::COLUMNS);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- 32 bits: fused multiply-adds
+// Products of 32-bit rows are made by the ordinary units: the matrix instructions round their operands to 11 bits or fewer.  Tiles of 128 features (gated: 64
+// of each half) x BN rows; a thread has 8 features x BN / 16 rows, operands go through registers into two stages of shared memory, read channel by
+// channel from rows of any alignment.  Bound by the multiply-adds.
+constexpr int FMA_THREADS = 256, FMA_DEEP = 16;
+template <int MODE, int BN>
+__global__ void __launch_bounds__(FMA_THREADS, BN == 128 ? 2 : 4) expert_product_f32_kernel(const float* __restrict__ a, size_t a_expert, size_t a_stride, const float* __restrict__ b, size_t b_stride,
+                                                                             const product_plan<float> p) {
+  constexpr int WIDE = 128, ROWS = BN / 16, PAD = 4;
+  __shared__ __align__(16) float sa[2][FMA_DEEP][WIDE + PAD], sb[2][FMA_DEEP][BN + PAD];
+  extern __shared__ int raw_spans[];
+  spans s;
+  s.at = raw_spans;
+  s.tiles = raw_spans + p.experts + 1;
+  if (threadIdx.x == 0 && blockIdx.x == 0 && p.first) p.hdr->error = 0;      // nothing here waits
+  read_spans(s, p.offsets, p.wide, p.experts, p.m, BN);
+  const bool gated = MODE == BY_ROWS && (p.activation & ACT_GATED), a_mn = MODE == BY_EXPERTS || p.a_mn;
+  // tiles are as wide as the features they have: half as wide where they are of two halves
+  const unsigned across = (unsigned)(p.features + (gated ? 63 : 127)) / (gated ? 64 : 128);
+  const unsigned tiles = gated ? across * (unsigned)s.tiles[p.experts] : tiles_of<MODE, WIDE, BN>(p, s);
+  constexpr int NA = FMA_DEEP * WIDE / FMA_THREADS, NB = FMA_DEEP * BN / FMA_THREADS;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  unsigned e = 0;
+  for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const product_tile tile = MODE == BY_ROWS && gated ? tile_at<MODE, 64, BN>(p, s, t, e) : tile_at<MODE, WIDE, BN>(p, s, t, e);
+    float acc[8][ROWS];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j) acc[i][j] = 0.f;
+    float ra[NA], rb[NB];
+    auto fetch = [&](int k0) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        const int at = threadIdx.x + i * FMA_THREADS, k = k0 + (a_mn ? at / WIDE : at % FMA_DEEP), w = a_mn ? at % WIDE : at / FMA_DEEP;
+        const int f = tile.feature + (gated && w >= 64 ? w - 64 : w);
+        const size_t g = (size_t)f + (gated && w >= 64 ? p.second : 0);
+        const bool there = k < tile.depth && f < p.features;
+        if (MODE == BY_ROWS) ra[i] = there ? a[tile.e * a_expert + (a_mn ? (size_t)k * a_stride + g : g * a_stride + k)] : 0.f;
+        else ra[i] = there ? a[((size_t)tile.row + k) * a_stride + g] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int at = threadIdx.x + i * FMA_THREADS;
+        if (MODE == BY_ROWS) {
+          const int k = k0 + at % FMA_DEEP, n = at / FMA_DEEP;
+          rb[i] = k < tile.depth && n < tile.rows ? b[((size_t)tile.row + n) * b_stride + k] : 0.f;
+        } else {
+          const int k = k0 + at / BN, n = at % BN;
+          rb[i] = k < tile.depth && n < tile.rows ? b[((size_t)tile.row + k) * b_stride + tile.other + n] : 0.f;
+        }
+      }
+    };
+    auto keep = [&](int stage) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        const int at = threadIdx.x + i * FMA_THREADS;
+        sa[stage][a_mn ? at / WIDE : at % FMA_DEEP][a_mn ? at % WIDE : at / FMA_DEEP] = ra[i];
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int at = threadIdx.x + i * FMA_THREADS;
+        sb[stage][MODE == BY_ROWS ? at % FMA_DEEP : at / BN][MODE == BY_ROWS ? at / FMA_DEEP : at % BN] = rb[i];
+      }
+    };
+    int stage = 0;
+    if (tile.depth > 0) { fetch(0); keep(0); }
+    __syncthreads();
+    for (int k = 0; k < tile.depth; k += FMA_DEEP, stage ^= 1) {
+      const bool more = k + FMA_DEEP < tile.depth;
+      if (more) fetch(k + FMA_DEEP);
+#pragma unroll
+      for (int i = 0; i < FMA_DEEP; ++i) {
+        float x[8], y[ROWS];
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(&sa[stage][i][tx * 4]);
+        *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(&sa[stage][i][64 + tx * 4]);
+        if constexpr (ROWS == 8) {
+          *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(&sb[stage][i][ty * 4]);
+          *reinterpret_cast<float4*>(y + 4) = *reinterpret_cast<const float4*>(&sb[stage][i][64 + ty * 4]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < ROWS; ++j) y[j] = sb[stage][i][ty * ROWS + j];
+        }
+#pragma unroll
+        for (int f = 0; f < 8; ++f)
+#pragma unroll
+          for (int j = 0; j < ROWS; ++j) acc[f][j] = fmaf(x[f], y[j], acc[f][j]);
+      }
+      if (more) keep(stage ^ 1);
+      __syncthreads();
+    }
+    const size_t width = p.features;
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+      const int n = ROWS == 8 ? (j < 4 ? ty * 4 + j : 60 + ty * 4 + j) : ty * ROWS + j;
+      if (n >= tile.rows) continue;
+      const size_t row = (size_t)tile.row + n;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (gated && i >= 4) continue;
+        const int f = tile.feature + (i < 4 ? tx * 4 + i : 60 + tx * 4 + i);
+        if (f >= p.features) continue;
+        float v = acc[i][j];
+        if (MODE == BY_ROWS) {
+          const int kind = p.activation & ~ACT_GATED;
+          const size_t both = gated ? 2 * width : width;
+          float u = acc[i < 4 ? i + 4 : i][j];
+          if (p.bias) { v += p.bias[tile.e * both + f]; if (gated) u += p.bias[tile.e * both + width + f]; }
+          if (p.before) { p.before[row * both + f] = v; if (gated) p.before[row * both + width + f] = u; }
+          v = activated<false>(v, kind);
+          if (gated) v *= u;
+          if (p.residual) v += p.residual[row * p.residual_stride + f];
+          p.out[row * width + f] = v;
+        } else {
+          float* const q = static_cast<float*>(p.matrix) + ((size_t)tile.e * p.others + tile.other + n) * width + f;
+          *q = p.accumulate ? *q + v : v;
+        }
+      }
+    }
+  }
+  if (MODE == BY_ROWS) clear_others(p, s, (size_t)blockIdx.x * FMA_THREADS + threadIdx.x, (size_t)gridDim.x * FMA_THREADS);
+}
+
+// ---------------------------------------------------------------------------------------------- the smaller parts
+// The gradient of bias: the sums of each expert's rows of dout.  A CTA has 64 features of one of `parts` pieces of an expert's rows; its warps take rows in turn and
+// meet in shared memory, parts meet in a second kernel, always in the same order.
+constexpr int SUM_BLOCK = 256;
+template <class T>
+__global__ void __launch_bounds__(SUM_BLOCK) row_sums_kernel(const T* __restrict__ x, size_t stride, const void* __restrict__ offsets, bool wide, unsigned experts, int m, int features,
+                                                             float* __restrict__ sums) {
+  const unsigned e = blockIdx.y, part = blockIdx.z, parts = gridDim.z;
+  const int a = read_offset(offsets, wide, e, m), end = read_offset(offsets, wide, e + 1, m), n = end > a ? end - a : 0, per = (n + (int)parts - 1) / (int)parts;
+  const int first = a + (int)part * per, last = (int)part * per + per < n ? first + per : a + n;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, f = blockIdx.x * 64 + lane;
+  float u = 0.f, v = 0.f;
+#pragma unroll 8
+  for (int r = first + warp; r < last; r += SUM_BLOCK / 32) {
+    const T* const row = x + (size_t)r * stride;
+    if (f < features) u += to_f32(row[f]);
+    if (f + 32 < features) v += to_f32(row[f + 32]);
+  }
+  __shared__ float met[SUM_BLOCK / 32][64];
+  met[warp][lane] = u;
+  met[warp][lane + 32] = v;
+  __syncthreads();
+  const int g = blockIdx.x * 64 + (int)threadIdx.x;
+  if (threadIdx.x < 64 && g < features) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < SUM_BLOCK / 32; ++w) sum += met[w][threadIdx.x];
+    sums[((size_t)part * experts + e) * features + g] = sum;
+  }
+}
+__global__ void __launch_bounds__(SUM_BLOCK) join_sums_kernel(const float* __restrict__ sums, size_t items, unsigned parts, float* __restrict__ out) {
+  const size_t i = (size_t)blockIdx.x * SUM_BLOCK + threadIdx.x;
+  if (i >= items) return;
+  float sum = 0.f;
+  for (unsigned q = 0; q < parts; ++q) sum += sums[q * items + i];
+  out[i] = sum;
+}
+
+// Rows that the copy engine does not take (they or their distances are not made of 16-byte pieces) as rows that it takes: `halves` pieces of `width` elements,
+// each on a boundary of 8.
+template <class T>
+__global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ from, size_t each, size_t outer, size_t stride, size_t rows, unsigned halves, unsigned width, T* __restrict__ to) {
+  const unsigned wide = (width + 7) / 8;
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * halves * wide) return;
+  const size_t line = i / wide, row = line / halves, c = (i - line * wide) * 8;
+  const T* const f = from + row / each * outer + row % each * stride + (line - row * halves) * width + c;
+  union { T at[8]; uint4 all; } v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v.at[j] = c + j < width ? f[j] : from_f32<T>(0.f);
+  reinterpret_cast<uint4*>(to)[i] = v.all;
+}
+
+// dbefore = dout * the activation's slope; gated with out = act(a) b: da = dout b act'(a), db = dout act(a).  Bound by the bytes.
+template <class T, int V>
+__global__ void __launch_bounds__(256) activation_grad_kernel(const T* __restrict__ dout, size_t stride, const T* __restrict__ before, size_t n, unsigned pieces, bool gated, int kind,
+                                                              T* __restrict__ dbefore) {
+  constexpr bool FAST = sizeof(T) == 2;
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n * pieces) return;
+  const size_t row = i / pieces, c = (i - row * pieces) * V, width = (size_t)pieces * V;
+  const T* const x = before + row * width * (gated ? 2 : 1) + c;
+  T* const to = dbefore + row * width * (gated ? 2 : 1) + c;
+  float d[V], a[V], b[V];
+  const words<T, V> dw = load_words<T, V>(dout + row * stride + c), aw = load_words<T, V>(x);
+  words<T, V> bw = aw;
+  if (gated) bw = load_words<T, V>(x + width);
+  channels(dw, d);
+  channels(aw, a);
+  channels(bw, b);
+  if (gated) {
+    float db[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) db[v] = d[v] * activated<FAST>(a[v], kind);
+    store_words<T, V>(to + width, to_words<T, V>(db));
+#pragma unroll
+    for (int v = 0; v < V; ++v) d[v] *= b[v];
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) d[v] *= slope<FAST>(a[v], kind);
+  store_words<T, V>(to, to_words<T, V>(d));
+}
+
+// ---------------------------------------------------------------------------------------------- calls
+using encode_call = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+encode_call encoder() {
+  static const encode_call call = []() -> encode_call {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+    return reinterpret_cast<encode_call>(f);
+  }();
+  return call;
+}
+// Matrices [count][rows][width], rows `stride` and matrices `outer` elements apart, in boxes of 64 neighbouring elements (128 bytes, swizzled) of `box` rows.
+template <class T> bool box_map(CUtensorMap& map, const void* at, size_t width, size_t rows, size_t stride, size_t count, size_t outer, unsigned box) {
+  const cuuint64_t dims[3] = {width, rows, count}, strides[2] = {stride * 2, (count > 1 ? outer : rows * stride) * 2};
+  const cuuint32_t boxes[3] = {64, box, 1}, steps[3] = {1, 1, 1};
+  return encoder() && encoder()(&map, std::is_same<T, f16>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, count ? 3 : 2, const_cast<void*>(at), dims, strides, boxes,
+                                steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Matrices as a kernel is given them: as they lie, or packed into the workspace.
+struct matrices {
+  const void* at;
+  size_t width, rows, stride, count, outer;      // count 0: one matrix
+  unsigned halves;                               // of the width, each on a boundary of 8
+  bool fits() const { return ((reinterpret_cast<uintptr_t>(at) | stride * 2 | (count > 1 ? outer * 2 : 0)) & 15) == 0 && (halves == 1 || width / halves % 8 == 0); }
+  size_t half() const { return width / halves; }
+  size_t packed_half() const { return (half() + 7) / 8 * 8; }
+  size_t all_rows() const { return rows * (count ? count : 1); }
+  size_t packed_bytes() const { return fits() ? 0 : tb200::align_up(all_rows() * halves * packed_half() * 2, 256); }
+};
+// into `room`, which is moved on; nothing where they fit
+template <class T> cudaError_t pack(matrices& x, char*& room, cudaStream_t stream) {
+  if (x.fits() || x.width == 0 || x.all_rows() == 0) return cudaSuccess;
+  const size_t bytes = x.packed_bytes(), pieces = x.all_rows() * x.halves * (x.packed_half() / 8);
+  if ((pieces + 255) / 256 > 0x7fffffffull) return cudaErrorInvalidValue;
+  pack_rows_kernel<T><<<(unsigned)((pieces + 255) / 256), 256, 0, stream>>>(static_cast<const T*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), reinterpret_cast<T*>(room));
+  x.at = room;
+  x.stride = x.halves * x.packed_half();
+  x.outer = x.rows * x.stride;
+  x.width = x.stride;
+  room += bytes;
+  return cudaGetLastError();
+}
+
+// How many CTAs: as many as can run, or as there can be tiles
+unsigned product_grid(size_t tiles, unsigned a_sm) {
+  const size_t most = (size_t)tb200::current_device_info().sm_count * a_sm;
+  return (unsigned)(tiles < most ? (tiles ? tiles : 1) : most);
+}
+size_t most_row_tiles(size_t m, size_t experts, size_t tall) { return m / tall + (m < experts ? m : experts); }
+
+template <class T, class O, int MODE, bool GATED, int BN, int STAGES>
+cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_plan<T>& p, cudaStream_t stream) {
+  using Shared = tc_shared<GATED, BN, STAGES>;
+  auto kernel = expert_product_kernel<T, O, MODE, GATED, BN, STAGES>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shared::bytes(MOST_EXPERTS));
+  if (e != cudaSuccess) return e;
+  const size_t across = ((size_t)p.features + 127) / 128;
+  const size_t tiles = MODE == BY_ROWS ? across * most_row_tiles(p.m, p.experts, BN) : across * (((size_t)p.others + BN - 1) / BN) * p.experts;
+  kernel<<<product_grid(tiles, 1), TC_THREADS, Shared::bytes(p.experts), stream>>>(a, b, p);
+  return cudaGetLastError();
+}
+
+// out[i] = rows[i] W[e] (+ the rest) of the expert that row i is of.  w: its matrices' rows are inputs (a_mn: the outputs of an input are neighbours), or outputs.
+template <class T> cudaError_t product_by_rows(matrices w, matrices x, product_plan<T> p, char* room, cudaStream_t stream) {
+  const bool gated = (p.activation & ACT_GATED) != 0, few = (size_t)p.m <= (size_t)32 * p.experts;
+  if constexpr (sizeof(T) == 4) {
+    const size_t wide = gated ? 64 : 128;
+    const size_t smem = (2 * (size_t)p.experts + 2) * 4, across = ((size_t)p.features + wide - 1) / wide;
+    p.second = p.features;
+    const float* const a = static_cast<const float*>(w.at);
+    const float* const b = static_cast<const float*>(x.at);
+    if (few) expert_product_f32_kernel<BY_ROWS, 32><<<product_grid(across * most_row_tiles(p.m, p.experts, 32), 4), FMA_THREADS, smem, stream>>>(a, w.outer, w.stride, b, x.stride, p);
+    else expert_product_f32_kernel<BY_ROWS, 128><<<product_grid(across * most_row_tiles(p.m, p.experts, 128), 2), FMA_THREADS, smem, stream>>>(a, w.outer, w.stride, b, x.stride, p);
+    return cudaGetLastError();
+  } else {
+    cudaError_t e = pack<T>(w, room, stream);
+    if (e == cudaSuccess) e = pack<T>(x, room, stream);
+    if (e != cudaSuccess) return e;
+    p.second = p.a_mn ? (int)(w.halves == 2 ? w.width / 2 : 0) : p.features;
+    p.box = few ? 16 : 64;
+    CUtensorMap a = {}, b = {};
+    if (p.k > 0 && (!box_map<T>(a, w.at, w.width, w.rows, w.stride, w.count, w.outer, p.a_mn ? 64 : 128) || !box_map<T>(b, x.at, x.width, x.rows, x.stride, 0, 0, (unsigned)p.box)))
+      return cudaErrorNotSupported;
+    if (gated) return few ? launch_tc<T, T, BY_ROWS, true, 64, 5>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, true, 128, 4>(a, b, p, stream);
+    return few ? launch_tc<T, T, BY_ROWS, false, 64, 8>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, false, 256, 4>(a, b, p, stream);
+  }
+}
+
+// matrix[e][o][f] = the sum over the expert's rows of others[row][o] features[row][f]
+template <class T, class O> cudaError_t product_by_experts(const matrices& features, const matrices& others, const product_plan<T>& p, cudaStream_t stream) {
+  if constexpr (sizeof(T) == 4) {
+    const size_t tiles = (((size_t)p.features + 127) / 128) * (((size_t)p.others + 127) / 128) * p.experts;
+    expert_product_f32_kernel<BY_EXPERTS, 128><<<product_grid(tiles, 2), FMA_THREADS, (2 * (size_t)p.experts + 2) * 4, stream>>>(static_cast<const float*>(features.at), 0, features.stride,
+                                                                                                            static_cast<const float*>(others.at), others.stride, p);
+    return cudaGetLastError();
+  } else {
+    CUtensorMap a = {}, b = {};
+    if (p.m > 0 && (!box_map<T>(a, features.at, features.width, features.rows, features.stride, 0, 0, 64) || !box_map<T>(b, others.at, others.width, others.rows, others.stride, 0, 0, 64)))
+      return cudaErrorNotSupported;
+    return launch_tc<T, O, BY_EXPERTS, false, 256, 4>(a, b, p, stream);
+  }
+}
+
+bool sizes_fit(size_t n, size_t experts, size_t in, size_t out) { return n <= MOST_ROWS && experts >= 1 && experts <= (size_t)MOST_EXPERTS && in < MOST_CHANNELS && out < MOST_CHANNELS; }
+bool activation_known(int a) { return a == ACT_NONE || (a & ~ACT_GATED) == ACT_SILU || (a & ~ACT_GATED) == ACT_GELU; }
+// weight as it lies: an input's outputs are neighbours, or an output's inputs
+matrices weights_of(const void* d_weight, size_t experts, size_t in, size_t out, size_t expert_stride, size_t stride, bool inputs_inside, unsigned halves) {
+  if (inputs_inside) return {d_weight, in, out, stride, experts, expert_stride, 1};
+  return {d_weight, out, in, stride, experts, expert_stride, halves};
+}
+bool weights_fit(size_t experts, size_t in, size_t out, size_t expert_stride, size_t stride, bool inputs_inside) {
+  const size_t width = inputs_inside ? in : out, rows = inputs_inside ? out : in;
+  return stride >= width && (experts == 1 || expert_stride >= (rows ? (rows - 1) * stride + width : 0));
+}
+// how many pieces of an expert's rows are added up side by side
+unsigned sum_parts(size_t n, size_t experts, size_t out) {
+  const size_t ctas = ((out + 63) / 64) * experts, most = (size_t)tb200::current_device_info().sm_count * 8, rows = n / experts / 64;
+  size_t parts = ctas ? most / ctas : 1;
+  if (parts > rows) parts = rows;
+  return (unsigned)(parts < 1 ? 1 : parts > 256 ? 256 : parts);
+}
+}  // namespace
+
+TB200_API int tb200_expert_product(const void* d_rows, size_t rows_stride, const void* d_offsets, int offset_t, const void* d_weight, size_t expert_stride, size_t weight_stride,
+                                   int inputs_inside, const void* d_bias, const void* d_residual, size_t residual_stride, int activation, size_t n, size_t num_experts, size_t in,
+                                   size_t out, int t, void* d_out, void* d_before, void* d_ws, size_t* ws_bytes, tb200_stream_t stream) {
+  return by_row_dtype(t, [&](auto tv) -> int {
+    using T = decltype(tv);
+    return by_index_dtype(offset_t, [&](auto iv) -> int {
+      const bool gated = (activation & ACT_GATED) != 0;
+      if (!sizes_fit(n, num_experts, in, out) || !activation_known(activation) || (gated && out % 2)) return ERR_INVALID;
+      const size_t width = gated ? out / 2 : out;
+      matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, gated ? 2 : 1), x = {d_rows, in, n, rows_stride, 0, 0, 1};
+      int rc;
+      if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header) + (sizeof(T) == 2 ? w.packed_bytes() + x.packed_bytes() : 0), rc)) return rc;
+      if (n == 0 || width == 0) return 0;
+      if (!d_offsets || !d_out || (in && (!d_rows || !d_weight)) || rows_stride < in || (d_residual && residual_stride < width) ||
+          !weights_fit(num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0))
+        return ERR_INVALID;
+      product_plan<T> p = {};
+      p.offsets = d_offsets;
+      p.wide = sizeof(iv) == 8;
+      p.experts = (unsigned)num_experts;
+      p.m = (int)n;
+      p.k = (int)in;
+      p.features = (int)width;
+      p.a_mn = !inputs_inside;
+      p.bias = static_cast<const T*>(d_bias);
+      p.residual = static_cast<const T*>(d_residual);
+      p.residual_stride = residual_stride;
+      p.out = static_cast<T*>(d_out);
+      p.before = static_cast<T*>(d_before);
+      p.activation = activation;
+      p.first = true;
+      p.hdr = static_cast<tb200::ws_header*>(d_ws);
+      return (int)product_by_rows<T>(w, x, p, static_cast<char*>(d_ws) + sizeof(tb200::ws_header), stream);
+    });
+  });
+}
+
+TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, const void* d_rows, size_t rows_stride, const void* d_offsets, int offset_t, const void* d_weight,
+                                        size_t expert_stride, size_t weight_stride, int inputs_inside, size_t n, size_t num_experts, size_t in, size_t out, int t, int grad_t,
+                                        int accumulate, void* d_drows, void* d_dweight, float* d_dbias, void* d_ws, size_t* ws_bytes, tb200_stream_t stream) {
+  return by_row_dtype(t, [&](auto tv) -> int {
+    using T = decltype(tv);
+    if (grad_t != t && grad_t != TB200_F32) return ERR_UNSUPPORTED;
+    return by_index_dtype(offset_t, [&](auto iv) -> int {
+      if (!sizes_fit(n, num_experts, in, out)) return ERR_INVALID;
+      matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, 1), x = {d_rows, in, n, rows_stride, 0, 0, 1},
+               d = {d_dout, out, n, dout_stride, 0, 0, 1};
+      const unsigned parts = d_dbias ? sum_parts(n, num_experts, out) : 1;
+      const size_t sums = parts > 1 ? tb200::align_up((size_t)parts * num_experts * out * 4, 256) : 0;
+      int rc;
+      if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header) + sums + (sizeof(T) == 2 ? w.packed_bytes() + x.packed_bytes() + d.packed_bytes() : 0), rc)) return rc;
+      if (out == 0 && (n == 0 || in == 0)) return 0;
+      if (!d_offsets || (in && n && (!d_drows || (out && (!d_rows || !d_weight)))) || (in && out && !d_dweight) || (out && n && !d_dout) || rows_stride < in || dout_stride < out ||
+          !weights_fit(num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0))
+        return ERR_INVALID;
+      char* room = static_cast<char*>(d_ws) + sizeof(tb200::ws_header);
+      float* const partial = reinterpret_cast<float*>(room);
+      room += sums;
+      cudaError_t e = cudaSuccess;
+      if constexpr (sizeof(T) == 2) {
+        e = pack<T>(w, room, stream);
+        if (e == cudaSuccess) e = pack<T>(x, room, stream);
+        if (e == cudaSuccess) e = pack<T>(d, room, stream);
+        if (e != cudaSuccess) return (int)e;
+      }
+      product_plan<T> p = {};
+      p.offsets = d_offsets;
+      p.wide = sizeof(iv) == 8;
+      p.experts = (unsigned)num_experts;
+      p.m = (int)n;
+      p.hdr = static_cast<tb200::ws_header*>(d_ws);
+      p.first = true;
+      if (n && in) {
+        product_plan<T> q = p;
+        q.k = (int)out;
+        q.features = (int)in;
+        q.a_mn = inputs_inside != 0;
+        q.out = static_cast<T*>(d_drows);
+        e = product_by_rows<T>(w, d, q, room, stream);
+        if (e != cudaSuccess) return (int)e;
+        p.first = false;
+      }
+      if (in && out) {
+        const matrices &inside = inputs_inside ? x : d, &around = inputs_inside ? d : x;
+        p.features = (int)(inputs_inside ? in : out);
+        p.others = (int)(inputs_inside ? out : in);
+        p.box = 64;
+        p.matrix = d_dweight;
+        p.accumulate = accumulate != 0;
+        e = grad_t == t ? product_by_experts<T, T>(inside, around, p, stream) : product_by_experts<T, float>(inside, around, p, stream);
+        if (e != cudaSuccess) return (int)e;
+      }
+      if (d_dbias && out) {
+        float* const to = parts > 1 ? partial : d_dbias;
+        row_sums_kernel<T><<<dim3((unsigned)((out + 63) / 64), (unsigned)num_experts, parts), SUM_BLOCK, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, d_offsets, sizeof(iv) == 8,
+                                                                                                                (unsigned)num_experts, (int)n, (int)out, to);
+        if (parts > 1) join_sums_kernel<<<(unsigned)((num_experts * out + SUM_BLOCK - 1) / SUM_BLOCK), SUM_BLOCK, 0, stream>>>(partial, num_experts * out, parts, d_dbias);
+        e = cudaGetLastError();
+      }
+      return (int)e;
+    });
+  });
+}
+
+TB200_API int tb200_expert_activation_grad(const void* d_dout, size_t dout_stride, const void* d_before, int activation, size_t n, size_t width, int t, void* d_dbefore,
+                                           tb200_stream_t stream) {
+  return by_row_dtype(t, [&](auto tv) -> int {
+    using T = decltype(tv);
+    const bool gated = (activation & ACT_GATED) != 0;
+    if (!activation_known(activation) || activation == ACT_NONE || n > MOST_ROWS || width >= MOST_CHANNELS) return ERR_INVALID;
+    if (n == 0 || width == 0) return 0;
+    if (!d_dout || !d_before || !d_dbefore || dout_stride < width) return ERR_INVALID;
+    auto go = [&](auto vv) -> int {
+      constexpr int V = decltype(vv)::value;
+      const size_t grid = (n * (width / V) + 255) / 256;
+      if (grid > 0x7fffffffull) return ERR_INVALID;
+      activation_grad_kernel<T, V><<<(unsigned)grid, 256, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, static_cast<const T*>(d_before), n, (unsigned)(width / V), gated,
+                                                                      activation & ~ACT_GATED, static_cast<T*>(d_dbefore));
+      return (int)cudaGetLastError();
+    };
+    if (in_16_bytes(d_dout, width, dout_stride, sizeof(T)) && in_16_bytes(d_before, width, width, sizeof(T)) && in_16_bytes(d_dbefore, width, width, sizeof(T)))
+      return go(std::integral_constant<int, 16 / sizeof(T)>());
+    return go(std::integral_constant<int, 1>());
+  });
+}

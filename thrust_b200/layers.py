@@ -2,7 +2,8 @@
 
 Rows looked up by token and the gradient of the table (embedding, embedding_grad); a gated linear recurrence along
 sequences, its gradient, and its form for one token of each sequence (gated_scan, gated_scan_grad, gated_step); rows sorted by
-expert and back, with both gradients (expert_dispatch, expert_combine, expert_combine_grad, expert_dispatch_grad).
+expert and back, with both gradients (expert_dispatch, expert_combine, expert_combine_grad, expert_dispatch_grad); which experts a token
+goes to (expert_route, expert_route_grad) and what they make of its row (expert_product, expert_activation_grad, expert_product_grad).
 
 Tensors live on the current CUDA device.  Rows are float32, float16 or bfloat16, their channels next to one another; the rows of an
 input may lie further apart than they are long, evenly (one half of a fused projection, say), everything else is contiguous.
@@ -19,11 +20,13 @@ from . import _lib, api
 from .api import _call_and_wait, _check, _raw_stream, _stream_captures
 
 __all__ = ["ExpertPlan", "embedding", "embedding_grad", "gated_scan", "gated_scan_grad", "gated_step", "expert_dispatch", "expert_combine",
-           "expert_combine_grad", "expert_dispatch_grad"]
+           "expert_combine_grad", "expert_dispatch_grad", "expert_route", "expert_route_grad", "expert_product", "expert_activation_grad", "expert_product_grad"]
 
 _ROW_CODE = {torch.float32: 8, torch.float16: 10, torch.bfloat16: 11}
 _ID_CODE = {torch.int32: 4, torch.int64: 6}
 _F32, _I32 = torch.float32, torch.int32
+_SCORES = {"softmax": 0, "sigmoid": 1}
+_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gated_silu": 5, "gated_gelu": 6}
 
 #: What expert_dispatch found out: slots [tokens, choices], the place of each assignment among the rows (-1: none); sources
 #: [tokens * choices], the assignment (token * choices + choice) at each place (-1 behind the last); offsets [experts + 1],
@@ -297,3 +300,152 @@ def expert_combine_grad(dout, rows, plan, weights):
 def expert_dispatch_grad(drows, plan):
     """The gradient of expert_dispatch's x: each token's rows added up."""
     return expert_combine(drows, plan)
+
+
+# ---------------------------------------------------------------------------------- routing
+def _logits(logits, choices, scores):
+    dev = _device_of("logits", logits)
+    step = _row_step("logits", logits, dev)
+    if logits.dim() != 2 or not 1 <= logits.shape[1] <= 1024:
+        raise ValueError("logits: [tokens, experts] of 1 to 1024 experts is needed")
+    if not 1 <= choices <= min(32, logits.shape[1]) or logits.shape[0] * choices >= 1 << 30:
+        raise ValueError("choices: 1 to 32, no more than there are experts, and less than 2^30 in all")
+    if scores not in _SCORES:
+        raise ValueError('scores: "softmax" or "sigmoid"')
+    return dev, step
+
+
+def expert_route(logits, choices, scores="softmax", bias=None, groups=1, group_choices=None, group_best=2, renormalize=True, scale=1.0):
+    """Which experts each token goes to: of logits [tokens, experts] the `choices` best by score + bias, the best first, the lower index
+    before an equal one.  scores: "softmax" over the token's open experts, or "sigmoid"; bias: float32 [experts], which takes part in the choice
+    alone.  An expert whose logit, or score + bias, is NaN or -infinity is not open and never chosen.  groups: only the group_choices (all by
+    default) best of so many equal groups of neighbouring experts take part, by the sum of their group_best (1 or 2) best score + bias.
+    Returns (experts, weights): int32 [tokens, choices], -1 where no open expert is left (expert_dispatch drops it); float32, scale times the
+    score, divided by the sum of the chosen ones' scores if renormalize, 0 where no expert is.  Scores are compared as 64-bit numbers."""
+    dev, step = _logits(logits, choices, scores)
+    n, e = logits.shape
+    group_choices = groups if group_choices is None else group_choices
+    if not 1 <= groups <= 32 or e % groups or not 1 <= group_choices <= groups or group_best not in (1, 2):
+        raise ValueError("groups: 1 to 32 that divide the experts, group_choices: 1 to groups, group_best: 1 or 2")
+    experts = torch.empty(n, choices, dtype=_I32, device=logits.device)
+    weights = torch.empty(n, choices, dtype=_F32, device=logits.device)
+    _check(_lib.load().tb200_expert_route(logits.data_ptr(), step, n, e, _ROW_CODE[logits.dtype], _maybe("bias", bias, _F32, (e,), dev), choices, _SCORES[scores], groups,
+                                          group_choices, group_best, int(renormalize), scale, experts.data_ptr(), weights.data_ptr(), _raw_stream(dev)), "expert_route")
+    return experts, weights
+
+
+def expert_route_grad(dweights, experts, logits, scores="softmax", renormalize=True, scale=1.0):
+    """The gradient of expert_route's logits, of their type, from that of its weights; experts is what it returned.  The choice has none, nor has
+    the bias.  A choice that is no open expert has no part; choices of the same expert add up."""
+    if experts.dim() != 2:
+        raise ValueError("experts: [tokens, choices] is needed")
+    choices = experts.shape[1]
+    dev, step = _logits(logits, choices, scores)
+    n, e = logits.shape
+    dlogits = torch.empty(n, e, dtype=logits.dtype, device=logits.device)
+    _check(_lib.load().tb200_expert_route_grad(_packed("dweights", dweights, _F32, (n, choices), dev), _packed("experts", experts, _I32, (n, choices), dev), logits.data_ptr(), step, n, e,
+                                               choices, _ROW_CODE[logits.dtype], _SCORES[scores], int(renormalize), scale, dlogits.data_ptr(), _raw_stream(dev)), "expert_route_grad")
+    return dlogits
+
+
+# ---------------------------------------------------------------------------------- experts' products
+def _matrices(what, t, dev):
+    """How [experts, in, out] lies: (experts' distance, rows' distance, whether inputs are neighbours instead of outputs)."""
+    if t.get_device() != dev:
+        raise ValueError("%s: a tensor on the current CUDA device is needed" % what)
+    if t.dim() != 3 or not 1 <= t.shape[0] <= 1024 or max(t.shape[1:]) >= 1 << 24:
+        raise ValueError("%s: [experts, in, out] of 1 to 1024 experts and less than 2^24 channels is needed" % what)
+    experts, inputs, outputs = t.shape
+    if t.is_contiguous():
+        return inputs * outputs, outputs, 0
+    each, i, o = t.stride()
+    for inside, size, step, near, rows in ((0, outputs, i, o, inputs), (1, inputs, o, i, outputs)):
+        if size == 1:
+            near = 1
+        if rows == 1:
+            step = size
+        if near == 1 and step >= size and (experts == 1 or each >= (rows - 1) * step + size):
+            return each if experts > 1 else rows * step, step, inside
+    raise ValueError("%s: inputs or outputs must be neighbours, and nothing may overlap: make it contiguous" % what)
+
+
+def _rows_and_experts(rows, offsets, weight):
+    dev = _device_of("rows", rows)
+    step, code = _row_step("rows", rows, dev), _ids("offsets", offsets, dev)
+    lies = _matrices("weight", weight, dev)
+    if weight.dtype != rows.dtype or rows.dim() != 2 or rows.shape[1] != weight.shape[1]:
+        raise ValueError("rows: [rows, in] and weight: [experts, in, out] of one type are needed")
+    if offsets.dim() != 1 or offsets.numel() != weight.shape[0] + 1:
+        raise ValueError("offsets: one more than there are experts")
+    return dev, step, code, lies
+
+
+def expert_product(rows, offsets, weight, bias=None, activation=None, residual=None, keep=False):
+    """Each expert's rows times its matrix: before[i] = rows[i] @ weight[e] + bias[e] for the rows from offsets[e] to offsets[e + 1] (ids [experts + 1],
+    not decreasing: expert_dispatch's plan.offsets), out = act(before) + residual; rows that are no expert's are zero.
+
+    rows [n, in], weight [experts, in, out], contiguous or the transpose of such (out, in) matrices, bias [experts, out], residual as out, all of one
+    type.  activation: None, "silu", "gelu" (by the error function), or "gated_silu", "gated_gelu": the outputs are halves [a | b], and act(a) * b comes
+    of them.  Sums are 32 bits, rounded once.  Returns out [n, out] (gated: [n, out / 2]); with keep (out, before), before [n, out] for expert_activation_grad."""
+    dev, step, code, lies = _rows_and_experts(rows, offsets, weight)
+    if activation not in _ACTIVATIONS:
+        raise ValueError("activation: None, or one of %s" % ", ".join(k for k in _ACTIVATIONS if k))
+    (experts, inputs, outputs), n, dtype, act = weight.shape, rows.shape[0], rows.dtype, _ACTIVATIONS[activation]
+    if act & 4 and outputs % 2:
+        raise ValueError("weight: a gated activation needs two halves of outputs")
+    width = outputs // 2 if act & 4 else outputs
+    to, extra = None, 0
+    if residual is not None:
+        if residual.shape != (n, width) or residual.dtype != dtype:
+            raise ValueError("residual: shape %s and type %s are needed" % ((n, width), dtype))
+        to, extra = residual.data_ptr(), _row_step("residual", residual, dev)
+    out = torch.empty(n, width, dtype=dtype, device=rows.device)
+    before = torch.empty(n, outputs, dtype=dtype, device=rows.device) if keep else None
+    _enqueue("expert_product", "expert_product", "tb200_expert_product", dev, rows.data_ptr(), step, offsets.data_ptr(), code, weight.data_ptr(), *lies,
+             _maybe("bias", bias, dtype, (experts, outputs), dev), to, extra, act, n, experts, inputs, outputs, _ROW_CODE[dtype], out.data_ptr(),
+             before.data_ptr() if keep else None)
+    return (out, before) if keep else out
+
+
+def expert_activation_grad(dout, before, activation):
+    """The gradient of what expert_product kept, from that of act(before): dout [n, width], before [n, width], or [n, 2 width] of a gated activation."""
+    dev = _device_of("before", before)
+    act = _ACTIVATIONS.get(activation, 0)
+    if not act:
+        raise ValueError("activation: one of %s" % ", ".join(k for k in _ACTIVATIONS if k))
+    if before.dim() != 2 or dout.dim() != 2 or before.shape != (dout.shape[0], dout.shape[1] * (2 if act & 4 else 1)) or dout.dtype != before.dtype or before.dtype not in _ROW_CODE:
+        raise ValueError("dout: [n, width] and before: [n, width], gated [n, 2 width], of one type are needed")
+    n, width = dout.shape
+    dbefore = torch.empty(before.shape, dtype=before.dtype, device=before.device)
+    _check(_lib.load().tb200_expert_activation_grad(dout.data_ptr(), _row_step("dout", dout, dev), _packed("before", before, before.dtype, before.shape, dev), act, n, width,
+                                                    _ROW_CODE[before.dtype], dbefore.data_ptr(), _raw_stream(dev)), "expert_activation_grad")
+    return dbefore
+
+
+def expert_product_grad(dout, rows, offsets, weight, bias=False, dtype=None, out=None, accumulate=False):
+    """The gradients of expert_product's rows, weight and (with bias) bias, from dout, that of `before` (expert_activation_grad's result; without an
+    activation out's; the residual's gradient is out's itself).  The gradient of weight is of type dtype (weight's by default, or float32) and lies as weight
+    does; accumulate: added to `out` (a gradient that several micro-batches share).  Returns (drows, dweight, dbias): as rows, as weight or `out`, and
+    float32 [experts, out] or None.  The order of the sums is fixed: the same inputs give the same bits."""
+    dev, step, code, lies = _rows_and_experts(rows, offsets, weight)
+    (experts, inputs, outputs), n = weight.shape, rows.shape[0]
+    if dout.shape != (n, outputs) or dout.dtype != rows.dtype:
+        raise ValueError("dout: shape %s and type %s are needed" % ((n, outputs), rows.dtype))
+    dstep = _row_step("dout", dout, dev)
+    if accumulate and out is None:
+        raise ValueError("accumulate adds to `out`")
+    dtype = out.dtype if out is not None and dtype is None else dtype or weight.dtype
+    if dtype not in (weight.dtype, _F32):
+        raise ValueError("dtype: weight's, or float32")
+    inside = lies[2]
+    if out is None:
+        out = torch.empty((experts, outputs, inputs) if inside else weight.shape, dtype=dtype, device=rows.device)
+        out = out.transpose(1, 2) if inside else out
+    if out.shape != weight.shape:
+        raise ValueError("out: shape %s is needed" % (tuple(weight.shape),))
+    to = _packed("out", out.transpose(1, 2) if inside else out, dtype, (experts, outputs, inputs) if inside else (experts, inputs, outputs), dev)
+    drows = torch.empty(n, inputs, dtype=rows.dtype, device=rows.device)
+    dbias = torch.empty(experts, outputs, dtype=_F32, device=rows.device) if bias else None
+    _enqueue("expert_product_grad", "expert_product_grad", "tb200_expert_product_grad", dev, dout.data_ptr(), dstep, rows.data_ptr(), step, offsets.data_ptr(), code, weight.data_ptr(),
+             *lies, n, experts, inputs, outputs, _ROW_CODE[rows.dtype], _ROW_CODE[dtype], int(accumulate), drows.data_ptr(), to, dbias.data_ptr() if bias else None)
+    return drows, out, dbias
