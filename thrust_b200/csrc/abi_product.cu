@@ -76,7 +76,8 @@ template <class T> struct product_plan {
   int m, k, features, others;
   int second;                 // gated: where the second half of the features begins in A
   bool a_mn;                  // A's features are neighbours (else its k)
-  int box;                    // rows in a box of B
+  int a_chunks, b_chunks;     // MN-major: how many 64 neighbours there are in a box
+  int box;                    // K-major: rows in a box of B
   const T *bias, *residual;
   size_t residual_stride;
   T *out, *before;
@@ -194,9 +195,13 @@ template <class O> __device__ __forceinline__ void put_column(O* p, size_t strid
   }
 }
 template <class O> __device__ __forceinline__ void get_column(const O* p, size_t stride, int count, O (&v)[32]) {
+  if (count >= 32) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (j < count) v[j] = p[(size_t)j * stride];
+    for (int j = 0; j < 32; ++j) v[j] = p[(size_t)j * stride];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = p[(size_t)(j < count ? j : count - 1) * stride];      // (no branch between the requests)
+  }
 }
 
 // D^T = A B^T by tiles of 128 features (gated: 128 of each half) x up to BN rows, one CTA a SM, which goes from tile to tile.  Features are the lanes of tensor
@@ -234,44 +239,46 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
   constexpr unsigned SETS = GATED ? 2 : 1;
 
   if (warp == 4) {
-    if (lane == 0) {
-      const unsigned base = tb200::smem_addr(stages);
-      unsigned count = 0, e = 0;      // stages filled so far
-      bool good = true;
-      for (unsigned t = blockIdx.x; good && t < tiles; t += gridDim.x) {
-        const product_tile tile = tile_at<MODE, 128, BN>(p, s, t, e);
-        const int boxes = (tile.rows + p.box - 1) / p.box;
-        const unsigned bytes = Shared::A * SETS + (MODE == BY_ROWS ? boxes * p.box * DEEP * 2 : boxes * BOX64);
-        for (int k = 0; k < tile.depth; k += DEEP, ++count) {
-          const unsigned stage = count % STAGES, to = base + stage * Shared::STAGE;
-          if (!await(&sh.empty[stage], (count / STAGES & 1) ^ 1, &sh.dead, p.hdr)) { good = false; break; }
-          unsigned long long* const bar = &sh.full[stage];
+    const unsigned base = tb200::smem_addr(stages);
+    unsigned count = 0, e = 0;      // stages filled so far
+    bool good = true;
+    for (unsigned t = blockIdx.x; good && t < tiles; t += gridDim.x) {
+      const product_tile tile = tile_at<MODE, 128, BN>(p, s, t, e);
+      const int boxes = MODE == BY_ROWS ? (tile.rows + p.box - 1) / p.box : (tile.rows + p.b_chunks * 64 - 1) / (p.b_chunks * 64);
+      const unsigned b_box = MODE == BY_ROWS ? p.box * DEEP * 2 : p.b_chunks * BOX64, bytes = Shared::A * SETS + boxes * b_box;
+      for (int k = 0; k < tile.depth; k += DEEP, ++count) {
+        const unsigned stage = count % STAGES, to = base + stage * Shared::STAGE;
+        good = __all_sync(tb200::FULL_MASK, await(&sh.empty[stage], (count / STAGES & 1) ^ 1, &sh.dead, p.hdr));
+        if (!good) break;
+        unsigned long long* const bar = &sh.full[stage];
+        if (tb200_tc::elected()) {
           tb200::mbar_arrive_expect(bar, bytes);
-          if (withheld(t)) continue;
-          if (MODE == BY_ROWS) {
-            for (unsigned h = 0; h < SETS; ++h) {
-              const int f = tile.feature + (h ? p.second : 0);
-              if (p.a_mn) {
-                tb200_tc::load_box(to + h * Shared::A, &map_a, f, k, tile.e, bar);
-                tb200_tc::load_box(to + h * Shared::A + BOX64, &map_a, f + 64, k, tile.e, bar);
-              } else {
-                tb200_tc::load_box(to + h * Shared::A, &map_a, k, f, tile.e, bar);
-              }
+          if (!withheld(t)) {
+            if (MODE == BY_EXPERTS || p.a_mn) {
+#pragma unroll
+              for (unsigned h = 0; h < SETS; ++h)
+                for (int c = 0; c < 2; c += p.a_chunks) {
+                  const int f = tile.feature + (h ? p.second : 0) + c * 64;
+                  tb200_tc::load_box(to + h * Shared::A + c * BOX64, &map_a, p.a_chunks == 1 ? f : 0, MODE == BY_ROWS ? k : tile.row + k, p.a_chunks == 1 ? 0 : f / 64, MODE == BY_ROWS ? tile.e : 0,
+                                     bar);
+                }
+            } else {
+#pragma unroll
+              for (unsigned h = 0; h < SETS; ++h) tb200_tc::load_box(to + h * Shared::A, &map_a, k, tile.feature + (h ? p.second : 0), 0, tile.e, bar);
             }
-            for (int b = 0; b < boxes; ++b) tb200_tc::load_box(to + SETS * Shared::A + b * p.box * DEEP * 2, &map_b, k, tile.row + b * p.box, bar);
-          } else {
-            tb200_tc::load_box(to, &map_a, tile.feature, tile.row + k, bar);
-            tb200_tc::load_box(to + BOX64, &map_a, tile.feature + 64, tile.row + k, bar);
-            for (int b = 0; b < boxes; ++b) tb200_tc::load_box(to + Shared::A + b * BOX64, &map_b, tile.other + b * 64, tile.row + k, bar);
+            for (int b = 0; b < boxes; ++b)
+              if (MODE == BY_ROWS) tb200_tc::load_box(to + SETS * Shared::A + b * b_box, &map_b, k, tile.row + b * p.box, 0, 0, bar);
+              else tb200_tc::load_box(to + Shared::A + b * b_box, &map_b, p.b_chunks == 1 ? tile.other + b * 64 : 0, tile.row + k, p.b_chunks == 1 ? 0 : tile.other / 64, 0, bar);
           }
         }
+        __syncwarp();
       }
-      // the last of each stage: brought, and no longer needed
-      for (unsigned i = 0; i < STAGES && i < count; ++i) {
-        const unsigned c = count - 1 - i;
-        outlast(&sh.full[c % STAGES], c / STAGES & 1);
-        if (good && !*(volatile int*)&sh.dead) outlast(&sh.empty[c % STAGES], c / STAGES & 1);
-      }
+    }
+    // the last of each stage: brought, and no longer needed
+    for (unsigned i = 0; i < STAGES && i < count; ++i) {
+      const unsigned c = count - 1 - i;
+      outlast(&sh.full[c % STAGES], c / STAGES & 1);
+      if (good && !*(volatile int*)&sh.dead) outlast(&sh.empty[c % STAGES], c / STAGES & 1);
     }
   } else if (warp == 5) {
     const unsigned base = tb200::smem_addr(stages);
@@ -302,20 +309,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
           __syncwarp();
         }
         tb200_tc::fence_after_sync();
-        if (lane == 0) {
+        if (tb200_tc::elected()) {
           unsigned long long a = tb200_tc::operand(from, a_mn, BOX64), b = tb200_tc::operand(from + SETS * Shared::A, b_mn, BOX64);
-          for (int i = 0; i < steps; ++i, a += a_step, b += b_step) {
-            tb200_tc::multiply(d, a, b, what, k > 0 || i > 0);
-            if (GATED) tb200_tc::multiply(d + BN, a + (Shared::A >> 4), b, what, k > 0 || i > 0);
-          }
+#pragma unroll
+          for (int i = 0; i < DEEP / 16; ++i, a += a_step, b += b_step)
+            if (i < steps) {
+              tb200_tc::multiply(d, a, b, what, k > 0 || i > 0);
+              if (GATED) tb200_tc::multiply(d + BN, a + (Shared::A >> 4), b, what, k > 0 || i > 0);
+            }
           tb200_tc::commit(&sh.empty[stage]);
         }
         __syncwarp();
       }
-      if (good && lane == 0) tb200_tc::commit(&sh.made[set]);
+      if (good && tb200_tc::elected()) tb200_tc::commit(&sh.made[set]);
       __syncwarp();
     }
-    if (lane == 0) { tb200_tc::commit(&sh.done); outlast(&sh.done, 0); }
+    if (tb200_tc::elected()) { tb200_tc::commit(&sh.done); outlast(&sh.done, 0); }
     __syncwarp();
   } else {
     unsigned made = 0, e = 0;
@@ -340,6 +349,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
       }
       for (int c = 0; c < tile.rows; c += 32) {
         float v[32], u[32];
+        T r[32];
+        const int count = tile.rows - c;
+        if (MODE == BY_ROWS && p.residual && there) get_column(p.residual + ((size_t)tile.row + c) * p.residual_stride + f, p.residual_stride, count, r);
         if (tile.depth && good) {
           tb200_tc::tmem_load(v, d + c);
           if (GATED) tb200_tc::tmem_load(u, d + BN + c);
@@ -354,7 +366,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
           for (int j = 0; j < 32; ++j) v[j] = u[j] = good ? 0.f : __int_as_float(0x7fffffff);
         }
         if (!there) continue;
-        const int count = tile.rows - c;
         if (MODE == BY_ROWS) {
           const size_t row = (size_t)tile.row + c, width = p.features;
 #pragma unroll
@@ -376,11 +387,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
             for (int j = 0; j < 32; ++j) v[j] *= u[j];
           }
           if (p.residual) {
-            T r[32];
-            get_column(p.residual + row * p.residual_stride + f, p.residual_stride, count, r);
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < count) v[j] += to_f32(r[j]);
+            for (int j = 0; j < 32; ++j) v[j] += to_f32(r[j]);
           }
           put_column(p.out + row * width + f, width, count, v);
         } else {
@@ -390,8 +398,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
             O old[32];
             get_column(q, p.features, count, old);
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < count) v[j] += to_f32(old[j]);
+            for (int j = 0; j < 32; ++j) v[j] += to_f32(old[j]);
           }
           put_column(q, p.features, count, v);
         }
@@ -625,14 +632,16 @@ encode_call encoder() {
   }();
   return call;
 }
-// Matrices [count][rows][width], rows `stride` and matrices `outer` elements apart, in boxes of 64 neighbouring elements (128 bytes, swizzled) of `box` rows.
-template <class T> bool box_map(CUtensorMap& map, const void* at, size_t width, size_t rows, size_t stride, size_t count, size_t outer, unsigned box) {
-  const cuuint64_t dims[3] = {width, rows, count}, strides[2] = {stride * 2, (count > 1 ? outer : rows * stride) * 2};
-  const cuuint32_t boxes[3] = {64, box, 1}, steps[3] = {1, 1, 1};
-  return encoder() && encoder()(&map, std::is_same<T, f16>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, count ? 3 : 2, const_cast<void*>(at), dims, strides, boxes,
-                                steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+// Matrices [count][rows][width], rows `stride` and matrices `outer` elements apart, in boxes of `chunks` times 64 neighbouring elements (128 bytes, swizzled) of
+// `box` rows; coordinates are element (of the 64, where there are several chunks), row, chunk, matrix.  Several chunks only where rows are made of whole ones: otherwise the
+// last would go on into the next row.
+template <class T> bool box_map(CUtensorMap& map, const void* at, size_t width, size_t rows, size_t stride, size_t count, size_t outer, unsigned box, unsigned chunks) {
+  const cuuint64_t apart = (count > 1 ? outer : rows * stride) * 2;
+  const cuuint64_t dims[4] = {chunks > 1 ? 64 : width, rows, chunks > 1 ? width / 64 : 1, count ? count : 1}, strides[3] = {stride * 2, 128, apart};
+  const cuuint32_t boxes[4] = {64, box, chunks, 1}, steps[4] = {1, 1, 1, 1};
+  return encoder() && encoder()(&map, std::is_same<T, f16>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(at), dims, strides, boxes, steps,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
 // Matrices as a kernel is given them: as they lie, or packed into the workspace.
 struct matrices {
   const void* at;
@@ -694,9 +703,10 @@ template <class T> cudaError_t product_by_rows(matrices w, matrices x, product_p
     if (e == cudaSuccess) e = pack<T>(x, room, stream);
     if (e != cudaSuccess) return e;
     p.second = p.a_mn ? (int)(w.halves == 2 ? w.width / 2 : 0) : p.features;
-    p.box = few ? 16 : 64;
+    p.box = few ? 16 : 128;
+    p.a_chunks = p.a_mn && w.half() % 64 == 0 ? 2 : 1;
     CUtensorMap a = {}, b = {};
-    if (p.k > 0 && (!box_map<T>(a, w.at, w.width, w.rows, w.stride, w.count, w.outer, p.a_mn ? 64 : 128) || !box_map<T>(b, x.at, x.width, x.rows, x.stride, 0, 0, (unsigned)p.box)))
+    if (p.k > 0 && (!box_map<T>(a, w.at, w.width, w.rows, w.stride, w.count, w.outer, p.a_mn ? 64 : 128, p.a_chunks) || !box_map<T>(b, x.at, x.width, x.rows, x.stride, 0, 0, (unsigned)p.box, 1)))
       return cudaErrorNotSupported;
     if (gated) return few ? launch_tc<T, T, BY_ROWS, true, 64, 5>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, true, 128, 4>(a, b, p, stream);
     return few ? launch_tc<T, T, BY_ROWS, false, 64, 8>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, false, 256, 4>(a, b, p, stream);
@@ -704,7 +714,7 @@ template <class T> cudaError_t product_by_rows(matrices w, matrices x, product_p
 }
 
 // matrix[e][o][f] = the sum over the expert's rows of others[row][o] features[row][f]
-template <class T, class O> cudaError_t product_by_experts(const matrices& features, const matrices& others, const product_plan<T>& p, cudaStream_t stream) {
+template <class T, class O> cudaError_t product_by_experts(const matrices& features, const matrices& others, product_plan<T> p, cudaStream_t stream) {
   if constexpr (sizeof(T) == 4) {
     const size_t tiles = (((size_t)p.features + 127) / 128) * (((size_t)p.others + 127) / 128) * p.experts;
     expert_product_f32_kernel<BY_EXPERTS, 128><<<product_grid(tiles, 2), FMA_THREADS, (2 * (size_t)p.experts + 2) * 4, stream>>>(static_cast<const float*>(features.at), 0, features.stride,
@@ -712,7 +722,10 @@ template <class T, class O> cudaError_t product_by_experts(const matrices& featu
     return cudaGetLastError();
   } else {
     CUtensorMap a = {}, b = {};
-    if (p.m > 0 && (!box_map<T>(a, features.at, features.width, features.rows, features.stride, 0, 0, 64) || !box_map<T>(b, others.at, others.width, others.rows, others.stride, 0, 0, 64)))
+    p.a_chunks = features.width % 64 == 0 ? 2 : 1;
+    p.b_chunks = others.width % 64 == 0 ? 4 : 1;
+    if (p.m > 0 && (!box_map<T>(a, features.at, features.width, features.rows, features.stride, 0, 0, 64, p.a_chunks) ||
+                    !box_map<T>(b, others.at, others.width, others.rows, others.stride, 0, 0, 64, p.b_chunks)))
       return cudaErrorNotSupported;
     return launch_tc<T, O, BY_EXPERTS, false, 256, 4>(a, b, p, stream);
   }
@@ -824,7 +837,6 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
         const matrices &inside = inputs_inside ? x : d, &around = inputs_inside ? d : x;
         p.features = (int)(inputs_inside ? in : out);
         p.others = (int)(inputs_inside ? out : in);
-        p.box = 64;
         p.matrix = d_dweight;
         p.accumulate = accumulate != 0;
         e = grad_t == t ? product_by_experts<T, T>(inside, around, p, stream) : product_by_experts<T, float>(inside, around, p, stream);

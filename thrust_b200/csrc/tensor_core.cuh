@@ -4,6 +4,14 @@
 
 namespace tb200_tc {
 
+// One lane of a whole warp, the same one each time.  What it issues has its operands in registers that the whole warp shares, and the compiler sees that they are: a
+// warp whose loop is one lane's alone (`if (lane == 0)`) took 130 cycles for each box it asked for and 120 for each matrix instruction.
+__device__ __forceinline__ bool elected() {
+  unsigned p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // ---------------------------------------------------------------- tensor memory, by whole warps
 __device__ __forceinline__ void tmem_alloc(unsigned* where, unsigned columns) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tb200::smem_addr(where)), "r"(columns) : "memory");
@@ -51,12 +59,8 @@ __device__ __forceinline__ void commit(unsigned long long* bar) {
 }
 
 // ---------------------------------------------------------------- boxes by the copy engine
-__device__ __forceinline__ void load_box(unsigned dst, const void* map, int x, int y, unsigned long long* bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(tb200::smem_addr(bar))
-               : "memory");
-}
-__device__ __forceinline__ void load_box(unsigned dst, const void* map, int x, int y, int z, unsigned long long* bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z),
+__device__ __forceinline__ void load_box(unsigned dst, const void* map, int x, int y, int z, int w, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w),
                "r"(tb200::smem_addr(bar))
                : "memory");
 }
