@@ -88,15 +88,15 @@ template <class T> struct product_plan {
 };
 struct product_tile { unsigned e; int row, rows, feature, other, depth; };
 
-// Tile t.  By rows: an expert's rows in tiles of equal height (multiples of 16), all features of one before the next.  `e`: the expert of the
+// Tile t.  By rows: an expert's rows in tiles of equal height (multiples of UNIT), all features of one before the next.  `e`: the expert of the
 // last tile asked for, from which the search goes on.
-template <int MODE, int WIDE, int BN, class T> __device__ __forceinline__ product_tile tile_at(const product_plan<T>& p, const spans& s, unsigned t, unsigned& e) {
+template <int MODE, int WIDE, int BN, int UNIT, class T> __device__ __forceinline__ product_tile tile_at(const product_plan<T>& p, const spans& s, unsigned t, unsigned& e) {
   product_tile r;
   const unsigned across = (unsigned)(p.features + WIDE - 1) / WIDE;
   if (MODE == BY_ROWS) {
     const unsigned index = t / across;
     while (index >= (unsigned)s.tiles[e + 1]) ++e;
-    const int n = rows_of(s, e), parts = (n + BN - 1) / BN, tall = ((n + parts - 1) / parts + 15) / 16 * 16, part = (int)(index - s.tiles[e]);
+    const int n = rows_of(s, e), parts = (n + BN - 1) / BN, tall = ((n + parts - 1) / parts + UNIT - 1) / UNIT * UNIT, part = (int)(index - s.tiles[e]);
     r.e = e;
     r.feature = (int)(t - index * across) * WIDE;
     r.row = s.at[e] + part * tall;
@@ -150,72 +150,83 @@ template <class T> __device__ __forceinline__ void clear_others(const product_pl
 #ifdef TB200_TEST_HOOKS
 // Test builds only: the copies of the first CTA's second tile are announced and not made.
 __device__ unsigned withhold_boxes;
-__device__ __forceinline__ bool withheld(unsigned t) { return withhold_boxes && blockIdx.x == 0 && t == gridDim.x; }
+__device__ __forceinline__ bool withheld(unsigned t, unsigned step) { return withhold_boxes && blockIdx.x == 0 && t == step; }
 #else
-__device__ __forceinline__ bool withheld(unsigned) { return false; }
+__device__ __forceinline__ bool withheld(unsigned, unsigned) { return false; }
 #endif
 
 constexpr int DEEP = 64;                      // of the contraction, a stage: 128 bytes
 constexpr int TC_THREADS = 192;               // warps 0 to 3 write results, 4 brings operands, 5 multiplies
 constexpr unsigned BOX64 = 64 * DEEP * 2;     // a box of 64 x 64
+constexpr unsigned A_BYTES = 2 * BOX64;       // a CTA's 128 features
 
-template <bool GATED, int BN, int STAGES> struct tc_shared {
-  static constexpr unsigned A = 128 * DEEP * 2, STAGE = A * (GATED ? 2 : 1) + BN * DEEP * 2;
-  static constexpr unsigned COLUMNS = 2 * BN * (GATED ? 2 : 1);
+template <bool PAIR, bool GATED, int BN, int STAGES> struct tc_shared {
+  static constexpr unsigned STAGE = A_BYTES + BN * DEEP * 2 / (PAIR ? 2 : 1), COLUMNS = 2 * BN;
   static_assert(COLUMNS <= 512, "two sets of sums in tensor memory");
-  unsigned long long full[STAGES], empty[STAGES], made[2], taken[2], done;
+  float halves[GATED ? 2 : 1][GATED ? 4 : 1][GATED ? 16 : 1][32];
+  unsigned long long full[STAGES], empty[STAGES], tail[STAGES], ready[STAGES], made[2], taken[2], done;
   unsigned tmem;
   int dead;
   static size_t bytes(unsigned experts) { return 1024 + (size_t)STAGES * STAGE + sizeof(tc_shared) + (2 * (size_t)experts + 2) * 4; }
 };
 // false: it did not come within the limit, or another warp has given up
-__device__ __forceinline__ bool await(unsigned long long* bar, unsigned parity, int* dead, tb200::ws_header* hdr) {
-  for (unsigned iter = 0; iter < tb200::MBAR_SPIN_LIMIT; ++iter) {
-    if (tb200::mbar_try_wait(bar, parity)) return true;
-    if (*(volatile int*)dead) return false;
+template <bool PAIR> __device__ __forceinline__ bool await(unsigned long long* bar, unsigned parity, int* dead, tb200::ws_header* hdr) {
+  bool good = false;
+  for (unsigned iter = 0; !good && iter < tb200::MBAR_SPIN_LIMIT; ++iter) {
+    good = PAIR ? tb200_tc::try_wait_pair(bar, parity) : tb200::mbar_try_wait(bar, parity);
+    if (!good && *(volatile int*)dead) break;
   }
-  *(volatile int*)dead = 1;
-  tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
-  return false;
+  good = __all_sync(tb200::FULL_MASK, good);
+  if (!good && !*(volatile int*)dead) {
+    *(volatile int*)dead = 1;
+    tb200::record_error(&hdr->error, tb200::ERR_LOOKBACK_TIMEOUT);
+  }
+  return good;
 }
 // at the end, dead or not: what was asked for is not left on its way
 __device__ __forceinline__ void outlast(unsigned long long* bar, unsigned parity) {
   for (unsigned iter = 0; iter < tb200::MBAR_SPIN_LIMIT && !tb200::mbar_try_wait(bar, parity); ++iter) {}
 }
 
-// results of 32 columns in a lane's registers go to p, p + stride, ...: the warp writes 32 neighbouring features at a time
-template <class O> __device__ __forceinline__ void put_column(O* p, size_t stride, int count, const float (&v)[32]) {
-  if (count >= 32) {
+// results of N columns in a lane's registers go to p, p + stride, ...: the warp writes 32 neighbouring features at a time
+template <class O, int N> __device__ __forceinline__ void put_column(O* p, size_t stride, int count, const float (&v)[N]) {
+  if (count >= N) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) p[(size_t)j * stride] = from_f32<O>(v[j]);
+    for (int j = 0; j < N; ++j) p[(size_t)j * stride] = from_f32<O>(v[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
+    for (int j = 0; j < N; ++j)
       if (j < count) p[(size_t)j * stride] = from_f32<O>(v[j]);
   }
 }
-template <class O> __device__ __forceinline__ void get_column(const O* p, size_t stride, int count, O (&v)[32]) {
-  if (count >= 32) {
+// and come from there (of columns past the count, the last one's: no branch between the requests); none: nothing
+template <class O, int N> __device__ __forceinline__ void get_column(const O* p, size_t stride, int count, O (&v)[N]) {
+  if (count >= N) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = p[(size_t)j * stride];
-  } else {
+    for (int j = 0; j < N; ++j) v[j] = p[(size_t)j * stride];
+  } else if (count > 0) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = p[(size_t)(j < count ? j : count - 1) * stride];      // (no branch between the requests)
+    for (int j = 0; j < N; ++j) v[j] = p[(size_t)(j < count ? j : count - 1) * stride];
   }
 }
 
-// D^T = A B^T by tiles of 128 features (gated: 128 of each half) x up to BN rows, one CTA a SM, which goes from tile to tile.  Features are the lanes of tensor
+// D^T = A B^T by tiles of 128 features (gated: 64 of each half) a CTA x up to BN rows; CTAs stay and go from tile to tile.  Features are the lanes of tensor
 // memory and rows its columns, so that a tile that has few rows takes a narrower instruction and no more time than they need: experts have as many rows as they have.
+// PAIR: two CTAs have a tile of twice as many features, half of its rows' operands each, and instructions that read both's shared memory, which the first
+// issues: 64 KB instead of 96 come from L2 for 256 features x 256 rows x 64.
 //
 // One warp keeps STAGES boxes of A and B on their way by the copy engine, one issues the matrix instructions as they come, four take the sums of the last
 // tile from tensor memory, while the next one's are made in its other half, and write them.  Sums are 32 bits from first to last; they
-// are rounded once, where they are stored, after bias, activation and residual.
+// are rounded once, where they are stored, after bias, activation and residual.  Gated: the two halves of a result are in lanes 64 apart, in warps that pass each
+// other half of their columns.
 //
 // By experts the contraction ends where the expert's rows do, in the middle of a box: what the box has of the next rows is cleared in shared memory, up to
-// the next 16, where the instructions end.
-template <class T, class O, int MODE, bool GATED, int BN, int STAGES>
+// the next 16, where the instructions end.  Such a box is counted by the barrier `tail` of the CTA that it is for, which clears it; the second CTA then says that its
+// is ready.
+template <class T, class O, int MODE, bool PAIR, bool GATED, int BN, int STAGES>
 __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const product_plan<T> p) {
-  using Shared = tc_shared<GATED, BN, STAGES>;
+  using Shared = tc_shared<PAIR, GATED, BN, STAGES>;
+  constexpr int CTAS = PAIR ? 2 : 1, OWN = GATED ? 64 : 128, WIDE = OWN * CTAS, UNIT = 16 * CTAS;
   extern __shared__ char raw[];
   char* const stages = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   Shared& sh = *reinterpret_cast<Shared*>(stages + STAGES * Shared::STAGE);
@@ -223,184 +234,232 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
   s.at = reinterpret_cast<int*>(&sh + 1);
   s.tiles = s.at + p.experts + 1;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const unsigned rank = PAIR ? tb200_tc::rank_in_pair() : 0;
   if (threadIdx.x == 0) {
     if (blockIdx.x == 0 && p.first) p.hdr->error = 0;      // a wait that runs out does so long after this
-    for (int i = 0; i < STAGES; ++i) { tb200::mbar_init(&sh.full[i], 1); tb200::mbar_init(&sh.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { tb200::mbar_init(&sh.made[i], 1); tb200::mbar_init(&sh.taken[i], 4); }
+    for (int i = 0; i < STAGES; ++i) {
+      for (unsigned long long* bar : {&sh.full[i], &sh.empty[i], &sh.tail[i], &sh.ready[i]}) tb200::mbar_init(bar, 1);
+    }
+    for (int i = 0; i < 2; ++i) { tb200::mbar_init(&sh.made[i], 1); tb200::mbar_init(&sh.taken[i], 4 * CTAS); }
     tb200::mbar_init(&sh.done, 1);
     sh.dead = 0;
     tb200::mbar_init_fence();
   }
-  if (warp == 5) tb200_tc::tmem_alloc(&sh.tmem, Shared::COLUMNS);
+  if (warp == 5) tb200_tc::tmem_alloc<PAIR>(&sh.tmem, Shared::COLUMNS);
   tb200_tc::fence_before_sync();
   read_spans(s, p.offsets, p.wide, p.experts, p.m, BN);
+  if (PAIR) tb200_tc::meet_pair();
   tb200_tc::fence_after_sync();
-  const unsigned tmem = sh.tmem, tiles = tiles_of<MODE, 128, BN>(p, s);
-  constexpr unsigned SETS = GATED ? 2 : 1;
+  const unsigned tmem = sh.tmem, tiles = tiles_of<MODE, WIDE, BN>(p, s), step = gridDim.x / CTAS;
+  // columns of a tile's instructions; of these each CTA brings its share of B
+  auto columns_of = [&](const product_tile& tile) { const int unit = MODE == BY_EXPERTS && p.b_chunks > 1 ? 64 * CTAS : UNIT; return (tile.rows + unit - 1) / unit * unit; };
+  auto is_tail = [&](const product_tile& tile, int k) { return MODE == BY_EXPERTS && tile.depth - k < DEEP && tile.depth % 16 != 0; };
+  // what a box has beyond the expert's rows
+  auto clear_tail = [&](unsigned stage, int valid, int boxes) {
+    const int pieces = (16 - valid % 16) * 8;
+    for (int i = lane; i < pieces * boxes; i += 32)
+      *reinterpret_cast<uint4*>(stages + stage * Shared::STAGE + i / pieces * BOX64 + valid * 128 + i % pieces * 16) = make_uint4(0, 0, 0, 0);
+    tb200::fence_async_smem();
+    __syncwarp();
+  };
 
   if (warp == 4) {
     const unsigned base = tb200::smem_addr(stages);
     unsigned count = 0, e = 0;      // stages filled so far
     bool good = true;
-    for (unsigned t = blockIdx.x; good && t < tiles; t += gridDim.x) {
-      const product_tile tile = tile_at<MODE, 128, BN>(p, s, t, e);
-      const int boxes = MODE == BY_ROWS ? (tile.rows + p.box - 1) / p.box : (tile.rows + p.b_chunks * 64 - 1) / (p.b_chunks * 64);
-      const unsigned b_box = MODE == BY_ROWS ? p.box * DEEP * 2 : p.b_chunks * BOX64, bytes = Shared::A * SETS + boxes * b_box;
+    for (unsigned t = blockIdx.x / CTAS; good && t < tiles; t += step) {
+      const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
+      const int share = columns_of(tile) / CTAS, feature = tile.feature + (int)rank * OWN, other = (MODE == BY_ROWS ? tile.row : tile.other) + (int)rank * share;
+      const int b_rows = MODE == BY_ROWS ? p.box : p.b_chunks * 64, boxes = (share + b_rows - 1) / b_rows;
+      const unsigned b_box = b_rows * DEEP * 2, bytes = A_BYTES + boxes * b_box;
       for (int k = 0; k < tile.depth; k += DEEP, ++count) {
         const unsigned stage = count % STAGES, to = base + stage * Shared::STAGE;
-        good = __all_sync(tb200::FULL_MASK, await(&sh.empty[stage], (count / STAGES & 1) ^ 1, &sh.dead, p.hdr));
+        good = await<PAIR>(&sh.empty[stage], (count / STAGES & 1) ^ 1, &sh.dead, p.hdr);
         if (!good) break;
-        unsigned long long* const bar = &sh.full[stage];
+        const bool tail = is_tail(tile, k);
         if (tb200_tc::elected()) {
-          tb200::mbar_arrive_expect(bar, bytes);
-          if (!withheld(t)) {
-            if (MODE == BY_EXPERTS || p.a_mn) {
-#pragma unroll
-              for (unsigned h = 0; h < SETS; ++h)
-                for (int c = 0; c < 2; c += p.a_chunks) {
-                  const int f = tile.feature + (h ? p.second : 0) + c * 64;
-                  tb200_tc::load_box(to + h * Shared::A + c * BOX64, &map_a, p.a_chunks == 1 ? f : 0, MODE == BY_ROWS ? k : tile.row + k, p.a_chunks == 1 ? 0 : f / 64, MODE == BY_ROWS ? tile.e : 0,
-                                     bar);
-                }
+          unsigned bar;
+          if (tail) {
+            tb200::mbar_arrive_expect(&sh.tail[stage], bytes);
+            if (rank == 0) tb200::mbar_arrive(&sh.full[stage]);
+            bar = tb200::smem_addr(&sh.tail[stage]);
+          } else {
+            if (rank == 0) tb200::mbar_arrive_expect(&sh.full[stage], bytes * CTAS);
+            bar = PAIR ? tb200_tc::first_ones(&sh.full[stage]) : tb200::smem_addr(&sh.full[stage]);
+          }
+          if (!withheld(t, step)) {
+            if (MODE == BY_EXPERTS) {
+              for (int c = 0; c < 2; c += p.a_chunks) {
+                const int f = feature + c * 64;
+                tb200_tc::load_box<PAIR>(to + c * BOX64, &map_a, p.a_chunks == 1 ? f : 0, tile.row + k, p.a_chunks == 1 ? 0 : f / 64, 0, bar);
+              }
+              for (int b = 0; b < boxes; ++b)
+                tb200_tc::load_box<PAIR>(to + A_BYTES + b * b_box, &map_b, p.b_chunks == 1 ? other + b * 64 : 0, tile.row + k, p.b_chunks == 1 ? 0 : other / 64, 0, bar);
             } else {
-#pragma unroll
-              for (unsigned h = 0; h < SETS; ++h) tb200_tc::load_box(to + h * Shared::A, &map_a, k, tile.feature + (h ? p.second : 0), 0, tile.e, bar);
+              if (p.a_mn) {
+                for (int c = 0; c < 2; c += p.a_chunks) {
+                  const int f = GATED && c ? p.second + feature : feature + c * 64;
+                  tb200_tc::load_box<PAIR>(to + c * BOX64, &map_a, p.a_chunks == 1 ? f : 0, k, p.a_chunks == 1 ? 0 : f / 64, tile.e, bar);
+                }
+              } else {
+                tb200_tc::load_box<PAIR>(to, &map_a, k, feature, 0, tile.e, bar);
+                if (GATED) tb200_tc::load_box<PAIR>(to + BOX64, &map_a, k, p.second + feature, 0, tile.e, bar);
+              }
+              for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + b * b_box, &map_b, k, other + b * p.box, 0, 0, bar);
             }
-            for (int b = 0; b < boxes; ++b)
-              if (MODE == BY_ROWS) tb200_tc::load_box(to + SETS * Shared::A + b * b_box, &map_b, k, tile.row + b * p.box, 0, 0, bar);
-              else tb200_tc::load_box(to + Shared::A + b * b_box, &map_b, p.b_chunks == 1 ? tile.other + b * 64 : 0, tile.row + k, p.b_chunks == 1 ? 0 : tile.other / 64, 0, bar);
           }
         }
         __syncwarp();
       }
     }
-    // the last of each stage: brought, and no longer needed
-    for (unsigned i = 0; i < STAGES && i < count; ++i) {
-      const unsigned c = count - 1 - i;
-      outlast(&sh.full[c % STAGES], c / STAGES & 1);
-      if (good && !*(volatile int*)&sh.dead) outlast(&sh.empty[c % STAGES], c / STAGES & 1);
-    }
+    // the last of each stage, no longer needed
+    if (good)
+      for (unsigned i = 0; i < STAGES && i < count; ++i) good = good && await<PAIR>(&sh.empty[(count - 1 - i) % STAGES], (count - 1 - i) / STAGES & 1, &sh.dead, p.hdr);
+    // given up: what is on its way is counted where this warp may not be able to see it; copies take microseconds
+    if (!good)
+      for (int i = 0; i < 20; ++i) __nanosleep(1000000);
   } else if (warp == 5) {
     const unsigned base = tb200::smem_addr(stages);
-    unsigned count = 0, made = 0, e = 0;
+    unsigned count = 0, made = 0, e = 0, tails = 0;      // tails: a bit for each stage's barrier
     bool good = true;
     const bool a_mn = MODE == BY_EXPERTS || p.a_mn;
     constexpr bool b_mn = MODE == BY_EXPERTS;
     const unsigned a_step = tb200_tc::step_of(a_mn), b_step = tb200_tc::step_of(b_mn);
-    for (unsigned t = blockIdx.x; good && t < tiles; t += gridDim.x) {
-      const product_tile tile = tile_at<MODE, 128, BN>(p, s, t, e);
-      if (tile.depth == 0) continue;
-      const unsigned set = made & 1, d = tmem + set * SETS * BN;
-      good = __all_sync(tb200::FULL_MASK, await(&sh.taken[set], (made / 2 & 1) ^ 1, &sh.dead, p.hdr));
-      if (!good) break;
-      ++made;
-      tb200_tc::fence_after_sync();
-      const unsigned what = tb200_tc::instruction(std::is_same<T, bf16>::value, a_mn, b_mn, (tile.rows + 15) / 16 * 16);
-      for (int k = 0; k < tile.depth; k += DEEP, ++count) {
-        const unsigned stage = count % STAGES, from = base + stage * Shared::STAGE;
-        good = __all_sync(tb200::FULL_MASK, await(&sh.full[stage], count / STAGES & 1, &sh.dead, p.hdr));
+    if (rank == 0) {
+      for (unsigned t = blockIdx.x / CTAS; good && t < tiles; t += step) {
+        const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
+        if (tile.depth == 0) continue;
+        const unsigned set = made & 1, d = tmem + set * BN;
+        good = await<PAIR>(&sh.taken[set], (made / 2 & 1) ^ 1, &sh.dead, p.hdr);
         if (!good) break;
-        const int valid = tile.depth - k < DEEP ? tile.depth - k : DEEP, steps = (valid + 15) / 16;
-        if (MODE == BY_EXPERTS && valid < steps * 16) {
-          const int pieces = (steps * 16 - valid) * 8, boxes = 2 + (tile.rows + 63) / 64;
-          for (int i = lane; i < pieces * boxes; i += 32)
-            *reinterpret_cast<uint4*>(stages + stage * Shared::STAGE + i / pieces * BOX64 + valid * 128 + i % pieces * 16) = make_uint4(0, 0, 0, 0);
-          tb200::fence_async_smem();
+        ++made;
+        tb200_tc::fence_after_sync();
+        const int columns = columns_of(tile);
+        const unsigned what = tb200_tc::instruction<PAIR>(std::is_same<T, bf16>::value, a_mn, b_mn, columns);
+        for (int k = 0; k < tile.depth; k += DEEP, ++count) {
+          const unsigned stage = count % STAGES, from = base + stage * Shared::STAGE;
+          good = await<PAIR>(&sh.full[stage], count / STAGES & 1, &sh.dead, p.hdr);
+          if (!good) break;
+          const int valid = tile.depth - k < DEEP ? tile.depth - k : DEEP, steps = (valid + 15) / 16;
+          if (is_tail(tile, k)) {
+            good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr);
+            if (!good) break;
+            clear_tail(stage, valid, 2 + (columns / CTAS + 63) / 64);
+            if (PAIR) good = await<PAIR>(&sh.ready[stage], tails >> stage & 1, &sh.dead, p.hdr);
+            if (!good) break;
+            tails ^= 1u << stage;
+          }
+          tb200_tc::fence_after_sync();
+          if (tb200_tc::elected()) {
+            unsigned long long a = tb200_tc::operand(from, a_mn, BOX64), b = tb200_tc::operand(from + A_BYTES, b_mn, BOX64);
+#pragma unroll
+            for (int i = 0; i < DEEP / 16; ++i, a += a_step, b += b_step)
+              if (i < steps) tb200_tc::multiply<PAIR>(d, a, b, what, k > 0 || i > 0);
+            tb200_tc::commit<PAIR>(&sh.empty[stage]);
+          }
           __syncwarp();
         }
-        tb200_tc::fence_after_sync();
-        if (tb200_tc::elected()) {
-          unsigned long long a = tb200_tc::operand(from, a_mn, BOX64), b = tb200_tc::operand(from + SETS * Shared::A, b_mn, BOX64);
-#pragma unroll
-          for (int i = 0; i < DEEP / 16; ++i, a += a_step, b += b_step)
-            if (i < steps) {
-              tb200_tc::multiply(d, a, b, what, k > 0 || i > 0);
-              if (GATED) tb200_tc::multiply(d + BN, a + (Shared::A >> 4), b, what, k > 0 || i > 0);
-            }
-          tb200_tc::commit(&sh.empty[stage]);
-        }
+        if (good && tb200_tc::elected()) tb200_tc::commit<PAIR>(&sh.made[set]);
         __syncwarp();
       }
-      if (good && tb200_tc::elected()) tb200_tc::commit(&sh.made[set]);
+      if (tb200_tc::elected()) { tb200_tc::commit<PAIR>(&sh.done); outlast(&sh.done, 0); }
       __syncwarp();
+    } else if (MODE == BY_EXPERTS) {
+      for (unsigned t = blockIdx.x / CTAS; good && t < tiles; t += step) {
+        const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
+        const unsigned blocks = (unsigned)(tile.depth + DEEP - 1) / DEEP, stage = (count + blocks - 1) % STAGES;
+        count += blocks;
+        if (blocks == 0 || !is_tail(tile, (int)(blocks - 1) * DEEP)) continue;
+        good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr);
+        if (!good) break;
+        tails ^= 1u << stage;
+        clear_tail(stage, tile.depth - (int)(blocks - 1) * DEEP, 2 + (columns_of(tile) / CTAS + 63) / 64);
+        if (lane == 0) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.ready[stage]));
+        __syncwarp();
+      }
     }
-    if (tb200_tc::elected()) { tb200_tc::commit(&sh.done); outlast(&sh.done, 0); }
-    __syncwarp();
   } else {
-    unsigned made = 0, e = 0;
+    unsigned made = 0, e = 0, turn = 0;
     bool good = true;
-    const bool gated = GATED;
-    const int kind = p.activation & ~ACT_GATED;
-    for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
-      const product_tile tile = tile_at<MODE, 128, BN>(p, s, t, e);
-      const unsigned set = made & 1, d = tmem + (warp * 32u << 16) + set * SETS * BN;
+    const int kind = p.activation & ~ACT_GATED, half = GATED ? warp / 2 : 0, within = GATED ? warp % 2 * 32 + lane : warp * 32 + lane;
+    constexpr int PUT = GATED ? 16 : 32;      // columns of results that a lane ends up with, of 32 of sums
+    for (unsigned t = blockIdx.x / CTAS; t < tiles; t += step) {
+      const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
+      const unsigned set = made & 1, d = tmem + (warp * 32u << 16) + set * BN;
       if (tile.depth) {
-        if (good) good = __all_sync(tb200::FULL_MASK, await(&sh.made[set], made / 2 & 1, &sh.dead, p.hdr));
+        if (good) good = await<PAIR>(&sh.made[set], made / 2 & 1, &sh.dead, p.hdr);
         ++made;
         tb200_tc::fence_after_sync();
       }
-      const int f = tile.feature + warp * 32 + lane;
+      const int f = tile.feature + (int)rank * OWN + within;
       const bool there = f < p.features;
-      float b0 = 0.f, b1 = 0.f;
-      if (MODE == BY_ROWS && p.bias && there) {
-        const T* const b = p.bias + (size_t)tile.e * p.features * (gated ? 2 : 1) + f;
-        b0 = to_f32(b[0]);
-        if (gated) b1 = to_f32(b[p.features]);
-      }
+      const size_t width = p.features, both = GATED ? 2 * width : width;
+      float b0 = 0.f;
+      if (MODE == BY_ROWS && p.bias && there) b0 = to_f32(p.bias[tile.e * both + half * width + f]);
       for (int c = 0; c < tile.rows; c += 32) {
-        float v[32], u[32];
-        T r[32];
-        const int count = tile.rows - c;
-        if (MODE == BY_ROWS && p.residual && there) get_column(p.residual + ((size_t)tile.row + c) * p.residual_stride + f, p.residual_stride, count, r);
+        float v[32];
+        T r[PUT];
+        const int mine = c + half * 16, count = tile.rows - mine;      // columns of results
+        if (MODE == BY_ROWS && p.residual && there) get_column(p.residual + ((size_t)tile.row + mine) * p.residual_stride + f, p.residual_stride, count, r);
         if (tile.depth && good) {
           tb200_tc::tmem_load(v, d + c);
-          if (GATED) tb200_tc::tmem_load(u, d + BN + c);
           tb200_tc::tmem_load_wait();
           if (c + 32 >= tile.rows) {      // the last of them: the next sums may be made there
             tb200_tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) tb200::mbar_arrive(&sh.taken[set]);
+            if (lane == 0) {
+              if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.taken[set]));
+              else tb200::mbar_arrive(&sh.taken[set]);
+            }
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = u[j] = good ? 0.f : __int_as_float(0x7fffffff);
+          for (int j = 0; j < 32; ++j) v[j] = good ? 0.f : __int_as_float(0x7fffffff);
         }
-        if (!there) continue;
         if (MODE == BY_ROWS) {
-          const size_t row = (size_t)tile.row + c, width = p.features;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) { v[j] += b0; if (GATED) u[j] += b1; }
-          if (p.before) {
-            T* const q = p.before + row * width * SETS + f;
-            put_column(q, width * SETS, count, v);
-            if (GATED) put_column(q + width, width * SETS, count, u);
+          for (int j = 0; j < 32; ++j) v[j] += b0;
+          if (p.before && there) put_column(p.before + ((size_t)tile.row + c) * both + half * width + f, both, tile.rows - c, v);
+          float w[PUT];
+          if constexpr (GATED) {
+            float (&out)[16][32] = sh.halves[turn][warp], (&in)[16][32] = sh.halves[turn][warp ^ 2];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) out[j][lane] = half ? v[j] : v[j + 16];
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + warp % 2) : "memory");
+            turn ^= 1;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) { const float x = in[j][lane]; w[j] = half ? x : v[j]; v[j] = half ? v[j + 16] : x; }      // act(w) v
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] = v[j];
           }
+          if (!there) continue;
           if (kind == ACT_SILU) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = activated<true>(v[j], ACT_SILU);
+            for (int j = 0; j < PUT; ++j) w[j] = activated<true>(w[j], ACT_SILU);
           } else if (kind == ACT_GELU) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = activated<true>(v[j], ACT_GELU);
+            for (int j = 0; j < PUT; ++j) w[j] = activated<true>(w[j], ACT_GELU);
           }
-          if (GATED) {
+          if constexpr (GATED) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= u[j];
+            for (int j = 0; j < PUT; ++j) w[j] *= v[j];
           }
           if (p.residual) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] += to_f32(r[j]);
+            for (int j = 0; j < PUT; ++j) w[j] += to_f32(r[j]);
           }
-          put_column(p.out + row * width + f, width, count, v);
-        } else {
-          O* const q = static_cast<O*>(p.matrix) + ((size_t)tile.e * p.others + tile.other + c) * p.features + f;
+          put_column(p.out + ((size_t)tile.row + mine) * width + f, width, count, w);
+        } else if (there) {
+          O* const q = static_cast<O*>(p.matrix) + ((size_t)tile.e * p.others + tile.other + c) * width + f;
           if (p.accumulate) {
             if (tile.depth == 0 && good) continue;      // nothing is added
             O old[32];
-            get_column(q, p.features, count, old);
+            get_column(q, width, tile.rows - c, old);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] += to_f32(old[j]);
           }
-          put_column(q, p.features, count, v);
+          put_column(q, width, tile.rows - c, v);
         }
       }
     }
@@ -408,9 +467,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
     tb200_tc::fence_before_sync();
   }
   __syncthreads();
+  if (PAIR) tb200_tc::meet_pair();      // neither ends while the other's instructions and arrivals come here
   if (warp == 5) {
     tb200_tc::fence_after_sync();
-    tb200_tc::tmem_free(tmem, Shared::COLUMNS);
+    tb200_tc::tmem_free<PAIR>(tmem, Shared::COLUMNS);
   }
 }
 
@@ -438,7 +498,7 @@ __global__ void __launch_bounds__(FMA_THREADS, BN == 128 ? 2 : 4) expert_product
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   unsigned e = 0;
   for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const product_tile tile = MODE == BY_ROWS && gated ? tile_at<MODE, 64, BN>(p, s, t, e) : tile_at<MODE, WIDE, BN>(p, s, t, e);
+    const product_tile tile = MODE == BY_ROWS && gated ? tile_at<MODE, 64, BN, 1>(p, s, t, e) : tile_at<MODE, WIDE, BN, 1>(p, s, t, e);
     float acc[8][ROWS];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -674,21 +734,32 @@ unsigned product_grid(size_t tiles, unsigned a_sm) {
 }
 size_t most_row_tiles(size_t m, size_t experts, size_t tall) { return m / tall + (m < experts ? m : experts); }
 
-template <class T, class O, int MODE, bool GATED, int BN, int STAGES>
+template <class T, class O, int MODE, bool PAIR, bool GATED, int BN, int STAGES>
 cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_plan<T>& p, cudaStream_t stream) {
-  using Shared = tc_shared<GATED, BN, STAGES>;
-  auto kernel = expert_product_kernel<T, O, MODE, GATED, BN, STAGES>;
+  using Shared = tc_shared<PAIR, GATED, BN, STAGES>;
+  constexpr size_t CTAS = PAIR ? 2 : 1, WIDE = (GATED ? 64 : 128) * CTAS;
+  auto kernel = expert_product_kernel<T, O, MODE, PAIR, GATED, BN, STAGES>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shared::bytes(MOST_EXPERTS));
   if (e != cudaSuccess) return e;
-  const size_t across = ((size_t)p.features + 127) / 128;
+  const size_t across = ((size_t)p.features + WIDE - 1) / WIDE;
   const size_t tiles = MODE == BY_ROWS ? across * most_row_tiles(p.m, p.experts, BN) : across * (((size_t)p.others + BN - 1) / BN) * p.experts;
-  kernel<<<product_grid(tiles, 1), TC_THREADS, Shared::bytes(p.experts), stream>>>(a, b, p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(PAIR ? product_grid(tiles * 2, 1) / 2 * 2 : product_grid(tiles, 1));
+  cfg.blockDim = dim3(TC_THREADS);
+  cfg.dynamicSmemBytes = Shared::bytes(p.experts);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CTAS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, a, b, p);
 }
 
 // out[i] = rows[i] W[e] (+ the rest) of the expert that row i is of.  w: its matrices' rows are inputs (a_mn: the outputs of an input are neighbours), or outputs.
 template <class T> cudaError_t product_by_rows(matrices w, matrices x, product_plan<T> p, char* room, cudaStream_t stream) {
-  const bool gated = (p.activation & ACT_GATED) != 0, few = (size_t)p.m <= (size_t)32 * p.experts;
+  const bool gated = (p.activation & ACT_GATED) != 0;
+  bool few = (size_t)p.m <= (size_t)32 * p.experts;
   if constexpr (sizeof(T) == 4) {
     const size_t wide = gated ? 64 : 128;
     const size_t smem = (2 * (size_t)p.experts + 2) * 4, across = ((size_t)p.features + wide - 1) / wide;
@@ -703,13 +774,18 @@ template <class T> cudaError_t product_by_rows(matrices w, matrices x, product_p
     if (e == cudaSuccess) e = pack<T>(x, room, stream);
     if (e != cudaSuccess) return e;
     p.second = p.a_mn ? (int)(w.halves == 2 ? w.width / 2 : 0) : p.features;
-    p.box = few ? 16 : 128;
-    p.a_chunks = p.a_mn && w.half() % 64 == 0 ? 2 : 1;
-    CUtensorMap a = {}, b = {};
-    if (p.k > 0 && (!box_map<T>(a, w.at, w.width, w.rows, w.stride, w.count, w.outer, p.a_mn ? 64 : 128, p.a_chunks) || !box_map<T>(b, x.at, x.width, x.rows, x.stride, 0, 0, (unsigned)p.box, 1)))
-      return cudaErrorNotSupported;
-    if (gated) return few ? launch_tc<T, T, BY_ROWS, true, 64, 5>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, true, 128, 4>(a, b, p, stream);
-    return few ? launch_tc<T, T, BY_ROWS, false, 64, 8>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, false, 256, 4>(a, b, p, stream);
+    // chunks of one box are neighbours, those of the two halves are not
+    p.a_chunks = p.a_mn && !gated && w.width % 64 == 0 ? 2 : 1;
+    for (;; few = true) {      // (again, by single CTAs, if there is no room for pairs)
+      p.box = few ? 16 : 128;
+      CUtensorMap a = {}, b = {};
+      if (p.k > 0 && (!box_map<T>(a, w.at, w.width, w.rows, w.stride, w.count, w.outer, p.a_mn || gated ? 64 : 128, p.a_chunks) ||
+                      !box_map<T>(b, x.at, x.width, x.rows, x.stride, 0, 0, (unsigned)p.box, 1)))
+        return cudaErrorNotSupported;
+      if (few) return gated ? launch_tc<T, T, BY_ROWS, false, true, 64, 8>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, false, false, 64, 8>(a, b, p, stream);
+      e = gated ? launch_tc<T, T, BY_ROWS, true, true, 256, 6>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, true, false, 256, 6>(a, b, p, stream);
+      if (!tb200::launch_refused(e)) return e;
+    }
   }
 }
 
@@ -721,13 +797,17 @@ template <class T, class O> cudaError_t product_by_experts(const matrices& featu
                                                                                                             static_cast<const float*>(others.at), others.stride, p);
     return cudaGetLastError();
   } else {
-    CUtensorMap a = {}, b = {};
     p.a_chunks = features.width % 64 == 0 ? 2 : 1;
-    p.b_chunks = others.width % 64 == 0 ? 4 : 1;
-    if (p.m > 0 && (!box_map<T>(a, features.at, features.width, features.rows, features.stride, 0, 0, 64, p.a_chunks) ||
-                    !box_map<T>(b, others.at, others.width, others.rows, others.stride, 0, 0, 64, p.b_chunks)))
-      return cudaErrorNotSupported;
-    return launch_tc<T, O, BY_EXPERTS, false, 256, 4>(a, b, p, stream);
+    for (bool pair = p.features > 128;; pair = false) {
+      CUtensorMap a = {}, b = {};
+      p.b_chunks = others.width % 64 == 0 ? pair ? 2 : 4 : 1;
+      if (p.m > 0 && (!box_map<T>(a, features.at, features.width, features.rows, features.stride, 0, 0, 64, p.a_chunks) ||
+                      !box_map<T>(b, others.at, others.width, others.rows, others.stride, 0, 0, 64, p.b_chunks)))
+        return cudaErrorNotSupported;
+      if (!pair) return launch_tc<T, O, BY_EXPERTS, false, false, 256, 4>(a, b, p, stream);
+      const cudaError_t e = launch_tc<T, O, BY_EXPERTS, true, false, 256, 6>(a, b, p, stream);
+      if (!tb200::launch_refused(e)) return e;
+    }
   }
 }
 

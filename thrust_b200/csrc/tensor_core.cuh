@@ -12,12 +12,20 @@ __device__ __forceinline__ bool elected() {
   return p != 0;
 }
 
-// ---------------------------------------------------------------- tensor memory, by whole warps
-__device__ __forceinline__ void tmem_alloc(unsigned* where, unsigned columns) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tb200::smem_addr(where)), "r"(columns) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+// ---------------------------------------------------------------- tensor memory, by whole warps; PAIR: by one of each of two CTAs, for both
+template <bool PAIR> __device__ __forceinline__ void tmem_alloc(unsigned* where, unsigned columns) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tb200::smem_addr(where)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tb200::smem_addr(where)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
 }
-__device__ __forceinline__ void tmem_free(unsigned at, unsigned columns) { asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns)); }
+template <bool PAIR> __device__ __forceinline__ void tmem_free(unsigned at, unsigned columns) {
+  if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+}
 
 // 32 columns of the 32 lanes that warp % 4 may read: lane l of the warp gets columns at, at + 1, ... of lane l
 __device__ __forceinline__ void tmem_load(float (&v)[32], unsigned at) {
@@ -46,23 +54,55 @@ __device__ __forceinline__ unsigned long long operand(unsigned smem, bool mn_maj
 // 16 k further on, in a descriptor's units of 16 bytes
 __device__ __forceinline__ unsigned step_of(bool mn_major) { return mn_major ? 2048 >> 4 : 32 >> 4; }
 
-// D (F32, 128 x n in tensor memory) = or += A (128 x 16) B (n x 16) of 16-bit elements; n a multiple of 16 up to 256
-__device__ __forceinline__ unsigned instruction(bool bf16, bool a_mn_major, bool b_mn_major, unsigned n) {
-  return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
+// D (F32, m x n in tensor memory) = or += A (m x 16) B (n x 16) of 16-bit elements: m = 128, n a multiple of 16 up to 256.  PAIR: m = 256, n a multiple of 32; each of
+// the two CTAs has half of A's m, half of B's n and the whole of n for its half of D's m.
+template <bool PAIR> __device__ __forceinline__ unsigned instruction(bool bf16, bool a_mn_major, bool b_mn_major, unsigned n) {
+  return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) | (n >> 3) << 17 | ((PAIR ? 256u : 128u) >> 4) << 24;
 }
-__device__ __forceinline__ void multiply(unsigned d, unsigned long long a, unsigned long long b, unsigned what, bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(what), "r"((unsigned)add) : "memory");
+template <bool PAIR> __device__ __forceinline__ void multiply(unsigned d, unsigned long long a, unsigned long long b, unsigned what, bool add) {
+  if (PAIR)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(what), "r"((unsigned)add) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(what), "r"((unsigned)add) : "memory");
 }
-// an arrival on `bar` once this thread's matrix instructions so far are done
-__device__ __forceinline__ void commit(unsigned long long* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tb200::smem_addr(bar)) : "memory");
+// an arrival on `bar`, PAIR: on that of both CTAs, once this thread's matrix instructions so far are done
+template <bool PAIR> __device__ __forceinline__ void commit(unsigned long long* bar) {
+  if (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(tb200::smem_addr(bar)), "h"((unsigned short)3) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tb200::smem_addr(bar)) : "memory");
+}
+
+// ---------------------------------------------------------------- two CTAs
+__device__ __forceinline__ unsigned rank_in_pair() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ unsigned first_ones(const void* p) {      // the first CTA's counterpart of something in shared memory
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(tb200::smem_addr(p)));
+  return r;
+}
+__device__ __forceinline__ void arrive_there(unsigned bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool try_wait_pair(unsigned long long* bar, unsigned parity) {
+  unsigned ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(tb200::smem_addr(bar)), "r"(parity), "r"(1000u) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void meet_pair() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- boxes by the copy engine
-__device__ __forceinline__ void load_box(unsigned dst, const void* map, int x, int y, int z, int w, unsigned long long* bar) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w),
-               "r"(tb200::smem_addr(bar))
-               : "memory");
+// into this CTA's shared memory; PAIR: counted by a barrier in that of either CTA
+template <bool PAIR> __device__ __forceinline__ void load_box(unsigned dst, const void* map, int x, int y, int z, int w, unsigned bar) {
+  if (PAIR)
+    asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y),
+                 "r"(z), "r"(w), "r"(bar)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w),
+                 "r"(bar)
+                 : "memory");
 }
 
 }  // namespace tb200_tc
