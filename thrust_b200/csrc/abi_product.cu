@@ -76,8 +76,8 @@ template <class T> struct product_plan {
   int m, k, features, others;
   int second;                 // gated: where the second half of the features begins in A
   bool a_mn;                  // A's features are neighbours (else its k)
-  int a_chunks, b_chunks;     // MN-major: how many 64 neighbours there are in a box
-  int box;                    // K-major: rows in a box of B
+  bool a_split, b_split;      // rows are made of whole chunks of 64 and mapped as such: a box has several
+  int box;                    // by rows: rows in a box of B
   const T *bias, *residual;
   size_t residual_stride;
   T *out, *before;
@@ -155,13 +155,13 @@ __device__ __forceinline__ bool withheld(unsigned t, unsigned step) { return wit
 __device__ __forceinline__ bool withheld(unsigned, unsigned) { return false; }
 #endif
 
-constexpr int DEEP = 64;                      // of the contraction, a stage: 128 bytes
+constexpr int DEEP = 128;                     // of the contraction, a stage
 constexpr int TC_THREADS = 192;               // warps 0 to 3 write results, 4 brings operands, 5 multiplies
-constexpr unsigned BOX64 = 64 * DEEP * 2;     // a box of 64 x 64
-constexpr unsigned A_BYTES = 2 * BOX64;       // a CTA's 128 features
+constexpr unsigned CHUNK = 64 * DEEP * 2;     // 64 neighbours by 128 of the other axis
+constexpr unsigned A_BYTES = 2 * CHUNK;       // a CTA's 128 features
 
 template <bool PAIR, bool GATED, int BN, int STAGES> struct tc_shared {
-  static constexpr unsigned STAGE = A_BYTES + BN * DEEP * 2 / (PAIR ? 2 : 1), COLUMNS = 2 * BN;
+  static constexpr unsigned B_CHUNK = BN * 128 / (PAIR ? 2 : 1), STAGE = A_BYTES + 2 * B_CHUNK, COLUMNS = 2 * BN;
   static_assert(COLUMNS <= 512, "two sets of sums in tensor memory");
   float halves[GATED ? 2 : 1][GATED ? 4 : 1][GATED ? 16 : 1][32];
   unsigned long long full[STAGES], empty[STAGES], tail[STAGES], ready[STAGES], made[2], taken[2], done;
@@ -252,13 +252,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
   tb200_tc::fence_after_sync();
   const unsigned tmem = sh.tmem, tiles = tiles_of<MODE, WIDE, BN>(p, s), step = gridDim.x / CTAS;
   // columns of a tile's instructions; of these each CTA brings its share of B
-  auto columns_of = [&](const product_tile& tile) { const int unit = MODE == BY_EXPERTS && p.b_chunks > 1 ? 64 * CTAS : UNIT; return (tile.rows + unit - 1) / unit * unit; };
+  auto columns_of = [&](const product_tile& tile) { const int unit = MODE == BY_EXPERTS && p.b_split ? 64 * CTAS : UNIT; return (tile.rows + unit - 1) / unit * unit; };
   auto is_tail = [&](const product_tile& tile, int k) { return MODE == BY_EXPERTS && tile.depth - k < DEEP && tile.depth % 16 != 0; };
   // what a box has beyond the expert's rows
   auto clear_tail = [&](unsigned stage, int valid, int boxes) {
     const int pieces = (16 - valid % 16) * 8;
     for (int i = lane; i < pieces * boxes; i += 32)
-      *reinterpret_cast<uint4*>(stages + stage * Shared::STAGE + i / pieces * BOX64 + valid * 128 + i % pieces * 16) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(stages + stage * Shared::STAGE + i / pieces * CHUNK + valid * 128 + i % pieces * 16) = make_uint4(0, 0, 0, 0);
     tb200::fence_async_smem();
     __syncwarp();
   };
@@ -270,8 +270,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
     for (unsigned t = blockIdx.x / CTAS; good && t < tiles; t += step) {
       const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
       const int share = columns_of(tile) / CTAS, feature = tile.feature + (int)rank * OWN, other = (MODE == BY_ROWS ? tile.row : tile.other) + (int)rank * share;
-      const int b_rows = MODE == BY_ROWS ? p.box : p.b_chunks * 64, boxes = (share + b_rows - 1) / b_rows;
-      const unsigned b_box = b_rows * DEEP * 2, bytes = A_BYTES + boxes * b_box;
+      // by rows B has two chunks of k, each of boxes of rows, unless a box has both; by experts two chunks of others, unless a box has both
+      const int boxes = MODE == BY_ROWS ? (share + p.box - 1) / p.box : p.b_split ? 2 : (share + 63) / 64;
+      const unsigned b_box = MODE == BY_ROWS ? p.box * 128 : CHUNK, bytes = A_BYTES + (MODE == BY_ROWS ? 2 : 1) * boxes * b_box;
       for (int k = 0; k < tile.depth; k += DEEP, ++count) {
         const unsigned stage = count % STAGES, to = base + stage * Shared::STAGE;
         good = await<PAIR>(&sh.empty[stage], (count / STAGES & 1) ^ 1, &sh.dead, p.hdr);
@@ -288,24 +289,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
             bar = PAIR ? tb200_tc::first_ones(&sh.full[stage]) : tb200::smem_addr(&sh.full[stage]);
           }
           if (!withheld(t, step)) {
+            const int row = MODE == BY_ROWS ? k : tile.row + k, e = MODE == BY_ROWS ? (int)tile.e : 0;
+            const bool both = p.a_split || (GATED && p.a_mn);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              if (c && both) continue;
+              tb200_tc::box_at at;
+              if (MODE == BY_EXPERTS || p.a_mn) at = {p.a_split ? 0 : feature + c * 64, row, p.a_split ? feature / 64 : 0, 0, e};
+              else at = {p.a_split ? 0 : k + c * 64, feature, p.a_split && !GATED ? k / 64 : 0, p.a_split && GATED ? k / 64 : 0, e};
+              tb200_tc::load_box<PAIR>(to + c * CHUNK, &map_a, at, bar);
+            }
             if (MODE == BY_EXPERTS) {
-              for (int c = 0; c < 2; c += p.a_chunks) {
-                const int f = feature + c * 64;
-                tb200_tc::load_box<PAIR>(to + c * BOX64, &map_a, p.a_chunks == 1 ? f : 0, tile.row + k, p.a_chunks == 1 ? 0 : f / 64, 0, bar);
-              }
-              for (int b = 0; b < boxes; ++b)
-                tb200_tc::load_box<PAIR>(to + A_BYTES + b * b_box, &map_b, p.b_chunks == 1 ? other + b * 64 : 0, tile.row + k, p.b_chunks == 1 ? 0 : other / 64, 0, bar);
+              if (p.b_split) tb200_tc::load_box<PAIR>(to + A_BYTES, &map_b, {0, row, other / 64, 0, 0}, bar);
+              else
+                for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + b * CHUNK, &map_b, {other + b * 64, row, 0, 0, 0}, bar);
+            } else if (PAIR && p.b_split) {
+              tb200_tc::load_box<PAIR>(to + A_BYTES, &map_b, {0, other, k / 64, 0, 0}, bar);
             } else {
-              if (p.a_mn) {
-                for (int c = 0; c < 2; c += p.a_chunks) {
-                  const int f = GATED && c ? p.second + feature : feature + c * 64;
-                  tb200_tc::load_box<PAIR>(to + c * BOX64, &map_a, p.a_chunks == 1 ? f : 0, k, p.a_chunks == 1 ? 0 : f / 64, tile.e, bar);
-                }
-              } else {
-                tb200_tc::load_box<PAIR>(to, &map_a, k, feature, 0, tile.e, bar);
-                if (GATED) tb200_tc::load_box<PAIR>(to + BOX64, &map_a, k, p.second + feature, 0, tile.e, bar);
-              }
-              for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + b * b_box, &map_b, k, other + b * p.box, 0, 0, bar);
+              for (int c = 0; c < 2; ++c)
+                for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + c * Shared::B_CHUNK + b * b_box, &map_b, {k + c * 64, other + b * p.box, 0, 0, 0}, bar);
             }
           }
         }
@@ -324,7 +326,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
     bool good = true;
     const bool a_mn = MODE == BY_EXPERTS || p.a_mn;
     constexpr bool b_mn = MODE == BY_EXPERTS;
-    const unsigned a_step = tb200_tc::step_of(a_mn), b_step = tb200_tc::step_of(b_mn);
+    // from one 16 k to the next, and from one 64 to the next, in a descriptor's units of 16 bytes
+    const unsigned a_step = a_mn ? 16 * 128 >> 4 : 2, a_jump = a_mn ? 64 * 128 >> 4 : CHUNK >> 4;
+    constexpr unsigned b_step = b_mn ? 16 * 128 >> 4 : 2, b_jump = b_mn ? 64 * 128 >> 4 : Shared::B_CHUNK >> 4;
     if (rank == 0) {
       for (unsigned t = blockIdx.x / CTAS; good && t < tiles; t += step) {
         const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
@@ -351,10 +355,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
           }
           tb200_tc::fence_after_sync();
           if (tb200_tc::elected()) {
-            unsigned long long a = tb200_tc::operand(from, a_mn, BOX64), b = tb200_tc::operand(from + A_BYTES, b_mn, BOX64);
+            const unsigned long long a = tb200_tc::operand(from, a_mn, CHUNK), b = tb200_tc::operand(from + A_BYTES, b_mn, CHUNK);
 #pragma unroll
-            for (int i = 0; i < DEEP / 16; ++i, a += a_step, b += b_step)
-              if (i < steps) tb200_tc::multiply<PAIR>(d, a, b, what, k > 0 || i > 0);
+            for (int i = 0; i < DEEP / 16; ++i)
+              if (i < steps) tb200_tc::multiply<PAIR>(d, a + i / 4 * a_jump + i % 4 * a_step, b + i / 4 * b_jump + i % 4 * b_step, what, k > 0 || i > 0);
             tb200_tc::commit<PAIR>(&sh.empty[stage]);
           }
           __syncwarp();
@@ -692,16 +696,22 @@ encode_call encoder() {
   }();
   return call;
 }
-// Matrices [count][rows][width], rows `stride` and matrices `outer` elements apart, in boxes of `chunks` times 64 neighbouring elements (128 bytes, swizzled) of
-// `box` rows; coordinates are element (of the 64, where there are several chunks), row, chunk, matrix.  Several chunks only where rows are made of whole ones: otherwise the
-// last would go on into the next row.
-template <class T> bool box_map(CUtensorMap& map, const void* at, size_t width, size_t rows, size_t stride, size_t count, size_t outer, unsigned box, unsigned chunks) {
-  const cuuint64_t apart = (count > 1 ? outer : rows * stride) * 2;
-  const cuuint64_t dims[4] = {chunks > 1 ? 64 : width, rows, chunks > 1 ? width / 64 : 1, count ? count : 1}, strides[3] = {stride * 2, 128, apart};
-  const cuuint32_t boxes[4] = {64, box, chunks, 1}, steps[4] = {1, 1, 1, 1};
-  return encoder() && encoder()(&map, std::is_same<T, f16>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(at), dims, strides, boxes, steps,
+// A tensor as the copy engine takes boxes from it, 128 bytes of its innermost axis at a time, swizzled.  apart: in elements, of all axes but the innermost.
+struct box_axes { size_t size[5], apart[4]; unsigned box[5]; };
+template <class T> bool box_map(CUtensorMap& map, const void* at, const box_axes& x) {
+  cuuint64_t dims[5], strides[4];
+  cuuint32_t boxes[5], steps[5];
+  for (int i = 0; i < 5; ++i) { dims[i] = x.size[i]; boxes[i] = x.box[i]; steps[i] = 1; }
+  for (int i = 0; i < 4; ++i) strides[i] = x.size[i + 1] > 1 ? x.apart[i] * 2 : 128;      // (an axis of one may lie anywhere)
+  return encoder() && encoder()(&map, std::is_same<T, f16>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(at), dims, strides, boxes, steps,
                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// Matrices of `rows` rows of `width` elements, in boxes of 64 (split: `chunks` times 64) neighbours by `box` rows.  Split only where rows are made of whole chunks: otherwise the last
+// would go on into the next row.
+box_axes plain_axes(size_t width, size_t rows, size_t stride, size_t count, size_t outer, unsigned box, bool split, unsigned chunks) {
+  return {{split ? 64 : width, rows, split ? width / 64 : 1, 1, count}, {stride, 64, 0, outer}, {64, box, split ? chunks : 1, 1, 1}};
+}
+
 // Matrices as a kernel is given them: as they lie, or packed into the workspace.
 struct matrices {
   const void* at;
@@ -774,16 +784,18 @@ template <class T> cudaError_t product_by_rows(matrices w, matrices x, product_p
     if (e == cudaSuccess) e = pack<T>(x, room, stream);
     if (e != cudaSuccess) return e;
     p.second = p.a_mn ? (int)(w.halves == 2 ? w.width / 2 : 0) : p.features;
-    // chunks of one box are neighbours, those of the two halves are not
-    p.a_chunks = p.a_mn && !gated && w.width % 64 == 0 ? 2 : 1;
+    p.a_split = w.width % 64 == 0 && !(gated && p.a_mn);
+    box_axes of_a = plain_axes(w.width, w.rows, w.stride, w.count, w.outer, 128, p.a_split, 2);
+    if (gated && p.a_mn) of_a = {{(size_t)p.features, w.rows, 2, 1, w.count}, {w.stride, (size_t)p.second, 0, w.outer}, {64, 128, 2, 1, 1}};      // 64 of either half
+    else if (gated) of_a = {{p.a_split ? 64 : w.width, (size_t)p.features, 2, p.a_split ? w.width / 64 : 1, w.count}, {w.stride, p.features * w.stride, 64, w.outer},
+                            {64, 64, 2, p.a_split ? 2u : 1u, 1}};
     for (;; few = true) {      // (again, by single CTAs, if there is no room for pairs)
       p.box = few ? 16 : 128;
+      p.b_split = !few && x.width % 64 == 0;
       CUtensorMap a = {}, b = {};
-      if (p.k > 0 && (!box_map<T>(a, w.at, w.width, w.rows, w.stride, w.count, w.outer, p.a_mn || gated ? 64 : 128, p.a_chunks) ||
-                      !box_map<T>(b, x.at, x.width, x.rows, x.stride, 0, 0, (unsigned)p.box, 1)))
-        return cudaErrorNotSupported;
-      if (few) return gated ? launch_tc<T, T, BY_ROWS, false, true, 64, 8>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, false, false, 64, 8>(a, b, p, stream);
-      e = gated ? launch_tc<T, T, BY_ROWS, true, true, 256, 6>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, true, false, 256, 6>(a, b, p, stream);
+      if (p.k > 0 && (!box_map<T>(a, w.at, of_a) || !box_map<T>(b, x.at, plain_axes(x.width, x.rows, x.stride, 1, 0, (unsigned)p.box, p.b_split, 2)))) return cudaErrorNotSupported;
+      if (few) return gated ? launch_tc<T, T, BY_ROWS, false, true, 64, 4>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, false, false, 64, 4>(a, b, p, stream);
+      e = gated ? launch_tc<T, T, BY_ROWS, true, true, 256, 3>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, true, false, 256, 3>(a, b, p, stream);
       if (!tb200::launch_refused(e)) return e;
     }
   }
@@ -797,17 +809,17 @@ template <class T, class O> cudaError_t product_by_experts(const matrices& featu
                                                                                                             static_cast<const float*>(others.at), others.stride, p);
     return cudaGetLastError();
   } else {
-    p.a_chunks = features.width % 64 == 0 ? 2 : 1;
-    for (bool pair = p.features > 128;; pair = false) {
-      CUtensorMap a = {}, b = {};
-      p.b_chunks = others.width % 64 == 0 ? pair ? 2 : 4 : 1;
-      if (p.m > 0 && (!box_map<T>(a, features.at, features.width, features.rows, features.stride, 0, 0, 64, p.a_chunks) ||
-                      !box_map<T>(b, others.at, others.width, others.rows, others.stride, 0, 0, 64, p.b_chunks)))
-        return cudaErrorNotSupported;
-      if (!pair) return launch_tc<T, O, BY_EXPERTS, false, false, 256, 4>(a, b, p, stream);
-      const cudaError_t e = launch_tc<T, O, BY_EXPERTS, true, false, 256, 6>(a, b, p, stream);
-      if (!tb200::launch_refused(e)) return e;
+    p.a_split = features.width % 64 == 0;
+    p.b_split = others.width % 64 == 0;
+    CUtensorMap a = {}, b = {};
+    if (p.m > 0 && (!box_map<T>(a, features.at, plain_axes(features.width, features.rows, features.stride, 1, 0, DEEP, p.a_split, 2)) ||
+                    !box_map<T>(b, others.at, plain_axes(others.width, others.rows, others.stride, 1, 0, DEEP, p.b_split, 2))))
+      return cudaErrorNotSupported;
+    if (p.features > 128) {
+      const cudaError_t e = launch_tc<T, O, BY_EXPERTS, true, false, 256, 3>(a, b, p, stream);
+      if (!tb200::launch_refused(e)) return e;      // (no room for pairs)
     }
+    return launch_tc<T, O, BY_EXPERTS, false, false, 128, 3>(a, b, p, stream);
   }
 }
 

@@ -46,14 +46,11 @@ __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence
 // ---------------------------------------------------------------- operands
 // Operands lie in shared memory as the copy engine leaves boxes of 128-byte rows with the 128-byte swizzle: 8 rows are an atom of 1024 bytes, on a
 // boundary of as much.  K-major: a row has 64 neighbouring k of one m (or n), atoms follow one another along m.  MN-major: a row has 64
-// neighbouring m of one k, atoms follow one another along k, and the next 64 m are `box` bytes on.
+// neighbouring m of one k, atoms follow one another along k, and the next 64 m are `chunk` bytes on.
 constexpr unsigned long long DESCRIPTOR = 1ull << 46 | 2ull << 61;      // version, 128-byte swizzle
-__device__ __forceinline__ unsigned long long operand(unsigned smem, bool mn_major, unsigned box) {
-  return DESCRIPTOR | (unsigned long long)(1024 >> 4) << 32 | (unsigned long long)(mn_major ? box >> 4 : 1) << 16 | (smem & 0x3ffff) >> 4;
+__device__ __forceinline__ unsigned long long operand(unsigned smem, bool mn_major, unsigned chunk) {
+  return DESCRIPTOR | (unsigned long long)(1024 >> 4) << 32 | (unsigned long long)(mn_major ? chunk >> 4 : 1) << 16 | (smem & 0x3ffff) >> 4;
 }
-// 16 k further on, in a descriptor's units of 16 bytes
-__device__ __forceinline__ unsigned step_of(bool mn_major) { return mn_major ? 2048 >> 4 : 32 >> 4; }
-
 // D (F32, m x n in tensor memory) = or += A (m x 16) B (n x 16) of 16-bit elements: m = 128, n a multiple of 16 up to 256.  PAIR: m = 256, n a multiple of 32; each of
 // the two CTAs has half of A's m, half of B's n and the whole of n for its half of D's m.
 template <bool PAIR> __device__ __forceinline__ unsigned instruction(bool bf16, bool a_mn_major, bool b_mn_major, unsigned n) {
@@ -94,14 +91,15 @@ __device__ __forceinline__ void meet_pair() {
 
 // ---------------------------------------------------------------- boxes by the copy engine
 // into this CTA's shared memory; PAIR: counted by a barrier in that of either CTA
-template <bool PAIR> __device__ __forceinline__ void load_box(unsigned dst, const void* map, int x, int y, int z, int w, unsigned bar) {
+struct box_at { int x, y, z, w, v; };
+template <bool PAIR> __device__ __forceinline__ void load_box(unsigned dst, const void* map, box_at c, unsigned bar) {
   if (PAIR)
-    asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y),
-                 "r"(z), "r"(w), "r"(bar)
+    asm volatile("cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(map), "r"(c.x),
+                 "r"(c.y), "r"(c.z), "r"(c.w), "r"(c.v), "r"(bar)
                  : "memory");
   else
-    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w),
-                 "r"(bar)
+    asm volatile("cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(map), "r"(c.x), "r"(c.y), "r"(c.z),
+                 "r"(c.w), "r"(c.v), "r"(bar)
                  : "memory");
 }
 
