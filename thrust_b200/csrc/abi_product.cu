@@ -76,6 +76,7 @@ template <class T> struct product_plan {
   int m, k, features, others;
   int second;                 // gated: where the second half of the features begins in A
   bool a_mn;                  // A's features are neighbours (else its k)
+  bool wide_out, wide_residual;      // rows are made of whole 16-byte pieces
   bool a_split, b_split;      // rows are made of whole chunks of 64 and mapped as such: a box has several
   int box;                    // by rows: rows in a box of B
   const T *bias, *residual;
@@ -156,14 +157,14 @@ __device__ __forceinline__ bool withheld(unsigned, unsigned) { return false; }
 #endif
 
 constexpr int DEEP = 128;                     // of the contraction, a stage
-constexpr int TC_THREADS = 192;               // warps 0 to 3 write results, 4 brings operands, 5 multiplies
+constexpr int WRITERS = 8, BRINGS = WRITERS, MULTIPLIES = WRITERS + 1, TC_THREADS = (WRITERS + 2) * 32;      // warps that write results, that bring operands, that multiply
 constexpr unsigned CHUNK = 64 * DEEP * 2;     // 64 neighbours by 128 of the other axis
 constexpr unsigned A_BYTES = 2 * CHUNK;       // a CTA's 128 features
 
 template <bool PAIR, bool GATED, int BN, int STAGES> struct tc_shared {
   static constexpr unsigned B_CHUNK = BN * 128 / (PAIR ? 2 : 1), STAGE = A_BYTES + 2 * B_CHUNK, COLUMNS = 2 * BN;
   static_assert(COLUMNS <= 512, "two sets of sums in tensor memory");
-  float halves[GATED ? 2 : 1][GATED ? 4 : 1][GATED ? 16 : 1][32];
+  alignas(16) unsigned char turn[WRITERS][2048];      // where a writer's results are turned round
   unsigned long long full[STAGES], empty[STAGES], tail[STAGES], ready[STAGES], made[2], taken[2], done;
   unsigned tmem;
   int dead;
@@ -188,8 +189,27 @@ __device__ __forceinline__ void outlast(unsigned long long* bar, unsigned parity
   for (unsigned iter = 0; iter < tb200::MBAR_SPIN_LIMIT && !tb200::mbar_try_wait(bar, parity); ++iter) {}
 }
 
-// results of N columns in a lane's registers go to p, p + stride, ...: the warp writes 32 neighbouring features at a time
-template <class O, int N> __device__ __forceinline__ void put_column(O* p, size_t stride, int count, const float (&v)[N]) {
+// Results of N columns in a lane's registers go to p, p + stride, ...; p: of the warp's first lane, whose neighbours' results lie next to its own.  With `wide` rows (whole
+// 16-byte pieces) of a 16-bit type they are turned round in shared memory and written 16 bytes a lane, `room` elements (of 32) being there; otherwise element by element.
+template <class O, int N> __device__ __forceinline__ void put_columns(O* p, size_t stride, int count, const float (&v)[N], int lane, int room, bool wide, unsigned char* turn) {
+  if constexpr (sizeof(O) == 2) {
+    if (wide) {
+      O* const t = reinterpret_cast<O*>(turn);
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < N; ++j) t[j * 32 + lane] = from_f32<O>(v[j]);
+      __syncwarp();
+      const int c = lane % 4 * 8;
+#pragma unroll
+      for (int i = 0; i < N / 8; ++i) {
+        const int j = i * 8 + lane / 4;
+        if (j < count && c < room) *reinterpret_cast<uint4*>(p + (size_t)j * stride + c) = *reinterpret_cast<const uint4*>(t + j * 32 + c);
+      }
+      return;
+    }
+  }
+  if (lane >= room) return;
+  p += lane;
   if (count >= N) {
 #pragma unroll
     for (int j = 0; j < N; ++j) p[(size_t)j * stride] = from_f32<O>(v[j]);
@@ -199,23 +219,52 @@ template <class O, int N> __device__ __forceinline__ void put_column(O* p, size_
       if (j < count) p[(size_t)j * stride] = from_f32<O>(v[j]);
   }
 }
-// and come from there (of columns past the count, the last one's: no branch between the requests); none: nothing
-template <class O, int N> __device__ __forceinline__ void get_column(const O* p, size_t stride, int count, O (&v)[N]) {
-  if (count >= N) {
+// The same the other way: requested, and (turned round) added to v
+template <class O, int N> struct columns_in {
+  static constexpr int W = sizeof(O) == 2 ? N / 8 : 1;
+  O at[N];
+  uint4 pieces[W];
+  __device__ __forceinline__ void request(const O* p, size_t stride, int count, int lane, int room, bool wide) {
+    if constexpr (sizeof(O) == 2) {
+      if (wide) {
+        const int c = lane % 4 * 8;
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = p[(size_t)j * stride];
-  } else if (count > 0) {
+        for (int i = 0; i < W; ++i) {
+          const int j = i * 8 + lane / 4;
+          if (j < count && c < room) pieces[i] = *reinterpret_cast<const uint4*>(p + (size_t)j * stride + c);
+        }
+        return;
+      }
+    }
+    if (lane >= room || count <= 0) return;
+    p += lane;
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = p[(size_t)(j < count ? j : count - 1) * stride];
+    for (int j = 0; j < N; ++j) at[j] = p[(size_t)(j < count ? j : count - 1) * stride];      // (no branch between the requests)
   }
-}
+  __device__ __forceinline__ void add(float (&v)[N], int lane, bool wide, unsigned char* turn) {
+    if constexpr (sizeof(O) == 2) {
+      if (wide) {
+        O* const t = reinterpret_cast<O*>(turn);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(t)[i * 32 + lane] = pieces[i];
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] += to_f32(t[j * 32 + lane]);
+        return;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] += to_f32(at[j]);
+  }
+};
 
 // D^T = A B^T by tiles of 128 features (gated: 64 of each half) a CTA x up to BN rows; CTAs stay and go from tile to tile.  Features are the lanes of tensor
 // memory and rows its columns, so that a tile that has few rows takes a narrower instruction and no more time than they need: experts have as many rows as they have.
 // PAIR: two CTAs have a tile of twice as many features, half of its rows' operands each, and instructions that read both's shared memory, which the first
 // issues: 64 KB instead of 96 come from L2 for 256 features x 256 rows x 64.
 //
-// One warp keeps STAGES boxes of A and B on their way by the copy engine, one issues the matrix instructions as they come, four take the sums of the last
+// One warp keeps STAGES boxes of A and B on their way by the copy engine, one issues the matrix instructions as they come, eight take the sums of the last
 // tile from tensor memory, while the next one's are made in its other half, and write them.  Sums are 32 bits from first to last; they
 // are rounded once, where they are stored, after bias, activation and residual.  Gated: the two halves of a result are in lanes 64 apart, in warps that pass each
 // other half of their columns.
@@ -240,12 +289,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
     for (int i = 0; i < STAGES; ++i) {
       for (unsigned long long* bar : {&sh.full[i], &sh.empty[i], &sh.tail[i], &sh.ready[i]}) tb200::mbar_init(bar, 1);
     }
-    for (int i = 0; i < 2; ++i) { tb200::mbar_init(&sh.made[i], 1); tb200::mbar_init(&sh.taken[i], 4 * CTAS); }
+    for (int i = 0; i < 2; ++i) { tb200::mbar_init(&sh.made[i], 1); tb200::mbar_init(&sh.taken[i], WRITERS * CTAS); }
     tb200::mbar_init(&sh.done, 1);
     sh.dead = 0;
     tb200::mbar_init_fence();
   }
-  if (warp == 5) tb200_tc::tmem_alloc<PAIR>(&sh.tmem, Shared::COLUMNS);
+  if (warp == MULTIPLIES) tb200_tc::tmem_alloc<PAIR>(&sh.tmem, Shared::COLUMNS);
   tb200_tc::fence_before_sync();
   read_spans(s, p.offsets, p.wide, p.experts, p.m, BN);
   if (PAIR) tb200_tc::meet_pair();
@@ -263,7 +312,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
     __syncwarp();
   };
 
-  if (warp == 4) {
+  if (warp == BRINGS) {
     const unsigned base = tb200::smem_addr(stages);
     unsigned count = 0, e = 0;      // stages filled so far
     bool good = true;
@@ -320,7 +369,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
     // given up: what is on its way is counted where this warp may not be able to see it; copies take microseconds
     if (!good)
       for (int i = 0; i < 20; ++i) __nanosleep(1000000);
-  } else if (warp == 5) {
+  } else if (warp == MULTIPLIES) {
     const unsigned base = tb200::smem_addr(stages);
     unsigned count = 0, made = 0, e = 0, tails = 0;      // tails: a bit for each stage's barrier
     bool good = true;
@@ -383,61 +432,71 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
       }
     }
   } else {
-    unsigned made = 0, e = 0, turn = 0;
+    // a writer has the 32 lanes that warp % 4 may read, and every other 32 columns; GATED: of these it finishes 16, of both halves
+    unsigned made = 0, e = 0;
     bool good = true;
-    const int kind = p.activation & ~ACT_GATED, half = GATED ? warp / 2 : 0, within = GATED ? warp % 2 * 32 + lane : warp * 32 + lane;
-    constexpr int PUT = GATED ? 16 : 32;      // columns of results that a lane ends up with, of 32 of sums
+    const int kind = p.activation & ~ACT_GATED, quarter = warp % 4, half = GATED ? quarter / 2 : 0, within = (GATED ? quarter % 2 : quarter) * 32;
+    unsigned char* const turn = sh.turn[warp];
+    constexpr int PUT = GATED ? 16 : 32;
     for (unsigned t = blockIdx.x / CTAS; t < tiles; t += step) {
       const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
-      const unsigned set = made & 1, d = tmem + (warp * 32u << 16) + set * BN;
-      if (tile.depth) {
-        if (good) good = await<PAIR>(&sh.made[set], made / 2 & 1, &sh.dead, p.hdr);
-        ++made;
-        tb200_tc::fence_after_sync();
-      }
-      const int f = tile.feature + (int)rank * OWN + within;
-      const bool there = f < p.features;
+      const unsigned set = made & 1, d = tmem + (quarter * 32u << 16) + set * BN;
+      const int f = tile.feature + (int)rank * OWN + within, room = p.features - f;      // the first lane's feature, and how many there are from there on
+      const bool there = lane < room;
       const size_t width = p.features, both = GATED ? 2 * width : width;
-      float b0 = 0.f;
-      if (MODE == BY_ROWS && p.bias && there) b0 = to_f32(p.bias[tile.e * both + half * width + f]);
-      for (int c = 0; c < tile.rows; c += 32) {
+      float bias = 0.f;
+      if (MODE == BY_ROWS && p.bias && there) bias = to_f32(p.bias[tile.e * both + half * width + f + lane]);
+      bool waited = tile.depth == 0;
+      for (int c = warp / 4 * 32;; c += 64) {
+        const bool any = c < tile.rows;
+        const int mine = c + half * 16;
+        columns_in<T, PUT> residual;
+        columns_in<O, 32> old;
+        O* const to = static_cast<O*>(p.matrix) + ((size_t)tile.e * p.others + tile.other + c) * width + f;
+        if (MODE == BY_ROWS && p.residual && any) residual.request(p.residual + ((size_t)tile.row + mine) * p.residual_stride + f, p.residual_stride, tile.rows - mine, lane, room, p.wide_residual);
+        if (MODE == BY_EXPERTS && p.accumulate && any) old.request(to, width, tile.rows - c, lane, room, p.wide_out);
+        if (!waited) {
+          if (good) good = await<PAIR>(&sh.made[set], made / 2 & 1, &sh.dead, p.hdr);
+          ++made;
+          waited = true;
+          tb200_tc::fence_after_sync();
+        }
         float v[32];
-        T r[PUT];
-        const int mine = c + half * 16, count = tile.rows - mine;      // columns of results
-        if (MODE == BY_ROWS && p.residual && there) get_column(p.residual + ((size_t)tile.row + mine) * p.residual_stride + f, p.residual_stride, count, r);
-        if (tile.depth && good) {
+        if (any && tile.depth && good) {
           tb200_tc::tmem_load(v, d + c);
           tb200_tc::tmem_load_wait();
-          if (c + 32 >= tile.rows) {      // the last of them: the next sums may be made there
-            tb200_tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-              if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.taken[set]));
-              else tb200::mbar_arrive(&sh.taken[set]);
-            }
-          }
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = good ? 0.f : __int_as_float(0x7fffffff);
         }
+        if (c + 64 >= tile.rows && tile.depth && good) {      // the last of them: the next sums may be made there
+          tb200_tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.taken[set]));
+            else tb200::mbar_arrive(&sh.taken[set]);
+          }
+        }
+        if (!any) break;
         if (MODE == BY_ROWS) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += b0;
-          if (p.before && there) put_column(p.before + ((size_t)tile.row + c) * both + half * width + f, both, tile.rows - c, v);
+          for (int j = 0; j < 32; ++j) v[j] += bias;
+          if (p.before) put_columns(p.before + ((size_t)tile.row + c) * both + half * width + f, both, tile.rows - c, v, lane, room, p.wide_out, turn);
           float w[PUT];
           if constexpr (GATED) {
-            float (&out)[16][32] = sh.halves[turn][warp], (&in)[16][32] = sh.halves[turn][warp ^ 2];
+            float (&out)[16][32] = *reinterpret_cast<float(*)[16][32]>(turn), (&in)[16][32] = *reinterpret_cast<float(*)[16][32]>(sh.turn[warp ^ 2]);
+            __syncwarp();
 #pragma unroll
             for (int j = 0; j < 16; ++j) out[j][lane] = half ? v[j] : v[j + 16];
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + warp % 2) : "memory");
-            turn ^= 1;
+            const int pair = 1 + warp / 4 * 2 + warp % 2;      // the barrier of the two warps
+            asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
 #pragma unroll
             for (int j = 0; j < 16; ++j) { const float x = in[j][lane]; w[j] = half ? x : v[j]; v[j] = half ? v[j + 16] : x; }      // act(w) v
+            asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
           } else {
 #pragma unroll
             for (int j = 0; j < 32; ++j) w[j] = v[j];
           }
-          if (!there) continue;
           if (kind == ACT_SILU) {
 #pragma unroll
             for (int j = 0; j < PUT; ++j) w[j] = activated<true>(w[j], ACT_SILU);
@@ -449,30 +508,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
 #pragma unroll
             for (int j = 0; j < PUT; ++j) w[j] *= v[j];
           }
-          if (p.residual) {
-#pragma unroll
-            for (int j = 0; j < PUT; ++j) w[j] += to_f32(r[j]);
-          }
-          put_column(p.out + ((size_t)tile.row + mine) * width + f, width, count, w);
-        } else if (there) {
-          O* const q = static_cast<O*>(p.matrix) + ((size_t)tile.e * p.others + tile.other + c) * width + f;
-          if (p.accumulate) {
-            if (tile.depth == 0 && good) continue;      // nothing is added
-            O old[32];
-            get_column(q, width, tile.rows - c, old);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] += to_f32(old[j]);
-          }
-          put_column(q, width, tile.rows - c, v);
+          if (p.residual) residual.add(w, lane, p.wide_residual, turn);
+          put_columns(p.out + ((size_t)tile.row + mine) * width + f, width, tile.rows - mine, w, lane, room, p.wide_out, turn);
+        } else if (!p.accumulate) {
+          put_columns(to, width, tile.rows - c, v, lane, room, p.wide_out, turn);
+        } else if (tile.depth || !good) {      // (an expert without rows adds nothing)
+          old.add(v, lane, p.wide_out, turn);
+          put_columns(to, width, tile.rows - c, v, lane, room, p.wide_out, turn);
         }
+        if (c + 64 >= tile.rows) break;
       }
     }
-    if (MODE == BY_ROWS) clear_others(p, s, (size_t)blockIdx.x * 128 + threadIdx.x, (size_t)gridDim.x * 128);
+    if (MODE == BY_ROWS) clear_others(p, s, (size_t)blockIdx.x * WRITERS * 32 + threadIdx.x, (size_t)gridDim.x * WRITERS * 32);
     tb200_tc::fence_before_sync();
   }
   __syncthreads();
   if (PAIR) tb200_tc::meet_pair();      // neither ends while the other's instructions and arrivals come here
-  if (warp == 5) {
+  if (warp == MULTIPLIES) {
     tb200_tc::fence_after_sync();
     tb200_tc::tmem_free<PAIR>(tmem, Shared::COLUMNS);
   }
@@ -602,33 +654,39 @@ __global__ void __launch_bounds__(FMA_THREADS, BN == 128 ? 2 : 4) expert_product
 }
 
 // ---------------------------------------------------------------------------------------------- the smaller parts
-// The gradient of bias: the sums of each expert's rows of dout.  A CTA has 64 features of one of `parts` pieces of an expert's rows; its warps take rows in turn and
+// The gradient of bias: the sums of each expert's rows of dout.  A CTA has 32 V features of one of `parts` pieces of an expert's rows; its warps take rows in turn and
 // meet in shared memory, parts meet in a second kernel, always in the same order.
 constexpr int SUM_BLOCK = 256;
-template <class T>
+template <class T, int V>
 __global__ void __launch_bounds__(SUM_BLOCK) row_sums_kernel(const T* __restrict__ x, size_t stride, const void* __restrict__ offsets, bool wide, unsigned experts, int m, int features,
                                                              float* __restrict__ sums) {
   const unsigned e = blockIdx.y, part = blockIdx.z, parts = gridDim.z;
   const int a = read_offset(offsets, wide, e, m), end = read_offset(offsets, wide, e + 1, m), n = end > a ? end - a : 0, per = (n + (int)parts - 1) / (int)parts;
   const int first = a + (int)part * per, last = (int)part * per + per < n ? first + per : a + n;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, f = blockIdx.x * 64 + lane;
-  float u = 0.f, v = 0.f;
-#pragma unroll 8
-  for (int r = first + warp; r < last; r += SUM_BLOCK / 32) {
-    const T* const row = x + (size_t)r * stride;
-    if (f < features) u += to_f32(row[f]);
-    if (f + 32 < features) v += to_f32(row[f + 32]);
-  }
-  __shared__ float met[SUM_BLOCK / 32][64];
-  met[warp][lane] = u;
-  met[warp][lane + 32] = v;
-  __syncthreads();
-  const int g = blockIdx.x * 64 + (int)threadIdx.x;
-  if (threadIdx.x < 64 && g < features) {
-    float sum = 0.f;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, f = (blockIdx.x * 32 + lane) * V;
+  float sum[V];
 #pragma unroll
-    for (int w = 0; w < SUM_BLOCK / 32; ++w) sum += met[w][threadIdx.x];
-    sums[((size_t)part * experts + e) * features + g] = sum;
+  for (int v = 0; v < V; ++v) sum[v] = 0.f;
+  if (f < features) {
+#pragma unroll 4
+    for (int r = first + warp; r < last; r += SUM_BLOCK / 32) {
+      float g[V];
+      channels(load_words<T, V>(x + (size_t)r * stride + f), g);
+#pragma unroll
+      for (int v = 0; v < V; ++v) sum[v] += g[v];
+    }
+  }
+  __shared__ float met[SUM_BLOCK / 32][32 * V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) met[warp][lane * V + v] = sum[v];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * V; i += SUM_BLOCK) {
+    const int g = blockIdx.x * 32 * V + i;
+    if (g >= features) break;
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < SUM_BLOCK / 32; ++w) all += met[w][i];
+    sums[((size_t)part * experts + e) * features + g] = all;
   }
 }
 __global__ void __launch_bounds__(SUM_BLOCK) join_sums_kernel(const float* __restrict__ sums, size_t items, unsigned parts, float* __restrict__ out) {
@@ -654,34 +712,47 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ fr
   reinterpret_cast<uint4*>(to)[i] = v.all;
 }
 
-// dbefore = dout * the activation's slope; gated with out = act(a) b: da = dout b act'(a), db = dout act(a).  Bound by the bytes.
+// dbefore = dout * the activation's slope; gated with out = act(a) b: da = dout b act'(a), db = dout act(a).  Bound by the bytes; a thread asks for two places' pieces before
+// it works on either.
 template <class T, int V>
 __global__ void __launch_bounds__(256) activation_grad_kernel(const T* __restrict__ dout, size_t stride, const T* __restrict__ before, size_t n, unsigned pieces, bool gated, int kind,
                                                               T* __restrict__ dbefore) {
   constexpr bool FAST = sizeof(T) == 2;
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n * pieces) return;
-  const size_t row = i / pieces, c = (i - row * pieces) * V, width = (size_t)pieces * V;
-  const T* const x = before + row * width * (gated ? 2 : 1) + c;
-  T* const to = dbefore + row * width * (gated ? 2 : 1) + c;
-  float d[V], a[V], b[V];
-  const words<T, V> dw = load_words<T, V>(dout + row * stride + c), aw = load_words<T, V>(x);
-  words<T, V> bw = aw;
-  if (gated) bw = load_words<T, V>(x + width);
-  channels(dw, d);
-  channels(aw, a);
-  channels(bw, b);
-  if (gated) {
-    float db[V];
+  constexpr int U = 2;
+  const size_t all = n * pieces, width = (size_t)pieces * V, both = gated ? 2 * width : width;
+  words<T, V> dw[U], aw[U], bw[U];
+  size_t at[U];
 #pragma unroll
-    for (int v = 0; v < V; ++v) db[v] = d[v] * activated<FAST>(a[v], kind);
-    store_words<T, V>(to + width, to_words<T, V>(db));
-#pragma unroll
-    for (int v = 0; v < V; ++v) d[v] *= b[v];
+  for (int u = 0; u < U; ++u) {
+    const size_t i = ((size_t)blockIdx.x * U + u) * 256 + threadIdx.x;
+    at[u] = ~(size_t)0;
+    if (i >= all) continue;
+    const size_t row = all <= 0xffffffffull ? (unsigned)i / pieces : i / pieces, c = (i - row * pieces) * V;
+    at[u] = row * both + c;
+    dw[u] = load_words<T, V>(dout + row * stride + c);
+    aw[u] = load_words<T, V>(before + at[u]);
+    if (gated) bw[u] = load_words<T, V>(before + at[u] + width);
   }
 #pragma unroll
-  for (int v = 0; v < V; ++v) d[v] *= slope<FAST>(a[v], kind);
-  store_words<T, V>(to, to_words<T, V>(d));
+  for (int u = 0; u < U; ++u) {
+    if (at[u] == ~(size_t)0) continue;
+    T* const to = dbefore + at[u];
+    float d[V], a[V];
+    channels(dw[u], d);
+    channels(aw[u], a);
+    if (gated) {
+      float b[V], db[V];
+      channels(bw[u], b);
+#pragma unroll
+      for (int v = 0; v < V; ++v) db[v] = d[v] * activated<FAST>(a[v], kind);
+      store_words<T, V>(to + width, to_words<T, V>(db));
+#pragma unroll
+      for (int v = 0; v < V; ++v) d[v] *= b[v];
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) d[v] *= slope<FAST>(a[v], kind);
+    store_words<T, V>(to, to_words<T, V>(d));
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- calls
@@ -784,6 +855,9 @@ template <class T> cudaError_t product_by_rows(matrices w, matrices x, product_p
     if (e == cudaSuccess) e = pack<T>(x, room, stream);
     if (e != cudaSuccess) return e;
     p.second = p.a_mn ? (int)(w.halves == 2 ? w.width / 2 : 0) : p.features;
+    const size_t both = (size_t)p.features * (gated ? 2 : 1);
+    p.wide_out = in_16_bytes(p.out, p.features, p.features, 2) && in_16_bytes(p.before, both, both, 2);
+    p.wide_residual = in_16_bytes(p.residual, p.features, p.residual_stride, 2);
     p.a_split = w.width % 64 == 0 && !(gated && p.a_mn);
     box_axes of_a = plain_axes(w.width, w.rows, w.stride, w.count, w.outer, 128, p.a_split, 2);
     if (gated && p.a_mn) of_a = {{(size_t)p.features, w.rows, 2, 1, w.count}, {w.stride, (size_t)p.second, 0, w.outer}, {64, 128, 2, 1, 1}};      // 64 of either half
@@ -809,6 +883,7 @@ template <class T, class O> cudaError_t product_by_experts(const matrices& featu
                                                                                                             static_cast<const float*>(others.at), others.stride, p);
     return cudaGetLastError();
   } else {
+    p.wide_out = in_16_bytes(p.matrix, p.features, p.features, sizeof(O));
     p.a_split = features.width % 64 == 0;
     p.b_split = others.width % 64 == 0;
     CUtensorMap a = {}, b = {};
@@ -834,10 +909,10 @@ bool weights_fit(size_t experts, size_t in, size_t out, size_t expert_stride, si
   const size_t width = inputs_inside ? in : out, rows = inputs_inside ? out : in;
   return stride >= width && (experts == 1 || expert_stride >= (rows ? (rows - 1) * stride + width : 0));
 }
-// how many pieces of an expert's rows are added up side by side
+// how many pieces of an expert's rows are added up side by side: as long as a warp has eight rows, enough CTAs for every SM to hold eight
 unsigned sum_parts(size_t n, size_t experts, size_t out) {
-  const size_t ctas = ((out + 63) / 64) * experts, most = (size_t)tb200::current_device_info().sm_count * 8, rows = n / experts / 64;
-  size_t parts = ctas ? most / ctas : 1;
+  const size_t ctas = ((out + 255) / 256) * experts, most = (size_t)tb200::current_device_info().sm_count * 8, rows = n / experts / 64;
+  size_t parts = ctas ? (most + ctas - 1) / ctas : 1;
   if (parts > rows) parts = rows;
   return (unsigned)(parts < 1 ? 1 : parts > 256 ? 256 : parts);
 }
@@ -936,8 +1011,13 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
       }
       if (d_dbias && out) {
         float* const to = parts > 1 ? partial : d_dbias;
-        row_sums_kernel<T><<<dim3((unsigned)((out + 63) / 64), (unsigned)num_experts, parts), SUM_BLOCK, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, d_offsets, sizeof(iv) == 8,
-                                                                                                                (unsigned)num_experts, (int)n, (int)out, to);
+        auto add = [&](auto vv) {
+          constexpr int V = decltype(vv)::value;
+          row_sums_kernel<T, V><<<dim3((unsigned)((out + 32 * V - 1) / (32 * V)), (unsigned)num_experts, parts), SUM_BLOCK, 0, stream>>>(
+              static_cast<const T*>(d_dout), dout_stride, d_offsets, sizeof(iv) == 8, (unsigned)num_experts, (int)n, (int)out, to);
+        };
+        if (in_16_bytes(d_dout, out, dout_stride, sizeof(T))) add(std::integral_constant<int, 16 / sizeof(T)>());
+        else add(std::integral_constant<int, 1>());
         if (parts > 1) join_sums_kernel<<<(unsigned)((num_experts * out + SUM_BLOCK - 1) / SUM_BLOCK), SUM_BLOCK, 0, stream>>>(partial, num_experts * out, parts, d_dbias);
         e = cudaGetLastError();
       }
@@ -956,7 +1036,7 @@ TB200_API int tb200_expert_activation_grad(const void* d_dout, size_t dout_strid
     if (!d_dout || !d_before || !d_dbefore || dout_stride < width) return ERR_INVALID;
     auto go = [&](auto vv) -> int {
       constexpr int V = decltype(vv)::value;
-      const size_t grid = (n * (width / V) + 255) / 256;
+      const size_t grid = (n * (width / V) + 511) / 512;
       if (grid > 0x7fffffffull) return ERR_INVALID;
       activation_grad_kernel<T, V><<<(unsigned)grid, 256, 0, stream>>>(static_cast<const T*>(d_dout), dout_stride, static_cast<const T*>(d_before), n, (unsigned)(width / V), gated,
                                                                       activation & ~ACT_GATED, static_cast<T*>(d_dbefore));
