@@ -15,154 +15,248 @@ struct route_plan {
   bool sigmoid, renormalize;
   float scale;
 };
+// the logits' order is the scores', and no scores are added up
+__device__ __forceinline__ bool exact_by_logits(const route_plan& p) { return !p.bias && !(p.groups > 1 && p.group_best > 1); }
 
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
-template <class R> __device__ __forceinline__ R lowest() { return -(R)INFINITY; }
-
-// the largest of the warp's values; an order on floats that the warp's integer reduction knows (no NaNs come here, no -0 either)
-__device__ __forceinline__ unsigned ordered(float x) { const unsigned u = __float_as_uint(x); return u & 0x80000000u ? ~u : u | 0x80000000u; }
-__device__ __forceinline__ float warp_max(float x) {
-  const unsigned u = __reduce_max_sync(ALL, ordered(x));
-  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
-}
-template <class R> __device__ __forceinline__ R warp_sum(R x) {
+// Up to 32 / L tokens a warp, L neighbouring lanes each; lane l of them has experts l * PER to l * PER + PER - 1.
+template <int L> __device__ __forceinline__ float lanes_sum(float x) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(ALL, x, o);
+  for (int o = L / 2; o; o >>= 1) x += __shfl_xor_sync(ALL, x, o);
   return x;
 }
-__device__ __forceinline__ double warp_max(double x) {
+template <int L> __device__ __forceinline__ double lanes_sum(double x) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) { const double y = __shfl_xor_sync(ALL, x, o); x = y > x ? y : x; }
+  for (int o = L / 2; o; o >>= 1) x += __shfl_xor_sync(ALL, x, o);
   return x;
 }
-
-// Of the softmax over a row's open experts: its largest logit and the sum of exp(logit - largest).  An infinite logit leaves the others nothing.
-template <class R> struct softmax_of {
-  R top, sum;
-  __device__ __forceinline__ R share(R x) const { return x == top ? (R)1 : exp_of(x - top); }      // times the sum
-};
-template <class R> __device__ __forceinline__ R sigmoid_of(R x) { return (R)1 / ((R)1 + exp_of(-x)); }
-
-template <class R> struct best_of { R value; int at; };
-// The best of a row's experts in [low, high) other than `but`, the first of equal ones; value -inf and no place where there is none.
-template <class R, int PER> __device__ __forceinline__ best_of<R> warp_best(const R (&order)[PER], int low, int high, int but) {
-  const int lane = threadIdx.x % 32;
-  R mine = lowest<R>();
-  int at = 0x7fffffff;
+template <int L> __device__ __forceinline__ unsigned lanes_max(unsigned x) {
+  if constexpr (L == 32) {
+    return __reduce_max_sync(ALL, x);
+  } else {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = i * 32 + lane;
-    if (order[i] > mine && e >= low && e < high && e != but) { mine = order[i]; at = e; }
+    for (int o = L / 2; o; o >>= 1) { const unsigned y = __shfl_xor_sync(ALL, x, o); x = y > x ? y : x; }
+    return x;
   }
-  best_of<R> b;
-  b.value = warp_max(mine);
-  b.at = (int)__reduce_min_sync(ALL, mine == b.value ? (unsigned)at : 0x7fffffffu);
-  return b;
+}
+template <int L> __device__ __forceinline__ unsigned long long lanes_max(unsigned long long x) {
+#pragma unroll
+  for (int o = L / 2; o; o >>= 1) { const unsigned long long y = __shfl_xor_sync(ALL, x, o); x = y > x ? y : x; }
+  return x;
 }
 
-// The choices of one row, choice c in lane c (-1: none), found by a warp that holds expert i * 32 + lane in order[i].
+// Numbers (no NaN, no -0) as integers in the same order, above 0, which stands for an expert that is not open.  FAST: functions good to a few 2^-22 and, of the
+// exponential's argument x, 2^-24 |x|.
+template <class R> struct ordered;
+template <> struct ordered<float> {
+  using key = unsigned;
+  static __device__ __forceinline__ key of(float x) { const unsigned u = __float_as_uint(x); return u & 0x80000000u ? ~u : u | 0x80000000u; }
+  static __device__ __forceinline__ float value(key k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+  static __device__ __forceinline__ float exp_of(float x) { return __expf(x); }
+  static __device__ __forceinline__ float over(float a, float b) { return __fdividef(a, b); }
+};
+template <> struct ordered<double> {
+  using key = unsigned long long;
+  static __device__ __forceinline__ key of(double x) { const unsigned long long u = (unsigned long long)__double_as_longlong(x); return u >> 63 ? ~u : u | 1ull << 63; }
+  static __device__ __forceinline__ double value(key k) { return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k)); }
+  static __device__ __forceinline__ double exp_of(double x) { return exp(x); }
+  static __device__ __forceinline__ double over(double a, double b) { return a / b; }
+};
+
+// the best of a lane's own experts in [low, high) other than `but`, the first of equal ones
+template <class K, int PER> __device__ __forceinline__ K best_of(const K (&order)[PER], int first, int low, int high, int but, int& at) {
+  K best = 0;
+  at = -1;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (order[i] > best && first + i >= low && first + i < high && first + i != but) { best = order[i]; at = first + i; }
+  return best;
+}
+template <class K> struct two { K first, second; };      // the best two of some
+template <class K> __device__ __forceinline__ two<K> both_of(two<K> a, two<K> b) {
+  const K less = a.first < b.first ? a.first : b.first, second = a.second > b.second ? a.second : b.second;
+  return {a.first > b.first ? a.first : b.first, less > second ? less : second};
+}
+
+// The choices of a token, choice c in its lane c (-1: none).
 //
 // Scores are compared as 64-bit numbers would be.  Where the order is the logits' (no bias, and no sums of scores of groups) it is exact as it is.
 // Otherwise the scores are 32-bit numbers that are off by up to `slack`: two neighbours in the order that are nearer than that, and the last group
-// kept and the first left out, are `unsure`, and the row is done again in 64 bits.  (Equal logits with equal biases are as equal there.)  Every
-// row in 64 bits takes three times as long.
-template <class R, int PER, class T> __device__ __forceinline__ bool choose(const route_plan& p, const T* row, int& chosen, softmax_of<R>& all) {
-  const int lane = threadIdx.x % 32;
-  const int experts = (int)p.experts;
+// kept and the first left out, are `unsure`, and the token is done again in 64 bits.  (Equal logits with equal biases are as equal there.)
+template <class R, int L, int PER, class T> __device__ __forceinline__ bool choose(const route_plan& p, const T* row, bool whole, int& chosen) {
+  using O = ordered<R>;
+  using K = typename O::key;
+  const int lane = threadIdx.x % L, first = lane * PER, experts = (int)p.experts;
   const bool sums = p.groups > 1 && p.group_best > 1, exact = sizeof(R) == 8 || (!p.bias && !sums);
-  R order[PER];
+  K order[PER];
+  {
+    float x[PER];
+    if (whole) {      // rows of whole 16-byte pieces, all of them experts
+      constexpr int V = 16 / sizeof(T) < PER ? 16 / sizeof(T) : PER;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = i * 32 + lane;
-    const float x = e < experts ? to_f32(row[e]) : -INFINITY;
-    order[i] = x > -INFINITY ? (R)x + (R)0 : lowest<R>();      // neither NaN nor -0
+      for (int i = 0; i < PER; i += V) {
+        float f[V];
+        channels(load_words<T, V>(row + first + i), f);
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[i + v] = f[v];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = first + i < experts ? to_f32(row[first + i]) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) order[i] = x[i] > -INFINITY ? O::of((R)x[i] + (R)0) : 0;      // neither NaN nor -0
   }
-  all.top = lowest<R>();
-  all.sum = (R)1;
-  if (!p.sigmoid && (!p.renormalize || p.bias || sums)) {
-    R mine = lowest<R>(), sum = 0;
+  // of the softmax: the largest logit, and the sum of exp(logit - largest); an infinite logit leaves the others nothing
+  R top = 0, sum = 1;
+  auto share = [&](R x) { return x == top ? (R)1 : O::exp_of(x - top); };
+  if (!p.sigmoid && !exact_by_logits(p)) {
+    K mine = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) mine = order[i] > mine ? order[i] : mine;
-    all.top = warp_max(mine);
+    const K best = lanes_max<L>(mine);
+    if (best) top = O::value(best);
+    R own = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (order[i] > lowest<R>()) sum += all.share(order[i]);
-    all.sum = warp_sum(sum);
+      if (order[i]) own += share(O::value(order[i]));
+    sum = lanes_sum<L>(own);
+    if (!best) sum = 1;
   }
-  auto score = [&](R x) { return p.sigmoid ? sigmoid_of(x) : all.share(x) / all.sum; };
+  const R under = (R)1 / sum;
+  auto score = [&](K k) { const R x = O::value(k); return p.sigmoid ? O::over((R)1, (R)1 + O::exp_of(-x)) : share(x) * under; };
   if (p.bias) {
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (order[i] > lowest<R>()) {
-        const R v = score(order[i]) + (R)p.bias[i * 32 + lane];
-        order[i] = v > lowest<R>() ? v + (R)0 : lowest<R>();
+      if (order[i]) {
+        const R v = score(order[i]) + (R)p.bias[first + i];
+        order[i] = v > -(R)INFINITY ? O::of(v + (R)0) : 0;
       }
   }
-  // sums of up to 1024 exponentials, whose arguments are rounded differences: good to 2^-18 of the largest score; a sum with a bias to 2^-24 of itself
-  const R largest = p.sigmoid ? (R)1 : (R)1 / all.sum;
+  // exponentials of rounded differences, sums of up to 1024 of them: good to 2^-18 of the largest score; a sum with a bias to 2^-24 of itself
+  const R largest = p.sigmoid ? (R)1 : under;
   auto slack = [&](R v) { return (R)0x1p-18 * largest + (R)0x1p-22 * (v < 0 ? -v : v); };
   bool unsure = false;
   if (p.groups > 1) {
-    const int size = experts / (int)p.groups;
-    R mine = lowest<R>();
-    for (int g = 0; g < (int)p.groups; ++g) {
-      const best_of<R> first = warp_best<R, PER>(order, g * size, (g + 1) * size, -1);
-      R sum = first.value;
-      if (sums && first.value > lowest<R>()) {
-        const best_of<R> second = warp_best<R, PER>(order, g * size, (g + 1) * size, first.at);
-        sum = p.bias ? first.value : score(first.value);
-        if (second.value > lowest<R>()) sum += p.bias ? second.value : score(second.value);
-        sum += (R)0;
+    const int size = experts / (int)p.groups, across = size / PER;
+    auto rank_of = [&](two<K> b) {      // what a group counts: the key of the sum, or of its best
+      if (!sums || !b.first) return b.first;
+      const R x = p.bias ? O::value(b.first) : score(b.first), y = !b.second ? (R)0 : p.bias ? O::value(b.second) : score(b.second);
+      return O::of(x + y + (R)0);
+    };
+    K mine = 0;                 // of the group whose number is `own`
+    int own, stride;            // group g's is known to lane g * stride
+    const bool aligned = size % PER == 0 && (across & (across - 1)) == 0;
+    if (aligned) {              // a lane's experts are of one group, the lanes of a group a power of two
+      two<K> b = {0, 0};
+#pragma unroll
+      for (int i = 0; i < PER; ++i) b = both_of(b, two<K>{order[i], 0});
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) {
+        const two<K> other = {__shfl_xor_sync(ALL, b.first, o), __shfl_xor_sync(ALL, b.second, o)};
+        if (o < across) b = both_of(b, other);
       }
-      if (lane == g) mine = sum;
+      mine = rank_of(b);
+      own = lane / across;
+      stride = across;
+      if (own >= (int)p.groups) mine = 0;
+    } else {
+      own = lane;
+      stride = 1;
+      for (int g = 0; g < (int)p.groups; ++g) {
+        two<K> b;
+        int at;
+        const K one = best_of(order, first, g * size, (g + 1) * size, -1, at);
+        b.first = lanes_max<L>(one);
+        // the lowest lane that has it gives up that one expert
+        const unsigned having = __ballot_sync(ALL, one == b.first) >> (threadIdx.x % 32 / L * L) & (L == 32 ? ~0u : (1u << L % 32) - 1);
+        const K two_ = best_of(order, first, g * size, (g + 1) * size, __ffs(having) - 1 == lane ? at : -1, at);
+        b.second = lanes_max<L>(two_);
+        const K r = rank_of(b);
+        if (lane == g) mine = r;
+      }
     }
     int before = 0;
     for (int g = 0; g < (int)p.groups; ++g) {
-      const R other = __shfl_sync(ALL, mine, g);
-      before += other > mine || (other == mine && g < lane);
+      const K other = __shfl_sync(ALL, mine, g * stride, L);
+      before += other > mine || (other == mine && g < own);
     }
-    const bool stays = lane < (int)p.groups && before < (int)p.group_choices;
-    const unsigned kept = __ballot_sync(ALL, stays);
+    const bool stays = own < (int)p.groups && before < (int)p.group_choices;
     if (!exact) {
-      const R last = -warp_max(stays ? -mine + (R)0 : lowest<R>()), next = warp_max(stays ? lowest<R>() : mine);
-      if (next > lowest<R>() && last - next < 2 * slack(last)) unsure = true;
+      const K last = ~lanes_max<L>(stays ? ~mine : (K)0), next = lanes_max<L>(stays ? (K)0 : mine);
+      if (next && O::value(last) - O::value(next) < 2 * slack(O::value(last))) unsure = true;
     }
+    if (aligned) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = i * 32 + lane;
-      if (e < experts && !(kept >> (e / size) & 1)) order[i] = lowest<R>();
+      for (int i = 0; i < PER; ++i)
+        if (!stays) order[i] = 0;
+    } else {
+      const unsigned kept = __ballot_sync(ALL, stays) >> (threadIdx.x % 32 / L * L);
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (first + i < experts && !(kept >> ((first + i) / size) & 1)) order[i] = 0;
     }
   }
   chosen = -1;
-  best_of<R> last = {(R)0, -1};
+  K last = 0;
+  int last_at = -1, at;
+  K mine = best_of(order, first, 0, 0x7fffffff, -1, at);
   for (int c = 0; c < (int)p.choices + (exact ? 0 : 1); ++c) {
-    const best_of<R> next = warp_best<R, PER>(order, 0, experts, -1);
-    if (!(next.value > lowest<R>())) break;
-    if (!exact && c > 0 && last.value - next.value < slack(last.value)) {
-      const float x = to_f32(row[last.at]), y = to_f32(row[next.at]);
-      unsure |= !(x == y && (!p.bias || p.bias[last.at] == p.bias[next.at]));
+    const K next = lanes_max<L>(mine);
+    const unsigned having = __ballot_sync(ALL, mine == next) >> (threadIdx.x % 32 / L * L) & (L == 32 ? ~0u : (1u << L % 32) - 1);
+    const int winner = __ffs(having) - 1, next_at = __shfl_sync(ALL, at, winner, L);
+    if (!exact && c > 0 && next && O::value(last) - O::value(next) < slack(O::value(last))) {
+      const float x = to_f32(row[last_at]), y = to_f32(row[next_at]);
+      unsure |= !(x == y && (!p.bias || p.bias[last_at] == p.bias[next_at]));
     }
-    if (lane == c && c < (int)p.choices) chosen = next.at;
+    if (next && lane == c && c < (int)p.choices) chosen = next_at;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (i * 32 + lane == next.at) order[i] = lowest<R>();
+      if (lane == winner && first + i == next_at) order[i] = 0;
+    mine = best_of(order, first, 0, 0x7fffffff, -1, at);
     last = next;
+    last_at = next_at;
   }
   return unsure;
 }
-// (not inlined: few rows come here, and its registers would be all rows')
-template <int PER, class T> __device__ __noinline__ int choose_in_64(const route_plan& p, const T* row) {
+// (not inlined: few tokens come here, and its registers would be all tokens')
+template <int L, int PER, class T> __device__ __noinline__ int choose_in_64(const route_plan& p, const T* row, bool whole) {
   int chosen;
-  softmax_of<double> all;
-  choose<double, PER>(p, row, chosen, all);
+  choose<double, L, PER>(p, row, whole, chosen);
   return chosen;
 }
 
-// w = scale * score (/ the sum of the chosen ones' scores) of the chosen expert's logit x.  Quotients are made of exponentials relative to the largest, so that
+// Of the softmax over a row's open experts: its largest logit and the sum of exp(logit - largest).
+struct softmax_of {
+  float top, sum;
+  __device__ __forceinline__ float share(float x) const { return x == top ? 1.f : expf(x - top); }      // times the sum
+};
+template <int L> __device__ __forceinline__ float lanes_max_of(float x) { return ordered<float>::value(lanes_max<L>(ordered<float>::of(x + 0.f))); }
+template <int L, int V, class T> __device__ __forceinline__ softmax_of softmax_over(const T* row, unsigned pieces) {
+  const unsigned lane = threadIdx.x % L;
+  softmax_of all;
+  float top = -INFINITY, sum = 0.f;
+  for (unsigned c = lane; c < pieces; c += L) {
+    float f[V];
+    channels(load_words<T, V>(row + c * V), f);
+#pragma unroll
+    for (int v = 0; v < V; ++v) top = f[v] > top ? f[v] : top;
+  }
+  all.top = lanes_max_of<L>(top);
+  for (unsigned c = lane; c < pieces; c += L) {
+    float f[V];
+    channels(load_words<T, V>(row + c * V), f);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (f[v] > -INFINITY) sum += all.share(f[v]);
+  }
+  all.sum = lanes_sum<L>(sum);
+  return all;
+}
+
+// w = score (/ the sum of the chosen ones' scores) of the chosen expert's logit x.  Quotients are made of exponentials relative to the largest, so that
 // they hold where the scores themselves vanish: with c = min(largest, 0), sigmoid(x) e^-c = e^(x - c) / (1 + e^x) for x <= 0.
 struct weight_of { float w, other; };      // the quotient or the score; 1 - sigmoid(x)
-__device__ __forceinline__ weight_of weigh(bool chosen, float x, bool sigmoid, bool renormalize, const softmax_of<float>& all) {
+template <int L> __device__ __forceinline__ weight_of weigh(bool chosen, float x, bool sigmoid, bool renormalize, const softmax_of& all) {
   weight_of r = {0.f, 0.f};
   if (sigmoid) {
     const float e = expf(-fabsf(x));
@@ -170,48 +264,50 @@ __device__ __forceinline__ weight_of weigh(bool chosen, float x, bool sigmoid, b
     if (!renormalize) {
       r.w = x >= 0.f ? 1.f / (1.f + e) : e / (1.f + e);
     } else {
-      const float c = fminf(warp_max(chosen ? x + 0.f : -INFINITY), 0.f);
+      const float c = fminf(lanes_max_of<L>(chosen ? x : -INFINITY), 0.f);
       r.w = x > 0.f ? 1.f / (1.f + e) : (x == c ? 1.f : expf(x - c)) / (1.f + e);
     }
   } else if (renormalize) {
-    softmax_of<float> some = {warp_max(chosen ? x + 0.f : -INFINITY), 1.f};
+    const softmax_of some = {lanes_max_of<L>(chosen ? x : -INFINITY), 1.f};
     r.w = some.share(x);
   } else {
     r.w = all.share(x) / all.sum;
   }
   if (!chosen) r.w = 0.f;
   if (renormalize) {
-    const float sum = warp_sum(r.w);
+    const float sum = lanes_sum<L>(r.w);
     r.w = sum > 0.f ? r.w / sum : 0.f;
   }
   return r;
 }
 
-// A warp a token.  Bound by how long its choices take one after another (each a comparison of what the lanes hold and two reductions).
-template <class T, int PER>
-__global__ void __launch_bounds__(BLOCK) expert_route_kernel(const T* __restrict__ logits, size_t stride, unsigned n, route_plan p, int* __restrict__ experts, float* __restrict__ weights) {
-  const unsigned token = blockIdx.x * (BLOCK / 32) + threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (token >= n) return;
+// Bound by how long a token's choices take one after another (each a comparison of what a lane holds, the lanes' maximum, and who has it).
+template <class T, int L, int PER>
+__global__ void __launch_bounds__(BLOCK) expert_route_kernel(const T* __restrict__ logits, size_t stride, unsigned n, route_plan p, bool whole, int* __restrict__ experts,
+                                                           float* __restrict__ weights) {
+  const unsigned place = blockIdx.x * (BLOCK / L) + threadIdx.x / L, token = place < n ? place : n - 1, lane = threadIdx.x % L;
   const T* const row = logits + token * stride;
   int chosen;
-  softmax_of<float> all;
-  if (choose<float, PER>(p, row, chosen, all)) chosen = choose_in_64<PER>(p, row);
+  const bool unsure = choose<float, L, PER>(p, row, whole, chosen);
+  if (__any_sync(ALL, unsure)) chosen = choose_in_64<L, PER>(p, row, whole);
+  softmax_of all = {0.f, 1.f};
+  constexpr unsigned V = 16 / sizeof(T);
+  if (!p.sigmoid && !p.renormalize) all = whole ? softmax_over<L, V>(row, p.experts / V) : softmax_over<L, 1>(row, p.experts);
   const float x = chosen >= 0 ? to_f32(row[chosen]) : 0.f;
-  const weight_of r = weigh(chosen >= 0, x, p.sigmoid, p.renormalize, all);
-  if (lane < p.choices) {
+  const weight_of r = weigh<L>(chosen >= 0, x, p.sigmoid, p.renormalize, all);
+  if (place < n && lane < p.choices) {
     experts[(size_t)token * p.choices + lane] = chosen;
     weights[(size_t)token * p.choices + lane] = p.scale * r.w;
   }
 }
 
-// A warp a token: what every expert's logit gets (zero but for the whole softmax), then the chosen ones' in their places.
+// L lanes a token: what every expert's logit gets (zero but for the whole softmax), then the chosen ones' in their places.
 //   renormalised: w_c (g_c - sum of g w) (sigmoid: times 1 - s_c);   softmax: p_e (G_e - sum of g p);   sigmoid: g_c s_c (1 - s_c),
 // with G_e the sum of g over the choices of e.  Bound by the launch and, from some thousand tokens on, by the bytes of dlogits.
-template <class T, int V, bool DENSE>
+template <class T, int L, int V, bool DENSE>
 __global__ void __launch_bounds__(BLOCK) expert_route_grad_kernel(const float* __restrict__ dweights, const int* __restrict__ ids, const T* __restrict__ logits, size_t stride, unsigned n,
                                                                 route_plan p, T* __restrict__ dlogits) {
-  const unsigned token = blockIdx.x * (BLOCK / 32) + threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (token >= n) return;
+  const unsigned place = blockIdx.x * (BLOCK / L) + threadIdx.x / L, token = place < n ? place : n - 1, lane = threadIdx.x % L;
   const T* const row = logits + token * stride;
   T* const to = dlogits + (size_t)token * p.experts;
   const unsigned pieces = p.experts / V;
@@ -220,47 +316,41 @@ __global__ void __launch_bounds__(BLOCK) expert_route_grad_kernel(const float* _
   const bool chosen = x > -INFINITY;
   x = chosen ? x : 0.f;
   const float g = chosen ? p.scale * dweights[(size_t)token * p.choices + lane] : 0.f;
-  softmax_of<float> all = {-INFINITY, 1.f};
-  if (DENSE) {
-    float top = -INFINITY, sum = 0.f;
-    for (unsigned c = lane; c < pieces; c += 32) {
-      float f[V];
-      channels(load_words<T, V>(row + c * V), f);
-#pragma unroll
-      for (int v = 0; v < V; ++v) top = f[v] > top ? f[v] : top;
-    }
-    all.top = warp_max(top + 0.f);
-    for (unsigned c = lane; c < pieces; c += 32) {
-      float f[V];
-      channels(load_words<T, V>(row + c * V), f);
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (f[v] > -INFINITY) sum += all.share(f[v]);
-    }
-    all.sum = warp_sum(sum);
-  }
-  const weight_of r = weigh(chosen, x, p.sigmoid, p.renormalize, all);
-  const float mean = p.renormalize || DENSE ? warp_sum(g * r.w) : 0.f;
+  softmax_of all = {0.f, 1.f};
+  if (DENSE) all = softmax_over<L, V>(row, pieces);
+  const weight_of r = weigh<L>(chosen, x, p.sigmoid, p.renormalize, all);
+  const float mean = p.renormalize || DENSE ? lanes_sum<L>(g * r.w) : 0.f;
   // of this choice; choices of the same expert are added up, in their order
   const float own = DENSE ? g : p.renormalize ? r.w * (g - mean) * (p.sigmoid ? r.other : 1.f) : g * r.w * r.other;
   float d = 0.f;
   for (unsigned c = 0; c < p.choices; ++c) {
-    const int other = __shfl_sync(ALL, chosen ? id : -1, c);
-    const float add = __shfl_sync(ALL, own, c);
+    const int other = __shfl_sync(ALL, chosen ? id : -1, c, L);
+    const float add = __shfl_sync(ALL, own, c, L);
     if (other == id) d += add;
   }
   if (DENSE) d = r.w * (d - mean);
-  for (unsigned c = lane; c < pieces; c += 32) {
-    float f[V];
-    if (DENSE) channels(load_words<T, V>(row + c * V), f);
+  if (place < n)
+    for (unsigned c = lane; c < pieces; c += L) {
+      float f[V];
+      if (DENSE) channels(load_words<T, V>(row + c * V), f);
 #pragma unroll
-    for (int v = 0; v < V; ++v) f[v] = DENSE && f[v] > -INFINITY ? -(all.share(f[v]) / all.sum) * mean : 0.f;
-    store_words<T, V>(to + c * V, to_words<T, V>(f));
-  }
+      for (int v = 0; v < V; ++v) f[v] = DENSE && f[v] > -INFINITY ? -(all.share(f[v]) / all.sum) * mean : 0.f;
+      store_words<T, V>(to + c * V, to_words<T, V>(f));
+    }
   __syncwarp();
-  if (chosen) to[id] = from_f32<T>(d);
+  if (chosen && place < n) to[id] = from_f32<T>(d);
 }
 
+// (lanes a token, experts a lane) for so many experts, and `held` choices or groups, one a lane: as few lanes as leave each about eight experts
+template <class F> int by_lanes(size_t experts, size_t held, F f) {
+  using std::integral_constant;
+  if (experts <= 32 && held <= 8) return f(integral_constant<int, 8>(), integral_constant<int, 4>());
+  if (experts <= 64 && held <= 8) return f(integral_constant<int, 8>(), integral_constant<int, 8>());
+  if (experts <= 128 && held <= 16) return f(integral_constant<int, 16>(), integral_constant<int, 8>());
+  if (experts <= 256) return f(integral_constant<int, 32>(), integral_constant<int, 8>());
+  if (experts <= 512) return f(integral_constant<int, 32>(), integral_constant<int, 16>());
+  return f(integral_constant<int, 32>(), integral_constant<int, 32>());
+}
 bool sizes_fit(size_t n, size_t experts, size_t choices) {
   return experts >= 1 && experts <= (size_t)MOST_EXPERTS && choices >= 1 && choices <= (size_t)MOST_CHOICES && choices <= experts && n <= 0x3fffffffull / choices;
 }
@@ -277,17 +367,12 @@ TB200_API int tb200_expert_route(const void* d_logits, size_t logits_stride, siz
     if (!d_logits || !d_experts || !d_weights || logits_stride < num_experts) return ERR_INVALID;
     route_plan p = {d_bias, (unsigned)num_experts, (unsigned)choices, (unsigned)groups, (unsigned)group_choices, (unsigned)group_best, scores == TB200_SIGMOID, renormalize != 0, scale};
     if (group_choices == groups) p.groups = 1;      // all of them stay
-    auto go = [&](auto per) -> int {
-      expert_route_kernel<T, decltype(per)::value><<<(unsigned)((n + BLOCK / 32 - 1) / (BLOCK / 32)), BLOCK, 0, stream>>>(static_cast<const T*>(d_logits), logits_stride, (unsigned)n, p, d_experts,
-                                                                                                                 d_weights);
+    return by_lanes(num_experts, choices > p.groups ? choices : p.groups, [&](auto lanes, auto per) -> int {
+      constexpr int L = decltype(lanes)::value, PER = decltype(per)::value, TOKENS = BLOCK / L;
+      const bool whole = num_experts == (size_t)L * PER && in_16_bytes(d_logits, num_experts, logits_stride, sizeof(T));
+      expert_route_kernel<T, L, PER><<<(unsigned)((n + TOKENS - 1) / TOKENS), BLOCK, 0, stream>>>(static_cast<const T*>(d_logits), logits_stride, (unsigned)n, p, whole, d_experts, d_weights);
       return (int)cudaGetLastError();
-    };
-    if (num_experts <= 32) return go(std::integral_constant<int, 1>());
-    if (num_experts <= 64) return go(std::integral_constant<int, 2>());
-    if (num_experts <= 128) return go(std::integral_constant<int, 4>());
-    if (num_experts <= 256) return go(std::integral_constant<int, 8>());
-    if (num_experts <= 512) return go(std::integral_constant<int, 16>());
-    return go(std::integral_constant<int, 32>());
+    });
   });
 }
 
@@ -300,14 +385,15 @@ TB200_API int tb200_expert_route_grad(const float* d_dweights, const int* d_expe
     if (!d_dweights || !d_experts || !d_logits || !d_dlogits || logits_stride < num_experts) return ERR_INVALID;
     const route_plan p = {nullptr, (unsigned)num_experts, (unsigned)choices, 1, 1, 1, scores == TB200_SIGMOID, renormalize != 0, scale};
     const bool dense = scores == TB200_SOFTMAX && !renormalize;
-    auto go = [&](auto vv) -> int {
-      constexpr int V = decltype(vv)::value;
-      (dense ? expert_route_grad_kernel<T, V, true> : expert_route_grad_kernel<T, V, false>)<<<(unsigned)((n + BLOCK / 32 - 1) / (BLOCK / 32)), BLOCK, 0, stream>>>(
+    auto go = [&](auto vv, auto lanes) -> int {
+      constexpr int V = decltype(vv)::value, L = decltype(lanes)::value, TOKENS = BLOCK / L;
+      (dense ? expert_route_grad_kernel<T, L, V, true> : expert_route_grad_kernel<T, L, V, false>)<<<(unsigned)((n + TOKENS - 1) / TOKENS), BLOCK, 0, stream>>>(
           d_dweights, d_experts, static_cast<const T*>(d_logits), logits_stride, (unsigned)n, p, static_cast<T*>(d_dlogits));
       return (int)cudaGetLastError();
     };
+    auto with = [&](auto vv) -> int { return choices <= 8 && num_experts <= 64 ? go(vv, std::integral_constant<int, 8>()) : go(vv, std::integral_constant<int, 32>()); };
     if ((!dense || in_16_bytes(d_logits, num_experts, logits_stride, sizeof(T))) && in_16_bytes(d_dlogits, num_experts, num_experts, sizeof(T)))
-      return go(std::integral_constant<int, 16 / sizeof(T)>());
-    return go(std::integral_constant<int, 1>());
+      return with(std::integral_constant<int, 16 / sizeof(T)>());
+    return with(std::integral_constant<int, 1>());
   });
 }
