@@ -75,7 +75,8 @@ def test_products_say_how_much_workspace_they_need():
     lib, need = _lib.load(), ctypes.c_size_t(0)
     ask = lambda t, i, o, rstride, each, stride, inside=0, act=0, at=None: lib.tb200_expert_product(  # noqa: E731
         at, rstride, None, I32, None, each, stride, inside, None, None, 0, act, 100, 3, i, o, t, None, None, None, ctypes.byref(need), None)
-    assert ask(F32, 7, 9, 7, 63, 9) == 0 and need.value == 256
+    assert ask(F32, 8, 12, 8, 96, 12) == 0 and need.value == 256
+    assert ask(F32, 7, 9, 7, 63, 9) == 0 and need.value >= 256 + 100 * 8 * 4 + 3 * 7 * 12 * 4        # both laid out anew
     assert ask(BF16, 64, 32, 64, 64 * 32, 32) == 0 and need.value == 256
     assert ask(BF16, 7, 32, 7, 7 * 32, 32) == 0 and need.value >= 256 + 100 * 8 * 2              # rows laid out anew
     assert ask(BF16, 64, 9, 64, 64 * 9, 9) == 0 and need.value >= 256 + 3 * 64 * 16 * 2           # the matrices

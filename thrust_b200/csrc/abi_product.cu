@@ -34,10 +34,12 @@ template <bool FAST> __device__ __forceinline__ sigmoid_pair sigmoid(float x) {
 }
 __device__ __forceinline__ float normal_below(float x) { return 0.5f * erfcf(-0.70710678118654752f * x); }
 template <bool FAST> __device__ __forceinline__ float activated(float x, int kind) { return kind == ACT_SILU ? x * sigmoid<FAST>(x).s : kind == ACT_GELU ? x * normal_below(x) : x; }
-// and its slope
-template <bool FAST> __device__ __forceinline__ float slope(float x, int kind) {
-  if (kind == ACT_SILU) { const sigmoid_pair p = sigmoid<FAST>(x); return p.s * fmaf(x, p.other, 1.f); }
-  return fmaf(x * 0.39894228040143268f, expf(-0.5f * x * x), normal_below(x));
+// and with its slope
+struct act_slope { float y, slope; };
+template <bool FAST> __device__ __forceinline__ act_slope with_slope(float x, int kind) {
+  if (kind == ACT_SILU) { const sigmoid_pair p = sigmoid<FAST>(x); return {x * p.s, p.s * fmaf(x, p.other, 1.f)}; }
+  const float below = normal_below(x);
+  return {x * below, fmaf(x * 0.39894228040143268f, expf(-0.5f * x * x), below)};
 }
 
 // ---------------------------------------------------------------------------------------------- where the experts' rows are
@@ -532,111 +534,171 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
 
 // ---------------------------------------------------------------------------------------------- 32 bits: fused multiply-adds
 // Products of 32-bit rows are made by the ordinary units: the matrix instructions round their operands to 11 bits or fewer.  Tiles of 128 features (gated: 64
-// of each half) x BN rows; a thread has 8 features x BN / 16 rows, operands go through registers into two stages of shared memory, read channel by
-// channel from rows of any alignment.  Bound by the multiply-adds.
-constexpr int FMA_THREADS = 256, FMA_DEEP = 16;
-template <int MODE, int BN>
-__global__ void __launch_bounds__(FMA_THREADS, BN == 128 ? 2 : 4) expert_product_f32_kernel(const float* __restrict__ a, size_t a_expert, size_t a_stride, const float* __restrict__ b, size_t b_stride,
-                                                                             const product_plan<float> p) {
-  constexpr int WIDE = 128, ROWS = BN / 16, PAD = 4;
-  __shared__ __align__(16) float sa[2][FMA_DEEP][WIDE + PAD], sb[2][FMA_DEEP][BN + PAD];
-  extern __shared__ int raw_spans[];
+// of each half) x BN rows; a lane has 2 FP features x 8 rows, eight lanes by four, two features side by side in its multiply-adds (f32x2).  Operands go 16 bytes at a time,
+// by asynchronous copies, into a ring of stages of shared memory, and lie there as they lie in memory: by k (rows of features or of others), or by m (rows of
+// k), of which a lane takes two k at a time.  Bound by the multiply-adds.
+constexpr int FMA_THREADS = 128, FMA_DEEP = 16, FMA_STAGES = 4;
+template <int WIDE, bool BY_K> struct fma_tile {      // an operand's part of a stage
+  static constexpr int STRIDE = BY_K ? WIDE + 4 : FMA_DEEP + 4, PIECES = WIDE * FMA_DEEP / 4 / FMA_THREADS;
+  float at[(BY_K ? FMA_DEEP : WIDE) * STRIDE];
+};
+template <int MODE, bool A_MN, int BN> struct fma_shared {
+  static constexpr bool A_BY_K = MODE == BY_EXPERTS || A_MN, B_BY_K = MODE == BY_EXPERTS;
+  fma_tile<128, A_BY_K> a[FMA_STAGES];
+  fma_tile<BN, B_BY_K> b[FMA_STAGES];
+  static size_t bytes(unsigned experts) { return sizeof(fma_shared) + (2 * (size_t)experts + 2) * 4; }
+};
+// 16 bytes on their way to shared memory, of which `words` are there; zero for the others
+__device__ __forceinline__ void copy_words(float* to, const float* from, int words) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tb200::smem_addr(to)), "l"(from), "r"(words * 4) : "memory");
+}
+__device__ __forceinline__ int within_four(int n) { return n < 0 ? 0 : n > 4 ? 4 : n; }
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pack2(float x, float y) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ float2 unpack2(f2 a) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
+template <int MODE, bool A_MN, int BN>
+__global__ void __launch_bounds__(FMA_THREADS, 3) expert_product_f32_kernel(const float* __restrict__ a, size_t a_expert, size_t a_stride, const float* __restrict__ b, size_t b_stride,
+                                                                            const product_plan<float> p) {
+  using Shared = fma_shared<MODE, A_MN, BN>;
+  constexpr bool A_BY_K = Shared::A_BY_K, B_BY_K = Shared::B_BY_K;
+  constexpr int FP = BN == 64 ? 4 : 2, ACROSS = 64 / (8 * FP), SA = fma_tile<128, A_BY_K>::STRIDE, SB = fma_tile<BN, B_BY_K>::STRIDE;
+  extern __shared__ __align__(16) char raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(raw);
   spans s;
-  s.at = raw_spans;
-  s.tiles = raw_spans + p.experts + 1;
+  s.at = reinterpret_cast<int*>(&sh + 1);
+  s.tiles = s.at + p.experts + 1;
   if (threadIdx.x == 0 && blockIdx.x == 0 && p.first) p.hdr->error = 0;      // nothing here waits
   read_spans(s, p.offsets, p.wide, p.experts, p.m, BN);
-  const bool gated = MODE == BY_ROWS && (p.activation & ACT_GATED), a_mn = MODE == BY_EXPERTS || p.a_mn;
+  const bool gated = MODE == BY_ROWS && (p.activation & ACT_GATED);
   // tiles are as wide as the features they have: half as wide where they are of two halves
   const unsigned across = (unsigned)(p.features + (gated ? 63 : 127)) / (gated ? 64 : 128);
-  const unsigned tiles = gated ? across * (unsigned)s.tiles[p.experts] : tiles_of<MODE, WIDE, BN>(p, s);
-  constexpr int NA = FMA_DEEP * WIDE / FMA_THREADS, NB = FMA_DEEP * BN / FMA_THREADS;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const unsigned tiles = gated ? across * (unsigned)s.tiles[p.experts] : tiles_of<MODE, 128, BN>(p, s);
+  // this lane's features (of either 64) and rows
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, x0 = warp % ACROSS * 8 * FP, y0 = warp / ACROSS * 32;
+  auto x_of = [&](int i) { return x0 + (A_BY_K ? lane % 8 * FP + i : lane % 8 + 8 * i); };
+  auto y_of = [&](int j) { return y0 + (B_BY_K ? lane / 8 * 4 + j % 4 + j / 4 * 16 : lane / 8 + 4 * j); };
   unsigned e = 0;
   for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const product_tile tile = MODE == BY_ROWS && gated ? tile_at<MODE, 64, BN, 1>(p, s, t, e) : tile_at<MODE, WIDE, BN, 1>(p, s, t, e);
-    float acc[8][ROWS];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < ROWS; ++j) acc[i][j] = 0.f;
-    float ra[NA], rb[NB];
-    auto fetch = [&](int k0) {
-#pragma unroll
-      for (int i = 0; i < NA; ++i) {
-        const int at = threadIdx.x + i * FMA_THREADS, k = k0 + (a_mn ? at / WIDE : at % FMA_DEEP), w = a_mn ? at % WIDE : at / FMA_DEEP;
-        const int f = tile.feature + (gated && w >= 64 ? w - 64 : w);
-        const size_t g = (size_t)f + (gated && w >= 64 ? p.second : 0);
-        const bool there = k < tile.depth && f < p.features;
-        if (MODE == BY_ROWS) ra[i] = there ? a[tile.e * a_expert + (a_mn ? (size_t)k * a_stride + g : g * a_stride + k)] : 0.f;
-        else ra[i] = there ? a[((size_t)tile.row + k) * a_stride + g] : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int at = threadIdx.x + i * FMA_THREADS;
-        if (MODE == BY_ROWS) {
-          const int k = k0 + at % FMA_DEEP, n = at / FMA_DEEP;
-          rb[i] = k < tile.depth && n < tile.rows ? b[((size_t)tile.row + n) * b_stride + k] : 0.f;
-        } else {
-          const int k = k0 + at / BN, n = at % BN;
-          rb[i] = k < tile.depth && n < tile.rows ? b[((size_t)tile.row + k) * b_stride + tile.other + n] : 0.f;
-        }
-      }
-    };
-    auto keep = [&](int stage) {
-#pragma unroll
-      for (int i = 0; i < NA; ++i) {
-        const int at = threadIdx.x + i * FMA_THREADS;
-        sa[stage][a_mn ? at / WIDE : at % FMA_DEEP][a_mn ? at % WIDE : at / FMA_DEEP] = ra[i];
-      }
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int at = threadIdx.x + i * FMA_THREADS;
-        sb[stage][MODE == BY_ROWS ? at % FMA_DEEP : at / BN][MODE == BY_ROWS ? at / FMA_DEEP : at % BN] = rb[i];
-      }
-    };
-    int stage = 0;
-    if (tile.depth > 0) { fetch(0); keep(0); }
-    __syncthreads();
-    for (int k = 0; k < tile.depth; k += FMA_DEEP, stage ^= 1) {
-      const bool more = k + FMA_DEEP < tile.depth;
-      if (more) fetch(k + FMA_DEEP);
-#pragma unroll
-      for (int i = 0; i < FMA_DEEP; ++i) {
-        float x[8], y[ROWS];
-        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(&sa[stage][i][tx * 4]);
-        *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(&sa[stage][i][64 + tx * 4]);
-        if constexpr (ROWS == 8) {
-          *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(&sb[stage][i][ty * 4]);
-          *reinterpret_cast<float4*>(y + 4) = *reinterpret_cast<const float4*>(&sb[stage][i][64 + ty * 4]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < ROWS; ++j) y[j] = sb[stage][i][ty * ROWS + j];
-        }
-#pragma unroll
-        for (int f = 0; f < 8; ++f)
-#pragma unroll
-          for (int j = 0; j < ROWS; ++j) acc[f][j] = fmaf(x[f], y[j], acc[f][j]);
-      }
-      if (more) keep(stage ^ 1);
-      __syncthreads();
+    const product_tile tile = MODE == BY_ROWS && gated ? tile_at<MODE, 64, BN, 1>(p, s, t, e) : tile_at<MODE, 128, BN, 1>(p, s, t, e);
+    const int wide = p.features - tile.feature < (gated ? 64 : 128) ? p.features - tile.feature : gated ? 64 : 128;      // features of the tile, gated of either half
+    // this thread's pieces of a stage: where they lie in the tile, where the first comes from (at k = 0), of A also the first of the upper 64 features
+    constexpr int PA = fma_tile<128, A_BY_K>::PIECES, PB = fma_tile<BN, B_BY_K>::PIECES;
+    const int ka = A_BY_K ? threadIdx.x / 32 : threadIdx.x % 4 * 4, wa = A_BY_K ? threadIdx.x % 32 * 4 : threadIdx.x / 4;
+    const int kb = B_BY_K ? threadIdx.x / (BN / 4) : threadIdx.x % 4 * 4, wb = B_BY_K ? threadIdx.x % (BN / 4) * 4 : threadIdx.x / 4;
+    constexpr int A_K = A_BY_K ? 4 : 0, A_W = A_BY_K ? 0 : 32, B_K = B_BY_K ? FMA_THREADS * 4 / BN : 0, B_W = B_BY_K ? 0 : 32;      // from one piece to the next
+    auto column_of = [&](int w) { return (size_t)tile.feature + (gated && w >= 64 ? p.second + w - 64 : w); };
+    auto left_of = [&](int w) { return wide - (gated && w >= 64 ? w - 64 : w); };      // features from w on
+    const float *a0, *a1;
+    if (A_BY_K) {
+      a0 = a + (MODE == BY_ROWS ? tile.e * a_expert : (size_t)tile.row * a_stride) + (size_t)ka * a_stride + column_of(wa);
+      a1 = a0;
+    } else {
+      a0 = a + tile.e * a_expert + column_of(wa) * a_stride + ka;
+      a1 = a + tile.e * a_expert + column_of(wa + 64) * a_stride + ka;
     }
+    const float* b0 = B_BY_K ? b + ((size_t)tile.row + kb) * b_stride + tile.other + wb : b + ((size_t)tile.row + wb) * b_stride + kb;
+    auto fetch = [&](int k0, int stage) {
+#pragma unroll
+      for (int i = 0; i < PA; ++i) {
+        const int k = ka + i * A_K, w = wa + i * A_W;
+        const int words = A_BY_K ? (k0 + k < tile.depth ? within_four(left_of(w)) : 0) : left_of(w) > 0 ? within_four(tile.depth - k0 - k) : 0;
+        const float* const from = A_BY_K ? a0 + (size_t)(i * A_K) * a_stride : (i < 2 ? a0 : a1) + (size_t)(i % 2 * A_W) * a_stride;
+        copy_words(&sh.a[stage].at[(A_BY_K ? k : w) * SA + (A_BY_K ? w : k)], words ? from : a, words);
+      }
+#pragma unroll
+      for (int i = 0; i < PB; ++i) {
+        const int k = kb + i * B_K, w = wb + i * B_W;
+        const int words = B_BY_K ? (k0 + k < tile.depth ? within_four(tile.rows - w) : 0) : w < tile.rows ? within_four(tile.depth - k0 - k) : 0;
+        const float* const from = b0 + (size_t)(B_BY_K ? i * B_K : i * B_W) * b_stride;
+        copy_words(&sh.b[stage].at[(B_BY_K ? k : w) * SB + (B_BY_K ? w : k)], words ? from : b, words);
+      }
+      a0 += A_BY_K ? FMA_DEEP * a_stride : FMA_DEEP;
+      a1 += A_BY_K ? FMA_DEEP * a_stride : FMA_DEEP;
+      b0 += B_BY_K ? FMA_DEEP * b_stride : FMA_DEEP;
+    };
+    f2 acc[FP][8];      // pairs of the lower features, then of the upper
+#pragma unroll
+    for (int i = 0; i < FP; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i][j] = pack2(0.f, 0.f);
+    const int blocks = (tile.depth + FMA_DEEP - 1) / FMA_DEEP;
+    __syncthreads();      // (the last tile's stages have been read)
+    for (int q = 0; q < FMA_STAGES - 1; ++q) {
+      if (q < blocks) fetch(q * FMA_DEEP, q);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    for (int q = 0; q < blocks; ++q) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(FMA_STAGES - 2) : "memory");
+      __syncthreads();
+      if (q + FMA_STAGES - 1 < blocks) fetch((q + FMA_STAGES - 1) * FMA_DEEP, (q + FMA_STAGES - 1) % FMA_STAGES);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      const float *const sa = sh.a[q % FMA_STAGES].at, *const sb = sh.b[q % FMA_STAGES].at;
+#pragma unroll
+      for (int k = 0; k < FMA_DEEP; k += 2) {
+        float2 xs[A_BY_K ? 1 : 2 * FP], ys[B_BY_K ? 1 : 8];      // two k of a feature, of a row
+        if constexpr (!A_BY_K) {
+#pragma unroll
+          for (int i = 0; i < 2 * FP; ++i) xs[i] = *reinterpret_cast<const float2*>(sa + ((i < FP ? 0 : 64) + x_of(i % FP)) * SA + k);
+        }
+        if constexpr (!B_BY_K) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ys[j] = *reinterpret_cast<const float2*>(sb + y_of(j) * SB + k);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          f2 x[FP];
+          float y[8];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float* const from = sa + (k + u) * SA + h * 64 + x_of(0);
+            if constexpr (!A_BY_K) {
+#pragma unroll
+              for (int i = 0; i < FP / 2; ++i) {
+                const float2 m = xs[h * FP + 2 * i], n = xs[h * FP + 2 * i + 1];
+                x[h * FP / 2 + i] = u ? pack2(m.y, n.y) : pack2(m.x, n.x);
+              }
+            } else if constexpr (FP == 4) {
+              *reinterpret_cast<ulonglong2*>(x + h * 2) = *reinterpret_cast<const ulonglong2*>(from);
+            } else {
+              x[h] = *reinterpret_cast<const f2*>(from);
+            }
+            if constexpr (B_BY_K) *reinterpret_cast<float4*>(y + h * 4) = *reinterpret_cast<const float4*>(sb + (k + u) * SB + y_of(h * 4));
+          }
+          if constexpr (!B_BY_K) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = u ? ys[j].y : ys[j].x;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const f2 both = pack2(y[j], y[j]);
+#pragma unroll
+            for (int f = 0; f < FP; ++f) acc[f][j] = fma2(x[f], both, acc[f][j]);
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     const size_t width = p.features;
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-      const int n = ROWS == 8 ? (j < 4 ? ty * 4 + j : 60 + ty * 4 + j) : ty * ROWS + j;
+    for (int j = 0; j < 8; ++j) {
+      const int n = y_of(j);
       if (n >= tile.rows) continue;
       const size_t row = (size_t)tile.row + n;
+      float sums[2 * FP];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (gated && i >= 4) continue;
-        const int f = tile.feature + (i < 4 ? tx * 4 + i : 60 + tx * 4 + i);
+      for (int i = 0; i < FP; ++i) { const float2 v = unpack2(acc[i][j]); sums[2 * i] = v.x; sums[2 * i + 1] = v.y; }
+#pragma unroll
+      for (int i = 0; i < 2 * FP; ++i) {
+        if (gated && i >= FP) continue;
+        const int f = tile.feature + (i < FP ? 0 : 64) + x_of(i % FP);
         if (f >= p.features) continue;
-        float v = acc[i][j];
+        float v = sums[i];
         if (MODE == BY_ROWS) {
           const int kind = p.activation & ~ACT_GATED;
           const size_t both = gated ? 2 * width : width;
-          float u = acc[i < 4 ? i + 4 : i][j];
+          float u = sums[i < FP ? i + FP : i];
           if (p.bias) { v += p.bias[tile.e * both + f]; if (gated) u += p.bias[tile.e * both + width + f]; }
           if (p.before) { p.before[row * both + f] = v; if (gated) p.before[row * both + width + f] = u; }
           v = activated<false>(v, kind);
@@ -697,18 +759,19 @@ __global__ void __launch_bounds__(SUM_BLOCK) join_sums_kernel(const float* __res
   out[i] = sum;
 }
 
-// Rows that the copy engine does not take (they or their distances are not made of 16-byte pieces) as rows that it takes: `halves` pieces of `width` elements,
-// each on a boundary of 8.
+// Rows that are not made of whole aligned 16-byte pieces, or whose distances are not, laid out so that they are: `halves` pieces of `width` elements, each on a
+// boundary.
 template <class T>
 __global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ from, size_t each, size_t outer, size_t stride, size_t rows, unsigned halves, unsigned width, T* __restrict__ to) {
-  const unsigned wide = (width + 7) / 8;
+  constexpr int V = 16 / sizeof(T);
+  const unsigned wide = (width + V - 1) / V;
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * halves * wide) return;
-  const size_t line = i / wide, row = line / halves, c = (i - line * wide) * 8;
+  const size_t line = i / wide, row = line / halves, c = (i - line * wide) * V;
   const T* const f = from + row / each * outer + row % each * stride + (line - row * halves) * width + c;
-  union { T at[8]; uint4 all; } v;
+  union { T at[V]; uint4 all; } v;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v.at[j] = c + j < width ? f[j] : from_f32<T>(0.f);
+  for (int j = 0; j < V; ++j) v.at[j] = c + j < width ? f[j] : from_f32<T>(0.f);
   reinterpret_cast<uint4*>(to)[i] = v.all;
 }
 
@@ -737,21 +800,18 @@ __global__ void __launch_bounds__(256) activation_grad_kernel(const T* __restric
   for (int u = 0; u < U; ++u) {
     if (at[u] == ~(size_t)0) continue;
     T* const to = dbefore + at[u];
-    float d[V], a[V];
+    float d[V], a[V], b[V];
     channels(dw[u], d);
     channels(aw[u], a);
-    if (gated) {
-      float b[V], db[V];
-      channels(bw[u], b);
+    if (gated) channels(bw[u], b);
 #pragma unroll
-      for (int v = 0; v < V; ++v) db[v] = d[v] * activated<FAST>(a[v], kind);
-      store_words<T, V>(to + width, to_words<T, V>(db));
-#pragma unroll
-      for (int v = 0; v < V; ++v) d[v] *= b[v];
+    for (int v = 0; v < V; ++v) {
+      const act_slope s = with_slope<FAST>(a[v], kind);
+      a[v] = (gated ? d[v] * b[v] : d[v]) * s.slope;
+      b[v] = d[v] * s.y;
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) d[v] *= slope<FAST>(a[v], kind);
-    store_words<T, V>(to, to_words<T, V>(d));
+    store_words<T, V>(to, to_words<T, V>(a));
+    if (gated) store_words<T, V>(to + width, to_words<T, V>(b));
   }
 }
 
@@ -787,21 +847,22 @@ box_axes plain_axes(size_t width, size_t rows, size_t stride, size_t count, size
 struct matrices {
   const void* at;
   size_t width, rows, stride, count, outer;      // count 0: one matrix
-  unsigned halves;                               // of the width, each on a boundary of 8
-  bool fits() const { return ((reinterpret_cast<uintptr_t>(at) | stride * 2 | (count > 1 ? outer * 2 : 0)) & 15) == 0 && (halves == 1 || width / halves % 8 == 0); }
+  unsigned halves;                               // of the width, each on a boundary of 16 bytes
+  size_t bytes;                                  // of an element
+  size_t pieces() const { return (half() * bytes + 15) / 16; }
+  bool fits() const { return ((reinterpret_cast<uintptr_t>(at) | stride * bytes | (count > 1 ? outer * bytes : 0) | (halves > 1 ? half() * bytes : 0)) & 15) == 0; }
   size_t half() const { return width / halves; }
-  size_t packed_half() const { return (half() + 7) / 8 * 8; }
   size_t all_rows() const { return rows * (count ? count : 1); }
-  size_t packed_bytes() const { return fits() ? 0 : tb200::align_up(all_rows() * halves * packed_half() * 2, 256); }
+  size_t packed_bytes() const { return fits() ? 0 : tb200::align_up(all_rows() * halves * pieces() * 16, 256); }
 };
 // into `room`, which is moved on; nothing where they fit
 template <class T> cudaError_t pack(matrices& x, char*& room, cudaStream_t stream) {
   if (x.fits() || x.width == 0 || x.all_rows() == 0) return cudaSuccess;
-  const size_t bytes = x.packed_bytes(), pieces = x.all_rows() * x.halves * (x.packed_half() / 8);
+  const size_t bytes = x.packed_bytes(), pieces = x.all_rows() * x.halves * x.pieces();
   if ((pieces + 255) / 256 > 0x7fffffffull) return cudaErrorInvalidValue;
   pack_rows_kernel<T><<<(unsigned)((pieces + 255) / 256), 256, 0, stream>>>(static_cast<const T*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), reinterpret_cast<T*>(room));
   x.at = room;
-  x.stride = x.halves * x.packed_half();
+  x.stride = x.halves * x.pieces() * 16 / sizeof(T);
   x.outer = x.rows * x.stride;
   x.width = x.stride;
   room += bytes;
@@ -837,24 +898,29 @@ cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_
   return cudaLaunchKernelEx(&cfg, kernel, a, b, p);
 }
 
+template <int MODE, bool A_MN, int BN> cudaError_t launch_fma(const matrices& a, const matrices& b, const product_plan<float>& p, cudaStream_t stream) {
+  using Shared = fma_shared<MODE, A_MN, BN>;
+  auto kernel = expert_product_f32_kernel<MODE, A_MN, BN>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shared::bytes(MOST_EXPERTS));
+  if (e != cudaSuccess) return e;
+  const size_t wide = MODE == BY_ROWS && (p.activation & ACT_GATED) ? 64 : 128, across = ((size_t)p.features + wide - 1) / wide;
+  const size_t tiles = MODE == BY_ROWS ? across * most_row_tiles(p.m, p.experts, BN) : across * (((size_t)p.others + BN - 1) / BN) * p.experts;
+  kernel<<<product_grid(tiles, 3), FMA_THREADS, Shared::bytes(p.experts), stream>>>(static_cast<const float*>(a.at), a.outer, a.stride, static_cast<const float*>(b.at), b.stride, p);
+  return cudaGetLastError();
+}
+
 // out[i] = rows[i] W[e] (+ the rest) of the expert that row i is of.  w: its matrices' rows are inputs (a_mn: the outputs of an input are neighbours), or outputs.
 template <class T> cudaError_t product_by_rows(matrices w, matrices x, product_plan<T> p, char* room, cudaStream_t stream) {
   const bool gated = (p.activation & ACT_GATED) != 0;
   bool few = (size_t)p.m <= (size_t)32 * p.experts;
+  cudaError_t e = pack<T>(w, room, stream);
+  if (e == cudaSuccess) e = pack<T>(x, room, stream);
+  if (e != cudaSuccess) return e;
+  p.second = p.a_mn ? (int)(w.halves == 2 ? w.width / 2 : 0) : p.features;
   if constexpr (sizeof(T) == 4) {
-    const size_t wide = gated ? 64 : 128;
-    const size_t smem = (2 * (size_t)p.experts + 2) * 4, across = ((size_t)p.features + wide - 1) / wide;
-    p.second = p.features;
-    const float* const a = static_cast<const float*>(w.at);
-    const float* const b = static_cast<const float*>(x.at);
-    if (few) expert_product_f32_kernel<BY_ROWS, 32><<<product_grid(across * most_row_tiles(p.m, p.experts, 32), 4), FMA_THREADS, smem, stream>>>(a, w.outer, w.stride, b, x.stride, p);
-    else expert_product_f32_kernel<BY_ROWS, 128><<<product_grid(across * most_row_tiles(p.m, p.experts, 128), 2), FMA_THREADS, smem, stream>>>(a, w.outer, w.stride, b, x.stride, p);
-    return cudaGetLastError();
+    if (p.a_mn) return few ? launch_fma<BY_ROWS, true, 32>(w, x, p, stream) : launch_fma<BY_ROWS, true, 64>(w, x, p, stream);
+    return few ? launch_fma<BY_ROWS, false, 32>(w, x, p, stream) : launch_fma<BY_ROWS, false, 64>(w, x, p, stream);
   } else {
-    cudaError_t e = pack<T>(w, room, stream);
-    if (e == cudaSuccess) e = pack<T>(x, room, stream);
-    if (e != cudaSuccess) return e;
-    p.second = p.a_mn ? (int)(w.halves == 2 ? w.width / 2 : 0) : p.features;
     const size_t both = (size_t)p.features * (gated ? 2 : 1);
     p.wide_out = in_16_bytes(p.out, p.features, p.features, 2) && in_16_bytes(p.before, both, both, 2);
     p.wide_residual = in_16_bytes(p.residual, p.features, p.residual_stride, 2);
@@ -878,10 +944,7 @@ template <class T> cudaError_t product_by_rows(matrices w, matrices x, product_p
 // matrix[e][o][f] = the sum over the expert's rows of others[row][o] features[row][f]
 template <class T, class O> cudaError_t product_by_experts(const matrices& features, const matrices& others, product_plan<T> p, cudaStream_t stream) {
   if constexpr (sizeof(T) == 4) {
-    const size_t tiles = (((size_t)p.features + 127) / 128) * (((size_t)p.others + 127) / 128) * p.experts;
-    expert_product_f32_kernel<BY_EXPERTS, 128><<<product_grid(tiles, 2), FMA_THREADS, (2 * (size_t)p.experts + 2) * 4, stream>>>(static_cast<const float*>(features.at), 0, features.stride,
-                                                                                                            static_cast<const float*>(others.at), others.stride, p);
-    return cudaGetLastError();
+    return launch_fma<BY_EXPERTS, true, 64>(features, others, p, stream);
   } else {
     p.wide_out = in_16_bytes(p.matrix, p.features, p.features, sizeof(O));
     p.a_split = features.width % 64 == 0;
@@ -901,9 +964,9 @@ template <class T, class O> cudaError_t product_by_experts(const matrices& featu
 bool sizes_fit(size_t n, size_t experts, size_t in, size_t out) { return n <= MOST_ROWS && experts >= 1 && experts <= (size_t)MOST_EXPERTS && in < MOST_CHANNELS && out < MOST_CHANNELS; }
 bool activation_known(int a) { return a == ACT_NONE || (a & ~ACT_GATED) == ACT_SILU || (a & ~ACT_GATED) == ACT_GELU; }
 // weight as it lies: an input's outputs are neighbours, or an output's inputs
-matrices weights_of(const void* d_weight, size_t experts, size_t in, size_t out, size_t expert_stride, size_t stride, bool inputs_inside, unsigned halves) {
-  if (inputs_inside) return {d_weight, in, out, stride, experts, expert_stride, 1};
-  return {d_weight, out, in, stride, experts, expert_stride, halves};
+matrices weights_of(const void* d_weight, size_t experts, size_t in, size_t out, size_t expert_stride, size_t stride, bool inputs_inside, unsigned halves, size_t bytes) {
+  if (inputs_inside) return {d_weight, in, out, stride, experts, expert_stride, 1, bytes};
+  return {d_weight, out, in, stride, experts, expert_stride, halves, bytes};
 }
 bool weights_fit(size_t experts, size_t in, size_t out, size_t expert_stride, size_t stride, bool inputs_inside) {
   const size_t width = inputs_inside ? in : out, rows = inputs_inside ? out : in;
@@ -927,9 +990,9 @@ TB200_API int tb200_expert_product(const void* d_rows, size_t rows_stride, const
       const bool gated = (activation & ACT_GATED) != 0;
       if (!sizes_fit(n, num_experts, in, out) || !activation_known(activation) || (gated && out % 2)) return ERR_INVALID;
       const size_t width = gated ? out / 2 : out;
-      matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, gated ? 2 : 1), x = {d_rows, in, n, rows_stride, 0, 0, 1};
+      matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, gated ? 2 : 1, sizeof(T)), x = {d_rows, in, n, rows_stride, 0, 0, 1, sizeof(T)};
       int rc;
-      if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header) + (sizeof(T) == 2 ? w.packed_bytes() + x.packed_bytes() : 0), rc)) return rc;
+      if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header) + w.packed_bytes() + x.packed_bytes(), rc)) return rc;
       if (n == 0 || width == 0) return 0;
       if (!d_offsets || !d_out || (in && (!d_rows || !d_weight)) || rows_stride < in || (d_residual && residual_stride < width) ||
           !weights_fit(num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0))
@@ -963,12 +1026,12 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
     if (grad_t != t && grad_t != TB200_F32) return ERR_UNSUPPORTED;
     return by_index_dtype(offset_t, [&](auto iv) -> int {
       if (!sizes_fit(n, num_experts, in, out)) return ERR_INVALID;
-      matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, 1), x = {d_rows, in, n, rows_stride, 0, 0, 1},
-               d = {d_dout, out, n, dout_stride, 0, 0, 1};
+      matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, 1, sizeof(T)), x = {d_rows, in, n, rows_stride, 0, 0, 1, sizeof(T)},
+               d = {d_dout, out, n, dout_stride, 0, 0, 1, sizeof(T)};
       const unsigned parts = d_dbias ? sum_parts(n, num_experts, out) : 1;
       const size_t sums = parts > 1 ? tb200::align_up((size_t)parts * num_experts * out * 4, 256) : 0;
       int rc;
-      if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header) + sums + (sizeof(T) == 2 ? w.packed_bytes() + x.packed_bytes() + d.packed_bytes() : 0), rc)) return rc;
+      if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header) + sums + w.packed_bytes() + x.packed_bytes() + d.packed_bytes(), rc)) return rc;
       if (out == 0 && (n == 0 || in == 0)) return 0;
       if (!d_offsets || (in && n && (!d_drows || (out && (!d_rows || !d_weight)))) || (in && out && !d_dweight) || (out && n && !d_dout) || rows_stride < in || dout_stride < out ||
           !weights_fit(num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0))
@@ -977,12 +1040,10 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
       float* const partial = reinterpret_cast<float*>(room);
       room += sums;
       cudaError_t e = cudaSuccess;
-      if constexpr (sizeof(T) == 2) {
-        e = pack<T>(w, room, stream);
-        if (e == cudaSuccess) e = pack<T>(x, room, stream);
-        if (e == cudaSuccess) e = pack<T>(d, room, stream);
-        if (e != cudaSuccess) return (int)e;
-      }
+      e = pack<T>(w, room, stream);
+      if (e == cudaSuccess) e = pack<T>(x, room, stream);
+      if (e == cudaSuccess) e = pack<T>(d, room, stream);
+      if (e != cudaSuccess) return (int)e;
       product_plan<T> p = {};
       p.offsets = d_offsets;
       p.wide = sizeof(iv) == 8;
