@@ -86,7 +86,7 @@ template <class T> struct product_plan {
   T *out, *before;
   int activation;
   void* matrix;
-  bool accumulate, first;     // first: of the call's kernels, the one that clears the status
+  bool accumulate, first;     // first: of the call's kernels, the one that clears the status; the others begin while those before them end
   tb200::ws_header* hdr;
 };
 struct product_tile { unsigned e; int row, rows, feature, other, depth; };
@@ -122,6 +122,27 @@ template <int MODE, int WIDE, int BN, class T> __device__ __forceinline__ unsign
   const unsigned across = (unsigned)(p.features + WIDE - 1) / WIDE;
   return MODE == BY_ROWS ? across * (unsigned)s.tiles[p.experts] : across * (unsigned)((p.others + BN - 1) / BN) * p.experts;
 }
+// Tiles are taken in turn by `takers`.  What is left over when all have had as many is cut into up to `most` parts each, as long as there are takers for them, so that the last
+// turn is as much shorter: 536 tiles for 74 pairs take 7.3 turns instead of 8 (16382 f16 rows of 4096 to 2048 through eight experts: 243 us against 254).
+struct turns {
+  unsigned whole, parts, count;
+  __device__ __forceinline__ turns(unsigned tiles, unsigned takers, unsigned most) {
+    whole = tiles / takers * takers;
+    const unsigned rest = tiles - whole;
+    parts = rest ? takers / rest : 1;
+    parts = parts > most ? most : parts;
+    count = whole + rest * parts;
+  }
+  __device__ __forceinline__ unsigned tile(unsigned t) const { return t < whole || parts == 1 ? t : whole + (t - whole) / parts; }
+  // of what a tile has of rows (by experts: of others); 0 where nothing is left for a part
+  __device__ __forceinline__ void cut(unsigned t, int unit, int& first, int& rows) const {
+    if (t < whole || parts == 1) return;
+    const int part = (int)((t - whole) % parts), each = ((rows + (int)parts - 1) / (int)parts + unit - 1) / unit * unit;
+    first += part * each;
+    rows = rows - part * each < each ? rows - part * each : each;
+    if (rows < 0) rows = 0;
+  }
+};
 
 // rows [first, last) of `width` packed elements are zeros
 template <class T> __device__ __forceinline__ void clear_rows(T* to, size_t first, size_t last, size_t width, size_t thread, size_t threads) {
@@ -159,7 +180,8 @@ __device__ __forceinline__ bool withheld(unsigned, unsigned) { return false; }
 #endif
 
 constexpr int DEEP = 128;                     // of the contraction, a stage
-constexpr int WRITERS = 8, BRINGS = WRITERS, MULTIPLIES = WRITERS + 1, TC_THREADS = (WRITERS + 2) * 32;      // warps that write results, that bring operands, that multiply
+constexpr int WRITERS = 8, BRINGS = WRITERS, MULTIPLIES = WRITERS + 1, CLEARS = WRITERS + 2;      // warps that write results, that bring operands, that multiply, that clear boxes' ends (by experts)
+template <int MODE> constexpr int TC_THREADS = (WRITERS + (MODE == BY_EXPERTS ? 3 : 2)) * 32;
 constexpr unsigned CHUNK = 64 * DEEP * 2;     // 64 neighbours by 128 of the other axis
 constexpr unsigned A_BYTES = 2 * CHUNK;       // a CTA's 128 features
 
@@ -272,10 +294,10 @@ template <class O, int N> struct columns_in {
 // other half of their columns.
 //
 // By experts the contraction ends where the expert's rows do, in the middle of a box: what the box has of the next rows is cleared in shared memory, up to
-// the next 16, where the instructions end.  Such a box is counted by the barrier `tail` of the CTA that it is for, which clears it; the second CTA then says that its
-// is ready.
+// the next 16, where the instructions end.  Such a box is counted by the barrier `tail` of the CTA that it is for, where a warp of its own clears it as soon as it is there and
+// says that it is ready.
 template <class T, class O, int MODE, bool PAIR, bool GATED, int BN, int STAGES>
-__global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const product_plan<T> p) {
+__global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const product_plan<T> p) {
   using Shared = tc_shared<PAIR, GATED, BN, STAGES>;
   constexpr int CTAS = PAIR ? 2 : 1, OWN = GATED ? 64 : 128, WIDE = OWN * CTAS, UNIT = 16 * CTAS;
   extern __shared__ char raw[];
@@ -285,11 +307,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
   s.at = reinterpret_cast<int*>(&sh + 1);
   s.tiles = s.at + p.experts + 1;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  tb200::grid_dependents_launch();
   const unsigned rank = PAIR ? tb200_tc::rank_in_pair() : 0;
   if (threadIdx.x == 0) {
     if (blockIdx.x == 0 && p.first) p.hdr->error = 0;      // a wait that runs out does so long after this
     for (int i = 0; i < STAGES; ++i) {
-      for (unsigned long long* bar : {&sh.full[i], &sh.empty[i], &sh.tail[i], &sh.ready[i]}) tb200::mbar_init(bar, 1);
+      for (unsigned long long* bar : {&sh.full[i], &sh.empty[i], &sh.tail[i]}) tb200::mbar_init(bar, 1);
+      tb200::mbar_init(&sh.ready[i], CTAS);
     }
     for (int i = 0; i < 2; ++i) { tb200::mbar_init(&sh.made[i], 1); tb200::mbar_init(&sh.taken[i], WRITERS * CTAS); }
     tb200::mbar_init(&sh.done, 1);
@@ -301,9 +325,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
   read_spans(s, p.offsets, p.wide, p.experts, p.m, BN);
   if (PAIR) tb200_tc::meet_pair();
   tb200_tc::fence_after_sync();
-  const unsigned tmem = sh.tmem, tiles = tiles_of<MODE, WIDE, BN>(p, s), step = gridDim.x / CTAS;
+  const unsigned tmem = sh.tmem, step = gridDim.x / CTAS;
+  const turns turn(tiles_of<MODE, WIDE, BN>(p, s), step, MODE == BY_ROWS ? 4 : 2);
   // columns of a tile's instructions; of these each CTA brings its share of B
-  auto columns_of = [&](const product_tile& tile) { const int unit = MODE == BY_EXPERTS && p.b_split ? 64 * CTAS : UNIT; return (tile.rows + unit - 1) / unit * unit; };
+  const int unit = MODE == BY_EXPERTS && p.b_split ? 64 * CTAS : UNIT;
+  auto columns_of = [&](const product_tile& tile) { return (tile.rows + unit - 1) / unit * unit; };
+  auto tile_of = [&](unsigned t, unsigned& e) {
+    product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, turn.tile(t), e);
+    turn.cut(t, unit, MODE == BY_ROWS ? tile.row : tile.other, tile.rows);
+    return tile;
+  };
   auto is_tail = [&](const product_tile& tile, int k) { return MODE == BY_EXPERTS && tile.depth - k < DEEP && tile.depth % 16 != 0; };
   // what a box has beyond the expert's rows
   auto clear_tail = [&](unsigned stage, int valid, int boxes) {
@@ -318,8 +349,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
     const unsigned base = tb200::smem_addr(stages);
     unsigned count = 0, e = 0;      // stages filled so far
     bool good = true;
-    for (unsigned t = blockIdx.x / CTAS; good && t < tiles; t += step) {
-      const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
+    for (unsigned t = blockIdx.x / CTAS; good && t < turn.count; t += step) {
+      const product_tile tile = tile_of(t, e);
+      if (tile.rows == 0) continue;
       const int share = columns_of(tile) / CTAS, feature = tile.feature + (int)rank * OWN, other = (MODE == BY_ROWS ? tile.row : tile.other) + (int)rank * share;
       // by rows B has two chunks of k, each of boxes of rows, unless a box has both; by experts two chunks of others, unless a box has both
       const int boxes = MODE == BY_ROWS ? (share + p.box - 1) / p.box : p.b_split ? 2 : (share + 63) / 64;
@@ -381,9 +413,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
     const unsigned a_step = a_mn ? 16 * 128 >> 4 : 2, a_jump = a_mn ? 64 * 128 >> 4 : CHUNK >> 4;
     constexpr unsigned b_step = b_mn ? 16 * 128 >> 4 : 2, b_jump = b_mn ? 64 * 128 >> 4 : Shared::B_CHUNK >> 4;
     if (rank == 0) {
-      for (unsigned t = blockIdx.x / CTAS; good && t < tiles; t += step) {
-        const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
-        if (tile.depth == 0) continue;
+      for (unsigned t = blockIdx.x / CTAS; good && t < turn.count; t += step) {
+        const product_tile tile = tile_of(t, e);
+        if (tile.depth == 0 || tile.rows == 0) continue;
         const unsigned set = made & 1, d = tmem + set * BN;
         good = await<PAIR>(&sh.taken[set], (made / 2 & 1) ^ 1, &sh.dead, p.hdr);
         if (!good) break;
@@ -397,10 +429,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
           if (!good) break;
           const int valid = tile.depth - k < DEEP ? tile.depth - k : DEEP, steps = (valid + 15) / 16;
           if (is_tail(tile, k)) {
-            good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr);
-            if (!good) break;
-            clear_tail(stage, valid, 2 + (columns / CTAS + 63) / 64);
-            if (PAIR) good = await<PAIR>(&sh.ready[stage], tails >> stage & 1, &sh.dead, p.hdr);
+            good = await<PAIR>(&sh.ready[stage], tails >> stage & 1, &sh.dead, p.hdr);
             if (!good) break;
             tails ^= 1u << stage;
           }
@@ -419,29 +448,36 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
       }
       if (tb200_tc::elected()) { tb200_tc::commit<PAIR>(&sh.done); outlast(&sh.done, 0); }
       __syncwarp();
-    } else if (MODE == BY_EXPERTS) {
-      for (unsigned t = blockIdx.x / CTAS; good && t < tiles; t += step) {
-        const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
-        const unsigned blocks = (unsigned)(tile.depth + DEEP - 1) / DEEP, stage = (count + blocks - 1) % STAGES;
-        count += blocks;
-        if (blocks == 0 || !is_tail(tile, (int)(blocks - 1) * DEEP)) continue;
-        good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr);
-        if (!good) break;
-        tails ^= 1u << stage;
-        clear_tail(stage, tile.depth - (int)(blocks - 1) * DEEP, 2 + (columns_of(tile) / CTAS + 63) / 64);
-        if (lane == 0) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.ready[stage]));
-        __syncwarp();
+    }
+  } else if (MODE == BY_EXPERTS && warp == CLEARS) {
+    unsigned count = 0, e = 0, tails = 0;
+    bool good = true;
+    for (unsigned t = blockIdx.x / CTAS; good && t < turn.count; t += step) {
+      const product_tile tile = tile_of(t, e);
+      if (tile.rows == 0) continue;
+      const unsigned blocks = (unsigned)(tile.depth + DEEP - 1) / DEEP, stage = (count + blocks - 1) % STAGES;
+      count += blocks;
+      if (blocks == 0 || !is_tail(tile, (int)(blocks - 1) * DEEP)) continue;
+      good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr);
+      if (!good) break;
+      tails ^= 1u << stage;
+      clear_tail(stage, tile.depth - (int)(blocks - 1) * DEEP, 2 + (columns_of(tile) / CTAS + 63) / 64);
+      if (lane == 0) {
+        if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.ready[stage]));
+        else tb200::mbar_arrive(&sh.ready[stage]);
       }
+      __syncwarp();
     }
   } else {
     // a writer has the 32 lanes that warp % 4 may read, and every other 32 columns; GATED: of these it finishes 16, of both halves
     unsigned made = 0, e = 0;
     bool good = true;
     const int kind = p.activation & ~ACT_GATED, quarter = warp % 4, half = GATED ? quarter / 2 : 0, within = (GATED ? quarter % 2 : quarter) * 32;
-    unsigned char* const turn = sh.turn[warp];
+    unsigned char* const room_of = sh.turn[warp];
     constexpr int PUT = GATED ? 16 : 32;
-    for (unsigned t = blockIdx.x / CTAS; t < tiles; t += step) {
-      const product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, t, e);
+    for (unsigned t = blockIdx.x / CTAS; t < turn.count; t += step) {
+      const product_tile tile = tile_of(t, e);
+      if (tile.rows == 0) continue;
       const unsigned set = made & 1, d = tmem + (quarter * 32u << 16) + set * BN;
       const int f = tile.feature + (int)rank * OWN + within, room = p.features - f;      // the first lane's feature, and how many there are from there on
       const bool there = lane < room;
@@ -483,10 +519,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
         if (MODE == BY_ROWS) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] += bias;
-          if (p.before) put_columns(p.before + ((size_t)tile.row + c) * both + half * width + f, both, tile.rows - c, v, lane, room, p.wide_out, turn);
+          if (p.before) put_columns(p.before + ((size_t)tile.row + c) * both + half * width + f, both, tile.rows - c, v, lane, room, p.wide_out, room_of);
           float w[PUT];
           if constexpr (GATED) {
-            float (&out)[16][32] = *reinterpret_cast<float(*)[16][32]>(turn), (&in)[16][32] = *reinterpret_cast<float(*)[16][32]>(sh.turn[warp ^ 2]);
+            float (&out)[16][32] = *reinterpret_cast<float(*)[16][32]>(room_of), (&in)[16][32] = *reinterpret_cast<float(*)[16][32]>(sh.turn[warp ^ 2]);
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < 16; ++j) out[j][lane] = half ? v[j] : v[j + 16];
@@ -510,13 +546,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
 #pragma unroll
             for (int j = 0; j < PUT; ++j) w[j] *= v[j];
           }
-          if (p.residual) residual.add(w, lane, p.wide_residual, turn);
-          put_columns(p.out + ((size_t)tile.row + mine) * width + f, width, tile.rows - mine, w, lane, room, p.wide_out, turn);
+          if (p.residual) residual.add(w, lane, p.wide_residual, room_of);
+          put_columns(p.out + ((size_t)tile.row + mine) * width + f, width, tile.rows - mine, w, lane, room, p.wide_out, room_of);
         } else if (!p.accumulate) {
-          put_columns(to, width, tile.rows - c, v, lane, room, p.wide_out, turn);
+          put_columns(to, width, tile.rows - c, v, lane, room, p.wide_out, room_of);
         } else if (tile.depth || !good) {      // (an expert without rows adds nothing)
-          old.add(v, lane, p.wide_out, turn);
-          put_columns(to, width, tile.rows - c, v, lane, room, p.wide_out, turn);
+          old.add(v, lane, p.wide_out, room_of);
+          put_columns(to, width, tile.rows - c, v, lane, room, p.wide_out, room_of);
         }
         if (c + 64 >= tile.rows) break;
       }
@@ -525,6 +561,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) expert_product_kernel(const __g
     tb200_tc::fence_before_sync();
   }
   __syncthreads();
+  tb200::grid_dependency_wait();      // (nothing here needs what ran before, but what comes after may)
   if (PAIR) tb200_tc::meet_pair();      // neither ends while the other's instructions and arrivals come here
   if (warp == MULTIPLIES) {
     tb200_tc::fence_after_sync();
@@ -726,6 +763,7 @@ __global__ void __launch_bounds__(SUM_BLOCK) row_sums_kernel(const T* __restrict
   const int a = read_offset(offsets, wide, e, m), end = read_offset(offsets, wide, e + 1, m), n = end > a ? end - a : 0, per = (n + (int)parts - 1) / (int)parts;
   const int first = a + (int)part * per, last = (int)part * per + per < n ? first + per : a + n;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, f = (blockIdx.x * 32 + lane) * V;
+  tb200::grid_dependents_launch();
   float sum[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[v] = 0.f;
@@ -750,9 +788,11 @@ __global__ void __launch_bounds__(SUM_BLOCK) row_sums_kernel(const T* __restrict
     for (int w = 0; w < SUM_BLOCK / 32; ++w) all += met[w][i];
     sums[((size_t)part * experts + e) * features + g] = all;
   }
+  tb200::grid_dependency_wait();      // (as the products': what comes after waits for them too)
 }
 __global__ void __launch_bounds__(SUM_BLOCK) join_sums_kernel(const float* __restrict__ sums, size_t items, unsigned parts, float* __restrict__ out) {
   const size_t i = (size_t)blockIdx.x * SUM_BLOCK + threadIdx.x;
+  tb200::grid_dependency_wait();
   if (i >= items) return;
   float sum = 0.f;
   for (unsigned q = 0; q < parts; ++q) sum += sums[q * items + i];
@@ -886,15 +926,24 @@ cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_
   const size_t across = ((size_t)p.features + WIDE - 1) / WIDE;
   const size_t tiles = MODE == BY_ROWS ? across * most_row_tiles(p.m, p.experts, BN) : across * (((size_t)p.others + BN - 1) / BN) * p.experts;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(PAIR ? product_grid(tiles * 2, 1) / 2 * 2 : product_grid(tiles, 1));
-  cfg.blockDim = dim3(TC_THREADS);
+  cfg.gridDim = dim3(product_grid(tiles * 4 * CTAS, 1) / CTAS * CTAS);      // (four: the parts of a tile)
+  cfg.blockDim = dim3(TC_THREADS<MODE>);
   cfg.dynamicSmemBytes = Shared::bytes(p.experts);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CTAS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  if (PAIR) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = CTAS; attr[n].val.clusterDim.y = 1; attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (!p.first) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = PAIR ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, a, b, p);
 }
 
@@ -1074,13 +1123,20 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
         float* const to = parts > 1 ? partial : d_dbias;
         auto add = [&](auto vv) {
           constexpr int V = decltype(vv)::value;
-          row_sums_kernel<T, V><<<dim3((unsigned)((out + 32 * V - 1) / (32 * V)), (unsigned)num_experts, parts), SUM_BLOCK, 0, stream>>>(
-              static_cast<const T*>(d_dout), dout_stride, d_offsets, sizeof(iv) == 8, (unsigned)num_experts, (int)n, (int)out, to);
+          cudaLaunchConfig_t cfg = {};
+          cfg.gridDim = dim3((unsigned)((out + 32 * V - 1) / (32 * V)), (unsigned)num_experts, parts);
+          cfg.blockDim = dim3(SUM_BLOCK);
+          cfg.stream = stream;
+          cudaLaunchAttribute attr[1];
+          attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+          attr[0].val.programmaticStreamSerializationAllowed = 1;
+          cfg.attrs = attr;
+          cfg.numAttrs = in ? 1 : 0;      // beside the products: they are this call's, so what dout comes from is done
+          return cudaLaunchKernelEx(&cfg, row_sums_kernel<T, V>, static_cast<const T*>(d_dout), dout_stride, d_offsets, sizeof(iv) == 8, (unsigned)num_experts, (int)n, (int)out, to);
         };
-        if (in_16_bytes(d_dout, out, dout_stride, sizeof(T))) add(std::integral_constant<int, 16 / sizeof(T)>());
-        else add(std::integral_constant<int, 1>());
-        if (parts > 1) join_sums_kernel<<<(unsigned)((num_experts * out + SUM_BLOCK - 1) / SUM_BLOCK), SUM_BLOCK, 0, stream>>>(partial, num_experts * out, parts, d_dbias);
-        e = cudaGetLastError();
+        e = in_16_bytes(d_dout, out, dout_stride, sizeof(T)) ? add(std::integral_constant<int, 16 / sizeof(T)>()) : add(std::integral_constant<int, 1>());
+        if (e == cudaSuccess && parts > 1)
+          e = tb200::launch_after(join_sums_kernel, (num_experts * out + SUM_BLOCK - 1) / SUM_BLOCK, SUM_BLOCK, 0, stream, partial, num_experts * out, parts, d_dbias);
       }
       return (int)e;
     });
