@@ -82,56 +82,62 @@ template <class K> __device__ __forceinline__ two<K> both_of(two<K> a, two<K> b)
 // Scores are compared as 64-bit numbers would be.  Where the order is the logits' (no bias, and no sums of scores of groups) it is exact as it is.
 // Otherwise the scores are 32-bit numbers that are off by up to `slack`: two neighbours in the order that are nearer than that, and the last group
 // kept and the first left out, are `unsure`, and the token is done again in 64 bits.  (Equal logits with equal biases are as equal there.)
-template <class R, int L, int PER, class T> __device__ __forceinline__ bool choose(const route_plan& p, const T* row, bool whole, int& chosen) {
+template <class R, int L, int PER, class T> __device__ __forceinline__ bool choose(const route_plan& p, const T* row, bool whole, uint2* candidates, int& chosen) {
   using O = ordered<R>;
   using K = typename O::key;
   const int lane = threadIdx.x % L, first = lane * PER, experts = (int)p.experts;
   const bool sums = p.groups > 1 && p.group_best > 1, exact = sizeof(R) == 8 || (!p.bias && !sums);
-  K order[PER];
-  {
-    float x[PER];
-    if (whole) {      // rows of whole 16-byte pieces, all of them experts
-      constexpr int V = 16 / sizeof(T) < PER ? 16 / sizeof(T) : PER;
+  R x[PER];      // logits; -inf: not open
+  if (whole) {   // rows of whole 16-byte pieces, all of them experts
+    constexpr int V = 16 / sizeof(T) < PER ? 16 / sizeof(T) : PER;
 #pragma unroll
-      for (int i = 0; i < PER; i += V) {
-        float f[V];
-        channels(load_words<T, V>(row + first + i), f);
+    for (int i = 0; i < PER; i += V) {
+      float f[V];
+      channels(load_words<T, V>(row + first + i), f);
 #pragma unroll
-        for (int v = 0; v < V; ++v) x[i + v] = f[v];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) x[i] = first + i < experts ? to_f32(row[first + i]) : -INFINITY;
+      for (int v = 0; v < V; ++v) x[i + v] = f[v] > -INFINITY ? (R)f[v] : -(R)INFINITY;
     }
+  } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) order[i] = x[i] > -INFINITY ? O::of((R)x[i] + (R)0) : 0;      // neither NaN nor -0
+    for (int i = 0; i < PER; ++i) {
+      const float f = first + i < experts ? to_f32(row[first + i]) : -INFINITY;
+      x[i] = f > -INFINITY ? (R)f : -(R)INFINITY;
+    }
   }
+  auto key_of = [&](R v) { return v > -(R)INFINITY ? O::of(v + (R)0) : (K)0; };      // neither NaN nor -0
   // of the softmax: the largest logit, and the sum of exp(logit - largest); an infinite logit leaves the others nothing
   R top = 0, sum = 1;
-  auto share = [&](R x) { return x == top ? (R)1 : O::exp_of(x - top); };
+  auto share = [&](R v) { return v == top ? (R)1 : O::exp_of(v - top); };
   if (!p.sigmoid && !exact_by_logits(p)) {
-    K mine = 0;
+    R mine = x[0];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) mine = order[i] > mine ? order[i] : mine;
-    const K best = lanes_max<L>(mine);
+    for (int i = 1; i < PER; ++i) mine = x[i] > mine ? x[i] : mine;
+    const K best = lanes_max<L>(key_of(mine));
     if (best) top = O::value(best);
     R own = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (order[i]) own += share(O::value(order[i]));
+    for (int i = 0; i < PER; ++i) own += x[i] > -(R)INFINITY ? share(x[i]) : (R)0;
     sum = lanes_sum<L>(own);
     if (!best) sum = 1;
   }
   const R under = (R)1 / sum;
-  auto score = [&](K k) { const R x = O::value(k); return p.sigmoid ? O::over((R)1, (R)1 + O::exp_of(-x)) : share(x) * under; };
+  auto score_of = [&](R v) { return p.sigmoid ? O::over((R)1, (R)1 + O::exp_of(-v)) : share(v) * under; };
+  auto score = [&](K k) { return score_of(O::value(k)); };
   if (p.bias) {
+    R bias[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (order[i]) {
-        const R v = score(order[i]) + (R)p.bias[first + i];
-        order[i] = v > -(R)INFINITY ? O::of(v + (R)0) : 0;
-      }
+    for (int i = 0; i < PER; ++i) bias[i] = first + i < experts ? (R)p.bias[first + i] : (R)0;
+    if (p.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = x[i] > -(R)INFINITY ? O::over((R)1, (R)1 + O::exp_of(-x[i])) + bias[i] : x[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = x[i] > -(R)INFINITY ? share(x[i]) * under + bias[i] : x[i];
+    }
   }
+  K order[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) order[i] = key_of(x[i]);
   // exponentials of rounded differences, sums of up to 1024 of them: good to 2^-18 of the largest score; a sum with a bias to 2^-24 of itself
   const R largest = p.sigmoid ? (R)1 : under;
   auto slack = [&](R v) { return (R)0x1p-18 * largest + (R)0x1p-22 * (v < 0 ? -v : v); };
@@ -197,22 +203,82 @@ template <class R, int L, int PER, class T> __device__ __forceinline__ bool choo
     }
   }
   chosen = -1;
-  K last = 0;
-  int last_at = -1, at;
-  K mine = best_of(order, first, 0, 0x7fffffff, -1, at);
+  // A whole warp sorts its lanes' best.  What is no worse than the last of those that are asked for, a few more than those, are the candidates; they are sorted, one a lane.
+  if constexpr (L == 32 && sizeof(R) == 4) {
+    const int asked = (int)p.choices + (exact ? 0 : 1);
+    if (asked <= 32) {
+      K mine = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) mine = order[i] > mine ? order[i] : mine;
+      K sorted = mine;
+#pragma unroll
+      for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size / 2; o; o >>= 1) {
+          const K other = __shfl_xor_sync(ALL, sorted, o);
+          const bool larger = ((lane & size) == 0) == ((lane & o) == 0);      // of the two, this lane keeps the larger
+          sorted = (other > sorted) == larger ? other : sorted;
+        }
+      K least = __shfl_sync(ALL, sorted, asked - 1);
+      least = least ? least : 1;
+      const unsigned below = (1u << lane) - 1;
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const bool is = order[i] >= least;
+        const unsigned these = __ballot_sync(ALL, is);
+        const int at = count + __popc(these & below);
+        if (is && at < 32) candidates[at] = make_uint2(order[i], (unsigned)(first + i));
+        count += __popc(these);
+      }
+      __syncwarp();
+      if (count <= 32) {
+        const uint2 c = lane < count ? candidates[lane] : make_uint2(0, 0xffffffffu);
+        K key = c.x;
+        unsigned at = c.y;
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+          for (int o = size / 2; o; o >>= 1) {
+            const K other = __shfl_xor_sync(ALL, key, o);
+            const unsigned other_at = __shfl_xor_sync(ALL, at, o);
+            const bool larger = ((lane & size) == 0) == ((lane & o) == 0);
+            if ((other > key || (other == key && other_at < at)) == larger) { key = other; at = other_at; }
+          }
+        if (lane < (int)p.choices && key) chosen = (int)at;
+        const K next = __shfl_down_sync(ALL, key, 1);
+        const unsigned next_at = __shfl_down_sync(ALL, at, 1);
+        if (!exact && lane < (int)p.choices && lane < 31 && next && O::value(key) - O::value(next) < slack(O::value(key))) {
+          const float u = to_f32(row[at]), v = to_f32(row[next_at]);
+          unsure |= !(u == v && (!p.bias || p.bias[at] == p.bias[next_at]));
+        }
+        return unsure;
+      }
+    }
+  }
+  K last = 0, mine = 0;
+  int last_at = -1, own_at = -1;      // own_at: which of this lane's experts is its best
+  auto best = [&] {
+    mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (order[i] > mine) { mine = order[i]; own_at = i; }
+  };
+  best();
+  const unsigned segment = threadIdx.x % 32 / L * L, all_lanes = L == 32 ? ~0u : (1u << L % 32) - 1;
   for (int c = 0; c < (int)p.choices + (exact ? 0 : 1); ++c) {
     const K next = lanes_max<L>(mine);
-    const unsigned having = __ballot_sync(ALL, mine == next) >> (threadIdx.x % 32 / L * L) & (L == 32 ? ~0u : (1u << L % 32) - 1);
-    const int winner = __ffs(having) - 1, next_at = __shfl_sync(ALL, at, winner, L);
+    const int winner = __ffs(__ballot_sync(ALL, mine == next) >> segment & all_lanes) - 1, next_at = __shfl_sync(ALL, first + own_at, winner, L);
     if (!exact && c > 0 && next && O::value(last) - O::value(next) < slack(O::value(last))) {
       const float x = to_f32(row[last_at]), y = to_f32(row[next_at]);
       unsure |= !(x == y && (!p.bias || p.bias[last_at] == p.bias[next_at]));
     }
     if (next && lane == c && c < (int)p.choices) chosen = next_at;
+    const int taken = lane == winner ? own_at : -1;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (lane == winner && first + i == next_at) order[i] = 0;
-    mine = best_of(order, first, 0, 0x7fffffff, -1, at);
+      if (i == taken) order[i] = 0;
+    best();
     last = next;
     last_at = next_at;
   }
@@ -221,7 +287,7 @@ template <class R, int L, int PER, class T> __device__ __forceinline__ bool choo
 // (not inlined: few tokens come here, and its registers would be all tokens')
 template <int L, int PER, class T> __device__ __noinline__ int choose_in_64(const route_plan& p, const T* row, bool whole) {
   int chosen;
-  choose<double, L, PER>(p, row, whole, chosen);
+  choose<double, L, PER>(p, row, whole, nullptr, chosen);
   return chosen;
 }
 
@@ -287,8 +353,9 @@ __global__ void __launch_bounds__(BLOCK) expert_route_kernel(const T* __restrict
                                                            float* __restrict__ weights) {
   const unsigned place = blockIdx.x * (BLOCK / L) + threadIdx.x / L, token = place < n ? place : n - 1, lane = threadIdx.x % L;
   const T* const row = logits + token * stride;
+  __shared__ uint2 candidates[L == 32 ? BLOCK : 1];
   int chosen;
-  const bool unsure = choose<float, L, PER>(p, row, whole, chosen);
+  const bool unsure = choose<float, L, PER>(p, row, whole, candidates + (L == 32 ? threadIdx.x / 32 * 32 : 0), chosen);
   if (__any_sync(ALL, unsure)) chosen = choose_in_64<L, PER>(p, row, whole);
   softmax_of all = {0.f, 1.f};
   constexpr unsigned V = 16 / sizeof(T);
