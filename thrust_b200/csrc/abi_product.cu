@@ -81,6 +81,8 @@ template <class T> struct product_plan {
   bool wide_out, wide_residual;      // rows are made of whole 16-byte pieces
   bool a_split, b_split;      // rows are made of whole chunks of 64 and mapped as such: a box has several
   int box;                    // by rows: rows in a box of B
+  int planes, segments;       // 32-bit operands are three of 16 bits each, and six products of them are added up; otherwise one and one
+  unsigned a_planes, b_planes;      // of which planes, two bits a segment
   const T *bias, *residual;
   size_t residual_stride;
   T *out, *before;
@@ -283,6 +285,11 @@ template <class O, int N> struct columns_in {
   }
 };
 
+// A 32-bit number is the sum of three of 16 bits (bf16), each the rest rounded.  Of the nine products of such planes the three smallest, 2^-24 of the whole together, are
+// left out; the others are segments of one contraction, the smaller ones first.  (Six instructions for one, at fifteen times the rate of multiply-adds.)
+constexpr int PLANES = 3, SEGMENTS = 6;
+constexpr unsigned A_PLANES = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, B_PLANES = 0 | 2 << 2 | 1 << 4 | 0 << 6 | 1 << 8 | 0 << 10;
+
 // D^T = A B^T by tiles of 128 features (gated: 64 of each half) a CTA x up to BN rows; CTAs stay and go from tile to tile.  Features are the lanes of tensor
 // memory and rows its columns, so that a tile that has few rows takes a narrower instruction and no more time than they need: experts have as many rows as they have.
 // PAIR: two CTAs have a tile of twice as many features, half of its rows' operands each, and instructions that read both's shared memory, which the first
@@ -356,7 +363,7 @@ __global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(con
       // by rows B has two chunks of k, each of boxes of rows, unless a box has both; by experts two chunks of others, unless a box has both
       const int boxes = MODE == BY_ROWS ? (share + p.box - 1) / p.box : p.b_split ? 2 : (share + 63) / 64;
       const unsigned b_box = MODE == BY_ROWS ? p.box * 128 : CHUNK, bytes = A_BYTES + (MODE == BY_ROWS ? 2 : 1) * boxes * b_box;
-      for (int k = 0; k < tile.depth; k += DEEP, ++count) {
+      for (int k = 0, segment = 0; k < tile.depth; ++count) {
         const unsigned stage = count % STAGES, to = base + stage * Shared::STAGE;
         good = await<PAIR>(&sh.empty[stage], (count / STAGES & 1) ^ 1, &sh.dead, p.hdr);
         if (!good) break;
@@ -372,29 +379,31 @@ __global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(con
             bar = PAIR ? tb200_tc::first_ones(&sh.full[stage]) : tb200::smem_addr(&sh.full[stage]);
           }
           if (!withheld(t, step)) {
-            const int row = MODE == BY_ROWS ? k : tile.row + k, e = MODE == BY_ROWS ? (int)tile.e : 0;
+            const int row = MODE == BY_ROWS ? k : tile.row + k, pa = (int)(p.a_planes >> 2 * segment & 3), pb = (int)(p.b_planes >> 2 * segment & 3);
+            const int of_a = MODE == BY_ROWS ? (int)tile.e * p.planes + pa : pa;
             const bool both = p.a_split || (GATED && p.a_mn);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               if (c && both) continue;
               tb200_tc::box_at at;
-              if (MODE == BY_EXPERTS || p.a_mn) at = {p.a_split ? 0 : feature + c * 64, row, p.a_split ? feature / 64 : 0, 0, e};
-              else at = {p.a_split ? 0 : k + c * 64, feature, p.a_split && !GATED ? k / 64 : 0, p.a_split && GATED ? k / 64 : 0, e};
+              if (MODE == BY_EXPERTS || p.a_mn) at = {p.a_split ? 0 : feature + c * 64, row, p.a_split ? feature / 64 : 0, 0, of_a};
+              else at = {p.a_split ? 0 : k + c * 64, feature, p.a_split && !GATED ? k / 64 : 0, p.a_split && GATED ? k / 64 : 0, of_a};
               tb200_tc::load_box<PAIR>(to + c * CHUNK, &map_a, at, bar);
             }
             if (MODE == BY_EXPERTS) {
-              if (p.b_split) tb200_tc::load_box<PAIR>(to + A_BYTES, &map_b, {0, row, other / 64, 0, 0}, bar);
+              if (p.b_split) tb200_tc::load_box<PAIR>(to + A_BYTES, &map_b, {0, row, other / 64, 0, pb}, bar);
               else
-                for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + b * CHUNK, &map_b, {other + b * 64, row, 0, 0, 0}, bar);
+                for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + b * CHUNK, &map_b, {other + b * 64, row, 0, 0, pb}, bar);
             } else if (PAIR && p.b_split) {
-              tb200_tc::load_box<PAIR>(to + A_BYTES, &map_b, {0, other, k / 64, 0, 0}, bar);
+              tb200_tc::load_box<PAIR>(to + A_BYTES, &map_b, {0, other, k / 64, 0, pb}, bar);
             } else {
               for (int c = 0; c < 2; ++c)
-                for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + c * Shared::B_CHUNK + b * b_box, &map_b, {k + c * 64, other + b * p.box, 0, 0, 0}, bar);
+                for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + c * Shared::B_CHUNK + b * b_box, &map_b, {k + c * 64, other + b * p.box, 0, 0, pb}, bar);
             }
           }
         }
         __syncwarp();
+        if ((k += DEEP) >= tile.depth && ++segment < p.segments) k = 0;
       }
     }
     // the last of each stage, no longer needed
@@ -422,8 +431,8 @@ __global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(con
         ++made;
         tb200_tc::fence_after_sync();
         const int columns = columns_of(tile);
-        const unsigned what = tb200_tc::instruction<PAIR>(std::is_same<T, bf16>::value, a_mn, b_mn, columns);
-        for (int k = 0; k < tile.depth; k += DEEP, ++count) {
+        const unsigned what = tb200_tc::instruction<PAIR>(!std::is_same<T, f16>::value, a_mn, b_mn, columns);
+        for (int k = 0, segment = 0; k < tile.depth; ++count) {
           const unsigned stage = count % STAGES, from = base + stage * Shared::STAGE;
           good = await<PAIR>(&sh.full[stage], count / STAGES & 1, &sh.dead, p.hdr);
           if (!good) break;
@@ -438,10 +447,11 @@ __global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(con
             const unsigned long long a = tb200_tc::operand(from, a_mn, CHUNK), b = tb200_tc::operand(from + A_BYTES, b_mn, CHUNK);
 #pragma unroll
             for (int i = 0; i < DEEP / 16; ++i)
-              if (i < steps) tb200_tc::multiply<PAIR>(d, a + i / 4 * a_jump + i % 4 * a_step, b + i / 4 * b_jump + i % 4 * b_step, what, k > 0 || i > 0);
+              if (i < steps) tb200_tc::multiply<PAIR>(d, a + i / 4 * a_jump + i % 4 * a_step, b + i / 4 * b_jump + i % 4 * b_step, what, segment > 0 || k > 0 || i > 0);
             tb200_tc::commit<PAIR>(&sh.empty[stage]);
           }
           __syncwarp();
+          if ((k += DEEP) >= tile.depth && ++segment < p.segments) k = 0;
         }
         if (good && tb200_tc::elected()) tb200_tc::commit<PAIR>(&sh.made[set]);
         __syncwarp();
@@ -455,18 +465,22 @@ __global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(con
     for (unsigned t = blockIdx.x / CTAS; good && t < turn.count; t += step) {
       const product_tile tile = tile_of(t, e);
       if (tile.rows == 0) continue;
-      const unsigned blocks = (unsigned)(tile.depth + DEEP - 1) / DEEP, stage = (count + blocks - 1) % STAGES;
-      count += blocks;
-      if (blocks == 0 || !is_tail(tile, (int)(blocks - 1) * DEEP)) continue;
-      good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr);
-      if (!good) break;
-      tails ^= 1u << stage;
-      clear_tail(stage, tile.depth - (int)(blocks - 1) * DEEP, 2 + (columns_of(tile) / CTAS + 63) / 64);
-      if (lane == 0) {
-        if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.ready[stage]));
-        else tb200::mbar_arrive(&sh.ready[stage]);
+      const unsigned blocks = (unsigned)(tile.depth + DEEP - 1) / DEEP;
+      const bool has = blocks > 0 && is_tail(tile, (int)(blocks - 1) * DEEP);
+      for (int segment = 0; good && segment < p.segments; ++segment) {
+        const unsigned stage = (count + blocks - 1) % STAGES;
+        count += blocks;
+        if (!has) continue;
+        good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr);
+        if (!good) break;
+        tails ^= 1u << stage;
+        clear_tail(stage, tile.depth - (int)(blocks - 1) * DEEP, 2 + (columns_of(tile) / CTAS + 63) / 64);
+        if (lane == 0) {
+          if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.ready[stage]));
+          else tb200::mbar_arrive(&sh.ready[stage]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
   } else {
     // a writer has the 32 lanes that warp % 4 may read, and every other 32 columns; GATED: of these it finishes 16, of both halves
@@ -537,10 +551,10 @@ __global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(con
           }
           if (kind == ACT_SILU) {
 #pragma unroll
-            for (int j = 0; j < PUT; ++j) w[j] = activated<true>(w[j], ACT_SILU);
+            for (int j = 0; j < PUT; ++j) w[j] = activated<sizeof(T) == 2>(w[j], ACT_SILU);
           } else if (kind == ACT_GELU) {
 #pragma unroll
-            for (int j = 0; j < PUT; ++j) w[j] = activated<true>(w[j], ACT_GELU);
+            for (int j = 0; j < PUT; ++j) w[j] = activated<sizeof(T) == 2>(w[j], ACT_GELU);
           }
           if constexpr (GATED) {
 #pragma unroll
@@ -815,6 +829,33 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ fr
   reinterpret_cast<uint4*>(to)[i] = v.all;
 }
 
+// The same rows as three planes of 16 bits, [matrix][plane][row][halves][wide], zeros behind a half's width.  A number that is not finite is in the first plane alone; one that
+// would be rounded to infinity is cut off instead.
+__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ from, size_t each, size_t outer, size_t stride, size_t rows, unsigned halves, unsigned width, unsigned wide,
+                                                         bf16* __restrict__ to) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const unsigned across = wide / 8;
+  if (i >= rows * halves * across) return;
+  const size_t line = i / across, row = line / halves, matrix = row / each, c = (i - line * across) * 8, h = line - row * halves;
+  const float* const f = from + matrix * outer + (row - matrix * each) * stride + h * width + c;
+  union { unsigned short at[8]; uint4 all; } v[PLANES];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float x = c + j < width ? f[j] : 0.f;
+#pragma unroll
+    for (int q = 0; q < PLANES; ++q) {
+      const unsigned bits = __float_as_uint(x);
+      unsigned short r = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+      if ((r & 0x7fff) == 0x7f80) r = (unsigned short)(bits >> 16);      // infinity stays, the largest numbers are cut off
+      v[q].at[j] = r;
+      x -= __uint_as_float((unsigned)r << 16);
+      if ((bits & 0x7f800000u) == 0x7f800000u) x = 0.f;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < PLANES; ++q) *reinterpret_cast<uint4*>(to + (((matrix * PLANES + q) * each + (row - matrix * each)) * halves + h) * wide + c) = v[q].all;
+}
+
 // dbefore = dout * the activation's slope; gated with out = act(a) b: da = dout b act'(a), db = dout act(a).  Bound by the bytes; a thread asks for two places' pieces before
 // it works on either.
 template <class T, int V>
@@ -889,22 +930,36 @@ struct matrices {
   size_t width, rows, stride, count, outer;      // count 0: one matrix
   unsigned halves;                               // of the width, each on a boundary of 16 bytes
   size_t bytes;                                  // of an element
+  bool split;                                    // to be laid out as planes
   size_t pieces() const { return (half() * bytes + 15) / 16; }
-  bool fits() const { return ((reinterpret_cast<uintptr_t>(at) | stride * bytes | (count > 1 ? outer * bytes : 0) | (halves > 1 ? half() * bytes : 0)) & 15) == 0; }
+  size_t wide() const { return (half() + 63) / 64 * 64; }      // of a half in a plane
+  bool fits() const { return !split && ((reinterpret_cast<uintptr_t>(at) | stride * bytes | (count > 1 ? outer * bytes : 0) | (halves > 1 ? half() * bytes : 0)) & 15) == 0; }
   size_t half() const { return width / halves; }
   size_t all_rows() const { return rows * (count ? count : 1); }
-  size_t packed_bytes() const { return fits() ? 0 : tb200::align_up(all_rows() * halves * pieces() * 16, 256); }
+  size_t packed_bytes() const { return fits() ? 0 : tb200::align_up(all_rows() * halves * (split ? PLANES * wide() * 2 : pieces() * 16), 256); }
 };
 // into `room`, which is moved on; nothing where they fit
 template <class T> cudaError_t pack(matrices& x, char*& room, cudaStream_t stream) {
   if (x.fits() || x.width == 0 || x.all_rows() == 0) return cudaSuccess;
-  const size_t bytes = x.packed_bytes(), pieces = x.all_rows() * x.halves * x.pieces();
+  const size_t bytes = x.packed_bytes(), pieces = x.all_rows() * x.halves * (x.split ? x.wide() / 8 : x.pieces());
   if ((pieces + 255) / 256 > 0x7fffffffull) return cudaErrorInvalidValue;
-  pack_rows_kernel<T><<<(unsigned)((pieces + 255) / 256), 256, 0, stream>>>(static_cast<const T*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), reinterpret_cast<T*>(room));
+  const unsigned grid = (unsigned)((pieces + 255) / 256);
+  if constexpr (sizeof(T) == 4) {
+    if (x.split) {
+      split_rows_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), (unsigned)x.wide(),
+                                                  reinterpret_cast<bf16*>(room));
+      x.width = x.stride = x.halves * x.wide();
+      x.count = (x.count ? x.count : 1) * PLANES;
+      x.bytes = 2;
+      x.split = false;
+    }
+  }
+  if (x.bytes == sizeof(T)) {
+    pack_rows_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), reinterpret_cast<T*>(room));
+    x.width = x.stride = x.halves * x.pieces() * 16 / sizeof(T);
+  }
   x.at = room;
-  x.stride = x.halves * x.pieces() * 16 / sizeof(T);
   x.outer = x.rows * x.stride;
-  x.width = x.stride;
   room += bytes;
   return cudaGetLastError();
 }
@@ -947,6 +1002,9 @@ cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_
   return cudaLaunchKernelEx(&cfg, kernel, a, b, p);
 }
 
+// So few rows an expert that a product is as long as it takes to read the matrices: narrow tiles, and nothing laid out anew that need not be
+bool few_rows(size_t m, size_t experts) { return m <= 32 * experts; }
+
 template <int MODE, bool A_MN, int BN> cudaError_t launch_fma(const matrices& a, const matrices& b, const product_plan<float>& p, cudaStream_t stream) {
   using Shared = fma_shared<MODE, A_MN, BN>;
   auto kernel = expert_product_f32_kernel<MODE, A_MN, BN>;
@@ -959,63 +1017,70 @@ template <int MODE, bool A_MN, int BN> cudaError_t launch_fma(const matrices& a,
 }
 
 // out[i] = rows[i] W[e] (+ the rest) of the expert that row i is of.  w: its matrices' rows are inputs (a_mn: the outputs of an input are neighbours), or outputs.
-template <class T> cudaError_t product_by_rows(matrices w, matrices x, product_plan<T> p, char* room, cudaStream_t stream) {
+// Both have been packed.
+template <class T> cudaError_t product_by_rows(const matrices& w, const matrices& x, product_plan<T> p, cudaStream_t stream) {
   const bool gated = (p.activation & ACT_GATED) != 0;
-  bool few = (size_t)p.m <= (size_t)32 * p.experts;
-  cudaError_t e = pack<T>(w, room, stream);
-  if (e == cudaSuccess) e = pack<T>(x, room, stream);
-  if (e != cudaSuccess) return e;
+  bool few = few_rows(p.m, p.experts);
   p.second = p.a_mn ? (int)(w.halves == 2 ? w.width / 2 : 0) : p.features;
   if constexpr (sizeof(T) == 4) {
-    if (p.a_mn) return few ? launch_fma<BY_ROWS, true, 32>(w, x, p, stream) : launch_fma<BY_ROWS, true, 64>(w, x, p, stream);
-    return few ? launch_fma<BY_ROWS, false, 32>(w, x, p, stream) : launch_fma<BY_ROWS, false, 64>(w, x, p, stream);
-  } else {
-    const size_t both = (size_t)p.features * (gated ? 2 : 1);
-    p.wide_out = in_16_bytes(p.out, p.features, p.features, 2) && in_16_bytes(p.before, both, both, 2);
-    p.wide_residual = in_16_bytes(p.residual, p.features, p.residual_stride, 2);
-    p.a_split = w.width % 64 == 0 && !(gated && p.a_mn);
-    box_axes of_a = plain_axes(w.width, w.rows, w.stride, w.count, w.outer, 128, p.a_split, 2);
-    if (gated && p.a_mn) of_a = {{(size_t)p.features, w.rows, 2, 1, w.count}, {w.stride, (size_t)p.second, 0, w.outer}, {64, 128, 2, 1, 1}};      // 64 of either half
-    else if (gated) of_a = {{p.a_split ? 64 : w.width, (size_t)p.features, 2, p.a_split ? w.width / 64 : 1, w.count}, {w.stride, p.features * w.stride, 64, w.outer},
-                            {64, 64, 2, p.a_split ? 2u : 1u, 1}};
-    for (;; few = true) {      // (again, by single CTAs, if there is no room for pairs)
-      p.box = few ? 16 : 128;
-      p.b_split = !few && x.width % 64 == 0;
-      CUtensorMap a = {}, b = {};
-      if (p.k > 0 && (!box_map<T>(a, w.at, of_a) || !box_map<T>(b, x.at, plain_axes(x.width, x.rows, x.stride, 1, 0, (unsigned)p.box, p.b_split, 2)))) return cudaErrorNotSupported;
-      if (few) return gated ? launch_tc<T, T, BY_ROWS, false, true, 64, 4>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, false, false, 64, 4>(a, b, p, stream);
-      e = gated ? launch_tc<T, T, BY_ROWS, true, true, 256, 3>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, true, false, 256, 3>(a, b, p, stream);
-      if (!tb200::launch_refused(e)) return e;
+    if (p.planes == 1) {
+      if (p.a_mn) return few ? launch_fma<BY_ROWS, true, 32>(w, x, p, stream) : launch_fma<BY_ROWS, true, 64>(w, x, p, stream);
+      return few ? launch_fma<BY_ROWS, false, 32>(w, x, p, stream) : launch_fma<BY_ROWS, false, 64>(w, x, p, stream);
     }
+  }
+  cudaError_t e = cudaSuccess;
+  const size_t both = (size_t)p.features * (gated ? 2 : 1);
+  p.wide_out = in_16_bytes(p.out, p.features, p.features, sizeof(T)) && in_16_bytes(p.before, both, both, sizeof(T));
+  p.wide_residual = in_16_bytes(p.residual, p.features, p.residual_stride, sizeof(T));
+  p.a_split = w.width % 64 == 0 && !(gated && p.a_mn);
+  box_axes of_a = plain_axes(w.width, w.rows, w.stride, w.count, w.outer, 128, p.a_split, 2);
+  if (gated && p.a_mn) of_a = {{(size_t)p.features, w.rows, 2, 1, w.count}, {w.stride, (size_t)p.second, 0, w.outer}, {64, 128, 2, 1, 1}};      // 64 of either half
+  else if (gated) of_a = {{p.a_split ? 64 : w.width, (size_t)p.features, 2, p.a_split ? w.width / 64 : 1, w.count}, {w.stride, p.features * w.stride, 64, w.outer},
+                          {64, 64, 2, p.a_split ? 2u : 1u, 1}};
+  for (;; few = true) {      // (again, by single CTAs, if there is no room for pairs)
+    p.box = few ? 16 : 128;
+    p.b_split = !few && x.width % 64 == 0;
+    CUtensorMap a = {}, b = {};
+    if (p.k > 0 && (!box_map<T>(a, w.at, of_a) || !box_map<T>(b, x.at, plain_axes(x.width, x.rows, x.stride, p.planes, x.outer, (unsigned)p.box, p.b_split, 2)))) return cudaErrorNotSupported;
+    if (few) return gated ? launch_tc<T, T, BY_ROWS, false, true, 64, 4>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, false, false, 64, 4>(a, b, p, stream);
+    e = gated ? launch_tc<T, T, BY_ROWS, true, true, 256, 3>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, true, false, 256, 3>(a, b, p, stream);
+    if (!tb200::launch_refused(e)) return e;
   }
 }
 
 // matrix[e][o][f] = the sum over the expert's rows of others[row][o] features[row][f]
 template <class T, class O> cudaError_t product_by_experts(const matrices& features, const matrices& others, product_plan<T> p, cudaStream_t stream) {
   if constexpr (sizeof(T) == 4) {
-    return launch_fma<BY_EXPERTS, true, 64>(features, others, p, stream);
-  } else {
-    p.wide_out = in_16_bytes(p.matrix, p.features, p.features, sizeof(O));
-    p.a_split = features.width % 64 == 0;
-    p.b_split = others.width % 64 == 0;
-    CUtensorMap a = {}, b = {};
-    if (p.m > 0 && (!box_map<T>(a, features.at, plain_axes(features.width, features.rows, features.stride, 1, 0, DEEP, p.a_split, 2)) ||
-                    !box_map<T>(b, others.at, plain_axes(others.width, others.rows, others.stride, 1, 0, DEEP, p.b_split, 2))))
-      return cudaErrorNotSupported;
-    if (p.features > 128) {
-      const cudaError_t e = launch_tc<T, O, BY_EXPERTS, true, false, 256, 3>(a, b, p, stream);
-      if (!tb200::launch_refused(e)) return e;      // (no room for pairs)
-    }
-    return launch_tc<T, O, BY_EXPERTS, false, false, 128, 3>(a, b, p, stream);
+    if (p.planes == 1) return launch_fma<BY_EXPERTS, true, 64>(features, others, p, stream);
   }
+  p.wide_out = in_16_bytes(p.matrix, p.features, p.features, sizeof(O));
+  p.a_split = features.width % 64 == 0;
+  p.b_split = others.width % 64 == 0;
+  CUtensorMap a = {}, b = {};
+  if (p.m > 0 && (!box_map<T>(a, features.at, plain_axes(features.width, features.rows, features.stride, p.planes, features.outer, DEEP, p.a_split, 2)) ||
+                  !box_map<T>(b, others.at, plain_axes(others.width, others.rows, others.stride, p.planes, others.outer, DEEP, p.b_split, 2))))
+    return cudaErrorNotSupported;
+  if (p.features > 128) {
+    const cudaError_t e = launch_tc<T, O, BY_EXPERTS, true, false, 256, 3>(a, b, p, stream);
+    if (!tb200::launch_refused(e)) return e;      // (no room for pairs)
+  }
+  return launch_tc<T, O, BY_EXPERTS, false, false, 128, 3>(a, b, p, stream);
 }
 
 bool sizes_fit(size_t n, size_t experts, size_t in, size_t out) { return n <= MOST_ROWS && experts >= 1 && experts <= (size_t)MOST_EXPERTS && in < MOST_CHANNELS && out < MOST_CHANNELS; }
+// 32-bit rows go to the tensor cores, as planes, where products are longer than it takes to lay the planes out: not few rows, and 64 or more channels on both sides
+template <class T> bool in_planes(size_t n, size_t experts, size_t in, size_t out) { return sizeof(T) == 4 && !few_rows(n, experts) && in >= 64 && out >= 64; }
+template <class T> void set_planes(product_plan<T>& p, bool split) {
+  p.planes = split ? PLANES : 1;
+  p.segments = split ? SEGMENTS : 1;
+  p.a_planes = split ? A_PLANES : 0;
+  p.b_planes = split ? B_PLANES : 0;
+}
 bool activation_known(int a) { return a == ACT_NONE || (a & ~ACT_GATED) == ACT_SILU || (a & ~ACT_GATED) == ACT_GELU; }
 // weight as it lies: an input's outputs are neighbours, or an output's inputs
-matrices weights_of(const void* d_weight, size_t experts, size_t in, size_t out, size_t expert_stride, size_t stride, bool inputs_inside, unsigned halves, size_t bytes) {
-  if (inputs_inside) return {d_weight, in, out, stride, experts, expert_stride, 1, bytes};
-  return {d_weight, out, in, stride, experts, expert_stride, halves, bytes};
+matrices weights_of(const void* d_weight, size_t experts, size_t in, size_t out, size_t expert_stride, size_t stride, bool inputs_inside, unsigned halves, size_t bytes, bool split) {
+  if (inputs_inside) return {d_weight, in, out, stride, experts, expert_stride, 1, bytes, split};
+  return {d_weight, out, in, stride, experts, expert_stride, halves, bytes, split};
 }
 bool weights_fit(size_t experts, size_t in, size_t out, size_t expert_stride, size_t stride, bool inputs_inside) {
   const size_t width = inputs_inside ? in : out, rows = inputs_inside ? out : in;
@@ -1039,7 +1104,8 @@ TB200_API int tb200_expert_product(const void* d_rows, size_t rows_stride, const
       const bool gated = (activation & ACT_GATED) != 0;
       if (!sizes_fit(n, num_experts, in, out) || !activation_known(activation) || (gated && out % 2)) return ERR_INVALID;
       const size_t width = gated ? out / 2 : out;
-      matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, gated ? 2 : 1, sizeof(T)), x = {d_rows, in, n, rows_stride, 0, 0, 1, sizeof(T)};
+      const bool split = in_planes<T>(n, num_experts, in, out);
+      matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, gated ? 2 : 1, sizeof(T), split), x = {d_rows, in, n, rows_stride, 0, 0, 1, sizeof(T), split};
       int rc;
       if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header) + w.packed_bytes() + x.packed_bytes(), rc)) return rc;
       if (n == 0 || width == 0) return 0;
@@ -1062,7 +1128,11 @@ TB200_API int tb200_expert_product(const void* d_rows, size_t rows_stride, const
       p.activation = activation;
       p.first = true;
       p.hdr = static_cast<tb200::ws_header*>(d_ws);
-      return (int)product_by_rows<T>(w, x, p, static_cast<char*>(d_ws) + sizeof(tb200::ws_header), stream);
+      set_planes(p, split);
+      char* room = static_cast<char*>(d_ws) + sizeof(tb200::ws_header);
+      cudaError_t e = pack<T>(w, room, stream);
+      if (e == cudaSuccess) e = pack<T>(x, room, stream);
+      return (int)(e == cudaSuccess ? product_by_rows<T>(w, x, p, stream) : e);
     });
   });
 }
@@ -1075,8 +1145,9 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
     if (grad_t != t && grad_t != TB200_F32) return ERR_UNSUPPORTED;
     return by_index_dtype(offset_t, [&](auto iv) -> int {
       if (!sizes_fit(n, num_experts, in, out)) return ERR_INVALID;
-      matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, 1, sizeof(T)), x = {d_rows, in, n, rows_stride, 0, 0, 1, sizeof(T)},
-               d = {d_dout, out, n, dout_stride, 0, 0, 1, sizeof(T)};
+      const bool split = in_planes<T>(n, num_experts, in, out);
+      matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, 1, sizeof(T), split), x = {d_rows, in, n, rows_stride, 0, 0, 1, sizeof(T), split},
+               d = {d_dout, out, n, dout_stride, 0, 0, 1, sizeof(T), split};
       const unsigned parts = d_dbias ? sum_parts(n, num_experts, out) : 1;
       const size_t sums = parts > 1 ? tb200::align_up((size_t)parts * num_experts * out * 4, 256) : 0;
       int rc;
@@ -1100,13 +1171,14 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
       p.m = (int)n;
       p.hdr = static_cast<tb200::ws_header*>(d_ws);
       p.first = true;
+      set_planes(p, split);
       if (n && in) {
         product_plan<T> q = p;
         q.k = (int)out;
         q.features = (int)in;
         q.a_mn = inputs_inside != 0;
         q.out = static_cast<T*>(d_drows);
-        e = product_by_rows<T>(w, d, q, room, stream);
+        e = product_by_rows<T>(w, d, q, stream);
         if (e != cudaSuccess) return (int)e;
         p.first = false;
       }
