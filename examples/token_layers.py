@@ -1,10 +1,10 @@
-"""A small token model whose memory-bound parts run on thrust_b200: tokens are looked up, mixed along the sequence by a gated recurrence, sent to
-experts and brought back, and scored against the same table; trained for a few steps, then used to write one token at a time.
+"""A small token model whose layers run on thrust_b200: tokens are looked up, mixed along the sequence by a gated recurrence, sent to the experts that a
+router chooses, multiplied there and brought back, and scored against the same table; trained for a few steps, then used to write one token at a time.
 
     python examples/token_layers.py [--steps 30]
 
-The matrix products are torch's; lookup, recurrence, dispatch and combination, and all their gradients, are the library's calls, wrapped as
-torch.autograd functions below.  The text is made up: a walk on the tokens in which each is followed by one of two others, so that a
+The dense matrix products are torch's; lookup, recurrence, routing, dispatch, the experts' products and combination, and all their gradients, are the
+library's calls, wrapped as torch.autograd functions below; nothing of a step is read back to the host.  The text is made up: a walk on the tokens in which each is followed by one of two others, so that a
 model which learns gets well below the loss of guessing, log(vocabulary).
 """
 import argparse
@@ -50,6 +50,38 @@ class Recurrence(torch.autograd.Function):
         return dx, dgate, None
 
 
+class Route(torch.autograd.Function):
+    """The best experts of each token and their weights, a softmax over those that were chosen."""
+
+    @staticmethod
+    def forward(ctx, logits, choices):
+        experts, weights = tb.expert_route(logits, choices)
+        ctx.save_for_backward(logits, experts)
+        ctx.mark_non_differentiable(experts)
+        return experts, weights
+
+    @staticmethod
+    def backward(ctx, _, grad):
+        logits, experts = ctx.saved_tensors
+        return tb.expert_route_grad(grad.contiguous(), experts, logits), None
+
+
+class Experts(torch.autograd.Function):
+    """silu(rows @ weight[e] + bias[e]) of the rows of each expert e."""
+
+    @staticmethod
+    def forward(ctx, rows, weight, bias, offsets):
+        out, before = tb.expert_product(rows, offsets, weight, bias, "silu", keep=True)
+        ctx.save_for_backward(rows, weight, before, offsets)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        rows, weight, before, offsets = ctx.saved_tensors
+        dbefore = tb.expert_activation_grad(grad.contiguous(), before, "silu")
+        return (*tb.expert_product_grad(dbefore, rows, offsets, weight, bias=True), None)
+
+
 class Dispatch(torch.autograd.Function):
     """Tokens' rows by expert, and the plan for the way back."""
 
@@ -90,21 +122,13 @@ class TokenModel(torch.nn.Module):
         self.mix = make(dim, 2 * dim)                 # x and gate of the recurrence, in one product
         self.router = make(dim, experts)
         self.expert = make(experts, dim, dim)
-
-    def route(self, h):
-        weights, experts = torch.topk(h @ self.router, self.choices, dim=1)
-        return torch.softmax(weights.float(), dim=1).contiguous(), experts
-
-    def apply_experts(self, rows, offsets):
-        ends = offsets.tolist()                       # how many rows each expert has: the host shapes the products by it
-        parts = [rows[a:b] @ self.expert[e] for e, (a, b) in enumerate(zip(ends[:-1], ends[1:]))]
-        return torch.nn.functional.silu(torch.cat(parts + [rows[ends[-1]:]]))
+        self.expert_bias = torch.nn.Parameter(torch.zeros(experts, dim, device="cuda"))
 
     def score(self, h):
         """Adds what the experts make of h, and scores every token of the table."""
-        weights, experts = self.route(h)
+        experts, weights = Route.apply(h @ self.router, self.choices)
         rows, *plan = Dispatch.apply(h, experts, self.experts)
-        made = self.apply_experts(rows, plan[2])
+        made = Experts.apply(rows, self.expert, self.expert_bias, plan[2])
         return (h + Combine.apply(made, weights, *plan)) @ self.table.t()
 
     def forward(self, tokens, offsets):

@@ -312,3 +312,26 @@ def test_refusals(tb):
                  lambda: tb.expert_activation_grad(d, e(8, 64)[:, ::2], "silu")):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_graphs_side_by_side(tb, dtype):
+    """Two graphs captured on one stream, with operands that are laid out anew, replayed at the same time."""
+    g = torch.Generator(device="cuda").manual_seed(15)
+    capture, streams, graphs, results, wants = torch.cuda.Stream(), [torch.cuda.Stream(), torch.cuda.Stream()], [], [], []
+    for counts in ([700, 0, 900, 811], [1500, 33, 640, 2]):
+        x, offsets, w = inputs(g, counts, 0, 3, 333, 517, dtype, "in_out")
+        d = rand(g, x.shape[0], 517, dtype=dtype)
+        wants.append((tb.expert_product(x, offsets, w), *tb.expert_product_grad(d, x, offsets, w, bias=True)))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=capture):
+            results.append((tb.expert_product(x, offsets, w), *tb.expert_product_grad(d, x, offsets, w, bias=True)))
+        graphs.append((graph, x, offsets, w, d))
+    for _ in range(10):
+        for s, (graph, *_) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for got, want in zip(results, wants):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))

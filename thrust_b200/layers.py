@@ -12,6 +12,7 @@ nothing: its result is zero, and what belongs to it, NaNs included, reaches no r
 
 Every call only enqueues work on the current stream, like reduce_to_device.  There is no fallback path.
 """
+import ctypes
 from collections import namedtuple
 
 import torch
@@ -349,6 +350,17 @@ def expert_route_grad(dweights, experts, logits, scores="softmax", renormalize=T
 
 
 # ---------------------------------------------------------------------------------- experts' products
+def _enqueue_product(what, fn, dev, *args):
+    """_enqueue, but a captured call has a workspace of its own, which belongs to the graph: operands are laid out anew there, and graphs that were captured
+    on one stream may be replayed side by side."""
+    if not _stream_captures():
+        return _enqueue(what, what, fn, dev, *args)
+    call, stream, need = getattr(_lib.load(), fn), _raw_stream(dev), ctypes.c_size_t(0)
+    _check(call(*args, None, ctypes.byref(need), stream), what)
+    room = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    _check(call(*args, room.data_ptr(), ctypes.byref(need), stream), what)
+
+
 def _matrices(what, t, dev):
     """How [experts, in, out] lies: (experts' distance, rows' distance, whether inputs are neighbours instead of outputs)."""
     if t.get_device() != dev:
@@ -386,7 +398,7 @@ def expert_product(rows, offsets, weight, bias=None, activation=None, residual=N
 
     rows [n, in], weight [experts, in, out], contiguous or the transpose of such (out, in) matrices, bias [experts, out], residual as out, all of one
     type.  activation: None, "silu", "gelu" (by the error function), or "gated_silu", "gated_gelu": the outputs are halves [a | b], and act(a) * b comes
-    of them.  Sums are 32 bits, rounded once.  Returns out [n, out] (gated: [n, out / 2]); with keep (out, before), before [n, out] for expert_activation_grad."""
+    of them.  Sums are 32 bits, rounded once; an infinite float32 operand may leave NaNs where the definition says infinity.  Returns out [n, out] (gated: [n, out / 2]); with keep (out, before), before [n, out] for expert_activation_grad."""
     dev, step, code, lies = _rows_and_experts(rows, offsets, weight)
     if activation not in _ACTIVATIONS:
         raise ValueError("activation: None, or one of %s" % ", ".join(k for k in _ACTIVATIONS if k))
@@ -401,7 +413,7 @@ def expert_product(rows, offsets, weight, bias=None, activation=None, residual=N
         to, extra = residual.data_ptr(), _row_step("residual", residual, dev)
     out = torch.empty(n, width, dtype=dtype, device=rows.device)
     before = torch.empty(n, outputs, dtype=dtype, device=rows.device) if keep else None
-    _enqueue("expert_product", "expert_product", "tb200_expert_product", dev, rows.data_ptr(), step, offsets.data_ptr(), code, weight.data_ptr(), *lies,
+    _enqueue_product("expert_product", "tb200_expert_product", dev, rows.data_ptr(), step, offsets.data_ptr(), code, weight.data_ptr(), *lies,
              _maybe("bias", bias, dtype, (experts, outputs), dev), to, extra, act, n, experts, inputs, outputs, _ROW_CODE[dtype], out.data_ptr(),
              before.data_ptr() if keep else None)
     return (out, before) if keep else out
@@ -446,6 +458,6 @@ def expert_product_grad(dout, rows, offsets, weight, bias=False, dtype=None, out
     to = _packed("out", out.transpose(1, 2) if inside else out, dtype, (experts, outputs, inputs) if inside else (experts, inputs, outputs), dev)
     drows = torch.empty(n, inputs, dtype=rows.dtype, device=rows.device)
     dbias = torch.empty(experts, outputs, dtype=_F32, device=rows.device) if bias else None
-    _enqueue("expert_product_grad", "expert_product_grad", "tb200_expert_product_grad", dev, dout.data_ptr(), dstep, rows.data_ptr(), step, offsets.data_ptr(), code, weight.data_ptr(),
-             *lies, n, experts, inputs, outputs, _ROW_CODE[rows.dtype], _ROW_CODE[dtype], int(accumulate), drows.data_ptr(), to, dbias.data_ptr() if bias else None)
+    _enqueue_product("expert_product_grad", "tb200_expert_product_grad", dev, dout.data_ptr(), dstep, rows.data_ptr(), step, offsets.data_ptr(), code, weight.data_ptr(), *lies, n, experts, inputs, outputs,
+                     _ROW_CODE[rows.dtype], _ROW_CODE[dtype], int(accumulate), drows.data_ptr(), to, dbias.data_ptr() if bias else None)
     return drows, out, dbias
