@@ -181,9 +181,11 @@ __device__ __forceinline__ bool withheld(unsigned t, unsigned step) { return wit
 __device__ __forceinline__ bool withheld(unsigned, unsigned) { return false; }
 #endif
 
-constexpr int DEEP = 128;                     // of the contraction, a stage
+constexpr int DEEP = 128, GROUP = 6;          // of the contraction, a stage; stages
 constexpr int WRITERS = 8, BRINGS = WRITERS, MULTIPLIES = WRITERS + 1, CLEARS = WRITERS + 2;      // warps that write results, that bring operands, that multiply, that clear boxes' ends (by experts)
-template <int MODE> constexpr int TC_THREADS = (WRITERS + (MODE == BY_EXPERTS ? 3 : 2)) * 32;
+// 32-bit results: the writers hold 128 sums a thread, of registers that the other four warps hand over (launched with 168 a thread; 2 x 216 + 72 = 3 x 168)
+template <int MODE, class O> constexpr int TC_THREADS = sizeof(O) == 4 ? 384 : (WRITERS + (MODE == BY_EXPERTS ? 3 : 2)) * 32;
+constexpr int WRITERS_REGISTERS = 216, OTHERS_REGISTERS = 72;
 constexpr unsigned CHUNK = 64 * DEEP * 2;     // 64 neighbours by 128 of the other axis
 constexpr unsigned A_BYTES = 2 * CHUNK;       // a CTA's 128 features
 
@@ -297,16 +299,20 @@ constexpr unsigned A_PLANES = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, B
 //
 // One warp keeps STAGES boxes of A and B on their way by the copy engine, one issues the matrix instructions as they come, eight take the sums of the last
 // tile from tensor memory, while the next one's are made in its other half, and write them.  Sums are 32 bits from first to last; they
-// are rounded once, where they are stored, after bias, activation and residual.  Gated: the two halves of a result are in lanes 64 apart, in warps that pass each
+// are rounded once, where they are stored, after bias, activation and residual.  The matrix instructions cut off what they add (1.2e-7 of the results for each
+// stage, and always the same way), which results of 16 bits do not see.  32-bit results (FINE) are made of sums over GROUP stages, which the writers add up in registers,
+// rounded to nearest, and put back to where the last ones were: three stages where an activation multiplies two results (off by 3.4e-7, and 6.8e-7 behind it, for any
+// length), six for matrices (7.3e-7; with four 4.7e-7, and 8198 rows' gradients take 103 us instead of 98).  Gated: the two halves of a result are in lanes 64 apart, in warps that pass each
 // other half of their columns.
 //
 // By experts the contraction ends where the expert's rows do, in the middle of a box: what the box has of the next rows is cleared in shared memory, up to
 // the next 16, where the instructions end.  Such a box is counted by the barrier `tail` of the CTA that it is for, where a warp of its own clears it as soon as it is there and
 // says that it is ready.
 template <class T, class O, int MODE, bool PAIR, bool GATED, int BN, int STAGES>
-__global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const product_plan<T> p) {
+__global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const product_plan<T> p) {
   using Shared = tc_shared<PAIR, GATED, BN, STAGES>;
   constexpr int CTAS = PAIR ? 2 : 1, OWN = GATED ? 64 : 128, WIDE = OWN * CTAS, UNIT = 16 * CTAS;
+  constexpr bool FINE = sizeof(O) == 4;
   extern __shared__ char raw[];
   char* const stages = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   Shared& sh = *reinterpret_cast<Shared*>(stages + STAGES * Shared::STAGE);
@@ -352,137 +358,150 @@ __global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(con
     __syncwarp();
   };
 
-  if (warp == BRINGS) {
-    const unsigned base = tb200::smem_addr(stages);
-    unsigned count = 0, e = 0;      // stages filled so far
-    bool good = true;
-    for (unsigned t = blockIdx.x / CTAS; good && t < turn.count; t += step) {
-      const product_tile tile = tile_of(t, e);
-      if (tile.rows == 0) continue;
-      const int share = columns_of(tile) / CTAS, feature = tile.feature + (int)rank * OWN, other = (MODE == BY_ROWS ? tile.row : tile.other) + (int)rank * share;
-      // by rows B has two chunks of k, each of boxes of rows, unless a box has both; by experts two chunks of others, unless a box has both
-      const int boxes = MODE == BY_ROWS ? (share + p.box - 1) / p.box : p.b_split ? 2 : (share + 63) / 64;
-      const unsigned b_box = MODE == BY_ROWS ? p.box * 128 : CHUNK, bytes = A_BYTES + (MODE == BY_ROWS ? 2 : 1) * boxes * b_box;
-      for (int k = 0, segment = 0; k < tile.depth; ++count) {
-        const unsigned stage = count % STAGES, to = base + stage * Shared::STAGE;
-        good = await<PAIR>(&sh.empty[stage], (count / STAGES & 1) ^ 1, &sh.dead, p.hdr);
-        if (!good) break;
-        const bool tail = is_tail(tile, k);
-        if (tb200_tc::elected()) {
-          unsigned bar;
-          if (tail) {
-            tb200::mbar_arrive_expect(&sh.tail[stage], bytes);
-            if (rank == 0) tb200::mbar_arrive(&sh.full[stage]);
-            bar = tb200::smem_addr(&sh.tail[stage]);
-          } else {
-            if (rank == 0) tb200::mbar_arrive_expect(&sh.full[stage], bytes * CTAS);
-            bar = PAIR ? tb200_tc::first_ones(&sh.full[stage]) : tb200::smem_addr(&sh.full[stage]);
-          }
-          if (!withheld(t, step)) {
-            const int row = MODE == BY_ROWS ? k : tile.row + k, pa = (int)(p.a_planes >> 2 * segment & 3), pb = (int)(p.b_planes >> 2 * segment & 3);
-            const int of_a = MODE == BY_ROWS ? (int)tile.e * p.planes + pa : pa;
-            const bool both = p.a_split || (GATED && p.a_mn);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              if (c && both) continue;
-              tb200_tc::box_at at;
-              if (MODE == BY_EXPERTS || p.a_mn) at = {p.a_split ? 0 : feature + c * 64, row, p.a_split ? feature / 64 : 0, 0, of_a};
-              else at = {p.a_split ? 0 : k + c * 64, feature, p.a_split && !GATED ? k / 64 : 0, p.a_split && GATED ? k / 64 : 0, of_a};
-              tb200_tc::load_box<PAIR>(to + c * CHUNK, &map_a, at, bar);
-            }
-            if (MODE == BY_EXPERTS) {
-              if (p.b_split) tb200_tc::load_box<PAIR>(to + A_BYTES, &map_b, {0, row, other / 64, 0, pb}, bar);
-              else
-                for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + b * CHUNK, &map_b, {other + b * 64, row, 0, 0, pb}, bar);
-            } else if (PAIR && p.b_split) {
-              tb200_tc::load_box<PAIR>(to + A_BYTES, &map_b, {0, other, k / 64, 0, pb}, bar);
-            } else {
-              for (int c = 0; c < 2; ++c)
-                for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + c * Shared::B_CHUNK + b * b_box, &map_b, {k + c * 64, other + b * p.box, 0, 0, pb}, bar);
-            }
-          }
-        }
-        __syncwarp();
-        if ((k += DEEP) >= tile.depth && ++segment < p.segments) k = 0;
-      }
-    }
-    // the last of each stage, no longer needed
-    if (good)
-      for (unsigned i = 0; i < STAGES && i < count; ++i) good = good && await<PAIR>(&sh.empty[(count - 1 - i) % STAGES], (count - 1 - i) / STAGES & 1, &sh.dead, p.hdr);
-    // given up: what is on its way is counted where this warp may not be able to see it; copies take microseconds
-    if (!good)
-      for (int i = 0; i < 20; ++i) __nanosleep(1000000);
-  } else if (warp == MULTIPLIES) {
-    const unsigned base = tb200::smem_addr(stages);
-    unsigned count = 0, made = 0, e = 0, tails = 0;      // tails: a bit for each stage's barrier
-    bool good = true;
-    const bool a_mn = MODE == BY_EXPERTS || p.a_mn;
-    constexpr bool b_mn = MODE == BY_EXPERTS;
-    // from one 16 k to the next, and from one 64 to the next, in a descriptor's units of 16 bytes
-    const unsigned a_step = a_mn ? 16 * 128 >> 4 : 2, a_jump = a_mn ? 64 * 128 >> 4 : CHUNK >> 4;
-    constexpr unsigned b_step = b_mn ? 16 * 128 >> 4 : 2, b_jump = b_mn ? 64 * 128 >> 4 : Shared::B_CHUNK >> 4;
-    if (rank == 0) {
+  if (warp >= WRITERS) {
+    static_assert(2 * WRITERS_REGISTERS + OTHERS_REGISTERS == 3 * 168, "no more registers than the CTA was launched with");
+    if constexpr (FINE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHERS_REGISTERS));
+    if (warp == BRINGS) {
+      const unsigned base = tb200::smem_addr(stages);
+      unsigned count = 0, e = 0;      // stages filled so far
+      bool good = true;
       for (unsigned t = blockIdx.x / CTAS; good && t < turn.count; t += step) {
         const product_tile tile = tile_of(t, e);
-        if (tile.depth == 0 || tile.rows == 0) continue;
-        const unsigned set = made & 1, d = tmem + set * BN;
-        good = await<PAIR>(&sh.taken[set], (made / 2 & 1) ^ 1, &sh.dead, p.hdr);
-        if (!good) break;
-        ++made;
-        tb200_tc::fence_after_sync();
-        const int columns = columns_of(tile);
-        const unsigned what = tb200_tc::instruction<PAIR>(!std::is_same<T, f16>::value, a_mn, b_mn, columns);
+        if (tile.rows == 0) continue;
+        const int share = columns_of(tile) / CTAS, feature = tile.feature + (int)rank * OWN, other = (MODE == BY_ROWS ? tile.row : tile.other) + (int)rank * share;
+        // by rows B has two chunks of k, each of boxes of rows, unless a box has both; by experts two chunks of others, unless a box has both
+        const int boxes = MODE == BY_ROWS ? (share + p.box - 1) / p.box : p.b_split ? 2 : (share + 63) / 64;
+        const unsigned b_box = MODE == BY_ROWS ? p.box * 128 : CHUNK, bytes = A_BYTES + (MODE == BY_ROWS ? 2 : 1) * boxes * b_box;
         for (int k = 0, segment = 0; k < tile.depth; ++count) {
-          const unsigned stage = count % STAGES, from = base + stage * Shared::STAGE;
-          good = await<PAIR>(&sh.full[stage], count / STAGES & 1, &sh.dead, p.hdr);
+          const unsigned stage = count % STAGES, to = base + stage * Shared::STAGE;
+          good = await<PAIR>(&sh.empty[stage], (count / STAGES & 1) ^ 1, &sh.dead, p.hdr);
           if (!good) break;
-          const int valid = tile.depth - k < DEEP ? tile.depth - k : DEEP, steps = (valid + 15) / 16;
-          if (is_tail(tile, k)) {
-            good = await<PAIR>(&sh.ready[stage], tails >> stage & 1, &sh.dead, p.hdr);
-            if (!good) break;
-            tails ^= 1u << stage;
-          }
-          tb200_tc::fence_after_sync();
+          const bool tail = is_tail(tile, k);
           if (tb200_tc::elected()) {
-            const unsigned long long a = tb200_tc::operand(from, a_mn, CHUNK), b = tb200_tc::operand(from + A_BYTES, b_mn, CHUNK);
+            unsigned bar;
+            if (tail) {
+              tb200::mbar_arrive_expect(&sh.tail[stage], bytes);
+              if (rank == 0) tb200::mbar_arrive(&sh.full[stage]);
+              bar = tb200::smem_addr(&sh.tail[stage]);
+            } else {
+              if (rank == 0) tb200::mbar_arrive_expect(&sh.full[stage], bytes * CTAS);
+              bar = PAIR ? tb200_tc::first_ones(&sh.full[stage]) : tb200::smem_addr(&sh.full[stage]);
+            }
+            if (!withheld(t, step)) {
+              const int row = MODE == BY_ROWS ? k : tile.row + k, pa = (int)(p.a_planes >> 2 * segment & 3), pb = (int)(p.b_planes >> 2 * segment & 3);
+              const int of_a = MODE == BY_ROWS ? (int)tile.e * p.planes + pa : pa;
+              const bool both = p.a_split || (GATED && p.a_mn);
 #pragma unroll
-            for (int i = 0; i < DEEP / 16; ++i)
-              if (i < steps) tb200_tc::multiply<PAIR>(d, a + i / 4 * a_jump + i % 4 * a_step, b + i / 4 * b_jump + i % 4 * b_step, what, segment > 0 || k > 0 || i > 0);
-            tb200_tc::commit<PAIR>(&sh.empty[stage]);
+              for (int c = 0; c < 2; ++c) {
+                if (c && both) continue;
+                tb200_tc::box_at at;
+                if (MODE == BY_EXPERTS || p.a_mn) at = {p.a_split ? 0 : feature + c * 64, row, p.a_split ? feature / 64 : 0, 0, of_a};
+                else at = {p.a_split ? 0 : k + c * 64, feature, p.a_split && !GATED ? k / 64 : 0, p.a_split && GATED ? k / 64 : 0, of_a};
+                tb200_tc::load_box<PAIR>(to + c * CHUNK, &map_a, at, bar);
+              }
+              if (MODE == BY_EXPERTS) {
+                if (p.b_split) tb200_tc::load_box<PAIR>(to + A_BYTES, &map_b, {0, row, other / 64, 0, pb}, bar);
+                else
+                  for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + b * CHUNK, &map_b, {other + b * 64, row, 0, 0, pb}, bar);
+              } else if (PAIR && p.b_split) {
+                tb200_tc::load_box<PAIR>(to + A_BYTES, &map_b, {0, other, k / 64, 0, pb}, bar);
+              } else {
+                for (int c = 0; c < 2; ++c)
+                  for (int b = 0; b < boxes; ++b) tb200_tc::load_box<PAIR>(to + A_BYTES + c * Shared::B_CHUNK + b * b_box, &map_b, {k + c * 64, other + b * p.box, 0, 0, pb}, bar);
+              }
+            }
           }
           __syncwarp();
           if ((k += DEEP) >= tile.depth && ++segment < p.segments) k = 0;
         }
-        if (good && tb200_tc::elected()) tb200_tc::commit<PAIR>(&sh.made[set]);
+      }
+      // the last of each stage, no longer needed
+      if (good)
+        for (unsigned i = 0; i < STAGES && i < count; ++i) good = good && await<PAIR>(&sh.empty[(count - 1 - i) % STAGES], (count - 1 - i) / STAGES & 1, &sh.dead, p.hdr);
+      // given up: what is on its way is counted where this warp may not be able to see it; copies take microseconds
+      if (!good)
+        for (int i = 0; i < 20; ++i) __nanosleep(1000000);
+    } else if (warp == MULTIPLIES) {
+      const unsigned base = tb200::smem_addr(stages);
+      unsigned count = 0, made = 0, e = 0, tails = 0;      // tails: a bit for each stage's barrier
+      bool good = true;
+      const bool a_mn = MODE == BY_EXPERTS || p.a_mn;
+      constexpr bool b_mn = MODE == BY_EXPERTS;
+      // from one 16 k to the next, and from one 64 to the next, in a descriptor's units of 16 bytes
+      const unsigned a_step = a_mn ? 16 * 128 >> 4 : 2, a_jump = a_mn ? 64 * 128 >> 4 : CHUNK >> 4;
+      constexpr unsigned b_step = b_mn ? 16 * 128 >> 4 : 2, b_jump = b_mn ? 64 * 128 >> 4 : Shared::B_CHUNK >> 4;
+      if (rank == 0) {
+        for (unsigned t = blockIdx.x / CTAS; good && t < turn.count; t += step) {
+          const product_tile tile = tile_of(t, e);
+          if (tile.depth == 0 || tile.rows == 0) continue;
+          const unsigned what = tb200_tc::instruction<PAIR>(!std::is_same<T, f16>::value, a_mn, b_mn, columns_of(tile));
+          unsigned set = 0, d = 0;
+          bool begun = false;      // these sums are
+          for (int k = 0, segment = 0, block = 0; k < tile.depth; ++count) {
+            if (!begun) {
+              set = made & 1;
+              d = tmem + set * BN;
+              good = await<PAIR>(&sh.taken[set], (made / 2 & 1) ^ 1, &sh.dead, p.hdr);
+              if (!good) break;
+              ++made;
+              tb200_tc::fence_after_sync();
+            }
+            const unsigned stage = count % STAGES, from = base + stage * Shared::STAGE;
+            good = await<PAIR>(&sh.full[stage], count / STAGES & 1, &sh.dead, p.hdr);
+            if (!good) break;
+            const int valid = tile.depth - k < DEEP ? tile.depth - k : DEEP, steps = (valid + 15) / 16;
+            if (is_tail(tile, k)) {
+              good = await<PAIR>(&sh.ready[stage], tails >> stage & 1, &sh.dead, p.hdr);
+              if (!good) break;
+              tails ^= 1u << stage;
+            }
+            tb200_tc::fence_after_sync();
+            if (tb200_tc::elected()) {
+              const unsigned long long a = tb200_tc::operand(from, a_mn, CHUNK), b = tb200_tc::operand(from + A_BYTES, b_mn, CHUNK);
+#pragma unroll
+              for (int i = 0; i < DEEP / 16; ++i)
+                if (i < steps) tb200_tc::multiply<PAIR>(d, a + i / 4 * a_jump + i % 4 * a_step, b + i / 4 * b_jump + i % 4 * b_step, what, begun || i > 0);
+              tb200_tc::commit<PAIR>(&sh.empty[stage]);
+            }
+            __syncwarp();
+            begun = true;
+            if ((k += DEEP) >= tile.depth && ++segment < p.segments) k = 0;
+            if (k >= tile.depth || (FINE && ++block % GROUP == 0)) {
+              if (tb200_tc::elected()) tb200_tc::commit<PAIR>(&sh.made[set]);
+              __syncwarp();
+              begun = false;
+            }
+          }
+        }
+        if (tb200_tc::elected()) { tb200_tc::commit<PAIR>(&sh.done); outlast(&sh.done, 0); }
         __syncwarp();
       }
-      if (tb200_tc::elected()) { tb200_tc::commit<PAIR>(&sh.done); outlast(&sh.done, 0); }
-      __syncwarp();
-    }
-  } else if (MODE == BY_EXPERTS && warp == CLEARS) {
-    unsigned count = 0, e = 0, tails = 0;
-    bool good = true;
-    for (unsigned t = blockIdx.x / CTAS; good && t < turn.count; t += step) {
-      const product_tile tile = tile_of(t, e);
-      if (tile.rows == 0) continue;
-      const unsigned blocks = (unsigned)(tile.depth + DEEP - 1) / DEEP;
-      const bool has = blocks > 0 && is_tail(tile, (int)(blocks - 1) * DEEP);
-      for (int segment = 0; good && segment < p.segments; ++segment) {
-        const unsigned stage = (count + blocks - 1) % STAGES;
-        count += blocks;
-        if (!has) continue;
-        good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr);
-        if (!good) break;
-        tails ^= 1u << stage;
-        clear_tail(stage, tile.depth - (int)(blocks - 1) * DEEP, 2 + (columns_of(tile) / CTAS + 63) / 64);
-        if (lane == 0) {
-          if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.ready[stage]));
-          else tb200::mbar_arrive(&sh.ready[stage]);
+    } else if (MODE == BY_EXPERTS && warp == CLEARS) {
+      unsigned count = 0, e = 0, tails = 0;
+      bool good = true;
+      for (unsigned t = blockIdx.x / CTAS; good && t < turn.count; t += step) {
+        const product_tile tile = tile_of(t, e);
+        if (tile.rows == 0) continue;
+        const unsigned blocks = (unsigned)(tile.depth + DEEP - 1) / DEEP;
+        const bool has = blocks > 0 && is_tail(tile, (int)(blocks - 1) * DEEP);
+        for (int segment = 0; good && segment < p.segments; ++segment) {
+          const unsigned stage = (count + blocks - 1) % STAGES;
+          count += blocks;
+          if (!has) continue;
+          good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr);
+          if (!good) break;
+          tails ^= 1u << stage;
+          clear_tail(stage, tile.depth - (int)(blocks - 1) * DEEP, 2 + (columns_of(tile) / CTAS + 63) / 64);
+          if (lane == 0) {
+            if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.ready[stage]));
+            else tb200::mbar_arrive(&sh.ready[stage]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
     }
   } else {
+    if constexpr (FINE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WRITERS_REGISTERS));
     // a writer has the 32 lanes that warp % 4 may read, and every other 32 columns; GATED: of these it finishes 16, of both halves
     unsigned made = 0, e = 0;
     bool good = true;
@@ -492,45 +511,26 @@ __global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(con
     for (unsigned t = blockIdx.x / CTAS; t < turn.count; t += step) {
       const product_tile tile = tile_of(t, e);
       if (tile.rows == 0) continue;
-      const unsigned set = made & 1, d = tmem + (quarter * 32u << 16) + set * BN;
       const int f = tile.feature + (int)rank * OWN + within, room = p.features - f;      // the first lane's feature, and how many there are from there on
       const bool there = lane < room;
       const size_t width = p.features, both = GATED ? 2 * width : width;
       float bias = 0.f;
       if (MODE == BY_ROWS && p.bias && there) bias = to_f32(p.bias[tile.e * both + half * width + f + lane]);
-      bool waited = tile.depth == 0;
-      for (int c = warp / 4 * 32;; c += 64) {
-        const bool any = c < tile.rows;
+      columns_in<T, PUT> residual;
+      columns_in<O, 32> old;
+      // what results of columns c on are added to is asked for
+      auto request = [&](int c) {
         const int mine = c + half * 16;
-        columns_in<T, PUT> residual;
-        columns_in<O, 32> old;
-        O* const to = static_cast<O*>(p.matrix) + ((size_t)tile.e * p.others + tile.other + c) * width + f;
-        if (MODE == BY_ROWS && p.residual && any) residual.request(p.residual + ((size_t)tile.row + mine) * p.residual_stride + f, p.residual_stride, tile.rows - mine, lane, room, p.wide_residual);
-        if (MODE == BY_EXPERTS && p.accumulate && any) old.request(to, width, tile.rows - c, lane, room, p.wide_out);
-        if (!waited) {
-          if (good) good = await<PAIR>(&sh.made[set], made / 2 & 1, &sh.dead, p.hdr);
-          ++made;
-          waited = true;
-          tb200_tc::fence_after_sync();
-        }
-        float v[32];
-        if (any && tile.depth && good) {
-          tb200_tc::tmem_load(v, d + c);
-          tb200_tc::tmem_load_wait();
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = good ? 0.f : __int_as_float(0x7fffffff);
-        }
-        if (c + 64 >= tile.rows && tile.depth && good) {      // the last of them: the next sums may be made there
-          tb200_tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) {
-            if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.taken[set]));
-            else tb200::mbar_arrive(&sh.taken[set]);
-          }
-        }
-        if (!any) break;
-        if (MODE == BY_ROWS) {
+        if (c >= tile.rows) return;
+        if (MODE == BY_ROWS && p.residual)
+          residual.request(p.residual + ((size_t)tile.row + mine) * p.residual_stride + f, p.residual_stride, tile.rows - mine, lane, room, p.wide_residual);
+        if (MODE == BY_EXPERTS && p.accumulate)
+          old.request(static_cast<O*>(p.matrix) + ((size_t)tile.e * p.others + tile.other + c) * width + f, width, tile.rows - c, lane, room, p.wide_out);
+      };
+      // the sums of 32 columns become results
+      auto finish = [&](int c, float (&v)[32]) {
+        const int mine = c + half * 16;
+        if constexpr (MODE == BY_ROWS) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] += bias;
           if (p.before) put_columns(p.before + ((size_t)tile.row + c) * both + half * width + f, both, tile.rows - c, v, lane, room, p.wide_out, room_of);
@@ -562,13 +562,75 @@ __global__ void __launch_bounds__(TC_THREADS<MODE>, 1) expert_product_kernel(con
           }
           if (p.residual) residual.add(w, lane, p.wide_residual, room_of);
           put_columns(p.out + ((size_t)tile.row + mine) * width + f, width, tile.rows - mine, w, lane, room, p.wide_out, room_of);
-        } else if (!p.accumulate) {
-          put_columns(to, width, tile.rows - c, v, lane, room, p.wide_out, room_of);
-        } else if (tile.depth || !good) {      // (an expert without rows adds nothing)
-          old.add(v, lane, p.wide_out, room_of);
+        } else {
+          O* const to = static_cast<O*>(p.matrix) + ((size_t)tile.e * p.others + tile.other + c) * width + f;
+          if (p.accumulate && tile.depth == 0 && good) return;      // (an expert without rows adds nothing)
+          if (p.accumulate) old.add(v, lane, p.wide_out, room_of);
           put_columns(to, width, tile.rows - c, v, lane, room, p.wide_out, room_of);
         }
-        if (c + 64 >= tile.rows) break;
+      };
+      auto await_sums = [&] {
+        if (good) good = await<PAIR>(&sh.made[made & 1], made / 2 & 1, &sh.dead, p.hdr);
+        tb200_tc::fence_after_sync();
+      };
+      auto sums_taken = [&] {      // the next ones may be made there
+        tb200_tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0 && good) {
+          if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.taken[made & 1]));
+          else tb200::mbar_arrive(&sh.taken[made & 1]);
+        }
+        ++made;
+      };
+      const unsigned lanes = quarter * 32u << 16;
+      bool waited = tile.depth == 0;
+      if constexpr (FINE) {
+        // the sums of all groups, added up in registers, take the last one's place
+        constexpr int N = BN / 64;
+        const int groups = ((tile.depth + DEEP - 1) / DEEP * p.segments + GROUP - 1) / GROUP;
+        if (groups > 1) {
+          float sums[N][32];
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sums[i][j] = 0.f;
+          for (int g = 0; g < groups; ++g) {
+            await_sums();
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const int c = warp / 4 * 32 + i * 64;
+              if (c >= tile.rows || !good) continue;
+              float v[32];
+              tb200_tc::tmem_load(v, tmem + lanes + (made & 1) * BN + c);
+              tb200_tc::tmem_load_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sums[i][j] += v[j];
+            }
+            if (g + 1 < groups) sums_taken();
+          }
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (warp / 4 * 32 + i * 64 < tile.rows) tb200_tc::tmem_store(sums[i], tmem + lanes + (made & 1) * BN + warp / 4 * 32 + i * 64);
+          tb200_tc::tmem_store_wait();
+          waited = true;
+        }
+      }
+      for (int c = warp / 4 * 32;; c += 64) {
+        const bool any = c < tile.rows, last = c + 64 >= tile.rows;
+        request(c);
+        if (!waited) await_sums();
+        waited = true;
+        float v[32];
+        if (any && tile.depth && good) {
+          tb200_tc::tmem_load(v, tmem + lanes + (made & 1) * BN + c);
+          tb200_tc::tmem_load_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = good ? 0.f : __int_as_float(0x7fffffff);
+        }
+        if (last && tile.depth) sums_taken();
+        if (any) finish(c, v);
+        if (last) break;
       }
     }
     if (MODE == BY_ROWS) clear_others(p, s, (size_t)blockIdx.x * WRITERS * 32 + threadIdx.x, (size_t)gridDim.x * WRITERS * 32);
@@ -982,7 +1044,7 @@ cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_
   const size_t tiles = MODE == BY_ROWS ? across * most_row_tiles(p.m, p.experts, BN) : across * (((size_t)p.others + BN - 1) / BN) * p.experts;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(product_grid(tiles * 4 * CTAS, 1) / CTAS * CTAS);      // (four: the parts of a tile)
-  cfg.blockDim = dim3(TC_THREADS<MODE>);
+  cfg.blockDim = dim3(TC_THREADS<MODE, O>);
   cfg.dynamicSmemBytes = Shared::bytes(p.experts);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
