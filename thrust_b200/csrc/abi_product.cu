@@ -876,14 +876,22 @@ __global__ void __launch_bounds__(SUM_BLOCK) join_sums_kernel(const float* __res
 }
 
 // Rows that are not made of whole aligned 16-byte pieces, or whose distances are not, laid out so that they are: `halves` pieces of `width` elements, each on a
-// boundary.
+// boundary.  With offsets, the matrices of experts without rows are left out: nobody reads them.
+struct which_experts {
+  const void* offsets;
+  bool wide;
+  int m;
+  __device__ __forceinline__ bool has_rows(size_t e) const { return !offsets || read_offset(offsets, wide, (unsigned)e + 1, m) > read_offset(offsets, wide, (unsigned)e, m); }
+};
 template <class T>
-__global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ from, size_t each, size_t outer, size_t stride, size_t rows, unsigned halves, unsigned width, T* __restrict__ to) {
+__global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ from, size_t each, size_t outer, size_t stride, size_t rows, unsigned halves, unsigned width, which_experts used,
+                                                        T* __restrict__ to) {
   constexpr int V = 16 / sizeof(T);
   const unsigned wide = (width + V - 1) / V;
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * halves * wide) return;
   const size_t line = i / wide, row = line / halves, c = (i - line * wide) * V;
+  if (!used.has_rows(row / each)) return;
   const T* const f = from + row / each * outer + row % each * stride + (line - row * halves) * width + c;
   union { T at[V]; uint4 all; } v;
 #pragma unroll
@@ -894,11 +902,12 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ fr
 // The same rows as three planes of 16 bits, [matrix][plane][row][halves][wide], zeros behind a half's width.  A number that is not finite is in the first plane alone; one that
 // would be rounded to infinity is cut off instead.
 __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ from, size_t each, size_t outer, size_t stride, size_t rows, unsigned halves, unsigned width, unsigned wide,
-                                                         bf16* __restrict__ to) {
+                                                         which_experts used, bf16* __restrict__ to) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
   const unsigned across = wide / 8;
   if (i >= rows * halves * across) return;
   const size_t line = i / across, row = line / halves, matrix = row / each, c = (i - line * across) * 8, h = line - row * halves;
+  if (!used.has_rows(matrix)) return;
   const float* const f = from + matrix * outer + (row - matrix * each) * stride + h * width + c;
   union { unsigned short at[8]; uint4 all; } v[PLANES];
 #pragma unroll
@@ -1001,14 +1010,14 @@ struct matrices {
   size_t packed_bytes() const { return fits() ? 0 : tb200::align_up(all_rows() * halves * (split ? PLANES * wide() * 2 : pieces() * 16), 256); }
 };
 // into `room`, which is moved on; nothing where they fit
-template <class T> cudaError_t pack(matrices& x, char*& room, cudaStream_t stream) {
+template <class T> cudaError_t pack(matrices& x, char*& room, which_experts used, cudaStream_t stream) {
   if (x.fits() || x.width == 0 || x.all_rows() == 0) return cudaSuccess;
   const size_t bytes = x.packed_bytes(), pieces = x.all_rows() * x.halves * (x.split ? x.wide() / 8 : x.pieces());
   if ((pieces + 255) / 256 > 0x7fffffffull) return cudaErrorInvalidValue;
   const unsigned grid = (unsigned)((pieces + 255) / 256);
   if constexpr (sizeof(T) == 4) {
     if (x.split) {
-      split_rows_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), (unsigned)x.wide(),
+      split_rows_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), (unsigned)x.wide(), used,
                                                   reinterpret_cast<bf16*>(room));
       x.width = x.stride = x.halves * x.wide();
       x.count = (x.count ? x.count : 1) * PLANES;
@@ -1017,7 +1026,7 @@ template <class T> cudaError_t pack(matrices& x, char*& room, cudaStream_t strea
     }
   }
   if (x.bytes == sizeof(T)) {
-    pack_rows_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), reinterpret_cast<T*>(room));
+    pack_rows_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), used, reinterpret_cast<T*>(room));
     x.width = x.stride = x.halves * x.pieces() * 16 / sizeof(T);
   }
   x.at = room;
@@ -1040,6 +1049,12 @@ cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_
   auto kernel = expert_product_kernel<T, O, MODE, PAIR, GATED, BN, STAGES>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shared::bytes(MOST_EXPERTS));
   if (e != cudaSuccess) return e;
+  if constexpr (sizeof(O) == 4) {      // the writers would wait for registers that the CTA does not have
+    static thread_local int registers = 0;
+    cudaFuncAttributes has;
+    if (registers == 0 && cudaFuncGetAttributes(&has, kernel) == cudaSuccess) registers = (has.numRegs + 7) / 8 * 8;
+    if (registers * 3 < 2 * WRITERS_REGISTERS + OTHERS_REGISTERS) return cudaErrorInvalidKernelImage;
+  }
   const size_t across = ((size_t)p.features + WIDE - 1) / WIDE;
   const size_t tiles = MODE == BY_ROWS ? across * most_row_tiles(p.m, p.experts, BN) : across * (((size_t)p.others + BN - 1) / BN) * p.experts;
   cudaLaunchConfig_t cfg = {};
@@ -1192,8 +1207,8 @@ TB200_API int tb200_expert_product(const void* d_rows, size_t rows_stride, const
       p.hdr = static_cast<tb200::ws_header*>(d_ws);
       set_planes(p, split);
       char* room = static_cast<char*>(d_ws) + sizeof(tb200::ws_header);
-      cudaError_t e = pack<T>(w, room, stream);
-      if (e == cudaSuccess) e = pack<T>(x, room, stream);
+      cudaError_t e = pack<T>(w, room, {d_offsets, p.wide, p.m}, stream);
+      if (e == cudaSuccess) e = pack<T>(x, room, {}, stream);
       return (int)(e == cudaSuccess ? product_by_rows<T>(w, x, p, stream) : e);
     });
   });
@@ -1222,9 +1237,9 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
       float* const partial = reinterpret_cast<float*>(room);
       room += sums;
       cudaError_t e = cudaSuccess;
-      e = pack<T>(w, room, stream);
-      if (e == cudaSuccess) e = pack<T>(x, room, stream);
-      if (e == cudaSuccess) e = pack<T>(d, room, stream);
+      e = pack<T>(w, room, {d_offsets, sizeof(iv) == 8, (int)n}, stream);
+      if (e == cudaSuccess) e = pack<T>(x, room, {}, stream);
+      if (e == cudaSuccess) e = pack<T>(d, room, {}, stream);
       if (e != cudaSuccess) return (int)e;
       product_plan<T> p = {};
       p.offsets = d_offsets;
