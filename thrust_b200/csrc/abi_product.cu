@@ -14,8 +14,8 @@ constexpr size_t MOST_ROWS = (1ull << 31) - 1024, MOST_CHANNELS = 1ull << 24;
 
 // ---------------------------------------------------------------------------------------------- activations
 // silu(x) = x s(x) with s(x) = 1 / (1 + exp(-x)); gelu(x) = x P(x) with P the normal distribution.  s and 1 - s are made of exp(-|x|), which cannot overflow
-// and keeps the smaller of the two good where it is tiny; P comes from erfc, which does not cancel where P is small.  FAST: s is good to a few 2^-22 (and
-// 2^-24 |x| for the exponential's argument) of itself, for results that are rounded to 16 bits.
+// and keeps the smaller of the two good where it is tiny; P comes from erfc, which does not cancel where P is small.  FAST: s and P are good to a few 2^-22 (and
+// 2^-24 |x|, 2^-23 x^2 for the exponential's argument) of themselves, for results that are rounded to 16 bits.
 enum : int { ACT_NONE = TB200_ACT_NONE, ACT_SILU = TB200_ACT_SILU, ACT_GELU = TB200_ACT_GELU, ACT_GATED = TB200_ACT_GATED };
 struct sigmoid_pair { float s, other; };
 template <bool FAST> __device__ __forceinline__ sigmoid_pair sigmoid(float x) {
@@ -32,13 +32,31 @@ template <bool FAST> __device__ __forceinline__ sigmoid_pair sigmoid(float x) {
   p.other = x >= 0.f ? e * r : r;
   return p;
 }
-__device__ __forceinline__ float normal_below(float x) { return 0.5f * erfcf(-0.70710678118654752f * x); }
-template <bool FAST> __device__ __forceinline__ float activated(float x, int kind) { return kind == ACT_SILU ? x * sigmoid<FAST>(x).s : kind == ACT_GELU ? x * normal_below(x) : x; }
+// P(x); FAST: from the Chebyshev fit of erfc in Numerical Recipes (Press et al., 6.2), good to 1.2e-7 of itself
+template <bool FAST> __device__ __forceinline__ float normal_below(float x) {
+  if (!FAST) return 0.5f * erfcf(-0.70710678118654752f * x);
+  const float z = 0.70710678118654752f * fabsf(x), t = __fdividef(1.f, fmaf(0.5f, z, 1.f));
+  float q = 0.17087277f;
+  q = fmaf(q, t, -0.82215223f);
+  q = fmaf(q, t, 1.48851587f);
+  q = fmaf(q, t, -1.13520398f);
+  q = fmaf(q, t, 0.27886807f);
+  q = fmaf(q, t, -0.18628806f);
+  q = fmaf(q, t, 0.09678418f);
+  q = fmaf(q, t, 0.37409196f);
+  q = fmaf(q, t, 1.00002368f);
+  q = fmaf(q, t, -1.26551223f);
+  float e;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(1.4426950408889634f * fmaf(-z, z, q)));
+  const float tail = 0.5f * t * e;      // P(-|x|)
+  return x >= 0.f ? 1.f - tail : tail;
+}
+template <bool FAST> __device__ __forceinline__ float activated(float x, int kind) { return kind == ACT_SILU ? x * sigmoid<FAST>(x).s : kind == ACT_GELU ? x * normal_below<FAST>(x) : x; }
 // and with its slope
 struct act_slope { float y, slope; };
 template <bool FAST> __device__ __forceinline__ act_slope with_slope(float x, int kind) {
   if (kind == ACT_SILU) { const sigmoid_pair p = sigmoid<FAST>(x); return {x * p.s, p.s * fmaf(x, p.other, 1.f)}; }
-  const float below = normal_below(x);
+  const float below = normal_below<FAST>(x);
   return {x * below, fmaf(x * 0.39894228040143268f, expf(-0.5f * x * x), below)};
 }
 
@@ -93,26 +111,49 @@ template <class T> struct product_plan {
 };
 struct product_tile { unsigned e; int row, rows, feature, other, depth; };
 
-// Tile t.  By rows: an expert's rows in tiles of equal height (multiples of UNIT), all features of one before the next.  `e`: the expert of the
-// last tile asked for, from which the search goes on.
-template <int MODE, int WIDE, int BN, int UNIT, class T> __device__ __forceinline__ product_tile tile_at(const product_plan<T>& p, const spans& s, unsigned t, unsigned& e) {
+// Division by what is the same throughout a kernel: the upper half of a product with ceil(2^32 / d), which is the quotient or one more.
+struct divisor {
+  unsigned d, inverse;
+  __device__ __forceinline__ explicit divisor(unsigned by) : d(by), inverse(by > 1 ? (unsigned)((0x100000000ull + by - 1) / by) : 0) {}
+  __device__ __forceinline__ unsigned into(unsigned n, unsigned& rest) const {
+    unsigned q = d > 1 ? __umulhi(n, inverse) : n;
+    rest = n - q * d;
+    if (rest >= d) { --q; rest += d; }      // (below zero)
+    return q;
+  }
+};
+// How tiles of WIDE features follow one another.
+template <int MODE, int BN> struct tiling {
+  divisor across, each;      // tiles of an index's features; by experts: tiles of an expert
+  template <class T> __device__ __forceinline__ tiling(const product_plan<T>& p, int wide)
+      : across((unsigned)(p.features + wide - 1) / wide), each(MODE == BY_ROWS ? 1u : across.d * ((unsigned)(p.others + BN - 1) / BN)) {}
+};
+
+// Tile t, asked for by whole warps.  By rows: an expert's rows in tiles of equal height (multiples of UNIT), all features of one before the next.  `e`: the expert of the
+// last tile asked for, from which the search goes on, 32 experts at a time.
+template <int MODE, int BN, int UNIT, class T>
+__device__ __forceinline__ product_tile tile_at(const product_plan<T>& p, const spans& s, const tiling<MODE, BN>& g, int wide, unsigned t, unsigned& e) {
   product_tile r;
-  const unsigned across = (unsigned)(p.features + WIDE - 1) / WIDE;
+  unsigned in;
   if (MODE == BY_ROWS) {
-    const unsigned index = t / across;
-    while (index >= (unsigned)s.tiles[e + 1]) ++e;
-    const int n = rows_of(s, e), parts = (n + BN - 1) / BN, tall = ((n + parts - 1) / parts + UNIT - 1) / UNIT * UNIT, part = (int)(index - s.tiles[e]);
+    const unsigned index = g.across.into(t, in), lane = threadIdx.x % 32;
+    for (unsigned found = 0; !found;) {
+      const unsigned at = e + 1 + lane;
+      found = __ballot_sync(tb200::FULL_MASK, index < (unsigned)s.tiles[at < p.experts ? at : p.experts]);
+      e += found ? (unsigned)__ffs(found) - 1 : 32;
+    }
+    const int n = rows_of(s, e), parts = (n + BN - 1) / BN, tall = ((parts == 1 ? n : (n + parts - 1) / parts) + UNIT - 1) / UNIT * UNIT, part = (int)(index - s.tiles[e]);
     r.e = e;
-    r.feature = (int)(t - index * across) * WIDE;
+    r.feature = (int)in * wide;
     r.row = s.at[e] + part * tall;
     r.rows = n - part * tall < tall ? n - part * tall : tall;
     r.other = 0;
     r.depth = p.k;
   } else {
-    const unsigned down = (unsigned)(p.others + BN - 1) / BN, each = across * down;
-    r.e = t / each;
-    const unsigned in = t - r.e * each, o = in / across;
-    r.feature = (int)(in - o * across) * WIDE;
+    r.e = g.each.into(t, in);
+    unsigned f;
+    const unsigned o = g.across.into(in, f);
+    r.feature = (int)f * wide;
     r.other = (int)o * BN;
     r.rows = p.others - r.other < BN ? p.others - r.other : BN;
     r.row = s.at[r.e];
@@ -340,11 +381,12 @@ __global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(
   tb200_tc::fence_after_sync();
   const unsigned tmem = sh.tmem, step = gridDim.x / CTAS;
   const turns turn(tiles_of<MODE, WIDE, BN>(p, s), step, MODE == BY_ROWS ? 4 : 2);
+  const tiling<MODE, BN> follow(p, WIDE);
   // columns of a tile's instructions; of these each CTA brings its share of B
   const int unit = MODE == BY_EXPERTS && p.b_split ? 64 * CTAS : UNIT;
   auto columns_of = [&](const product_tile& tile) { return (tile.rows + unit - 1) / unit * unit; };
   auto tile_of = [&](unsigned t, unsigned& e) {
-    product_tile tile = tile_at<MODE, WIDE, BN, UNIT>(p, s, turn.tile(t), e);
+    product_tile tile = tile_at<MODE, BN, UNIT>(p, s, follow, WIDE, turn.tile(t), e);
     turn.cut(t, unit, MODE == BY_ROWS ? tile.row : tile.other, tile.rows);
     return tile;
   };
@@ -524,7 +566,7 @@ __global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(
         if (c >= tile.rows) return;
         if (MODE == BY_ROWS && p.residual)
           residual.request(p.residual + ((size_t)tile.row + mine) * p.residual_stride + f, p.residual_stride, tile.rows - mine, lane, room, p.wide_residual);
-        if (MODE == BY_EXPERTS && p.accumulate)
+        if (MODE == BY_EXPERTS && p.accumulate && tile.depth)
           old.request(static_cast<O*>(p.matrix) + ((size_t)tile.e * p.others + tile.other + c) * width + f, width, tile.rows - c, lane, room, p.wide_out);
       };
       // the sums of 32 columns become results
@@ -549,12 +591,16 @@ __global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(
 #pragma unroll
             for (int j = 0; j < 32; ++j) w[j] = v[j];
           }
-          if (kind == ACT_SILU) {
 #pragma unroll
-            for (int j = 0; j < PUT; ++j) w[j] = activated<sizeof(T) == 2>(w[j], ACT_SILU);
-          } else if (kind == ACT_GELU) {
+          for (int part = 0; part < PUT; part += 8) {      // (few rows: not for columns that are not there)
+            if (mine + part >= tile.rows) break;
+            if (kind == ACT_SILU) {
 #pragma unroll
-            for (int j = 0; j < PUT; ++j) w[j] = activated<sizeof(T) == 2>(w[j], ACT_GELU);
+              for (int j = part; j < part + 8; ++j) w[j] = activated<sizeof(T) == 2>(w[j], ACT_SILU);
+            } else if (kind == ACT_GELU) {
+#pragma unroll
+              for (int j = part; j < part + 8; ++j) w[j] = activated<sizeof(T) == 2>(w[j], ACT_GELU);
+            }
           }
           if constexpr (GATED) {
 #pragma unroll
@@ -688,13 +734,15 @@ __global__ void __launch_bounds__(FMA_THREADS, 3) expert_product_f32_kernel(cons
   // tiles are as wide as the features they have: half as wide where they are of two halves
   const unsigned across = (unsigned)(p.features + (gated ? 63 : 127)) / (gated ? 64 : 128);
   const unsigned tiles = gated ? across * (unsigned)s.tiles[p.experts] : tiles_of<MODE, 128, BN>(p, s);
+  const tiling<MODE, BN> follow(p, gated ? 64 : 128);
   // this lane's features (of either 64) and rows
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, x0 = warp % ACROSS * 8 * FP, y0 = warp / ACROSS * 32;
   auto x_of = [&](int i) { return x0 + (A_BY_K ? lane % 8 * FP + i : lane % 8 + 8 * i); };
   auto y_of = [&](int j) { return y0 + (B_BY_K ? lane / 8 * 4 + j % 4 + j / 4 * 16 : lane / 8 + 4 * j); };
   unsigned e = 0;
   for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const product_tile tile = MODE == BY_ROWS && gated ? tile_at<MODE, 64, BN, 1>(p, s, t, e) : tile_at<MODE, 128, BN, 1>(p, s, t, e);
+    const product_tile tile = tile_at<MODE, BN, 1>(p, s, follow, gated ? 64 : 128, t, e);
+    if (MODE == BY_EXPERTS && tile.depth == 0 && p.accumulate) continue;      // nothing is added
     const int wide = p.features - tile.feature < (gated ? 64 : 128) ? p.features - tile.feature : gated ? 64 : 128;      // features of the tile, gated of either half
     // this thread's pieces of a stage: where they lie in the tile, where the first comes from (at k = 0), of A also the first of the upper 64 features
     constexpr int PA = fma_tile<128, A_BY_K>::PIECES, PB = fma_tile<BN, B_BY_K>::PIECES;
