@@ -349,6 +349,11 @@ constexpr unsigned A_PLANES = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, B
 // By experts the contraction ends where the expert's rows do, in the middle of a box: what the box has of the next rows is cleared in shared memory, up to
 // the next 16, where the instructions end.  Such a box is counted by the barrier `tail` of the CTA that it is for, where a warp of its own clears it as soon as it is there and
 // says that it is ready.
+//
+// Large products are bound by the power limit: 131072 bf16 rows of 2048 to 1536, gated, with what is kept, through 128 experts: 780 us (1020 TFLOP/s at 1.0 to 1.2 GHz, 79 % of the
+// cycles the tensor cores'; without results written 680), 16382 f16 rows of 4096 to 2048 through eight 255 us (1080), 98304 rows' gradients 1024 to 2048 through 64
+// 775 us for both products (1040).  Few rows are bound by the matrices' bytes: 132 rows of 2048 to 2048 through 64 experts 76 us with the call (6200 GB/s).  What had
+// counted before: asking for boxes and issuing instructions lane by lane (950 us for the first), stages of 64 (884), single CTAs with tiles of 128 x 256 (951).
 template <class T, class O, int MODE, bool PAIR, bool GATED, int BN, int STAGES>
 __global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const product_plan<T> p) {
   using Shared = tc_shared<PAIR, GATED, BN, STAGES>;
@@ -695,7 +700,8 @@ __global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(
 // Products of 32-bit rows are made by the ordinary units: the matrix instructions round their operands to 11 bits or fewer.  Tiles of 128 features (gated: 64
 // of each half) x BN rows; a lane has 2 FP features x 8 rows, eight lanes by four, two features side by side in its multiply-adds (f32x2).  Operands go 16 bytes at a time,
 // by asynchronous copies, into a ring of stages of shared memory, and lie there as they lie in memory: by k (rows of features or of others), or by m (rows of
-// k), of which a lane takes two k at a time.  Bound by the multiply-adds.
+// k), of which a lane takes two k at a time.  Bound by the multiply-adds: 2048 rows of 1000 to 1501 through six experts took 176 us (35 TFLOP/s; tiles of
+// 128 x 128 read element by element 298), which the tensor cores take 61 for.  They have the products of few rows and of few channels.
 constexpr int FMA_THREADS = 128, FMA_DEEP = 16, FMA_STAGES = 4;
 template <int WIDE, bool BY_K> struct fma_tile {      // an operand's part of a stage
   static constexpr int STRIDE = BY_K ? WIDE + 4 : FMA_DEEP + 4, PIECES = WIDE * FMA_DEEP / 4 / FMA_THREADS;
@@ -878,7 +884,7 @@ __global__ void __launch_bounds__(FMA_THREADS, 3) expert_product_f32_kernel(cons
 
 // ---------------------------------------------------------------------------------------------- the smaller parts
 // The gradient of bias: the sums of each expert's rows of dout.  A CTA has 32 V features of one of `parts` pieces of an expert's rows; its warps take rows in turn and
-// meet in shared memory, parts meet in a second kernel, always in the same order.
+// meet in shared memory, parts meet in a second kernel, always in the same order.  Bound by latency: 8198 bf16 rows of 1280 for 16 experts 10 us and 4, beside the products.
 constexpr int SUM_BLOCK = 256;
 template <class T, int V>
 __global__ void __launch_bounds__(SUM_BLOCK) row_sums_kernel(const T* __restrict__ x, size_t stride, const void* __restrict__ offsets, bool wide, unsigned experts, int m, int features,
@@ -976,7 +982,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict
 }
 
 // dbefore = dout * the activation's slope; gated with out = act(a) b: da = dout b act'(a), db = dout act(a).  Bound by the bytes; a thread asks for two places' pieces before
-// it works on either.
+// it works on either.  98304 bf16 rows of 1024, gated: 156 us with the call (6450 GB/s; one place at a time, and an exponential each for value and slope, 195).
 template <class T, int V>
 __global__ void __launch_bounds__(256) activation_grad_kernel(const T* __restrict__ dout, size_t stride, const T* __restrict__ before, size_t n, unsigned pieces, bool gated, int kind,
                                                               T* __restrict__ dbefore) {
