@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(
             }
           }
         }
-        if (tb200_tc::elected()) { tb200_tc::commit<PAIR>(&sh.done); outlast(&sh.done, 0); }
+        if (tb200_tc::elected()) { tb200_tc::commit_here<PAIR>(&sh.done); outlast(&sh.done, 0); }
         __syncwarp();
       }
     } else if (MODE == BY_EXPERTS && warp == CLEARS) {

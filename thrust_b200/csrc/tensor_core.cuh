@@ -82,6 +82,12 @@ template <bool PAIR> __device__ __forceinline__ void commit(unsigned long long* 
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tb200::smem_addr(bar)) : "memory");
 }
 
+// the same on this CTA's alone
+template <bool PAIR> __device__ __forceinline__ void commit_here(unsigned long long* bar) {
+  if (PAIR) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tb200::smem_addr(bar)) : "memory");
+  else commit<false>(bar);
+}
+
 // ---------------------------------------------------------------- two CTAs
 __device__ __forceinline__ unsigned rank_in_pair() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ unsigned first_ones(const void* p) {      // the first CTA's counterpart of something in shared memory
