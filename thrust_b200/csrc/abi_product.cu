@@ -223,14 +223,17 @@ __device__ __forceinline__ bool withheld(unsigned, unsigned) { return false; }
 #endif
 
 constexpr int DEEP = 128, GROUP = 6;          // of the contraction, a stage; stages
-constexpr int WRITERS = 8, BRINGS = WRITERS, MULTIPLIES = WRITERS + 1, CLEARS = WRITERS + 2;      // warps that write results, that bring operands, that multiply, that clear boxes' ends (by experts)
-// 32-bit results: the writers hold 128 sums a thread, of registers that the other four warps hand over (launched with 168 a thread; 2 x 216 + 72 = 3 x 168)
-template <int MODE, class O> constexpr int TC_THREADS = sizeof(O) == 4 ? 384 : (WRITERS + (MODE == BY_EXPERTS ? 3 : 2)) * 32;
+// Warps: WRITERS that write results, then one that brings operands, one that multiplies, and (by experts) one that clears boxes' ends.  Few rows: four writers, and two CTAs a SM.
+// 32-bit results: the writers hold 128 sums a thread, of registers that the other four warps hand over (launched with 168 a thread; 2 x 216 + 72 = 3 x 168).
+template <int MODE, class O, bool PAIR> struct tc_warps {
+  static constexpr bool FINE = sizeof(O) == 4, FEW = MODE == BY_ROWS && !PAIR && !FINE;
+  static constexpr int WRITERS = FEW ? 4 : 8, THREADS = FINE ? 384 : (WRITERS + (MODE == BY_EXPERTS ? 3 : 2)) * 32, A_SM = FEW ? 2 : 1;
+};
 constexpr int WRITERS_REGISTERS = 216, OTHERS_REGISTERS = 72;
 constexpr unsigned CHUNK = 64 * DEEP * 2;     // 64 neighbours by 128 of the other axis
 constexpr unsigned A_BYTES = 2 * CHUNK;       // a CTA's 128 features
 
-template <bool PAIR, bool GATED, int BN, int STAGES> struct tc_shared {
+template <bool PAIR, int WRITERS, int BN, int STAGES> struct tc_shared {
   static constexpr unsigned B_CHUNK = BN * 128 / (PAIR ? 2 : 1), STAGE = A_BYTES + 2 * B_CHUNK, COLUMNS = 2 * BN;
   static_assert(COLUMNS <= 512, "two sets of sums in tensor memory");
   alignas(16) unsigned char turn[WRITERS][2048];      // where a writer's results are turned round
@@ -338,7 +341,7 @@ constexpr unsigned A_PLANES = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, B
 // PAIR: two CTAs have a tile of twice as many features, half of its rows' operands each, and instructions that read both's shared memory, which the first
 // issues: 64 KB instead of 96 come from L2 for 256 features x 256 rows x 64.
 //
-// One warp keeps STAGES boxes of A and B on their way by the copy engine, one issues the matrix instructions as they come, eight take the sums of the last
+// One warp keeps STAGES boxes of A and B on their way by the copy engine, one issues the matrix instructions as they come, the writers take the sums of the last
 // tile from tensor memory, while the next one's are made in its other half, and write them.  Sums are 32 bits from first to last; they
 // are rounded once, where they are stored, after bias, activation and residual.  The matrix instructions cut off what they add (1.2e-7 of the results for each
 // stage, and always the same way), which results of 16 bits do not see.  32-bit results (FINE) are made of sums over GROUP stages, which the writers add up in registers,
@@ -355,10 +358,12 @@ constexpr unsigned A_PLANES = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, B
 // 775 us for both products (1040).  Few rows are bound by the matrices' bytes: 132 rows of 2048 to 2048 through 64 experts 76 us with the call (6200 GB/s).  What had
 // counted before: asking for boxes and issuing instructions lane by lane (950 us for the first), stages of 64 (884), single CTAs with tiles of 128 x 256 (951).
 template <class T, class O, int MODE, bool PAIR, bool GATED, int BN, int STAGES>
-__global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const product_plan<T> p) {
-  using Shared = tc_shared<PAIR, GATED, BN, STAGES>;
+__global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MODE, O, PAIR>::A_SM) expert_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const product_plan<T> p) {
+  using Warps = tc_warps<MODE, O, PAIR>;
+  constexpr int WRITERS = Warps::WRITERS, BRINGS = WRITERS, MULTIPLIES = WRITERS + 1, CLEARS = WRITERS + 2, APART = WRITERS * 8;
+  using Shared = tc_shared<PAIR, WRITERS, BN, STAGES>;
   constexpr int CTAS = PAIR ? 2 : 1, OWN = GATED ? 64 : 128, WIDE = OWN * CTAS, UNIT = 16 * CTAS;
-  constexpr bool FINE = sizeof(O) == 4;
+  constexpr bool FINE = Warps::FINE;
   extern __shared__ char raw[];
   char* const stages = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   Shared& sh = *reinterpret_cast<Shared*>(stages + STAGES * Shared::STAGE);
@@ -549,7 +554,7 @@ __global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(
     }
   } else {
     if constexpr (FINE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WRITERS_REGISTERS));
-    // a writer has the 32 lanes that warp % 4 may read, and every other 32 columns; GATED: of these it finishes 16, of both halves
+    // a writer has the 32 lanes that warp % 4 may read, and 32 columns of every APART; GATED: of these it finishes 16, of both halves
     unsigned made = 0, e = 0;
     bool good = true;
     const int kind = p.activation & ~ACT_GATED, quarter = warp % 4, half = GATED ? quarter / 2 : 0, within = (GATED ? quarter % 2 : quarter) * 32;
@@ -637,7 +642,7 @@ __global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(
       bool waited = tile.depth == 0;
       if constexpr (FINE) {
         // the sums of all groups, added up in registers, take the last one's place
-        constexpr int N = BN / 64;
+        constexpr int N = BN / APART;
         const int groups = ((tile.depth + DEEP - 1) / DEEP * p.segments + GROUP - 1) / GROUP;
         if (groups > 1) {
           float sums[N][32];
@@ -649,7 +654,7 @@ __global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(
             await_sums();
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-              const int c = warp / 4 * 32 + i * 64;
+              const int c = warp / 4 * 32 + i * APART;
               if (c >= tile.rows || !good) continue;
               float v[32];
               tb200_tc::tmem_load(v, tmem + lanes + (made & 1) * BN + c);
@@ -661,13 +666,13 @@ __global__ void __launch_bounds__(TC_THREADS<MODE, O>, 1) expert_product_kernel(
           }
 #pragma unroll
           for (int i = 0; i < N; ++i)
-            if (warp / 4 * 32 + i * 64 < tile.rows) tb200_tc::tmem_store(sums[i], tmem + lanes + (made & 1) * BN + warp / 4 * 32 + i * 64);
+            if (warp / 4 * 32 + i * APART < tile.rows) tb200_tc::tmem_store(sums[i], tmem + lanes + (made & 1) * BN + warp / 4 * 32 + i * APART);
           tb200_tc::tmem_store_wait();
           waited = true;
         }
       }
-      for (int c = warp / 4 * 32;; c += 64) {
-        const bool any = c < tile.rows, last = c + 64 >= tile.rows;
+      for (int c = warp / 4 * 32;; c += APART) {
+        const bool any = c < tile.rows, last = c + APART >= tile.rows;
         request(c);
         if (!waited) await_sums();
         waited = true;
@@ -1098,7 +1103,8 @@ size_t most_row_tiles(size_t m, size_t experts, size_t tall) { return m / tall +
 
 template <class T, class O, int MODE, bool PAIR, bool GATED, int BN, int STAGES>
 cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_plan<T>& p, cudaStream_t stream) {
-  using Shared = tc_shared<PAIR, GATED, BN, STAGES>;
+  using Warps = tc_warps<MODE, O, PAIR>;
+  using Shared = tc_shared<PAIR, Warps::WRITERS, BN, STAGES>;
   constexpr size_t CTAS = PAIR ? 2 : 1, WIDE = (GATED ? 64 : 128) * CTAS;
   auto kernel = expert_product_kernel<T, O, MODE, PAIR, GATED, BN, STAGES>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shared::bytes(MOST_EXPERTS));
@@ -1112,8 +1118,8 @@ cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_
   const size_t across = ((size_t)p.features + WIDE - 1) / WIDE;
   const size_t tiles = MODE == BY_ROWS ? across * most_row_tiles(p.m, p.experts, BN) : across * (((size_t)p.others + BN - 1) / BN) * p.experts;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(product_grid(tiles * 4 * CTAS, 1) / CTAS * CTAS);      // (four: the parts of a tile)
-  cfg.blockDim = dim3(TC_THREADS<MODE, O>);
+  cfg.gridDim = dim3(product_grid(tiles * 4 * CTAS, Warps::A_SM) / CTAS * CTAS);      // (four: the parts of a tile)
+  cfg.blockDim = dim3(Warps::THREADS);
   cfg.dynamicSmemBytes = Shared::bytes(p.experts);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -1173,7 +1179,7 @@ template <class T> cudaError_t product_by_rows(const matrices& w, const matrices
     p.b_split = !few && x.width % 64 == 0;
     CUtensorMap a = {}, b = {};
     if (p.k > 0 && (!box_map<T>(a, w.at, of_a) || !box_map<T>(b, x.at, plain_axes(x.width, x.rows, x.stride, p.planes, x.outer, (unsigned)p.box, p.b_split, 2)))) return cudaErrorNotSupported;
-    if (few) return gated ? launch_tc<T, T, BY_ROWS, false, true, 64, 4>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, false, false, 64, 4>(a, b, p, stream);
+    if (few) return gated ? launch_tc<T, T, BY_ROWS, false, true, 64, 2>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, false, false, 64, 2>(a, b, p, stream);
     e = gated ? launch_tc<T, T, BY_ROWS, true, true, 256, 3>(a, b, p, stream) : launch_tc<T, T, BY_ROWS, true, false, 256, 3>(a, b, p, stream);
     if (!tb200::launch_refused(e)) return e;
   }
