@@ -935,55 +935,67 @@ __global__ void __launch_bounds__(SUM_BLOCK) join_sums_kernel(const float* __res
 }
 
 // Rows that are not made of whole aligned 16-byte pieces, or whose distances are not, laid out so that they are: `halves` pieces of `width` elements, each on a
-// boundary.  With offsets, the matrices of experts without rows are left out: nobody reads them.
+// boundary.  With offsets, the matrices of experts without rows are left out: nobody reads them (85 matrices of 512 x 589, three in use: 8 us; a thread for each piece of all, 32).
 struct which_experts {
   const void* offsets;
   bool wide;
   int m;
   __device__ __forceinline__ bool has_rows(size_t e) const { return !offsets || read_offset(offsets, wide, (unsigned)e + 1, m) > read_offset(offsets, wide, (unsigned)e, m); }
 };
+// The pieces (16 bytes of T, or 8 numbers) of a matrix's halves of rows, 2^spread threads a half: f(row, half, piece) for those of this thread; a matrix for each blockIdx.y.
+template <class F> __device__ __forceinline__ void each_piece(size_t rows, unsigned halves, unsigned pieces, unsigned spread, F f) {
+  const size_t thread = (size_t)blockIdx.x * 256 + threadIdx.x, lines = rows * halves, step = (size_t)gridDim.x * 256 >> spread;
+  for (size_t line = thread >> spread; line < lines; line += step)
+    for (unsigned c = (unsigned)thread & ((1u << spread) - 1); c < pieces; c += 1u << spread) f(halves == 2 ? line >> 1 : line, halves == 2 ? (unsigned)line & 1 : 0u, c);
+}
 template <class T>
-__global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ from, size_t each, size_t outer, size_t stride, size_t rows, unsigned halves, unsigned width, which_experts used,
-                                                        T* __restrict__ to) {
+__global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ from, size_t each, size_t outer, size_t stride, unsigned halves, unsigned width, unsigned pieces, unsigned spread,
+                                                        which_experts used, T* __restrict__ to) {
   constexpr int V = 16 / sizeof(T);
-  const unsigned wide = (width + V - 1) / V;
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * halves * wide) return;
-  const size_t line = i / wide, row = line / halves, c = (i - line * wide) * V;
-  if (!used.has_rows(row / each)) return;
-  const T* const f = from + row / each * outer + row % each * stride + (line - row * halves) * width + c;
-  union { T at[V]; uint4 all; } v;
+  if (!used.has_rows(blockIdx.y)) return;
+  from += blockIdx.y * outer;
+  to += blockIdx.y * each * halves * pieces * V;
+  each_piece(each, halves, pieces, spread, [&](size_t row, unsigned h, unsigned piece) {
+    const unsigned c = piece * V;
+    const T* const f = from + row * stride + (size_t)h * width + c;
+    union { T at[V]; uint4 all; } v;
 #pragma unroll
-  for (int j = 0; j < V; ++j) v.at[j] = c + j < width ? f[j] : from_f32<T>(0.f);
-  reinterpret_cast<uint4*>(to)[i] = v.all;
+    for (int j = 0; j < V; ++j) v.at[j] = c + j < width ? f[j] : from_f32<T>(0.f);
+    reinterpret_cast<uint4*>(to)[(row * halves + h) * pieces + piece] = v.all;
+  });
 }
 
 // The same rows as three planes of 16 bits, [matrix][plane][row][halves][wide], zeros behind a half's width.  A number that is not finite is in the first plane alone; one that
 // would be rounded to infinity is cut off instead.
-__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ from, size_t each, size_t outer, size_t stride, size_t rows, unsigned halves, unsigned width, unsigned wide,
+__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ from, size_t each, size_t outer, size_t stride, unsigned halves, unsigned width, unsigned pieces, unsigned spread,
                                                          which_experts used, bf16* __restrict__ to) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  const unsigned across = wide / 8;
-  if (i >= rows * halves * across) return;
-  const size_t line = i / across, row = line / halves, matrix = row / each, c = (i - line * across) * 8, h = line - row * halves;
-  if (!used.has_rows(matrix)) return;
-  const float* const f = from + matrix * outer + (row - matrix * each) * stride + h * width + c;
-  union { unsigned short at[8]; uint4 all; } v[PLANES];
+  if (!used.has_rows(blockIdx.y)) return;
+  from += blockIdx.y * outer;
+  const size_t plane = each * halves * pieces;      // in pieces
+  to += blockIdx.y * PLANES * plane * 8;
+  each_piece(each, halves, pieces, spread, [&](size_t row, unsigned h, unsigned piece) {
+    const unsigned c = piece * 8;
+    const float* const f = from + row * stride + (size_t)h * width + c;
+    float at[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float x = c + j < width ? f[j] : 0.f;
+    for (int j = 0; j < 8; ++j) at[j] = c + j < width ? f[j] : 0.f;
+    union { unsigned short at[8]; uint4 all; } v[PLANES];
 #pragma unroll
-    for (int q = 0; q < PLANES; ++q) {
-      const unsigned bits = __float_as_uint(x);
-      unsigned short r = __bfloat16_as_ushort(__float2bfloat16_rn(x));
-      if ((r & 0x7fff) == 0x7f80) r = (unsigned short)(bits >> 16);      // infinity stays, the largest numbers are cut off
-      v[q].at[j] = r;
-      x -= __uint_as_float((unsigned)r << 16);
-      if ((bits & 0x7f800000u) == 0x7f800000u) x = 0.f;
+    for (int j = 0; j < 8; ++j) {
+      float x = at[j];
+#pragma unroll
+      for (int q = 0; q < PLANES; ++q) {
+        const unsigned bits = __float_as_uint(x);
+        unsigned short r = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+        if ((r & 0x7fff) == 0x7f80) r = (unsigned short)(bits >> 16);      // infinity stays, the largest numbers are cut off
+        v[q].at[j] = r;
+        x -= __uint_as_float((unsigned)r << 16);
+        if ((bits & 0x7f800000u) == 0x7f800000u) x = 0.f;
+      }
     }
-  }
 #pragma unroll
-  for (int q = 0; q < PLANES; ++q) *reinterpret_cast<uint4*>(to + (((matrix * PLANES + q) * each + (row - matrix * each)) * halves + h) * wide + c) = v[q].all;
+    for (int q = 0; q < PLANES; ++q) reinterpret_cast<uint4*>(to)[q * plane + (row * halves + h) * pieces + piece] = v[q].all;
+  });
 }
 
 // dbefore = dout * the activation's slope; gated with out = act(a) b: da = dout b act'(a), db = dout act(a).  Bound by the bytes; a thread asks for two places' pieces before
@@ -1071,22 +1083,22 @@ struct matrices {
 // into `room`, which is moved on; nothing where they fit
 template <class T> cudaError_t pack(matrices& x, char*& room, which_experts used, cudaStream_t stream) {
   if (x.fits() || x.width == 0 || x.all_rows() == 0) return cudaSuccess;
-  const size_t bytes = x.packed_bytes(), pieces = x.all_rows() * x.halves * (x.split ? x.wide() / 8 : x.pieces());
-  if ((pieces + 255) / 256 > 0x7fffffffull) return cudaErrorInvalidValue;
-  const unsigned grid = (unsigned)((pieces + 255) / 256);
-  if constexpr (sizeof(T) == 4) {
-    if (x.split) {
-      split_rows_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), (unsigned)x.wide(), used,
+  const size_t bytes = x.packed_bytes(), many = x.count ? x.count : 1, pieces = x.split ? x.wide() / 8 : x.pieces();
+  const unsigned spread = spread_of(pieces, 5);
+  // as many CTAs as can run twice over, all matrices together
+  const size_t want = ((x.rows * x.halves << spread) + 255) / 256, most = ((size_t)tb200::current_device_info().sm_count * 16 + many - 1) / many;
+  const dim3 grid((unsigned)(want < most ? want : most), (unsigned)many);
+  if (x.split) {
+    if constexpr (sizeof(T) == 4)
+      split_rows_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(x.at), x.rows, x.outer, x.stride, x.halves, (unsigned)x.half(), (unsigned)pieces, spread, used,
                                                   reinterpret_cast<bf16*>(room));
-      x.width = x.stride = x.halves * x.wide();
-      x.count = (x.count ? x.count : 1) * PLANES;
-      x.bytes = 2;
-      x.split = false;
-    }
-  }
-  if (x.bytes == sizeof(T)) {
-    pack_rows_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T*>(x.at), x.rows, x.outer, x.stride, x.all_rows(), x.halves, (unsigned)x.half(), used, reinterpret_cast<T*>(room));
-    x.width = x.stride = x.halves * x.pieces() * 16 / sizeof(T);
+    x.width = x.stride = x.halves * x.wide();
+    x.count = many * PLANES;
+    x.bytes = 2;
+    x.split = false;
+  } else {
+    pack_rows_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T*>(x.at), x.rows, x.outer, x.stride, x.halves, (unsigned)x.half(), (unsigned)pieces, spread, used, reinterpret_cast<T*>(room));
+    x.width = x.stride = x.halves * pieces * 16 / sizeof(T);
   }
   x.at = room;
   x.outer = x.rows * x.stride;
