@@ -242,10 +242,12 @@ template <bool PAIR, int WRITERS, int BN, int STAGES> struct tc_shared {
   int dead;
   static size_t bytes(unsigned experts) { return 1024 + (size_t)STAGES * STAGE + sizeof(tc_shared) + (2 * (size_t)experts + 2) * 4; }
 };
-// false: it did not come within the limit, or another warp has given up
-template <bool PAIR> __device__ __forceinline__ bool await(unsigned long long* bar, unsigned parity, int* dead, tb200::ws_header* hdr) {
+// false: it did not come within the limit (of about a second), or another warp has given up.  stages: how many of the contraction it may have to wait for; 65536 of them
+// take less than a tenth of the limit.
+template <bool PAIR> __device__ __forceinline__ bool await(unsigned long long* bar, unsigned parity, int* dead, tb200::ws_header* hdr, unsigned stages = 0) {
   bool good = false;
-  for (unsigned iter = 0; !good && iter < tb200::MBAR_SPIN_LIMIT; ++iter) {
+  const unsigned long long limit = (unsigned long long)tb200::MBAR_SPIN_LIMIT * (1 + (stages >> 16));
+  for (unsigned long long iter = 0; !good && iter < limit; ++iter) {
     good = PAIR ? tb200_tc::try_wait_pair(bar, parity) : tb200::mbar_try_wait(bar, parity);
     if (!good && *(volatile int*)dead) break;
   }
@@ -540,7 +542,7 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
           const unsigned stage = (count + blocks - 1) % STAGES;
           count += blocks;
           if (!has) continue;
-          good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr);
+          good = await<PAIR>(&sh.tail[stage], tails >> stage & 1, &sh.dead, p.hdr, 2 * blocks);
           if (!good) break;
           tails ^= 1u << stage;
           clear_tail(stage, tile.depth - (int)(blocks - 1) * DEEP, 2 + (columns_of(tile) / CTAS + 63) / 64);
@@ -626,7 +628,7 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
         }
       };
       auto await_sums = [&] {
-        if (good) good = await<PAIR>(&sh.made[made & 1], made / 2 & 1, &sh.dead, p.hdr);
+        if (good) good = await<PAIR>(&sh.made[made & 1], made / 2 & 1, &sh.dead, p.hdr, FINE ? 0u : (unsigned)(tile.depth / DEEP));
         tb200_tc::fence_after_sync();
       };
       auto sums_taken = [&] {      // the next ones may be made there
