@@ -343,27 +343,27 @@ def test_long_sums_in_32_bits(tb, dtype):
     they add up to is two thirds of the result on average: 48 of them between sums that are rounded (24 by rows) are 1.9e-6; without those sums 30000 rows
     would be 7e-5."""
     g = torch.Generator(device="cuda").manual_seed(16)
-    x, offsets, w = inputs(g, [30000], 0, 0, 64, 136, dtype, "in_out")
+    x, offsets, w = inputs(g, [30000], 0, 0, 72, 136, dtype, "in_out")
     d = rand(g, 30000, 136, dtype=dtype)
     want = x.double().t() @ d.double()
     got = tb.expert_product_grad(d, x, offsets, w, dtype=torch.float32)[1][0].double()
     assert float((got - want).norm()) <= 1.9e-6 * float(want.norm())
     if dtype == torch.float32:
-        x, offsets, w = inputs(g, [400], 0, 0, 6000, 64, dtype, "out_in")
+        x, offsets, w = inputs(g, [400], 0, 0, 6000, 128, dtype, "out_in")
         want = x.double() @ w[0].double()
         assert float((tb.expert_product(x, offsets, w).double() - want).norm()) <= 1.9e-6 * float(want.norm())
 
 
 def test_numbers_at_the_ends_of_32_bits(tb):
     """As three planes of 16 bits: the largest and the smallest numbers, and infinities, which leave what is not finite and stay in their rows."""
-    x = torch.zeros(200, 64, device="cuda")
+    x = torch.zeros(200, 128, device="cuda")
     x[:, 0] = 1.0
     x[0, 0], x[1, 0], x[2, 0], x[3, 0], x[4, 0] = torch.finfo(torch.float32).max, -3.3961e38, 1e-30, 1.1754944e-38, 1 + 2.0 ** -23
     x[5, 3], x[6, 3] = float("inf"), float("-inf")
-    w = torch.zeros(1, 64, 64, device="cuda")
+    w = torch.zeros(1, 128, 128, device="cuda")
     w[0, 0] = 1.0
     w[0, 3] = 0.5
     offsets = torch.tensor([0, 200], device="cuda")
     out = tb.expert_product(x, offsets, w)
-    assert torch.equal(out[:5], x[:5, :1].expand(5, 64)) and torch.equal(out[7:], torch.ones(193, 64, device="cuda"))
+    assert torch.equal(out[:5], x[:5, :1].expand(5, 128)) and torch.equal(out[7:], torch.ones(193, 128, device="cuda"))
     assert not out[5:7].isfinite().any()

@@ -1153,8 +1153,10 @@ cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_
   return cudaLaunchKernelEx(&cfg, kernel, a, b, p);
 }
 
-// So few rows an expert that a product is as long as it takes to read the matrices: narrow tiles, and nothing laid out anew that need not be
-bool few_rows(size_t m, size_t experts) { return m <= 32 * experts; }
+// So few rows an expert that a product is as long as it takes to read the matrices: narrow tiles, and nothing laid out anew that need not be.  64 bf16 rows of 2048 for each of
+// 64 experts' 2048 outputs, gated: 94 us against 99, 96 rows 122 against 105; of 512 to 512 21 against 25, 27 against 17; 64 32-bit rows of 1024 for 16 experts' 1024 outputs 70
+// against 84, 96 rows 97 against 86.
+bool few_rows(size_t m, size_t experts) { return m <= 64 * experts; }
 
 template <int MODE, bool A_MN, int BN> cudaError_t launch_fma(const matrices& a, const matrices& b, const product_plan<float>& p, cudaStream_t stream) {
   using Shared = fma_shared<MODE, A_MN, BN>;
@@ -1211,7 +1213,7 @@ template <class T, class O> cudaError_t product_by_experts(const matrices& featu
   if (p.m > 0 && (!box_map<T>(a, features.at, plain_axes(features.width, features.rows, features.stride, p.planes, features.outer, DEEP, p.a_split, 2)) ||
                   !box_map<T>(b, others.at, plain_axes(others.width, others.rows, others.stride, p.planes, others.outer, DEEP, p.b_split, 2))))
     return cudaErrorNotSupported;
-  if (p.features > 128) {
+  if (p.features > 128) {      // (a pair's tile has 256: of fewer than half of them the second CTA would have nothing)
     const cudaError_t e = launch_tc<T, O, BY_EXPERTS, true, false, 256, 3>(a, b, p, stream);
     if (!tb200::launch_refused(e)) return e;      // (no room for pairs)
   }
@@ -1219,8 +1221,12 @@ template <class T, class O> cudaError_t product_by_experts(const matrices& featu
 }
 
 bool sizes_fit(size_t n, size_t experts, size_t in, size_t out) { return n <= MOST_ROWS && experts >= 1 && experts <= (size_t)MOST_EXPERTS && in < MOST_CHANNELS && out < MOST_CHANNELS; }
-// 32-bit rows go to the tensor cores, as planes, where products are longer than it takes to lay the planes out: not few rows, and 64 or more channels on both sides
-template <class T> bool in_planes(size_t n, size_t experts, size_t in, size_t out) { return sizeof(T) == 4 && !few_rows(n, experts) && in >= 64 && out >= 64; }
+// 32-bit rows go to the tensor cores, as planes, where products are longer than it takes to lay the planes out: not few rows, and 128 or more channels on both sides (256 rows of
+// 64 for 16 experts' 64 outputs: 14 us by multiply-adds against 21; 256 of 128 to 2048: 98 against 42).  Sums over very many rows do too, because one
+// multiply-add after another rounds them too often.
+template <class T> bool in_planes(size_t n, size_t experts, size_t in, size_t out, bool grad) {
+  return sizeof(T) == 4 && !few_rows(n, experts) && ((in >= 128 && out >= 128) || (grad && n >= 2048 * experts));
+}
 template <class T> void set_planes(product_plan<T>& p, bool split) {
   p.planes = split ? PLANES : 1;
   p.segments = split ? SEGMENTS : 1;
@@ -1255,7 +1261,7 @@ TB200_API int tb200_expert_product(const void* d_rows, size_t rows_stride, const
       const bool gated = (activation & ACT_GATED) != 0;
       if (!sizes_fit(n, num_experts, in, out) || !activation_known(activation) || (gated && out % 2)) return ERR_INVALID;
       const size_t width = gated ? out / 2 : out;
-      const bool split = in_planes<T>(n, num_experts, in, out);
+      const bool split = in_planes<T>(n, num_experts, in, out, false);
       matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, gated ? 2 : 1, sizeof(T), split), x = {d_rows, in, n, rows_stride, 0, 0, 1, sizeof(T), split};
       int rc;
       if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header) + w.packed_bytes() + x.packed_bytes(), rc)) return rc;
@@ -1296,7 +1302,7 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
     if (grad_t != t && grad_t != TB200_F32) return ERR_UNSUPPORTED;
     return by_index_dtype(offset_t, [&](auto iv) -> int {
       if (!sizes_fit(n, num_experts, in, out)) return ERR_INVALID;
-      const bool split = in_planes<T>(n, num_experts, in, out);
+      const bool split = in_planes<T>(n, num_experts, in, out, true);
       matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, 1, sizeof(T), split), x = {d_rows, in, n, rows_stride, 0, 0, 1, sizeof(T), split},
                d = {d_dout, out, n, dout_stride, 0, 0, 1, sizeof(T), split};
       const unsigned parts = d_dbias ? sum_parts(n, num_experts, out) : 1;
