@@ -1225,7 +1225,7 @@ bool sizes_fit(size_t n, size_t experts, size_t in, size_t out) { return n <= MO
 // 64 for 16 experts' 64 outputs: 14 us by multiply-adds against 21; 256 of 128 to 2048: 98 against 42).  Sums over very many rows do too, because one
 // multiply-add after another rounds them too often.
 template <class T> bool in_planes(size_t n, size_t experts, size_t in, size_t out, bool grad) {
-  return sizeof(T) == 4 && !few_rows(n, experts) && ((in >= 128 && out >= 128) || (grad && n >= 2048 * experts));
+  return sizeof(T) == 4 && in && out && !few_rows(n, experts) && ((in >= 128 && out >= 128) || (grad && n >= 2048 * experts));
 }
 template <class T> void set_planes(product_plan<T>& p, bool split) {
   p.planes = split ? PLANES : 1;
@@ -1307,8 +1307,9 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
                d = {d_dout, out, n, dout_stride, 0, 0, 1, sizeof(T), split};
       const unsigned parts = d_dbias ? sum_parts(n, num_experts, out) : 1;
       const size_t sums = parts > 1 ? tb200::align_up((size_t)parts * num_experts * out * 4, 256) : 0;
+      const bool products = n && in && out;      // otherwise what is left are zeros and the gradient of bias, and no product reads an operand (they may be NULL)
       int rc;
-      if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header) + sums + w.packed_bytes() + x.packed_bytes() + d.packed_bytes(), rc)) return rc;
+      if (workspace_gate(d_ws, ws_bytes, sizeof(tb200::ws_header) + sums + (products ? w.packed_bytes() + x.packed_bytes() + d.packed_bytes() : 0), rc)) return rc;
       if (out == 0 && (n == 0 || in == 0)) return 0;
       if (!d_offsets || (in && n && (!d_drows || (out && (!d_rows || !d_weight)))) || (in && out && !d_dweight) || (out && n && !d_dout) || rows_stride < in || dout_stride < out ||
           !weights_fit(num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0))
@@ -1317,10 +1318,12 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
       float* const partial = reinterpret_cast<float*>(room);
       room += sums;
       cudaError_t e = cudaSuccess;
-      e = pack<T>(w, room, {d_offsets, sizeof(iv) == 8, (int)n}, stream);
-      if (e == cudaSuccess) e = pack<T>(x, room, {}, stream);
-      if (e == cudaSuccess) e = pack<T>(d, room, {}, stream);
-      if (e != cudaSuccess) return (int)e;
+      if (products) {
+        e = pack<T>(w, room, {d_offsets, sizeof(iv) == 8, (int)n}, stream);
+        if (e == cudaSuccess) e = pack<T>(x, room, {}, stream);
+        if (e == cudaSuccess) e = pack<T>(d, room, {}, stream);
+        if (e != cudaSuccess) return (int)e;
+      }
       product_plan<T> p = {};
       p.offsets = d_offsets;
       p.wide = sizeof(iv) == 8;
