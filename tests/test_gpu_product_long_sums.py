@@ -1,0 +1,52 @@
+"""Results do not get worse with the length of a contraction: sums of numbers of one sign, which the matrix instructions make too small, always."""
+import pytest
+import torch
+
+from layers_util import STORE, TINY, U
+
+pytestmark = pytest.mark.gpu
+# What a matrix instruction adds to its sum are 16 products, each cut off at a bit of the sum, and so is the sum: 17 U of it at most.  A group is 8 instructions for each of its
+# stages; its sum is half as large on average as at the end.  Groups' sums are added up rounded to nearest, U each.
+GROUP = {torch.float16: 32, torch.bfloat16: 128}      # stages of 128
+
+
+def limit(dtype, length):
+    stages = -(-length // 128)
+    return STORE[dtype] + (8 * min(GROUP[dtype], stages) / 2 * 17 + -(-stages // GROUP[dtype])) * U
+
+
+def inputs(dtype, *shape):
+    """Around 1 / sqrt(length), so that results are around 1"""
+    g = torch.Generator(device="cuda").manual_seed(sum(shape))
+    return lambda length, *shape: ((0.5 + torch.rand(*shape, generator=g, device="cuda")) * length ** -0.5).to(dtype)
+
+
+def check(got, want, length):
+    assert bool(((got.double() - want).abs() <= limit(got.dtype, length) * want + TINY[got.dtype]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("counts", [[1 << 20], [3, (1 << 19) + 77, 0, 200000]])
+@pytest.mark.parametrize("i, o", [(64, 40), (24, 264)])
+def test_gradients_of_matrices(tb, dtype, counts, i, o):
+    make = inputs(dtype, sum(counts), i, o)
+    offsets = torch.tensor([0] + counts, device="cuda").cumsum(0)
+    x, d, w = make(max(counts), sum(counts), i), make(max(counts), sum(counts), o), make(1, len(counts), i, o)
+    dw = tb.expert_product_grad(d, x, offsets, w)[1]
+    at = offsets.tolist()
+    for e, c in enumerate(counts):
+        check(dw[e], x[at[e]:at[e + 1]].double().t() @ d[at[e]:at[e + 1]].double(), c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lies", ["in_out", "out_in"])
+@pytest.mark.parametrize("n, k", [(9, 1 << 19), (200, 1 << 19), (300, 20008), (70, 4096), (70, 4104)])
+def test_products_of_long_rows(tb, dtype, lies, n, k):
+    make = inputs(dtype, n, k)
+    x, w = make(k, n, k), make(k, 1, k, 160) if lies == "in_out" else make(k, 1, 160, k).transpose(1, 2)
+    offsets = torch.tensor([0, n], device="cuda")
+    want = x.double() @ w[0].double()
+    check(tb.expert_product(x, offsets, w), want, k)
+    check(tb.expert_product(x, offsets, w, None, "gated_silu", keep=True)[1], want, k)
+    # the same sums as a gradient of rows, by the same matrix the other way round
+    check(tb.expert_product_grad(x, make(1, n, 160), offsets, w.transpose(1, 2))[0], want, k)

@@ -222,7 +222,9 @@ __device__ __forceinline__ bool withheld(unsigned t, unsigned step) { return wit
 __device__ __forceinline__ bool withheld(unsigned, unsigned) { return false; }
 #endif
 
-constexpr int DEEP = 128, GROUP = 6;          // of the contraction, a stage; stages
+constexpr int DEEP = 128;                     // of the contraction, a stage
+// How many stages the matrix instructions add up; then the writers go on, with sums that are rounded to nearest.  See expert_product_kernel.
+template <class O> constexpr int GROUP = sizeof(O) == 4 ? 6 : std::is_same<O, f16>::value ? 32 : 128;
 // Warps: WRITERS that write results, then one that brings operands, one that multiplies, and (by experts) one that clears boxes' ends.  Few rows: four writers, and two CTAs a SM.
 // 32-bit results: the writers hold 128 sums a thread, of registers that the other four warps hand over (launched with 168 a thread; 2 x 216 + 72 = 3 x 168).
 template <int MODE, class O, bool PAIR> struct tc_warps {
@@ -345,8 +347,11 @@ constexpr unsigned A_PLANES = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, B
 //
 // One warp keeps STAGES boxes of A and B on their way by the copy engine, one issues the matrix instructions as they come, the writers take the sums of the last
 // tile from tensor memory, while the next one's are made in its other half, and write them.  Sums are 32 bits from first to last; they
-// are rounded once, where they are stored, after bias, activation and residual.  The matrix instructions cut off what they add (1.2e-7 of the results for each
-// stage, and always the same way), which results of 16 bits do not see.  32-bit results (FINE) are made of sums over GROUP stages, which the writers add up in registers,
+// are rounded once, where they are stored, after bias, activation and residual.  The matrix instructions cut off what they add (of sums
+// of one sign up to 1.5e-6 for each stage, and always the same way), so that they add up GROUP stages, and the writers add up those sums, rounded to nearest.  Results of 16 bits: 32 stages for
+// f16 and 128 for bf16, which are off by 2.4e-5 and 9.6e-5, a tenth and a twentieth of the least half step; a longer contraction goes on in the other set, by way of the writers, which add
+// the one to the other.  Sums of 2^20 numbers of one sign are off by half a step as those of 2^12 are (in one set: by 6e-3); 16384 f16 rows of 8192 to 512 take 142 us instead of 140,
+// of 16384 234 instead of 225.  32-bit results (FINE) are made of sums over six stages, which the writers add up in registers,
 // rounded to nearest, and put back to where the last ones were: three stages where an activation multiplies two results (off by 3.4e-7, and 6.8e-7 behind it, for any
 // length), six for matrices (7.3e-7; with four 4.7e-7, and 8198 rows' gradients take 103 us instead of 98).  Gated: the two halves of a result are in lanes 64 apart, in warps that pass each
 // other half of their columns.
@@ -520,7 +525,7 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
             __syncwarp();
             begun = true;
             if ((k += DEEP) >= tile.depth && ++segment < p.segments) k = 0;
-            if (k >= tile.depth || (FINE && ++block % GROUP == 0)) {
+            if (k >= tile.depth || ++block % GROUP<O> == 0) {
               if (tb200_tc::elected()) tb200_tc::commit<PAIR>(&sh.made[set]);
               __syncwarp();
               begun = false;
@@ -628,24 +633,44 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
         }
       };
       auto await_sums = [&] {
-        if (good) good = await<PAIR>(&sh.made[made & 1], made / 2 & 1, &sh.dead, p.hdr, FINE ? 0u : (unsigned)(tile.depth / DEEP));
+        if (good) good = await<PAIR>(&sh.made[made & 1], made / 2 & 1, &sh.dead, p.hdr);
         tb200_tc::fence_after_sync();
       };
-      auto sums_taken = [&] {      // the next ones may be made there
+      auto set_free = [&](unsigned set) {      // the next sums may be made there
         tb200_tc::fence_before_sync();
         __syncwarp();
         if (lane == 0 && good) {
-          if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.taken[made & 1]));
-          else tb200::mbar_arrive(&sh.taken[made & 1]);
+          if (PAIR) tb200_tc::arrive_there(tb200_tc::first_ones(&sh.taken[set]));
+          else tb200::mbar_arrive(&sh.taken[set]);
         }
-        ++made;
       };
+      auto sums_taken = [&] { set_free(made++ & 1); };
       const unsigned lanes = quarter * 32u << 16;
       bool waited = tile.depth == 0;
-      if constexpr (FINE) {
+      const int groups = ((tile.depth + DEEP - 1) / DEEP * p.segments + GROUP<O> - 1) / GROUP<O>;
+      if constexpr (!FINE) {
+        // each group's sums are added to those of all before it, in the other set, which the group after it may then have
+        for (int g = 0; g + 1 < groups; ++g) {
+          if (g == 0) await_sums();
+          ++made;
+          await_sums();
+          const unsigned at = tmem + lanes + (made & 1) * BN, before = tmem + lanes + (~made & 1) * BN;
+          for (int c = warp / 4 * 32; c < tile.rows && good; c += APART) {
+            float v[32], sums[32];
+            tb200_tc::tmem_load(sums, before + c);
+            tb200_tc::tmem_load(v, at + c);
+            tb200_tc::tmem_load_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += sums[j];
+            tb200_tc::tmem_store(v, at + c);
+          }
+          tb200_tc::tmem_store_wait();
+          set_free(~made & 1);
+          waited = true;
+        }
+      } else {
         // the sums of all groups, added up in registers, take the last one's place
         constexpr int N = BN / APART;
-        const int groups = ((tile.depth + DEEP - 1) / DEEP * p.segments + GROUP - 1) / GROUP;
         if (groups > 1) {
           float sums[N][32];
 #pragma unroll
