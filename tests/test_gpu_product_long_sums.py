@@ -50,3 +50,33 @@ def test_products_of_long_rows(tb, dtype, lies, n, k):
     check(tb.expert_product(x, offsets, w, None, "gated_silu", keep=True)[1], want, k)
     # the same sums as a gradient of rows, by the same matrix the other way round
     check(tb.expert_product_grad(x, make(1, n, 160), offsets, w.transpose(1, 2))[0], want, k)
+
+
+# 32 bits by multiply-adds.  A rounding is off by at most 2^-24 of the sum, 2^-24 / 3^0.5 of it in the norm, in either direction.  1024 of them while a sum grows evenly are a walk of
+# (1024 / 3)^0.5 such steps, 6.4e-7; one of up to 512 sums of so many adds 4.5e-7; twice both together is 1.6e-6.  A chain of 500000 would be 1.4e-5, of 65536 5e-6.
+LIMIT_32 = 1.6e-6
+
+
+@pytest.mark.parametrize("experts, n, i, o", [(256, 500000, 64, 64), (1024, 65536, 200, 136), (1024, 66000, 33, 50), (300, 500000, 8, 300)])
+def test_all_rows_of_one_of_many_experts(tb, experts, n, i, o):
+    """The rows of an expert on average are few, those of one are all."""
+    make = inputs(torch.float32, n, i, o)
+    offsets = torch.zeros(experts + 1, dtype=torch.int32, device="cuda")
+    offsets[experts // 2 + 1:] = n
+    x, d, w = make(1, n, i), make(1, n, o), make(1, experts, i, o)
+    dw = tb.expert_product_grad(d, x, offsets, w)[1]
+    want = x.double().t() @ d.double()
+    assert float((dw[experts // 2].double() - want).norm()) <= LIMIT_32 * float(want.norm())
+    assert float(dw[:experts // 2].abs().max()) == 0 and float(dw[experts // 2 + 1:].abs().max()) == 0
+
+
+@pytest.mark.parametrize("lies", ["in_out", "out_in"])
+@pytest.mark.parametrize("activation", [None, "gated_silu"])
+@pytest.mark.parametrize("n, k", [(5, 300000), (60, 70001), (200, 1024), (3, 1025), (3, 2049)])
+def test_few_long_rows(tb, lies, activation, n, k):
+    make = inputs(torch.float32, n, k)
+    x, w = make(k, n, k), make(k, 3, k, 70) if lies == "in_out" else make(k, 3, 70, k).transpose(1, 2)
+    offsets = torch.tensor([0, n // 2, n // 2, n], device="cuda")
+    want = torch.cat([x[:n // 2].double() @ w[0].double(), x[n // 2:].double() @ w[2].double()])
+    got = tb.expert_product(x, offsets, w, None, "gated_silu", keep=True)[1] if activation else tb.expert_product(x, offsets, w)
+    assert float((got.double() - want).norm()) <= LIMIT_32 * float(want.norm())

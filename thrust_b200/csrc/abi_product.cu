@@ -734,7 +734,10 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
 // by asynchronous copies, into a ring of stages of shared memory, and lie there as they lie in memory: by k (rows of features or of others), or by m (rows of
 // k), of which a lane takes two k at a time.  Bound by the multiply-adds: 2048 rows of 1000 to 1501 through six experts took 176 us (35 TFLOP/s; tiles of
 // 128 x 128 read element by element 298), which the tensor cores take 61 for.  They have the products of few rows and of few channels.
-constexpr int FMA_THREADS = 128, FMA_DEEP = 16, FMA_STAGES = 4;
+//
+// One multiply-add after another rounds a sum each time: FMA_GROUP stages (1024 of the contraction) are added up that way, and those sums to one another, so that 500000 rows of one
+// expert's gradient are off by 3e-7 in the norm (one after another: 9e-6), whatever the other experts have.
+constexpr int FMA_THREADS = 128, FMA_DEEP = 16, FMA_STAGES = 4, FMA_GROUP = 64;
 template <int WIDE, bool BY_K> struct fma_tile {      // an operand's part of a stage
   static constexpr int STRIDE = BY_K ? WIDE + 4 : FMA_DEEP + 4, PIECES = WIDE * FMA_DEEP / 4 / FMA_THREADS;
   float at[(BY_K ? FMA_DEEP : WIDE) * STRIDE];
@@ -753,6 +756,7 @@ __device__ __forceinline__ int within_four(int n) { return n < 0 ? 0 : n > 4 ? 4
 using f2 = unsigned long long;
 __device__ __forceinline__ f2 pack2(float x, float y) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
 __device__ __forceinline__ float2 unpack2(f2 a) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a)); return r; }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 
 template <int MODE, bool A_MN, int BN>
@@ -822,6 +826,7 @@ __global__ void __launch_bounds__(FMA_THREADS, 3) expert_product_f32_kernel(cons
     for (int i = 0; i < FP; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[i][j] = pack2(0.f, 0.f);
+    volatile f2 all[FP * 8];      // sums of long contractions, in local memory
     const int blocks = (tile.depth + FMA_DEEP - 1) / FMA_DEEP;
     __syncthreads();      // (the last tile's stages have been read)
     for (int q = 0; q < FMA_STAGES - 1; ++q) {
@@ -877,8 +882,23 @@ __global__ void __launch_bounds__(FMA_THREADS, 3) expert_product_f32_kernel(cons
           }
         }
       }
+      if (q % FMA_GROUP == FMA_GROUP - 1 && q + 1 < blocks) {
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            all[i * 8 + j] = q < FMA_GROUP ? acc[i][j] : add2(all[i * 8 + j], acc[i][j]);
+            acc[i][j] = pack2(0.f, 0.f);
+          }
+      }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (blocks > FMA_GROUP) {
+#pragma unroll
+      for (int i = 0; i < FP; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = add2(all[i * 8 + j], acc[i][j]);
+    }
     const size_t width = p.features;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
