@@ -80,3 +80,21 @@ def test_few_long_rows(tb, lies, activation, n, k):
     want = torch.cat([x[:n // 2].double() @ w[0].double(), x[n // 2:].double() @ w[2].double()])
     got = tb.expert_product(x, offsets, w, None, "gated_silu", keep=True)[1] if activation else tb.expert_product(x, offsets, w)
     assert float((got.double() - want).norm()) <= LIMIT_32 * float(want.norm())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("o", [8, 5])
+def test_bias_of_one_of_many_experts(tb, dtype, o):
+    """Two parts of 4000000 rows, of either 250000 a warp: 244 sums of 1024 each, as above, and the sixteen warps' walks are not one another's: a quarter of a single
+    one's.  (Chains of 250000: (250000 / 3)^0.5 2^-24 / 3^0.5 / 4 = 2.5e-6.)"""
+    n, experts = 4000000, 1024
+    make = inputs(torch.float32, n, o)
+    offsets = torch.zeros(experts + 1, dtype=torch.int32, device="cuda")
+    offsets[1:] = 7
+    offsets[100:] = n - 3
+    d = make(1, n, o).to(dtype)
+    d[:7], d[-3:] = float("nan"), float("nan")
+    db = tb.expert_product_grad(d, make(1, n, 8).to(dtype), offsets, make(1, experts, 8, o).to(dtype), bias=True)[2]
+    want = d[7:-3].double().sum(0)
+    assert float((db[99].double() - want).norm()) <= LIMIT_32 / 4 * float(want.norm())
+    assert float(db[100:].abs().max()) == 0 and float(db[1:99].abs().max()) == 0

@@ -937,7 +937,9 @@ __global__ void __launch_bounds__(FMA_THREADS, 3) expert_product_f32_kernel(cons
 // ---------------------------------------------------------------------------------------------- the smaller parts
 // The gradient of bias: the sums of each expert's rows of dout.  A CTA has 32 V features of one of `parts` pieces of an expert's rows; its warps take rows in turn and
 // meet in shared memory, parts meet in a second kernel, always in the same order.  Bound by latency: 8198 bf16 rows of 1280 for 16 experts 10 us and 4, beside the products.
-constexpr int SUM_BLOCK = 256;
+// SUM_GROUP rows, of which a warp adds up 1024, make a sum of their own: how many parts there are goes by the rows of an expert on average, and one expert may have nearly all
+// (4000000 rows of numbers of one sign: off by 7.7e-8, in chains of 250000 by 1.5e-6).
+constexpr int SUM_BLOCK = 256, SUM_GROUP = 1024 * SUM_BLOCK / 32;
 template <class T, int V>
 __global__ void __launch_bounds__(SUM_BLOCK) row_sums_kernel(const T* __restrict__ x, size_t stride, const void* __restrict__ offsets, bool wide, unsigned experts, int m, int features,
                                                              float* __restrict__ sums) {
@@ -949,14 +951,21 @@ __global__ void __launch_bounds__(SUM_BLOCK) row_sums_kernel(const T* __restrict
   float sum[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[v] = 0.f;
-  if (f < features) {
+  for (int begin = first; f < features && begin < last;) {
+    const int stop = last - begin > SUM_GROUP ? begin + SUM_GROUP : last;
+    float some[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) some[v] = 0.f;
 #pragma unroll 4
-    for (int r = first + warp; r < last; r += SUM_BLOCK / 32) {
+    for (int r = begin + warp; r < stop; r += SUM_BLOCK / 32) {
       float g[V];
       channels(load_words<T, V>(x + (size_t)r * stride + f), g);
 #pragma unroll
-      for (int v = 0; v < V; ++v) sum[v] += g[v];
+      for (int v = 0; v < V; ++v) some[v] += g[v];
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum[v] += some[v];
+    begin = stop;
   }
   __shared__ float met[SUM_BLOCK / 32][32 * V];
 #pragma unroll
