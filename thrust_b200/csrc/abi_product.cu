@@ -335,9 +335,14 @@ template <class O, int N> struct columns_in {
   }
 };
 
-// A 32-bit number is the sum of three of 16 bits (bf16), each the rest rounded.  Of the nine products of such planes the three smallest, 2^-24 of the whole together, are
-// left out; the others are segments of one contraction, the smaller ones first.  (Six instructions for one, at fifteen times the rate of multiply-adds.)
+// A 32-bit number is a + b / 128 + c / 128^2 with three numbers of 16 bits (bf16), each the rest rounded: scaled by SCALE, rests of the smallest numbers are numbers of 16 bits too (2^-133
+// is the least of them, so that c ends at 2^-147, where a 32-bit number's last bit is at 2^-149), and those of the largest, which would be rounded to infinity and are cut off instead, stay
+// below it, with sums of products below the whole product.  Of the nine products of such planes the three smallest, 2^-24 of the whole together, are left out; the others are segments of
+// one contraction, the smaller ones first: three of 1 / 128^2, two of 1 / 128, one of 1, and what is there is scaled as the next level begins.  (Six instructions for one, at fifteen times
+// the rate of multiply-adds.)
 constexpr int PLANES = 3, SEGMENTS = 6;
+constexpr float SCALE = 128.f;
+__host__ __device__ constexpr bool next_level(int segment) { return segment == 3 || segment == 5; }
 constexpr unsigned A_PLANES = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, B_PLANES = 0 | 2 << 2 | 1 << 4 | 0 << 6 | 1 << 8 | 0 << 10;
 
 // D^T = A B^T by tiles of 128 features (gated: 64 of each half) a CTA x up to BN rows; CTAs stay and go from tile to tile.  Features are the lanes of tensor
@@ -524,8 +529,13 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
             }
             __syncwarp();
             begun = true;
-            if ((k += DEEP) >= tile.depth && ++segment < p.segments) k = 0;
-            if (k >= tile.depth || ++block % GROUP<O> == 0) {
+            bool cut = ++block == GROUP<O>;
+            if ((k += DEEP) >= tile.depth) {
+              if (++segment < p.segments) k = 0;
+              cut = cut || segment == p.segments || next_level(segment);
+            }
+            if (cut) {
+              block = 0;
               if (tb200_tc::elected()) tb200_tc::commit<PAIR>(&sh.made[set]);
               __syncwarp();
               begun = false;
@@ -647,10 +657,11 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
       auto sums_taken = [&] { set_free(made++ & 1); };
       const unsigned lanes = quarter * 32u << 16;
       bool waited = tile.depth == 0;
-      const int groups = ((tile.depth + DEEP - 1) / DEEP * p.segments + GROUP<O> - 1) / GROUP<O>;
+      const int blocks = (tile.depth + DEEP - 1) / DEEP;
+      auto groups_of = [&](int segments) { return (blocks * segments + GROUP<O> - 1) / GROUP<O>; };
       if constexpr (!FINE) {
         // each group's sums are added to those of all before it, in the other set, which the group after it may then have
-        for (int g = 0; g + 1 < groups; ++g) {
+        for (int g = 0; g + 1 < groups_of(1); ++g) {
           if (g == 0) await_sums();
           ++made;
           await_sums();
@@ -671,25 +682,29 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
       } else {
         // the sums of all groups, added up in registers, take the last one's place
         constexpr int N = BN / APART;
-        if (groups > 1) {
+        if (tile.depth && (p.segments > 1 || groups_of(1) > 1)) {
           float sums[N][32];
 #pragma unroll
           for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int j = 0; j < 32; ++j) sums[i][j] = 0.f;
-          for (int g = 0; g < groups; ++g) {
-            await_sums();
+          for (int level = p.segments > 1 ? 3 : 1; level > 0; --level) {      // so many segments have its scale
+            const int groups = groups_of(level);
+            for (int g = 0; g < groups; ++g) {
+              const float scale = g == 0 && level < 3 ? 1.f / SCALE : 1.f;
+              await_sums();
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-              const int c = warp / 4 * 32 + i * APART;
-              if (c >= tile.rows || !good) continue;
-              float v[32];
-              tb200_tc::tmem_load(v, tmem + lanes + (made & 1) * BN + c);
-              tb200_tc::tmem_load_wait();
+              for (int i = 0; i < N; ++i) {
+                const int c = warp / 4 * 32 + i * APART;
+                if (c >= tile.rows || !good) continue;
+                float v[32];
+                tb200_tc::tmem_load(v, tmem + lanes + (made & 1) * BN + c);
+                tb200_tc::tmem_load_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) sums[i][j] += v[j];
+                for (int j = 0; j < 32; ++j) sums[i][j] = fmaf(sums[i][j], scale, v[j]);
+              }
+              if (level > 1 || g + 1 < groups) sums_taken();
             }
-            if (g + 1 < groups) sums_taken();
           }
 #pragma unroll
           for (int i = 0; i < N; ++i)
@@ -1021,8 +1036,7 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ fr
   });
 }
 
-// The same rows as three planes of 16 bits, [matrix][plane][row][halves][wide], zeros behind a half's width.  A number that is not finite is in the first plane alone; one that
-// would be rounded to infinity is cut off instead.
+// The same rows as three planes of 16 bits, [matrix][plane][row][halves][wide], zeros behind a half's width.  A number that is not finite is in the first plane alone.
 __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ from, size_t each, size_t outer, size_t stride, unsigned halves, unsigned width, unsigned pieces, unsigned spread,
                                                          which_experts used, bf16* __restrict__ to) {
   if (!used.has_rows(blockIdx.y)) return;
@@ -1045,7 +1059,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict
         unsigned short r = __bfloat16_as_ushort(__float2bfloat16_rn(x));
         if ((r & 0x7fff) == 0x7f80) r = (unsigned short)(bits >> 16);      // infinity stays, the largest numbers are cut off
         v[q].at[j] = r;
-        x -= __uint_as_float((unsigned)r << 16);
+        x = SCALE * (x - __uint_as_float((unsigned)r << 16));      // (both exact)
         if ((bits & 0x7f800000u) == 0x7f800000u) x = 0.f;
       }
     }
