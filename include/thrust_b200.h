@@ -420,8 +420,9 @@ enum tb200_scores { TB200_SOFTMAX = 0, TB200_SIGMOID = 1 };
 /* Which experts a token goes to, and with what weights: of row i of d_logits (num_experts <= 1024 of type t, logits_stride apart) the `choices` <= 32
  * best by score + bias, best first, the lower index before an equal one; d_experts[i * choices + c] (-1 where there is none) and d_weights (F32),
  * scale times the score (without the bias), divided by the sum of the chosen ones' scores if renormalize != 0.
- *   scores   TB200_SOFTMAX: over the row's open experts; TB200_SIGMOID: 1 / (1 + exp(-logit)).
- *   d_bias   F32, num_experts; NULL: the order is the logits'.
+ *   scores   TB200_SOFTMAX: over the row's experts whose logit is neither NaN nor -infinity; TB200_SIGMOID: 1 / (1 + exp(-logit)).
+ *   d_bias   F32, num_experts, which takes part in the choice alone: an expert that it closes keeps its share of the softmax.  NULL: the order is the
+ *            logits'.
  *   open     are experts whose logit, and logit's score + bias, is neither NaN nor -infinity; the others are never chosen.  A row without open experts
  *            has -1 and weights of zero throughout.
  *   groups   <= 32, dividing num_experts: only the group_choices best of the groups of neighbouring experts take part, by the sum of the group_best (1 or 2)
@@ -432,7 +433,7 @@ int tb200_expert_route(const void* d_logits, size_t logits_stride, size_t n, siz
                        int renormalize, float scale, int* d_experts, float* d_weights, tb200_stream_t stream);
 
 /* Its gradient: d_dlogits (packed) from that of d_weights and the chosen d_experts; the choice itself has none, nor has the bias.  A choice outside
- * [0, num_experts), or of an expert that is not open, has no part; choices of the same expert add up. */
+ * [0, num_experts), or of an expert whose logit is NaN or -infinity, has no part; choices of the same expert add up. */
 int tb200_expert_route_grad(const float* d_dweights, const int* d_experts, const void* d_logits, size_t logits_stride,
                             size_t n, size_t num_experts, size_t choices, int t, int scores, int renormalize,
                             float scale, void* d_dlogits, tb200_stream_t stream);

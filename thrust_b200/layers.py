@@ -318,8 +318,8 @@ def _logits(logits, choices, scores):
 
 def expert_route(logits, choices, scores="softmax", bias=None, groups=1, group_choices=None, group_best=2, renormalize=True, scale=1.0):
     """Which experts each token goes to: of logits [tokens, experts] the `choices` best by score + bias, the best first, the lower index
-    before an equal one.  scores: "softmax" over the token's open experts, or "sigmoid"; bias: float32 [experts], which takes part in the choice
-    alone.  An expert whose logit, or score + bias, is NaN or -infinity is not open and never chosen.  groups: only the group_choices (all by
+    before an equal one.  scores: "softmax" over the token's experts whose logit is neither NaN nor -infinity, or "sigmoid"; bias: float32 [experts], which takes
+    part in the choice alone (an expert that it closes keeps its share of the softmax).  An expert whose logit, or score + bias, is NaN or -infinity is not open and never chosen.  groups: only the group_choices (all by
     default) best of so many equal groups of neighbouring experts take part, by the sum of their group_best (1 or 2) best score + bias.
     Returns (experts, weights): int32 [tokens, choices], -1 where no open expert is left (expert_dispatch drops it); float32, scale times the
     score, divided by the sum of the chosen ones' scores if renormalize, 0 where no expert is.  Scores are compared as 64-bit numbers."""
@@ -337,7 +337,7 @@ def expert_route(logits, choices, scores="softmax", bias=None, groups=1, group_c
 
 def expert_route_grad(dweights, experts, logits, scores="softmax", renormalize=True, scale=1.0):
     """The gradient of expert_route's logits, of their type, from that of its weights; experts is what it returned.  The choice has none, nor has
-    the bias.  A choice that is no open expert has no part; choices of the same expert add up."""
+    the bias.  A choice that is no expert, or one whose logit is NaN or -infinity, has no part; choices of the same expert add up."""
     if experts.dim() != 2:
         raise ValueError("experts: [tokens, choices] is needed")
     choices = experts.shape[1]
