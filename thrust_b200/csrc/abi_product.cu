@@ -99,7 +99,7 @@ template <class T> struct product_plan {
   bool wide_out, wide_residual;      // rows are made of whole 16-byte pieces
   bool a_split, b_split;      // rows are made of whole chunks of 64 and mapped as such: a box has several
   int box;                    // by rows: rows in a box of B
-  int planes, segments;       // 32-bit operands are three of 16 bits each, and six products of them are added up; otherwise one and one
+  int planes;                 // 32-bit operands are three of 16 bits each, and six products of them are added up
   unsigned a_planes, b_planes;      // of which planes, two bits a segment
   const T *bias, *residual;
   size_t residual_stride;
@@ -376,6 +376,7 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
   using Shared = tc_shared<PAIR, WRITERS, BN, STAGES>;
   constexpr int CTAS = PAIR ? 2 : 1, OWN = GATED ? 64 : 128, WIDE = OWN * CTAS, UNIT = 16 * CTAS;
   constexpr bool FINE = Warps::FINE;
+  constexpr int SEGS = sizeof(T) == 4 ? SEGMENTS : 1, LEVELS = sizeof(T) == 4 ? 3 : 1;      // (32-bit rows come here as planes)
   extern __shared__ char raw[];
   char* const stages = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   Shared& sh = *reinterpret_cast<Shared*>(stages + STAGES * Shared::STAGE);
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
             }
           }
           __syncwarp();
-          if ((k += DEEP) >= tile.depth && ++segment < p.segments) k = 0;
+          if ((k += DEEP) >= tile.depth && ++segment < SEGS) k = 0;
         }
       }
       // the last of each stage, no longer needed
@@ -531,8 +532,8 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
             begun = true;
             bool cut = ++block == GROUP<O>;
             if ((k += DEEP) >= tile.depth) {
-              if (++segment < p.segments) k = 0;
-              cut = cut || segment == p.segments || next_level(segment);
+              if (++segment < SEGS) k = 0;
+              cut = cut || segment == SEGS || next_level(segment);
             }
             if (cut) {
               block = 0;
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
         if (tile.rows == 0) continue;
         const unsigned blocks = (unsigned)(tile.depth + DEEP - 1) / DEEP;
         const bool has = blocks > 0 && is_tail(tile, (int)(blocks - 1) * DEEP);
-        for (int segment = 0; good && segment < p.segments; ++segment) {
+        for (int segment = 0; good && segment < SEGS; ++segment) {
           const unsigned stage = (count + blocks - 1) % STAGES;
           count += blocks;
           if (!has) continue;
@@ -682,16 +683,16 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
       } else {
         // the sums of all groups, added up in registers, take the last one's place
         constexpr int N = BN / APART;
-        if (tile.depth && (p.segments > 1 || groups_of(1) > 1)) {
+        if (tile.depth && (LEVELS > 1 || groups_of(1) > 1)) {
           float sums[N][32];
 #pragma unroll
           for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int j = 0; j < 32; ++j) sums[i][j] = 0.f;
-          for (int level = p.segments > 1 ? 3 : 1; level > 0; --level) {      // so many segments have its scale
+          for (int level = LEVELS; level > 0; --level) {      // so many segments have its scale
             const int groups = groups_of(level);
             for (int g = 0; g < groups; ++g) {
-              const float scale = g == 0 && level < 3 ? 1.f / SCALE : 1.f;
+              const float scale = g == 0 && level < LEVELS ? 1.f / SCALE : 1.f;
               await_sums();
 #pragma unroll
               for (int i = 0; i < N; ++i) {
@@ -1297,7 +1298,6 @@ template <class T> bool in_planes(size_t n, size_t experts, size_t in, size_t ou
 }
 template <class T> void set_planes(product_plan<T>& p, bool split) {
   p.planes = split ? PLANES : 1;
-  p.segments = split ? SEGMENTS : 1;
   p.a_planes = split ? A_PLANES : 0;
   p.b_planes = split ? B_PLANES : 0;
 }
