@@ -46,3 +46,16 @@ def test_operands_that_are_not_read_may_be_null(tb, dtype, t, n, experts):
     assert grad(n, experts, 0, 9, t, d=d.data_ptr(), offsets=offsets.data_ptr(), db=db.data_ptr(), need=room, stream=stream) == 0 and room.value <= ws.numel()
     assert grad(n, experts, 0, 9, t, d=d.data_ptr(), offsets=offsets.data_ptr(), db=db.data_ptr(), ws=ws.data_ptr(), need=need, stream=stream) == 0
     assert torch.equal(db, offsets.diff().float()[:, None].expand(experts, 9))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n, experts", [(100, 3), (5000, 1), (0, 2)])
+def test_a_gradient_of_bias_alone_leaves_a_status(tb, n, experts):
+    """As the other calls' kernels, its own clear what is in the workspace."""
+    ws = torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda")
+    offsets = torch.linspace(0, n, experts + 1, device="cuda").int()
+    stream, status, need = torch.cuda.current_stream().cuda_stream, ctypes.c_uint(7), ctypes.c_size_t(ws.numel())
+    d, db = torch.ones(n + 1, 12, device="cuda"), torch.empty(experts, 9, device="cuda")
+    assert grad(n, experts, 0, 9, F32, d=d.data_ptr(), offsets=offsets.data_ptr(), db=db.data_ptr(), ws=ws.data_ptr(), need=need, stream=stream) == 0
+    assert _lib.load().tb200_workspace_status(ws.data_ptr(), stream, ctypes.byref(status)) == 0 and status.value == 0
+    assert torch.equal(db, offsets.diff().float()[:, None].expand(experts, 9))

@@ -958,12 +958,13 @@ __global__ void __launch_bounds__(FMA_THREADS, 3) expert_product_f32_kernel(cons
 constexpr int SUM_BLOCK = 256, SUM_GROUP = 1024 * SUM_BLOCK / 32;
 template <class T, int V>
 __global__ void __launch_bounds__(SUM_BLOCK) row_sums_kernel(const T* __restrict__ x, size_t stride, const void* __restrict__ offsets, bool wide, unsigned experts, int m, int features,
-                                                             float* __restrict__ sums) {
+                                                             float* __restrict__ sums, tb200::ws_header* hdr) {
   const unsigned e = blockIdx.y, part = blockIdx.z, parts = gridDim.z;
   const int a = read_offset(offsets, wide, e, m), end = read_offset(offsets, wide, e + 1, m), n = end > a ? end - a : 0, per = (n + (int)parts - 1) / (int)parts;
   const int first = a + (int)part * per, last = (int)part * per + per < n ? first + per : a + n;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, f = (blockIdx.x * 32 + lane) * V;
   tb200::grid_dependents_launch();
+  if (hdr && threadIdx.x == 0 && blockIdx.x + blockIdx.y + blockIdx.z == 0) hdr->error = 0;      // no product has cleared it, and nothing here waits
   float sum[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[v] = 0.f;
@@ -1432,7 +1433,8 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
           attr[0].val.programmaticStreamSerializationAllowed = 1;
           cfg.attrs = attr;
           cfg.numAttrs = in ? 1 : 0;      // beside the products: they are this call's, so what dout comes from is done
-          return cudaLaunchKernelEx(&cfg, row_sums_kernel<T, V>, static_cast<const T*>(d_dout), dout_stride, d_offsets, sizeof(iv) == 8, (unsigned)num_experts, (int)n, (int)out, to);
+          return cudaLaunchKernelEx(&cfg, row_sums_kernel<T, V>, static_cast<const T*>(d_dout), dout_stride, d_offsets, sizeof(iv) == 8, (unsigned)num_experts, (int)n, (int)out, to,
+                                    in ? nullptr : p.hdr);
         };
         e = in_16_bytes(d_dout, out, dout_stride, sizeof(T)) ? add(std::integral_constant<int, 16 / sizeof(T)>()) : add(std::integral_constant<int, 1>());
         if (e == cudaSuccess && parts > 1)
