@@ -357,8 +357,8 @@ constexpr unsigned A_PLANES = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, B
 // f16 and 128 for bf16, which are off by 2.4e-5 and 9.6e-5, a tenth and a twentieth of the least half step; a longer contraction goes on in the other set, by way of the writers, which add
 // the one to the other.  Sums of 2^20 numbers of one sign are off by half a step as those of 2^12 are (in one set: by 6e-3); 16384 f16 rows of 8192 to 512 take 142 us instead of 140,
 // of 16384 234 instead of 225.  32-bit results (FINE) are made of sums over six stages, which the writers add up in registers,
-// rounded to nearest, and put back to where the last ones were: three stages where an activation multiplies two results (off by 3.4e-7, and 6.8e-7 behind it, for any
-// length), six for matrices (7.3e-7; with four 4.7e-7, and 8198 rows' gradients take 103 us instead of 98).  Gated: the two halves of a result are in lanes 64 apart, in warps that pass each
+// rounded to nearest, and put back to where the last ones were: off by 7.3e-7 in the norm (9.8e-7 where 2^20 are added up), twice that behind an activation that multiplies two
+// results; with four stages 4.7e-7, and 8198 rows' gradients take 103 us instead of 98.  Gated: the two halves of a result are in lanes 64 apart, in warps that pass each
 // other half of their columns.
 //
 // By experts the contraction ends where the expert's rows do, in the middle of a box: what the box has of the next rows is cleared in shared memory, up to
@@ -1223,7 +1223,8 @@ cudaError_t launch_tc(const CUtensorMap& a, const CUtensorMap& b, const product_
   return cudaLaunchKernelEx(&cfg, kernel, a, b, p);
 }
 
-// So few rows an expert that a product is as long as it takes to read the matrices: narrow tiles, and nothing laid out anew that need not be.  64 bf16 rows of 2048 for each of
+// So few rows an expert that a product is as long as it takes to read the matrices: narrow tiles, and nothing laid out anew that need not be.  Both sides were measured
+// with as many rows for each expert; the rule knows the mean alone, and where most rows are a few experts' the wide tiles would take less from fewer rows on.  64 bf16 rows of 2048 for each of
 // 64 experts' 2048 outputs, gated: 94 us against 99, 96 rows 122 against 105; of 512 to 512 21 against 25, 27 against 17; 64 32-bit rows of 1024 for 16 experts' 1024 outputs 70
 // against 84, 96 rows 97 against 86.
 bool few_rows(size_t m, size_t experts) { return m <= 64 * experts; }
