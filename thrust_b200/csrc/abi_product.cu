@@ -215,11 +215,11 @@ template <class T> __device__ __forceinline__ void clear_others(const product_pl
 
 // ---------------------------------------------------------------------------------------------- 16 bits: tensor cores
 #ifdef TB200_TEST_HOOKS
-// Test builds only: the copies of the first CTA's second tile are announced and not made.
+// Test builds only: the copies of the first CTA's second tile are announced and not made, from stage withhold_boxes - 1 on.
 __device__ unsigned withhold_boxes;
-__device__ __forceinline__ bool withheld(unsigned t, unsigned step) { return withhold_boxes && blockIdx.x == 0 && t == step; }
+__device__ __forceinline__ bool withheld(unsigned t, unsigned step, int stage) { return withhold_boxes && blockIdx.x == 0 && t == step && (unsigned)stage + 1 >= withhold_boxes; }
 #else
-__device__ __forceinline__ bool withheld(unsigned, unsigned) { return false; }
+__device__ __forceinline__ bool withheld(unsigned, unsigned, int) { return false; }
 #endif
 
 constexpr int DEEP = 128;                     // of the contraction, a stage
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(tc_warps<MODE, O, PAIR>::THREADS, tc_warps<MOD
               if (rank == 0) tb200::mbar_arrive_expect(&sh.full[stage], bytes * CTAS);
               bar = PAIR ? tb200_tc::first_ones(&sh.full[stage]) : tb200::smem_addr(&sh.full[stage]);
             }
-            if (!withheld(t, step)) {
+            if (!withheld(t, step, k / DEEP)) {
               const int row = MODE == BY_ROWS ? k : tile.row + k, pa = (int)(p.a_planes >> 2 * segment & 3), pb = (int)(p.b_planes >> 2 * segment & 3);
               const int of_a = MODE == BY_ROWS ? (int)tile.e * p.planes + pa : pa;
               const bool both = p.a_split || (GATED && p.a_mn);
