@@ -448,7 +448,7 @@ enum tb200_activation { TB200_ACT_NONE = 0, TB200_ACT_SILU = 1, TB200_ACT_GELU =
  * W is in x out; element (i, o) of expert e's is at e * expert_stride + i * weight_stride + o, or with inputs_inside != 0 at e * expert_stride + o * weight_stride
  * + i (experts' matrices must not overlap).  d_bias (packed, num_experts x out) and d_residual may be NULL, and so may d_before (n x out), which a gradient
  * needs.  d_out is n x out, gated n x out / 2.  Rows that are no expert's are zero in d_out and d_before.  All are of type t; in, out < 2^24, n < 2^31 - 1024.
- * The size of the workspace depends on all arguments but d_ws: operands that are not made of 16-byte pieces are laid out anew there, and so are
+ * The size of the workspace, which is 16-byte aligned, depends on all arguments but d_ws: operands that are not made of 16-byte pieces are laid out anew there, and so are
  * F32 operands where there are many rows: as three bf16 numbers each, the second and third scaled (exact from 2^-123 on,
  * to 2^-148 below), of whose products those of 2^-24 of the whole are left out.  An infinite F32 operand leaves results that are infinite or NaN.
  * Waits inside a CTA and between two are bounded: one that ran out leaves NaNs and status 1. */

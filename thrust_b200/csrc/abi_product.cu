@@ -1291,6 +1291,8 @@ template <class T, class O> cudaError_t product_by_experts(const matrices& featu
   return launch_tc<T, O, BY_EXPERTS, false, false, 128, 3>(a, b, p, stream);
 }
 
+// what is laid out anew is read 16 bytes at a time, and by the copy engine
+bool on_16_bytes(const void* d_ws) { return (reinterpret_cast<uintptr_t>(d_ws) & 15) == 0; }
 bool sizes_fit(size_t n, size_t experts, size_t in, size_t out) { return n <= MOST_ROWS && experts >= 1 && experts <= (size_t)MOST_EXPERTS && in < MOST_CHANNELS && out < MOST_CHANNELS; }
 // 32-bit rows go to the tensor cores, as planes, where products are longer than it takes to lay the planes out: not few rows, and 128 or more channels on both sides (256 rows of
 // 64 for 16 experts' 64 outputs: 14 us by multiply-adds against 21; 256 of 128 to 2048: 98 against 42).  Sums over very many rows do too, because one
@@ -1329,7 +1331,7 @@ TB200_API int tb200_expert_product(const void* d_rows, size_t rows_stride, const
     using T = decltype(tv);
     return by_index_dtype(offset_t, [&](auto iv) -> int {
       const bool gated = (activation & ACT_GATED) != 0;
-      if (!sizes_fit(n, num_experts, in, out) || !activation_known(activation) || (gated && out % 2)) return ERR_INVALID;
+      if (!sizes_fit(n, num_experts, in, out) || !activation_known(activation) || (gated && out % 2) || !on_16_bytes(d_ws)) return ERR_INVALID;
       const size_t width = gated ? out / 2 : out;
       const bool split = in_planes<T>(n, num_experts, in, out, false);
       matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, gated ? 2 : 1, sizeof(T), split), x = {d_rows, in, n, rows_stride, 0, 0, 1, sizeof(T), split};
@@ -1371,7 +1373,7 @@ TB200_API int tb200_expert_product_grad(const void* d_dout, size_t dout_stride, 
     using T = decltype(tv);
     if (grad_t != t && grad_t != TB200_F32) return ERR_UNSUPPORTED;
     return by_index_dtype(offset_t, [&](auto iv) -> int {
-      if (!sizes_fit(n, num_experts, in, out)) return ERR_INVALID;
+      if (!sizes_fit(n, num_experts, in, out) || !on_16_bytes(d_ws)) return ERR_INVALID;
       const bool split = in_planes<T>(n, num_experts, in, out, true);
       matrices w = weights_of(d_weight, num_experts, in, out, expert_stride, weight_stride, inputs_inside != 0, 1, sizeof(T), split), x = {d_rows, in, n, rows_stride, 0, 0, 1, sizeof(T), split},
                d = {d_dout, out, n, dout_stride, 0, 0, 1, sizeof(T), split};
